@@ -132,6 +132,47 @@ class PointwiseDesc(Structure):
                 ("params", PointwiseParams)]
 
 
+class CacheDesc(Structure):
+    _fields_ = [("k", TensorDesc), ("v", TensorDesc), ("k_params", TensorDesc),
+                ("v_params", TensorDesc), ("batch", c_int64),
+                ("pages_per_sequence", c_int64), ("page_stride", c_int64)]
+
+
+class CachePointers(Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_params", c_void_p),
+                ("v_params", c_void_p), ("pages", c_void_p),
+                ("lengths", c_void_p)]
+
+    @staticmethod
+    def make(k, v, pages, lengths, k_params=None, v_params=None) -> "CachePointers":
+        """Of DeviceBuffers or addresses, which the caller keeps."""
+        return CachePointers(*(_p(x) for x in (k, v, k_params, v_params, pages, lengths)))
+
+
+class SdpaPackedDesc(Structure):
+    _fields_ = [("q", TensorDesc), ("k", TensorDesc), ("v", TensorDesc),
+                ("o", TensorDesc), ("batch", c_int64),
+                ("has_kv_offsets", c_int32), ("is_causal", c_int32),
+                ("has_scale", c_int32), ("scale", c_float)]
+
+
+class SdpaPagedDesc(Structure):
+    _fields_ = [("q", TensorDesc), ("o", TensorDesc), ("cache", CacheDesc),
+                ("is_causal", c_int32), ("has_scale", c_int32),
+                ("scale", c_float)]
+
+
+class CacheAppendDesc(Structure):
+    _fields_ = [("k", TensorDesc), ("v", TensorDesc), ("q", TensorDesc),
+                ("rotation", TensorDesc), ("q_out", TensorDesc),
+                ("k_out", TensorDesc), ("cache", CacheDesc),
+                ("has_positions", c_int32), ("interleaved", c_int32)]
+
+
+class CacheReadDesc(Structure):
+    _fields_ = [("k", TensorDesc), ("v", TensorDesc), ("cache", CacheDesc)]
+
+
 def epilogue_op(mode: int, result_dtype: int, *, scalar: Optional[float] = None,
                 operand: Optional[TensorDesc] = None, operand_index: int = 0,
                 acc_is_in1: bool = False,
@@ -206,6 +247,19 @@ SYMBOLS = {
     "fhip_sdpa_fwd_workspace_size": (c_int, [POINTER(SdpaDesc), POINTER(c_size_t)]),
     "fhip_sdpa_fwd_supported": (c_int, [POINTER(SdpaDesc)]),
     "fhip_sdpa_fwd": (c_int, [_P, POINTER(SdpaDesc), _P, _P, _P, _P, _P, _P, c_size_t]),
+    "fhip_sdpa_packed_fwd_workspace_size": (c_int, [POINTER(SdpaPackedDesc), POINTER(c_size_t)]),
+    "fhip_sdpa_packed_fwd_supported": (c_int, [POINTER(SdpaPackedDesc)]),
+    "fhip_sdpa_packed_fwd": (c_int, [_P, POINTER(SdpaPackedDesc), _P, _P, _P, _P, _P, _P, _P, c_size_t]),
+    "fhip_sdpa_paged_fwd_workspace_size": (c_int, [POINTER(SdpaPagedDesc), POINTER(c_size_t)]),
+    "fhip_sdpa_paged_fwd_supported": (c_int, [POINTER(SdpaPagedDesc)]),
+    "fhip_sdpa_paged_fwd": (c_int, [_P, POINTER(SdpaPagedDesc), POINTER(CachePointers), _P, _P, _P, _P, c_size_t]),
+    "fhip_cache_append_workspace_size": (c_int, [POINTER(CacheAppendDesc), POINTER(c_size_t)]),
+    "fhip_cache_append_supported": (c_int, [POINTER(CacheAppendDesc)]),
+    "fhip_cache_append": (c_int, [_P, POINTER(CacheAppendDesc), POINTER(CachePointers), _P, _P, _P, _P, _P, _P,
+                                  _P, _P, _P, c_size_t]),
+    "fhip_cache_read_workspace_size": (c_int, [POINTER(CacheReadDesc), POINTER(c_size_t)]),
+    "fhip_cache_read_supported": (c_int, [POINTER(CacheReadDesc)]),
+    "fhip_cache_read": (c_int, [_P, POINTER(CacheReadDesc), POINTER(CachePointers), _P, _P, _P, _P, c_size_t]),
     "fhip_norm_fwd_workspace_size": (c_int, [POINTER(NormDesc), POINTER(c_size_t)]),
     "fhip_norm_fwd_supported": (c_int, [POINTER(NormDesc)]),
     "fhip_norm_fwd": (c_int, [_P, POINTER(NormDesc), _P, _P, _P, POINTER(_P), _P, _P, _P, _P, c_size_t]),
@@ -438,6 +492,52 @@ class Context:
     def sdpa_fwd(self, d: SdpaDesc, q, k, v, o, mask=None):
         self._check(self.lib.fhip_sdpa_fwd(self.handle, byref(d), _p(q), _p(k),
                                            _p(v), _p(mask), _p(o), None, 0))
+
+    def sdpa_packed_workspace(self, d: SdpaPackedDesc) -> int:
+        n = c_size_t(0)
+        if self.lib.fhip_sdpa_packed_fwd_workspace_size(byref(d), byref(n)) != 0:
+            raise FusilliHipError(self.lib.fhip_last_error(None).decode())
+        return n.value
+
+    def sdpa_packed_fwd(self, d: SdpaPackedDesc, q, k, v, offsets, o,
+                        kv_offsets=None, workspace=None):
+        """`workspace`: a DeviceBuffer or address of at least
+        sdpa_packed_workspace(d) bytes; allocated here when omitted."""
+        need = self.sdpa_packed_workspace(d)
+        if need and workspace is None:
+            workspace = self.alloc(need)
+        self._check(self.lib.fhip_sdpa_packed_fwd(
+            self.handle, byref(d), _p(q), _p(k), _p(v), _p(offsets),
+            _p(kv_offsets), _p(o), _p(workspace), need))
+
+    def sdpa_paged_workspace(self, d: SdpaPagedDesc) -> int:
+        n = c_size_t(0)
+        if self.lib.fhip_sdpa_paged_fwd_workspace_size(byref(d), byref(n)) != 0:
+            raise FusilliHipError(self.lib.fhip_last_error(None).decode())
+        return n.value
+
+    def sdpa_paged_fwd(self, d: SdpaPagedDesc, cache: CachePointers, q, offsets,
+                       o, workspace=None):
+        """`workspace`: a DeviceBuffer or address of at least
+        sdpa_paged_workspace(d) bytes; allocated here when omitted."""
+        need = self.sdpa_paged_workspace(d)
+        if need and workspace is None:
+            workspace = self.alloc(need)
+        self._check(self.lib.fhip_sdpa_paged_fwd(
+            self.handle, byref(d), byref(cache), _p(q), _p(offsets), _p(o),
+            _p(workspace), need))
+
+    def cache_append(self, d: CacheAppendDesc, cache: CachePointers, k, v, offsets,
+                     q=None, rotation=None, positions=None, q_out=None, k_out=None):
+        self._check(self.lib.fhip_cache_append(
+            self.handle, byref(d), byref(cache), _p(q), _p(k), _p(v),
+            _p(rotation), _p(offsets), _p(positions), _p(q_out), _p(k_out),
+            None, 0))
+
+    def cache_read(self, d: CacheReadDesc, cache: CachePointers, offsets, k, v):
+        self._check(self.lib.fhip_cache_read(
+            self.handle, byref(d), byref(cache), _p(offsets), _p(k), _p(v),
+            None, 0))
 
     def norm_fwd(self, d: NormDesc, x, scale, bias, out, mean=None, rstd=None,
                  epilogue_operands=()):

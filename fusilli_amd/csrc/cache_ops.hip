@@ -1,0 +1,370 @@
+// A key / value cache in pages: appending packed rows to it, positions rotated
+// into queries and keys on the way, and reading rows back.
+//
+// This file holds the entry points and the kernels for any type, size and
+// stride: one wavefront per row of one head.
+#include "paged_cache.h"
+#include "fast_paths.h"
+
+namespace {
+
+struct AppendArgs {
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  const float *rotation;
+  const int32_t *offsets, *positions;
+  FhipCacheView cache;
+  int64_t q_s[2], k_s[2], v_s[2], qo_s[2], ko_s[2]; // row and head strides
+  int64_t rot_s;
+  int32_t dtype, T, Hq, Hkv, D, Dv, R, table_rows, interleaved;
+};
+
+// Rounds a group's values (in LDS) and stores a row of a pool.
+__device__ void store_row(const FhipCacheView &c, const FhipPool &p, int page, int slot, int h, const float *x, int D,
+                          int lane) {
+  const int64_t at = page * p.page + h * p.head + slot * p.slot;
+  if (!c.group) {
+    for (int e = lane; e < D; e += 64)
+      fhip_store<float>(p.data, c.dtype, at + e, x[e]);
+    return;
+  }
+  _Float16 *pairs = p.params + page * p.params_page + h * p.params_head + slot * p.params_slot;
+  for (int e = lane * 2; e < D; e += 128) {
+    const float *of = x + e / c.group * c.group;
+    float lo = of[0], hi = of[0];
+    bool number = true;
+    for (int i = 0; i < c.group; ++i) {
+      lo = fminf(lo, of[i]), hi = fmaxf(hi, of[i]);
+      number &= __builtin_fabsf(of[i]) < INFINITY;
+    }
+    const FhipGroup g = fhip_group_of(number ? lo : INFINITY, hi);
+    ((uint8_t *)p.data)[at + e / 2] = (uint8_t)(fhip_code_of(g, x[e]) | fhip_code_of(g, x[e + 1]) << 4);
+    if (e % c.group == 0)
+      pairs[e / c.group * 2] = g.scale, pairs[e / c.group * 2 + 1] = g.low;
+  }
+}
+
+__global__ __launch_bounds__(64) void append_rows_kernel(AppendArgs g) {
+#pragma clang fp contract(off)
+  __shared__ float row[kCacheMaxDim];
+  const int heads = g.Hq + 2 * g.Hkv;
+  const int t = (int)(blockIdx.x / (uint32_t)heads), which = (int)(blockIdx.x % (uint32_t)heads);
+  const int lane = threadIdx.x;
+  const int b = fhip_sequence_of(g.offsets, g.cache.batch, t);
+  if (b < 0)
+    return;
+  const int64_t place = (int64_t)g.cache.lengths[b] - g.offsets[b + 1] + t;
+  const int64_t pos = g.positions ? g.positions[t] : place;
+  const bool turned = !g.R || (pos >= 0 && pos < g.table_rows);
+  const int page = place >= 0 && place < kCacheMaxKeys ? fhip_page_of(g.cache, b, (int)place) : -1;
+  const int slot = page < 0 ? 0 : (int)(place % g.cache.page_size);
+  if (which >= g.Hq + g.Hkv) { // a row of V
+    const int h = which - g.Hq - g.Hkv;
+    if (page < 0 || !turned)
+      return;
+    for (int e = lane; e < g.Dv; e += 64)
+      row[e] = fhip_load<float>(g.v, g.dtype, t * g.v_s[0] + h * g.v_s[1] + e);
+    __syncthreads();
+    store_row(g.cache, g.cache.v, page, slot, h, row, g.Dv, lane);
+    return;
+  }
+  const bool is_q = which < g.Hq;
+  const int h = is_q ? which : which - g.Hq;
+  const void *x = is_q ? g.q : g.k;
+  const int64_t at = t * (is_q ? g.q_s[0] : g.k_s[0]) + h * (is_q ? g.q_s[1] : g.k_s[1]);
+  const float *angles = g.R && turned ? g.rotation + pos * g.rot_s : nullptr;
+  const int half = g.R / 2;
+  for (int e = lane; e < g.D; e += 64) {
+    float y = fhip_load<float>(x, g.dtype, at + e);
+    if (e < g.R) {
+      // (the pair's first and second element, each with its own sign)
+      const int i = g.interleaved ? e >> 1 : e % half;
+      const bool second = g.interleaved ? e & 1 : e >= half;
+      const int other = g.interleaved ? e ^ 1 : second ? e - half : e + half;
+      const float z = fhip_load<float>(x, g.dtype, at + other);
+      if (angles) {
+        const float c = angles[i], s = angles[half + i];
+        const float yc = y * c, zs = z * s;
+        y = second ? yc + zs : yc - zs;
+      }
+    }
+    row[e] = turned ? fhip_round_through<float>(g.dtype, y) : __builtin_nanf("");
+  }
+  __syncthreads();
+  void *out = is_q ? g.q_out : g.k_out;
+  if (out) {
+    const int64_t to = t * (is_q ? g.qo_s[0] : g.ko_s[0]) + h * (is_q ? g.qo_s[1] : g.ko_s[1]);
+    for (int e = lane; e < g.D; e += 64)
+      fhip_store<float>(out, g.dtype, to + e, row[e]);
+  }
+  if (!is_q && page >= 0 && turned)
+    store_row(g.cache, g.cache.k, page, slot, h, row, g.D, lane);
+}
+
+struct ReadArgs {
+  void *k, *v;
+  const int32_t *offsets;
+  FhipCacheView cache;
+  int64_t k_s[2], v_s[2];
+  int32_t dtype, T, Hkv, D, Dv;
+};
+
+__global__ __launch_bounds__(64) void read_rows_kernel(ReadArgs g) {
+  const int t = (int)(blockIdx.x / (uint32_t)(2 * g.Hkv)), which = (int)(blockIdx.x % (uint32_t)(2 * g.Hkv));
+  const int b = fhip_sequence_of(g.offsets, g.cache.batch, t);
+  if (b < 0)
+    return;
+  const int64_t place = (int64_t)g.cache.lengths[b] - g.offsets[b + 1] + t;
+  const int page = place >= 0 && place < kCacheMaxKeys ? fhip_page_of(g.cache, b, (int)place) : -1;
+  const int slot = page < 0 ? 0 : (int)(place % g.cache.page_size);
+  const bool is_k = which < g.Hkv;
+  const int h = is_k ? which : which - g.Hkv, D = is_k ? g.D : g.Dv;
+  const FhipPool &p = is_k ? g.cache.k : g.cache.v;
+  void *out = is_k ? g.k : g.v;
+  const int64_t to = t * (is_k ? g.k_s[0] : g.v_s[0]) + h * (is_k ? g.k_s[1] : g.v_s[1]);
+  for (int e = threadIdx.x; e < D; e += 64)
+    fhip_store<float>(out, g.dtype, to + e,
+                      page < 0 ? __builtin_nanf("") : fhip_cache_value(g.cache, p, page, slot, h, e));
+}
+
+// Ranges of memory that a tensor of non-negative strides spans.
+bool same_tensor(const fhip_tensor_desc &a, const fhip_tensor_desc &b) {
+  for (int i = 0; i < a.rank; ++i)
+    if (a.dim[i] > 1 && a.stride[i] != b.stride[i])
+      return false;
+  return a.dtype == b.dtype;
+}
+
+} // namespace
+
+FhipCacheView fhip_cache_view(const fhip_cache_desc &c, const fhip_cache_ptrs &p) {
+  FhipCacheView w{};
+  auto pool = [&](const fhip_tensor_desc &t, const fhip_tensor_desc &pt, void *data, void *params) {
+    auto st = [](const fhip_tensor_desc &x, int i) { return x.dim[i] > 1 ? x.stride[i] : 0; };
+    FhipPool o{(char *)data, (_Float16 *)params, st(t, 0), st(t, 1), st(t, 2), 0, 0, 0};
+    if (pt.rank)
+      o.params_page = st(pt, 0), o.params_head = st(pt, 1), o.params_slot = st(pt, 2);
+    return o;
+  };
+  w.k = pool(c.k, c.k_params, p.k, p.k_params);
+  w.v = pool(c.v, c.v_params, p.v, p.v_params);
+  w.table = (const int32_t *)p.pages;
+  w.lengths = (const int32_t *)p.lengths;
+  w.table_stride = c.batch > 1 ? c.page_stride : 0;
+  w.batch = (int32_t)c.batch;
+  w.table_pages = (int32_t)c.pages_per_sequence;
+  w.pool_pages = (int32_t)c.k.dim[0];
+  w.page_size = (int32_t)c.k.dim[2];
+  w.group = c.k_params.rank ? (int32_t)(2 * c.k.dim[3] / (c.k_params.dim[3] / 2)) : 0;
+  w.dtype = c.k.dtype;
+  return w;
+}
+
+int fhip_check_rows(fhip_ctx *ctx, const char *who, const char *what, const fhip_tensor_desc &t, bool written) {
+  if (!fhip_check_desc(ctx, t, what))
+    return 1;
+  FHIP_REQUIRE(ctx, t.rank == 3, "%s: %s must be rank 3 [rows, heads, head dim]", who, what);
+  FHIP_REQUIRE(ctx, t.dtype == FHIP_FLOAT || t.dtype == FHIP_BFLOAT16 || t.dtype == FHIP_HALF,
+               "%s: %s must be f32, bf16 or f16", who, what);
+  FHIP_REQUIRE(ctx, t.dim[0] < (1ll << 31) - 1 && t.dim[1] < (1 << 20) && t.dim[2] <= kCacheMaxDim,
+               "%s: %s has rows, heads or a head dim (above %d) out of range", who, what, kCacheMaxDim);
+  FHIP_REQUIRE(ctx, t.dim[2] == 1 || t.stride[2] == 1, "%s: %s must have a unit stride in its last dim", who, what);
+  FHIP_REQUIRE(ctx, !written || ((t.dim[0] == 1 || t.stride[0] > 0) && (t.dim[1] == 1 || t.stride[1] > 0)),
+               "%s: %s is written and has a stride of 0", who, what);
+  return 0;
+}
+
+int fhip_check_cache(fhip_ctx *ctx, const char *who, const fhip_cache_desc &c, int dtype, int64_t heads, int64_t D,
+                     int64_t Dv) {
+  if (!fhip_check_desc(ctx, c.k, "cache K") || !fhip_check_desc(ctx, c.v, "cache V"))
+    return 1;
+  FHIP_REQUIRE(ctx, c.k.rank == 4 && c.v.rank == 4,
+               "%s: the cache's K and V must be rank 4 [pages, heads, page size, head dim]", who);
+  for (int i = 0; i < 3; ++i)
+    FHIP_REQUIRE(ctx, c.k.dim[i] == c.v.dim[i], "%s: the cache's K and V differ in dim %d", who, i);
+  FHIP_REQUIRE(ctx, c.k.dim[0] < (1ll << 31) && c.k.dim[2] <= (1 << 24), "%s: pages or page size out of range", who);
+  FHIP_REQUIRE(ctx, c.k.dim[1] == heads, "%s: the cache has %lld heads, the rows %lld", who, (long long)c.k.dim[1],
+               (long long)heads);
+  FHIP_REQUIRE(ctx, c.k.dtype == c.v.dtype, "%s: the cache's K and V differ in type", who);
+  const bool packed = c.k.dtype == FHIP_UINT8;
+  FHIP_REQUIRE(ctx, packed || c.k.dtype == dtype, "%s: the cache must have the rows' type, or be Uint8 with parameters",
+               who);
+  FHIP_REQUIRE(ctx, packed == (c.k_params.rank != 0) && packed == (c.v_params.rank != 0),
+               "%s: parameters go with a Uint8 cache, and only with one", who);
+  const int64_t div = packed ? 2 : 1;
+  FHIP_REQUIRE(ctx, D % div == 0 && Dv % div == 0 && c.k.dim[3] == D / div && c.v.dim[3] == Dv / div,
+               "%s: the cache's head dims do not fit the rows'", who);
+  const fhip_tensor_desc *ts[4] = {&c.k, &c.v, &c.k_params, &c.v_params};
+  for (int i = 0; i < (packed ? 4 : 2); ++i) {
+    const fhip_tensor_desc &t = *ts[i];
+    if (i >= 2) {
+      if (!fhip_check_desc(ctx, t, "cache parameters"))
+        return 1;
+      FHIP_REQUIRE(ctx, t.rank == 4 && t.dtype == FHIP_HALF && t.dim[0] == c.k.dim[0] && t.dim[1] == heads &&
+                            t.dim[2] == c.k.dim[2],
+                   "%s: the cache's parameters must be Half [pages, heads, page size, pairs]", who);
+    }
+    FHIP_REQUIRE(ctx, t.dim[3] == 1 || t.stride[3] == 1, "%s: the cache needs a unit stride in its last dim", who);
+    for (int j = 0; j < 3; ++j)
+      FHIP_REQUIRE(ctx, t.dim[j] == 1 || t.stride[j] > 0, "%s: the cache has a stride of 0", who);
+  }
+  if (packed) {
+    const int64_t nk = c.k_params.dim[3] / 2, nv = c.v_params.dim[3] / 2;
+    FHIP_REQUIRE(ctx, c.k_params.dim[3] % 2 == 0 && c.v_params.dim[3] % 2 == 0 && nk > 0 && nv > 0 && D % nk == 0 &&
+                          Dv % nv == 0 && D / nk % 2 == 0 && D / nk == Dv / nv,
+                 "%s: groups must be of an even number of elements that divides the head dims, the same for K and V",
+                 who);
+  }
+  FHIP_REQUIRE(ctx, c.batch >= 1 && c.batch < (1 << 30), "%s: batch %lld out of range", who, (long long)c.batch);
+  FHIP_REQUIRE(ctx, c.pages_per_sequence >= 1 && c.pages_per_sequence < (1ll << 31) &&
+                        c.pages_per_sequence * c.k.dim[2] <= kCacheMaxKeys,
+               "%s: the page table holds more than 2^30 keys per sequence, or none", who);
+  FHIP_REQUIRE(ctx, c.batch == 1 || c.page_stride >= c.pages_per_sequence, "%s: the page table's rows overlap", who);
+  return 0;
+}
+
+int fhip_check_cache_ptrs(fhip_ctx *ctx, const char *who, const fhip_cache_desc &c, const fhip_cache_ptrs *p) {
+  FHIP_REQUIRE(ctx, p && p->k && p->v && p->pages && p->lengths, "%s: null cache pointer", who);
+  FHIP_REQUIRE(ctx, (c.k_params.rank != 0) == (p->k_params != nullptr) &&
+                        (c.v_params.rank != 0) == (p->v_params != nullptr),
+               "%s: parameter pointers and descriptors disagree", who);
+  return 0;
+}
+
+static int append_validate(fhip_ctx *ctx, const fhip_cache_append_desc *d) {
+  static const char who[] = "fhip_cache_append";
+  FHIP_REQUIRE(ctx, d != nullptr, "%s: null descriptor", who);
+  if (fhip_check_rows(ctx, who, "K", d->k, false) || fhip_check_rows(ctx, who, "V", d->v, false))
+    return 1;
+  const int64_t T = d->k.dim[0], Hkv = d->k.dim[1], D = d->k.dim[2], Dv = d->v.dim[2];
+  FHIP_REQUIRE(ctx, d->v.dim[0] == T && d->v.dim[1] == Hkv && d->v.dtype == d->k.dtype,
+               "%s: K and V differ in rows, heads or type", who);
+  FHIP_REQUIRE(ctx, (d->q.rank != 0) == (d->q_out.rank != 0), "%s: Q and Q_OUT go together", who);
+  if (d->q.rank) {
+    if (fhip_check_rows(ctx, who, "Q", d->q, false) || fhip_check_rows(ctx, who, "Q_OUT", d->q_out, true))
+      return 1;
+    for (int i = 0; i < 3; ++i)
+      FHIP_REQUIRE(ctx, d->q.dim[i] == d->q_out.dim[i], "%s: Q_OUT dims differ from Q's", who);
+    FHIP_REQUIRE(ctx, d->q.dim[0] == T && d->q.dim[2] == D && d->q.dtype == d->k.dtype && d->q_out.dtype == d->k.dtype,
+                 "%s: Q, Q_OUT and K differ in rows, head dim or type", who);
+  }
+  if (d->k_out.rank) {
+    if (fhip_check_rows(ctx, who, "K_OUT", d->k_out, true))
+      return 1;
+    for (int i = 0; i < 3; ++i)
+      FHIP_REQUIRE(ctx, d->k.dim[i] == d->k_out.dim[i], "%s: K_OUT dims differ from K's", who);
+    FHIP_REQUIRE(ctx, d->k_out.dtype == d->k.dtype, "%s: K_OUT has another type than K", who);
+  }
+  if (d->rotation.rank) {
+    const fhip_tensor_desc &r = d->rotation;
+    if (!fhip_check_desc(ctx, r, "ROTATION"))
+      return 1;
+    FHIP_REQUIRE(ctx, r.rank == 2 && r.dtype == FHIP_FLOAT && r.stride[1] == 1 && r.dim[0] < (1ll << 31),
+                 "%s: ROTATION must be Float [positions, R] with a unit stride in its last dim", who);
+    FHIP_REQUIRE(ctx, r.dim[1] % 2 == 0 && r.dim[1] <= D, "%s: ROTATION turns %lld of %lld dims", who,
+                 (long long)r.dim[1], (long long)D);
+  }
+  const int64_t heads = (d->q.rank ? d->q.dim[1] : 0) + 2 * Hkv;
+  FHIP_REQUIRE(ctx, T * heads < (1ll << 31), "%s: more than 2^31 rows of heads", who);
+  return fhip_check_cache(ctx, who, d->cache, d->k.dtype, Hkv, D, Dv);
+}
+
+static int read_validate(fhip_ctx *ctx, const fhip_cache_read_desc *d) {
+  static const char who[] = "fhip_cache_read";
+  FHIP_REQUIRE(ctx, d != nullptr, "%s: null descriptor", who);
+  if (fhip_check_rows(ctx, who, "K", d->k, true) || fhip_check_rows(ctx, who, "V", d->v, true))
+    return 1;
+  FHIP_REQUIRE(ctx, d->v.dim[0] == d->k.dim[0] && d->v.dim[1] == d->k.dim[1] && d->v.dtype == d->k.dtype,
+               "%s: K and V differ in rows, heads or type", who);
+  FHIP_REQUIRE(ctx, d->k.dim[0] * d->k.dim[1] < (1ll << 30), "%s: more than 2^30 rows of heads", who);
+  return fhip_check_cache(ctx, who, d->cache, d->k.dtype, d->k.dim[1], d->k.dim[2], d->v.dim[2]);
+}
+
+extern "C" {
+
+int fhip_cache_append_workspace_size(const fhip_cache_append_desc *d, size_t *bytes) {
+  FHIP_REQUIRE(nullptr, d && bytes, "fhip_cache_append_workspace_size: null");
+  *bytes = 0;
+  return 0;
+}
+
+int fhip_cache_append_supported(const fhip_cache_append_desc *d) {
+  if (!d || append_validate(nullptr, d) != 0)
+    return 0;
+  return 1;
+}
+
+int fhip_cache_append(fhip_ctx *ctx, const fhip_cache_append_desc *d, const fhip_cache_ptrs *cache, const void *q,
+                      const void *k, const void *v, const void *rotation, const void *offsets, const void *positions,
+                      void *q_out, void *k_out, void *workspace, size_t workspace_bytes) {
+  static const char who[] = "fhip_cache_append";
+  FHIP_REQUIRE(ctx, ctx != nullptr, "%s: null context", who);
+  if (append_validate(ctx, d) != 0 || fhip_check_cache_ptrs(ctx, who, d->cache, cache) != 0)
+    return 1;
+  FHIP_REQUIRE(ctx, k && v && offsets, "%s: null tensor pointer", who);
+  FHIP_REQUIRE(ctx, (d->q.rank != 0) == (q != nullptr) && (d->q.rank != 0) == (q_out != nullptr),
+               "%s: Q / Q_OUT pointers and descriptors disagree", who);
+  FHIP_REQUIRE(ctx, (d->k_out.rank != 0) == (k_out != nullptr), "%s: K_OUT pointer and descriptor disagree", who);
+  FHIP_REQUIRE(ctx, (d->rotation.rank != 0) == (rotation != nullptr), "%s: ROTATION pointer and descriptor disagree",
+               who);
+  FHIP_REQUIRE(ctx, (d->has_positions != 0) == (positions != nullptr), "%s: positions and has_positions disagree", who);
+  FHIP_REQUIRE(ctx, (q_out != q || same_tensor(d->q, d->q_out)) && (k_out != k || same_tensor(d->k, d->k_out)),
+               "%s: a row that is turned in place needs the same strides", who);
+  (void)workspace;
+  (void)workspace_bytes;
+  FHIP_HIP_CHECK(ctx, hipSetDevice(ctx->device));
+  fhip_note_kernel(ctx, "cache_append_rows");
+  AppendArgs g{};
+  g.q = q, g.k = k, g.v = v, g.q_out = q_out, g.k_out = k_out;
+  g.rotation = (const float *)rotation;
+  g.offsets = (const int32_t *)offsets, g.positions = (const int32_t *)positions;
+  g.cache = fhip_cache_view(d->cache, *cache);
+  auto st = [](const fhip_tensor_desc &t, int64_t(&s)[2]) { s[0] = t.stride[0], s[1] = t.stride[1]; };
+  st(d->q, g.q_s), st(d->k, g.k_s), st(d->v, g.v_s), st(d->q_out, g.qo_s), st(d->k_out, g.ko_s);
+  g.dtype = d->k.dtype;
+  g.T = (int32_t)d->k.dim[0], g.Hq = d->q.rank ? (int32_t)d->q.dim[1] : 0, g.Hkv = (int32_t)d->k.dim[1];
+  g.D = (int32_t)d->k.dim[2], g.Dv = (int32_t)d->v.dim[2];
+  if (d->rotation.rank)
+    g.R = (int32_t)d->rotation.dim[1], g.table_rows = (int32_t)d->rotation.dim[0], g.rot_s = d->rotation.stride[0];
+  g.interleaved = d->interleaved != 0;
+  hipLaunchKernelGGL(append_rows_kernel, dim3((unsigned)((int64_t)g.T * (g.Hq + 2 * g.Hkv))), dim3(64), 0, ctx->stream,
+                     g);
+  FHIP_HIP_CHECK(ctx, hipGetLastError());
+  return 0;
+}
+
+int fhip_cache_read_workspace_size(const fhip_cache_read_desc *d, size_t *bytes) {
+  FHIP_REQUIRE(nullptr, d && bytes, "fhip_cache_read_workspace_size: null");
+  *bytes = 0;
+  return 0;
+}
+
+int fhip_cache_read_supported(const fhip_cache_read_desc *d) {
+  if (!d || read_validate(nullptr, d) != 0)
+    return 0;
+  return 1;
+}
+
+int fhip_cache_read(fhip_ctx *ctx, const fhip_cache_read_desc *d, const fhip_cache_ptrs *cache, const void *offsets,
+                    void *k, void *v, void *workspace, size_t workspace_bytes) {
+  static const char who[] = "fhip_cache_read";
+  FHIP_REQUIRE(ctx, ctx != nullptr, "%s: null context", who);
+  if (read_validate(ctx, d) != 0 || fhip_check_cache_ptrs(ctx, who, d->cache, cache) != 0)
+    return 1;
+  FHIP_REQUIRE(ctx, k && v && offsets, "%s: null tensor pointer", who);
+  (void)workspace;
+  (void)workspace_bytes;
+  FHIP_HIP_CHECK(ctx, hipSetDevice(ctx->device));
+  fhip_note_kernel(ctx, "cache_read_rows");
+  ReadArgs g{};
+  g.k = k, g.v = v, g.offsets = (const int32_t *)offsets;
+  g.cache = fhip_cache_view(d->cache, *cache);
+  g.k_s[0] = d->k.stride[0], g.k_s[1] = d->k.stride[1], g.v_s[0] = d->v.stride[0], g.v_s[1] = d->v.stride[1];
+  g.dtype = d->k.dtype;
+  g.T = (int32_t)d->k.dim[0], g.Hkv = (int32_t)d->k.dim[1], g.D = (int32_t)d->k.dim[2], g.Dv = (int32_t)d->v.dim[2];
+  hipLaunchKernelGGL(read_rows_kernel, dim3((unsigned)((int64_t)g.T * 2 * g.Hkv)), dim3(64), 0, ctx->stream, g);
+  FHIP_HIP_CHECK(ctx, hipGetLastError());
+  return 0;
+}
+
+} // extern "C"

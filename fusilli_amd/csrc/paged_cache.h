@@ -1,0 +1,115 @@
+// Packed sequences and a key / value cache in pages, as kernels see them: which
+// sequence a row belongs to, where a key lies, and what 4-bit codes stand for.
+// Offsets, lengths and page numbers come from device memory that no call has
+// checked: every lookup here stays inside the tensors whatever they hold.
+#ifndef FUSILLI_AMD_CSRC_PAGED_CACHE_H
+#define FUSILLI_AMD_CSRC_PAGED_CACHE_H
+
+#include "common.h"
+
+constexpr int kCacheMaxDim = 512; // of a head
+constexpr int64_t kCacheMaxKeys = (1ll << 30); // of a sequence: places stay 32-bit numbers
+
+// One pool of a cache: K or V.  Strides in elements (bytes, in 4 bits).
+struct FhipPool {
+  char *data;
+  _Float16 *params; // null: not in 4 bits
+  int64_t page, head, slot;                   // strides of data
+  int64_t params_page, params_head, params_slot;
+};
+
+struct FhipCacheView {
+  FhipPool k, v;
+  const int32_t *table, *lengths;
+  int64_t table_stride;
+  int32_t batch, table_pages; // rows and columns of the table
+  int32_t pool_pages, page_size;
+  int32_t group;              // elements per (scale, low) pair; 0: the pool's own type
+  int32_t dtype;              // of the pools, without 4 bits
+};
+
+FhipCacheView fhip_cache_view(const fhip_cache_desc &c, const fhip_cache_ptrs &p);
+
+// The checks that append, read and attention share: a cache of `heads` heads of K rows
+// of `D` and V rows of `Dv` elements of type `dtype` (or 4 bits).
+int fhip_check_cache(fhip_ctx *ctx, const char *who, const fhip_cache_desc &c, int dtype,
+                     int64_t heads, int64_t D, int64_t Dv);
+int fhip_check_cache_ptrs(fhip_ctx *ctx, const char *who, const fhip_cache_desc &c,
+                          const fhip_cache_ptrs *p);
+// A rank-3 tensor [rows, heads, dim] of f32, bf16 or f16 with neighbouring elements side
+// by side.  `written`: no two elements may share memory, as far as strides of 0 say.
+int fhip_check_rows(fhip_ctx *ctx, const char *who, const char *what, const fhip_tensor_desc &t,
+                    bool written);
+
+#if defined(__HIPCC__)
+
+// Sequence of packed row `row`: the last b with offsets[b] <= row, so that rows of empty
+// sequences are skipped; -1 where the row lies in front of the first or behind the last.
+__device__ __forceinline__ int fhip_sequence_of(const int32_t *offsets, int batch, int row) {
+  int lo = 0, hi = batch; // offsets[lo] <= row < offsets[hi]
+  if (row < offsets[0] || row >= offsets[batch])
+    return -1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (offsets[mid] <= row)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// Page of key `j` of sequence `b`, -1 where the table or the pool has none.
+__device__ __forceinline__ int fhip_page_of(const FhipCacheView &c, int b, int j) {
+  const uint32_t i = (uint32_t)j / (uint32_t)c.page_size;
+  if (j < 0 || i >= (uint32_t)c.table_pages)
+    return -1;
+  const int page = c.table[b * c.table_stride + i];
+  return (uint32_t)page < (uint32_t)c.pool_pages ? page : -1;
+}
+
+// Element e of the row at (page, slot) of head h as a float.
+__device__ __forceinline__ float fhip_cache_value(const FhipCacheView &c, const FhipPool &p, int page, int slot,
+                                                  int h, int e) {
+  const int64_t at = page * p.page + h * p.head + slot * p.slot;
+  if (!c.group)
+    return fhip_load<float>(p.data, c.dtype, at + e);
+  const uint8_t two = ((const uint8_t *)p.data)[at + e / 2];
+  const _Float16 *pair = p.params + page * p.params_page + h * p.params_head + slot * p.params_slot + e / c.group * 2;
+  return (float)pair[1] + (float)pair[0] * (float)(e & 1 ? two >> 4 : two & 15);
+}
+
+// (scale, low) of a group of values from `lo` to `hi`, both NaN where `lo` or `hi` is no
+// number or half cannot hold them.  Every step is a single rounding in f32 (no fused
+// multiply-add), so that the same formula anywhere gives the same codes.
+struct FhipGroup {
+  _Float16 scale, low;
+  float by; // 1 / scale, 0 where the codes are 0
+};
+__device__ __forceinline__ FhipGroup fhip_group_of(float lo, float hi) {
+#pragma clang fp contract(off)
+  FhipGroup g;
+  g.low = (_Float16)lo;
+  const float l = (float)g.low;
+  float wide = hi - l;
+  wide = wide < 0.f ? 0.f : wide;
+  g.scale = (_Float16)(wide / 15.0f);
+  const float s = (float)g.scale;
+  if (!(__builtin_fabsf(l) < INFINITY) || !(s < INFINITY)) {
+    g.scale = g.low = (_Float16)__builtin_nanf("");
+    g.by = 0.f;
+  } else {
+    g.by = s > 0.f ? 1.0f / s : 0.f;
+  }
+  return g;
+}
+__device__ __forceinline__ uint32_t fhip_code_of(const FhipGroup &g, float x) {
+#pragma clang fp contract(off)
+  const float c = __builtin_rintf((x - (float)g.low) * g.by);
+  // (a NaN's code is 0)
+  return (uint32_t)(c > 0.f ? (c < 15.f ? c : 15.f) : 0.f);
+}
+
+#endif // __HIPCC__
+
+#endif // FUSILLI_AMD_CSRC_PAGED_CACHE_H

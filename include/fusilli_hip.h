@@ -340,6 +340,158 @@ int fhip_sdpa_fwd(fhip_ctx *ctx, const fhip_sdpa_desc *d, const void *q,
                   const void *k, const void *v, const void *mask, void *o,
                   void *workspace, size_t workspace_bytes);
 
+/* ---- attention of language models in service.  The reference has none of
+ *      the following; they stand beside fhip_sdpa_fwd, share its conventions
+ *      and extend it to batches whose sequences differ in length.
+ *
+ *      Rows ("tokens") of all sequences lie packed in tensors [T, heads, dim].
+ *      `offsets`, a dense Int32 vector of batch + 1 elements on the device,
+ *      says where they are: sequence b has rows offsets[b] .. offsets[b + 1] - 1
+ *      (ascending; an empty sequence has none).  Rows of an output in front of
+ *      the first sequence and behind the last are left as they were.
+ *
+ *      A cache keeps keys and values of past tokens in pages that lie anywhere
+ *      in two pools [pages, heads, page size, dim].  `pages` is a table Int32
+ *      [batch, pages_per_sequence]: key j of sequence b lies in page
+ *      pages[b][j / page size], row j % page size; entries behind a sequence's
+ *      last key are not read.  `lengths`, a dense Int32 vector of batch
+ *      elements, counts each sequence's keys, the rows of the running call
+ *      among them: row i of its n rows has the place lengths[b] - n + i.
+ *
+ *      The pools hold the packed rows' type (f32, bf16 or f16), or 4 bits:
+ *      Uint8 [pages, heads, page size, dim / 2], element 2 j in the low half of
+ *      byte j and element 2 j + 1 in the high half, beside Half parameters
+ *      [pages, heads, page size, 2 * dim / G], a (scale, low) pair for each
+ *      group of G neighbouring elements.  Code c stands for low + scale * c:
+ *        low = half(min), scale = half((max - low) / 15) (at least 0),
+ *        c = round((x - low) * (1 / scale)) within 0 .. 15, 0 where scale is 0,
+ *      in f32 with ties to even.  A group that holds an infinity or a NaN, or
+ *      whose low or scale is beyond half's range, is kept as (NaN, NaN).
+ *
+ *      Offsets, lengths and page numbers are device data and are not checked
+ *      by the calls.  Whatever they hold, kernels stay inside the tensors: a
+ *      row whose place is negative, behind the page table or in a page that
+ *      the pool does not have is not stored by fhip_cache_append and read as
+ *      NaN, and makes the attention rows that see it NaN. ---------------- */
+typedef struct {
+  fhip_tensor_desc k;        /* [pages, Hkv, page size, D]  (4 bits: D / 2)   */
+  fhip_tensor_desc v;        /* [pages, Hkv, page size, Dv] (4 bits: Dv / 2)  */
+  fhip_tensor_desc k_params; /* 4 bits: [pages, Hkv, page size, 2 * D / G];
+                                rank 0 otherwise.  Of all four the last stride
+                                is 1; the others are free */
+  fhip_tensor_desc v_params;
+  int64_t batch, pages_per_sequence;
+  int64_t page_stride; /* elements between the table's rows */
+} fhip_cache_desc;
+
+/* Device pointers of a cache; the parameters null without 4 bits. */
+typedef struct {
+  void *k, *v, *k_params, *v_params;
+  const void *pages, *lengths;
+} fhip_cache_ptrs;
+
+/* Attention of packed sequences on each other: every row over the keys and
+ * values of its own sequence.  Without kv_offsets K and V are packed like Q
+ * (whole prompts); with them sequence b's keys are rows kv_offsets[b] ..
+ * kv_offsets[b + 1] - 1 of K and V, such as a prefix read back from a cache and
+ * the rows themselves.  is_causal: row i of n sees the first m - n + i + 1 of m
+ * keys (the last row sees all).  A row that sees no key is 0.  Heads are
+ * grouped like fhip_sdpa_fwd's.  supported: 2 for bf16 / f16, D = Dv = 64 or
+ * 128, positive scale, rows (heads, and tensors at the call) on 16 bytes and below
+ * 2 GiB per K or V tensor; 1 for other sizes to 512 and f32. */
+typedef struct {
+  fhip_tensor_desc q; /* [T, Hq, D] */
+  fhip_tensor_desc k; /* [Tk, Hkv, D]; Tk = T without kv_offsets */
+  fhip_tensor_desc v; /* [Tk, Hkv, Dv] */
+  fhip_tensor_desc o; /* [T, Hq, Dv] */
+  int64_t batch;
+  int32_t has_kv_offsets;
+  int32_t is_causal;
+  int32_t has_scale;
+  float scale; /* used when has_scale; else 1/sqrt(D) */
+} fhip_sdpa_packed_desc;
+
+int fhip_sdpa_packed_fwd_workspace_size(const fhip_sdpa_packed_desc *d,
+                                        size_t *bytes);
+int fhip_sdpa_packed_fwd_supported(const fhip_sdpa_packed_desc *d);
+int fhip_sdpa_packed_fwd(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d,
+                         const void *q, const void *k, const void *v,
+                         const void *offsets, const void *kv_offsets, void *o,
+                         void *workspace, size_t workspace_bytes);
+
+/* Attention of each sequence's newest rows over its keys in a cache: single
+ * tokens, drafts of several, chunks of a prompt.  is_causal: row i sees the
+ * keys up to its own place; otherwise every row sees lengths[b] keys.  A row
+ * that sees no key is 0.  Needs 256-byte aligned workspace of
+ * fhip_sdpa_paged_fwd_workspace_size bytes (parts of long sequences; it holds
+ * nothing between calls, and calls that overlap need one each).  supported: 2 for
+ * bf16 / f16, D = Dv = 64 or 128, pages of a multiple of 16 rows, groups of 32, 64
+ * or 128, rows and parameters aligned to 16 and 4 bytes; otherwise 1. */
+typedef struct {
+  fhip_tensor_desc q; /* [T, Hq, D] */
+  fhip_tensor_desc o; /* [T, Hq, Dv] */
+  fhip_cache_desc cache;
+  int32_t is_causal;
+  int32_t has_scale;
+  float scale;
+} fhip_sdpa_paged_desc;
+
+int fhip_sdpa_paged_fwd_workspace_size(const fhip_sdpa_paged_desc *d,
+                                       size_t *bytes);
+int fhip_sdpa_paged_fwd_supported(const fhip_sdpa_paged_desc *d);
+int fhip_sdpa_paged_fwd(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d,
+                        const fhip_cache_ptrs *cache, const void *q,
+                        const void *offsets, void *o, void *workspace,
+                        size_t workspace_bytes);
+
+/* Puts packed keys and values into their places in a cache, and turns queries
+ * and keys by their positions on the way.  rotation: row p holds the R / 2
+ * cosines of position p's angles and then their sines; it turns the pairs
+ * (i, i + R / 2) of a head's first R dims, interleaved (2 i, 2 i + 1), as
+ * (a cos - b sin, b cos + a sin) in f32 with one rounding.  A row's position is
+ * its place, or positions[row] (dense Int32 vector of T elements); a row whose
+ * position the table does not have is not stored and NaN in q_out and k_out.
+ * The cache holds the turned and rounded keys.  q_out may be q and k_out k (the
+ * very pointers and strides).  Two rows with the same place: either is stored,
+ * or parts of both.  supported: 2 for 16-bit rows of a multiple of 8 dims on 16
+ * bytes, R a multiple of 16, groups of 32, 64, 128 or 256 dims; otherwise 1. */
+typedef struct {
+  fhip_tensor_desc k;        /* [T, Hkv, D]  */
+  fhip_tensor_desc v;        /* [T, Hkv, Dv] */
+  fhip_tensor_desc q;        /* [T, Hq, D]; rank 0 = absent */
+  fhip_tensor_desc rotation; /* Float [positions, R]; rank 0 = no rotation */
+  fhip_tensor_desc q_out;    /* as q; absent when q is */
+  fhip_tensor_desc k_out;    /* as k; rank 0 = not wanted */
+  fhip_cache_desc cache;
+  int32_t has_positions;
+  int32_t interleaved;
+} fhip_cache_append_desc;
+
+int fhip_cache_append_workspace_size(const fhip_cache_append_desc *d,
+                                     size_t *bytes);
+int fhip_cache_append_supported(const fhip_cache_append_desc *d);
+int fhip_cache_append(fhip_ctx *ctx, const fhip_cache_append_desc *d,
+                      const fhip_cache_ptrs *cache, const void *q,
+                      const void *k, const void *v, const void *rotation,
+                      const void *offsets, const void *positions, void *q_out,
+                      void *k_out, void *workspace, size_t workspace_bytes);
+
+/* Brings the last offsets[b + 1] - offsets[b] keys and values of each sequence
+ * back to packed rows (f32, bf16 or f16; values in 4 bits are rounded to it once;
+ * 16-bit and f32 caches are read in their own type). */
+typedef struct {
+  fhip_tensor_desc k; /* [T, Hkv, D]  */
+  fhip_tensor_desc v; /* [T, Hkv, Dv] */
+  fhip_cache_desc cache;
+} fhip_cache_read_desc;
+
+int fhip_cache_read_workspace_size(const fhip_cache_read_desc *d,
+                                   size_t *bytes);
+int fhip_cache_read_supported(const fhip_cache_read_desc *d);
+int fhip_cache_read(fhip_ctx *ctx, const fhip_cache_read_desc *d,
+                    const fhip_cache_ptrs *cache, const void *offsets, void *k,
+                    void *v, void *workspace, size_t workspace_bytes);
+
 /* ---- RMSNorm / LayerNorm forward (node/rmsnorm_node.h:38-219,
  *      node/layernorm_node.h:38-264, node/norm_utils.h:27-99;
  *      aten.rms_norm / aten.(native_)layer_norm,
