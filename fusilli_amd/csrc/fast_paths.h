@@ -123,6 +123,13 @@ double fhip_flash_sdpa_us(const fhip_sdpa_desc *d);
 int fhip_decode_sdpa(fhip_ctx *ctx, const fhip_sdpa_desc *d, const void *q,
                      const void *k, const void *v, void *o, bool *handled);
 
+// Attention over a paged cache on MFMA: 16-bit rows, head dim 64 or 128, pages of a
+// multiple of 16 rows.  `handled` false where a pointer's alignment does not fit.
+bool fhip_fast_sdpa_paged_applicable(const fhip_sdpa_paged_desc *d);
+size_t fhip_fast_sdpa_paged_workspace(const fhip_sdpa_paged_desc *d);
+int fhip_fast_sdpa_paged(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d, const fhip_cache_ptrs *cache,
+                         const void *q, const void *offsets, void *o, void *workspace, bool *handled);
+
 bool fhip_fast_norm_applicable(const fhip_norm_desc *d);
 int fhip_fast_norm(fhip_ctx *ctx, const fhip_norm_desc *d, const void *x,
                    const void *scale, const void *bias, const DevEpilogue &epi,

@@ -204,13 +204,17 @@ int fhip_sdpa_packed_fwd(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const vo
 int fhip_sdpa_paged_fwd_workspace_size(const fhip_sdpa_paged_desc *d, size_t *bytes) {
   FHIP_REQUIRE(nullptr, d && bytes, "fhip_sdpa_paged_fwd_workspace_size: null");
   *bytes = 0;
+  if (paged_validate(nullptr, d) != 0)
+    return 1;
+  if (fhip_fast_sdpa_paged_applicable(d))
+    *bytes = fhip_fast_sdpa_paged_workspace(d);
   return 0;
 }
 
 int fhip_sdpa_paged_fwd_supported(const fhip_sdpa_paged_desc *d) {
   if (!d || paged_validate(nullptr, d) != 0)
     return 0;
-  return 1;
+  return fhip_fast_sdpa_paged_applicable(d) ? 2 : 1;
 }
 
 int fhip_sdpa_paged_fwd(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d, const fhip_cache_ptrs *cache, const void *q,
@@ -220,9 +224,16 @@ int fhip_sdpa_paged_fwd(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d, const fhip
   if (paged_validate(ctx, d) != 0 || fhip_check_cache_ptrs(ctx, who, d->cache, cache) != 0)
     return 1;
   FHIP_REQUIRE(ctx, q && offsets && o, "%s: null tensor pointer", who);
-  (void)workspace;
-  (void)workspace_bytes;
   FHIP_HIP_CHECK(ctx, hipSetDevice(ctx->device));
+  if (fhip_fast_sdpa_paged_applicable(d)) {
+    const size_t need = fhip_fast_sdpa_paged_workspace(d);
+    FHIP_REQUIRE(ctx, need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0),
+                 "%s: needs %zu bytes of 256-byte aligned workspace, got %zu", who, need, workspace_bytes);
+    bool handled = false;
+    const int rc = fhip_fast_sdpa_paged(ctx, d, cache, q, offsets, o, workspace, &handled);
+    if (handled)
+      return rc;
+  }
   fhip_note_kernel(ctx, "sdpa_rows paged");
   RowsArgs g{};
   g.q = q, g.o = o, g.offsets = (const int32_t *)offsets;
