@@ -21,13 +21,22 @@
 // the type's own numbers (a nibble below the exponent of 128 in bf16, of 1024 in f16
 // is 128 + c or 1024 + c exactly; K's offset is in the accumulator's start or
 // taken off, V's comes from a product with ones), scales and lows act on sums and
-// probabilities in f32.  P scale is rounded where P would be: one rounding as in
-// 16 bits.  Each product's 32 dims (K) or 16 columns (V) lie within a group.
+// probabilities in f32.  P scale is rounded where P would be; so that its rounding
+// meets no larger numbers than in 16 bits, the codes count from the middle, as
+// c - 8, and 8 (P . scale) goes with the lows.  Each product's 32 dims (K) or 16 columns (V) lie within a group.
 //
-// Work: no one but the device knows the lengths.  Every workgroup reads all of
-// them, cuts the sum of all sequences' chunks into about `target` equal pieces
-// (whole sequences where they are short), and finds its own piece.  Pieces of one
-// sequence meet in the workspace, in a fixed order, in a second kernel.
+// In 4 bits a chunk is 4 KB, and more of them have to be on their way: rows and parameters go
+// to a ring of stages in the wavefront's own LDS by LDS-DMA, from which each lane takes
+// what its fragments need.
+//
+// Work: no one but the device knows the lengths.  All sequences' chunks, one
+// tile and head after another, are one line that is cut into equal pieces, one per
+// workgroup; each reads all lengths and finds its own.  What a workgroup does of
+// a (sequence, tile, head) is a segment: whole ones it stores, parts meet in the
+// workspace, in a fixed order, in a second kernel.  A cut near a segment's end moves
+// there: a new segment waits for its first loads, 3 us in which its workgroup reads nothing.
+// Where the page table has room for few keys only, or there are many tiles, a workgroup
+// takes one whole (sequence, tile, head).
 #include "paged_cache.h"
 #include "fast_paths.h"
 
@@ -43,10 +52,12 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 #define PG_AS1 __attribute__((address_space(1)))
+#define PG_AS3 __attribute__((address_space(3)))
 
 constexpr int kWaves = 4;
 constexpr int kChunk = 32; // keys of a step
 constexpr float kNegBig = -1.0e30f;
+constexpr int kNear = 4; // a cut moves by up to a quarter of a piece
 
 struct PagedArgs {
   const char *q;
@@ -55,13 +66,16 @@ struct PagedArgs {
   const int32_t *offsets;
   FhipCacheView cache;
   int32_t T, Hkv, group; // group: query heads per key head
-  int32_t causal, target, least; // pieces wanted, chunks that a piece has at least
+  int32_t causal;
+  int32_t pieces, least; // workgroups that share the line, chunks that each has at least
   float scale_log2e;
   // of sequences in several pieces (null: there are none)
-  int32_t *info;  // [T] (first part of the row's sequence, its pieces per tile and head, position)
-  float *part;    // [parts][16][HD] sums
-  float *part_ml; // [parts][16] (m, l)
-  int32_t parts;
+  struct Info {
+    int32_t first; // the sequence's place on the line
+    int32_t chunks, pos, tiles, per;
+  } *info;        // [T]
+  float *part;    // [piece][2][16][HD] sums: of a segment that another piece began, and of one that it goes on with
+  float *part_ml; // [piece][2][16] (m, l)
 };
 
 template <bool BF16>
@@ -97,12 +111,73 @@ template <bool BF16> __device__ __forceinline__ void pg_store(char *o, int64_t a
     ((PG_AS1 _Float16 *)o)[at] = (_Float16)v;
 }
 
-// Nibbles i and i + 4 of a word as two 16-bit numbers, both `kOffset` too large.
+// Nibbles i and i + 4 of a word as two 16-bit numbers, both `kOffset` too large.  (The masks are
+// hidden from the compiler, which would otherwise take two instructions for what v_and_or_b32
+// does with one scalar and one vector operand.)
 template <bool BF16> struct Codes {
   static constexpr float kOffset = BF16 ? 128.f : 1024.f;
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, int i) {
-    return ((w >> (4 * i)) & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u);
+  uint32_t mask = 0x000f000fu, exponent = BF16 ? 0x43004300u : 0x64006400u;
+  __device__ __forceinline__ Codes() { asm("" : "+s"(mask), "+v"(exponent)); }
+  __device__ __forceinline__ uint32_t pair(uint32_t w, int i) const { return ((w >> (4 * i)) & mask) | exponent; }
+};
+
+// LDS reads that the compiler does not see as memory accesses (it would make each wait for every
+// LDS-DMA in flight), and the wait that goes with them.
+template <int OFFSET> __device__ __forceinline__ void pg_read(u32x4 &to, uint32_t from) {
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(to) : "v"(from), "n"(OFFSET));
+}
+template <int OFFSET> __device__ __forceinline__ void pg_read(u32x2 &to, uint32_t from) {
+  asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(to) : "v"(from), "n"(OFFSET));
+}
+template <int OFFSET> __device__ __forceinline__ void pg_read(uint32_t &to, uint32_t from) {
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(to) : "v"(from), "n"(OFFSET));
+}
+template <int OFFSET> __device__ __forceinline__ void pg_read16(uint32_t &to, uint32_t from) {
+  asm volatile("ds_read_u16 %0, %1 offset:%2" : "=v"(to) : "v"(from), "n"(OFFSET));
+}
+template <int OFFSET> __device__ __forceinline__ void pg_read8(uint32_t &to, uint32_t from) {
+  asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(to) : "v"(from), "n"(OFFSET));
+}
+__device__ __forceinline__ void pg_lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// (behind the wait: nothing that uses `x` moves in front of it)
+template <typename V> __device__ __forceinline__ void pg_pin(V &x) { asm volatile("" : "+v"(x)); }
+
+template <int N, typename F> __device__ __forceinline__ void pg_static_for(F &&f) {
+  if constexpr (N > 0) {
+    pg_static_for<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
   }
+}
+
+// 16 or 4 bytes per lane from memory to LDS, lane after lane from `to`.  (The builtin takes its size as
+// a literal, and 16 only for this device.)
+#if defined(__HIP_DEVICE_COMPILE__)
+#define PG_DMA(BYTES)                                                                            \
+  __builtin_amdgcn_global_load_lds((const PG_AS1 void *)from,                                    \
+                                   (PG_AS3 void *)(uintptr_t)__builtin_amdgcn_readfirstlane(to), \
+                                   BYTES, 0, 0)
+#else
+#define PG_DMA(BYTES)
+#endif
+__device__ __forceinline__ void pg_dma16(const char *from, uint32_t to) { PG_DMA(16); }
+__device__ __forceinline__ void pg_dma4(const char *from, uint32_t to) { PG_DMA(4); }
+
+// s_waitcnt vmcnt(vm) alone.
+__device__ __forceinline__ constexpr int pg_wait_imm(int vm) {
+  return (vm & 0xF) | ((vm >> 4) << 14) | (0x7 << 4) | (0xF << 8);
+}
+
+// Bytes of LDS per wavefront: its sums in the end (17 floats per column of O); in 4 bits before that a ring of stages,
+// each 32 rows of K, of V and their (scale, low) pairs.
+template <int HD, int G> struct PagedShape {
+  static constexpr bool kQ4 = G != 0;
+  static constexpr int kGroups = HD / (kQ4 ? G : HD);
+  static constexpr int kRow = HD / 2; // bytes of a row in 4 bits
+  static constexpr int kPairs = 64 * kRow;
+  static constexpr int kStage = kPairs + 256 * kGroups;
+  static constexpr int kStages = kGroups == 4 ? 3 : 4; // (two workgroups' in 160 KB)
+  static constexpr int kSums = HD * 17 * 4;
+  static constexpr int kBytes = kQ4 && kStages * kStage > kSums ? kStages * kStage : kSums;
 };
 
 // Inclusive sums over the wavefront's lanes.
@@ -157,88 +232,520 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
   constexpr int KD = HD / 32;      // MFMA steps of a score tile
   constexpr int SG = GG / 32;      // of them per group
   constexpr int PITCH = 17;        // floats per column of O in LDS
-  __shared__ float sums[kWaves][HD * PITCH];
+  // (f16: P scale stays a number for scales up to half's range / 15)
+  constexpr float kRedo = Q4 && !BF16 ? 7.0f : 8192.0f;
+  using S = PagedShape<HD, G>;
+  constexpr int ROW = S::kRow, SEGS = ROW / 16; // 4 bits: bytes of a row, 16-byte pieces of it
+  constexpr int VB = GG / 32;      // bytes of a V row and group per lane
+  static_assert(!Q4 || VB == 4 || VB == 2 || VB == 1, "groups of 32, 64 or 128");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float ml[kWaves][2][16];
-  // (scale, low) of 32 keys, K's and V's
-  __shared__ __attribute__((aligned(16))) uint32_t params[Q4 ? kWaves : 1][2][Q4 ? 32 * NG : 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l = threadIdx.x & 63, lq = l & 15, lg = l >> 4;
   const FhipCacheView &c = g.cache;
+  const Codes<BF16> codes;
+  float *const sums = (float *)(smem + wave * S::kBytes);
+  const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * S::kBytes);
 
-  // ---- this workgroup's piece ------------------------------------------------
-  // (the first 64 sequences stay in the lanes for the second walk)
-  const Sequence front = l < c.batch ? pg_sequence(g, l) : Sequence{};
-  float work = (float)front.tiles * (float)front.chunks;
-  for (int b = l + 64; b < c.batch; b += 64) {
-    const Sequence s = pg_sequence(g, b);
-    work += (float)s.tiles * (float)s.chunks;
-  }
-  work = pg_lane(pg_scan(work), 63) * (float)g.Hkv;
-  int per = (int)(work / (float)g.target) + 1; // chunks of a piece
-  per = per < g.least ? g.least : per;
-  int b = -1, index = 0, splits = 1, part = 0; // part: of the sequence's first piece
-  Sequence seq{};
-  int done = 0, parted = 0;
-  for (int b0 = 0; b0 < c.batch; b0 += 64) {
-    const Sequence s = b0 == 0 ? front : b0 + l < c.batch ? pg_sequence(g, b0 + l) : Sequence{};
-    const int cut = (s.chunks + per - 1) / per, mine = s.tiles * g.Hkv * cut;
-    const int upto = pg_scan(mine), parts_upto = pg_scan(cut > 1 ? mine : 0);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(done + upto > (int)blockIdx.x);
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      b = b0 + at;
-      splits = pg_lane(cut, at);
-      index = (int)blockIdx.x - (done + pg_lane(upto - mine, at));
-      part = parted + pg_lane(parts_upto, at) - pg_lane(mine, at);
-      seq = Sequence{pg_lane(s.start, at), pg_lane(s.rows, at), pg_lane(s.length, at), pg_lane(s.tiles, at),
-                     pg_lane(s.chunks, at)};
-      break;
-    }
-    done += pg_lane(upto, 63);
-    parted += pg_lane(parts_upto, 63);
-  }
-  // (the tiles of a head are Hkv * splits workgroups apart, on one XCD where that is a
-  // multiple of 8: they read the same keys)
-  const int qt = b < 0 ? 0 : index / (g.Hkv * splits), rest = b < 0 ? 0 : index % (g.Hkv * splits);
-  const int split = rest / g.Hkv, hk = rest % g.Hkv;
-  // (what offsets that overlap could lead to)
-  if (b < 0 || index < 0 || qt >= seq.tiles || (splits > 1 && (part < 0 || part + index >= g.parts)))
-    return;
-  const int room = c.table_pages * c.page_size;
-  const int keys = seq.length < room ? seq.length : room;
-  const int left = seq.rows * g.group - qt * 16; // of the sequence's packed rows from this tile's first
-  const int row = qt * 16 + (lq < left ? lq : left - 1);
-  const int pos = row / g.group, hg = row - pos * g.group;
-  // keys that this lane's row sees
-  int seen = g.causal ? seq.length - seq.rows + pos + 1 : seq.length;
-  const bool beyond = seen > keys; // of the page table
-  seen = seen < 0 ? 0 : beyond ? keys : seen;
-  if (g.info && hk == 0 && split == 0 && threadIdx.x < 16) {
-    PG_AS1 int32_t *to = (PG_AS1 int32_t *)g.info + (int64_t)(seq.start + pos) * 3;
-    to[0] = part, to[1] = splits, to[2] = pos;
-  }
-
-  // ---- Q fragments (B operand of S^T = K Q^T) ----------------------------------
-  // step u of lane group lg: dims u * 32 + lg * 8 .. + 7; in 4 bits, step s of group n:
-  // n * GG + lg * GG / 4 + s * 8 .. + 7, as a lane's codes of a group lie side by side
-  uint32_t qf[KD][4];
-  float qsum[NG]; // of this lane's row over a group's dims
+  // ---- this workgroup's piece of the line ----------------------------------------
+  const bool cut = g.info != nullptr;
+  auto work_of = [&](const Sequence &s) { // chunks, or whole segments; fewer than 2^31 in all
+    return s.tiles * g.Hkv * (cut ? s.chunks : 1);
+  };
+  // The first 64 sequences are kept for the segments' search, in LDS: registers are what limits the wavefronts.
+  __shared__ Sequence front[64];
+  __shared__ int front_upto[64];
+  int total;
   {
-    const char *src = g.q + ((int64_t)(seq.start + pos) * g.q_st + (int64_t)(hk * g.group + hg) * g.q_sh) * 2;
-#pragma unroll
-    for (int u = 0; u < KD; ++u) {
-      const int d = Q4 ? u / SG * GG + lg * (GG / 4) + u % SG * 8 : u * 32 + lg * 8;
-      const u32x4 x = *(const PG_AS1 u32x4 *)(src + d * 2);
-      if constexpr (Q4) { // the pairs that Codes::pair gives: (0, 4), (1, 5), (2, 6), (3, 7)
-        qf[u][0] = __builtin_amdgcn_perm(x.z, x.x, 0x05040100u);
-        qf[u][1] = __builtin_amdgcn_perm(x.z, x.x, 0x07060302u);
-        qf[u][2] = __builtin_amdgcn_perm(x.w, x.y, 0x05040100u);
-        qf[u][3] = __builtin_amdgcn_perm(x.w, x.y, 0x07060302u);
+    const Sequence s = l < c.batch ? pg_sequence(g, l) : Sequence{};
+    const int upto = pg_scan(work_of(s));
+    front_upto[l] = upto; // (every wavefront writes the same)
+    front[l] = s;
+    total = pg_lane(upto, 63);
+  }
+  const int front_all = total;
+  for (int b0 = 64; b0 < c.batch; b0 += 64)
+    total += pg_lane(pg_scan(b0 + l < c.batch ? work_of(pg_sequence(g, b0 + l)) : 0), 63);
+  int block_at = 0, block = 0; // a block of 64 sequences and its place on the line
+  int b = -1, first = 0;       // a sequence and its place
+  Sequence seq{};
+  auto find = [&](int at) { // the sequence that holds `at`, not in front of the last one's block
+    b = -1;
+    for (; block < c.batch; block += 64) {
+      Sequence s{};
+      int all = front_all, upto;
+      if (block == 0) {
+        s = front[l];
+        upto = front_upto[l];
       } else {
-        qf[u][0] = x.x, qf[u][1] = x.y, qf[u][2] = x.z, qf[u][3] = x.w;
+        if (block + l < c.batch)
+          s = pg_sequence(g, block + l);
+        upto = pg_scan(work_of(s));
+        all = pg_lane(upto, 63);
+      }
+      const uint64_t past = __builtin_amdgcn_ballot_w64(block_at + upto > at);
+      if (past) {
+        const int i = __builtin_ctzll(past);
+        b = block + i;
+        first = pg_lane(block_at + upto - work_of(s), i);
+        seq = Sequence{pg_lane(s.start, i), pg_lane(s.rows, i), pg_lane(s.length, i), pg_lane(s.tiles, i),
+                       pg_lane(s.chunks, i)};
+        return;
+      }
+      block_at += all;
+    }
+  };
+  int at = (int)blockIdx.x, stop = at + 1, per = 1;
+  if (cut) {
+    per = (total - 1) / g.pieces + 1;
+    per = per < g.least ? g.least : per;
+    // the piece's ends, each at a segment's own where that is near
+    const int64_t from = (int64_t)blockIdx.x * per;
+    auto snapped = [&](int64_t x) {
+      if (x >= total)
+        return total;
+      find((int)x);
+      if (b < 0)
+        return total;
+      const int near = per / kNear, inside = ((int)x - first) % seq.chunks;
+      return inside < near ? (int)x - inside : seq.chunks - inside < near ? (int)x - inside + seq.chunks : (int)x;
+    };
+    const int begin = snapped(from), at_block = block, at_place = block_at;
+    stop = snapped(from + per);
+    at = begin, block = at_block, block_at = at_place;
+  }
+  if (at >= total)
+    return;
+  stop = stop < total ? stop : total;
+  while (at < stop) {
+    find(at);
+    // (b < 0 and items behind the last: what offsets that overlap could lead to)
+    const int unit = cut ? seq.chunks : 1;
+    const int item = b < 0 ? 0 : (at - first) / unit;
+    int c0 = at - first - item * unit;
+    if (b < 0 || seq.tiles <= 0 || item < 0 || c0 < 0 || item / seq.tiles >= g.Hkv)
+      return;
+    int c1 = stop - at < unit - c0 ? c0 + stop - at : unit;
+    at += c1 - c0;
+    const bool whole = c0 == 0 && c1 == unit;
+    const int slot = c0 == 0 ? 1 : 0;
+    if (!cut)
+      c1 = seq.chunks;
+    // (tiles of a head side by side: they read the same keys)
+    const int hk = item / seq.tiles, qt = item % seq.tiles;
+    const int room = c.table_pages * c.page_size;
+    const int keys = seq.length < room ? seq.length : room;
+    const int left = seq.rows * g.group - qt * 16; // of the sequence's packed rows from this tile's first
+    const int row = qt * 16 + (lq < left ? lq : left - 1);
+    const int pos = row / g.group, hg = row - pos * g.group;
+    // keys that this lane's row sees
+    int seen = g.causal ? seq.length - seq.rows + pos + 1 : seq.length;
+    const bool beyond = seen > keys; // of the page table
+    seen = seen < 0 ? 0 : beyond ? keys : seen;
+    int all_see = seen, any_sees = seen; // what every row sees: chunks up to it need no mask
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      const int x = __shfl_xor(all_see, o, 64), y = __shfl_xor(any_sees, o, 64);
+      all_see = x < all_see ? x : all_see;
+      any_sees = y > any_sees ? y : any_sees;
+    }
+    all_see = __builtin_amdgcn_readfirstlane(all_see);
+    if (cut && hk == 0 && slot == 1 && threadIdx.x < 16)
+      g.info[seq.start + pos] = PagedArgs::Info{first, seq.chunks, pos, seq.tiles, per};
+    // chunks behind the last key that any row sees have nothing
+    const int need = (__builtin_amdgcn_readfirstlane(any_sees) + kChunk - 1) / kChunk;
+    c1 = c1 < need ? c1 : need;
+    const int steps = (c1 - c0 - wave + kWaves - 1) / kWaves; // this wavefront's chunks c0 + wave + 4 i
+
+    // ---- Q fragments (B operand of S^T = K Q^T) ----------------------------------
+    // step u of lane group lg: dims u * 32 + lg * 8 .. + 7; in 4 bits, step s of group n:
+    // n * GG + lg * GG / 4 + s * 8 .. + 7, as a lane's codes of a group lie side by side
+    uint32_t qf[KD][4];
+    float qsum[NG]; // of this lane's row over a group's dims
+    {
+      const char *src = g.q + ((int64_t)(seq.start + pos) * g.q_st + (int64_t)(hk * g.group + hg) * g.q_sh) * 2;
+#pragma unroll
+      for (int u = 0; u < KD; ++u) {
+        const int d = Q4 ? u / SG * GG + lg * (GG / 4) + u % SG * 8 : u * 32 + lg * 8;
+        const u32x4 x = *(const PG_AS1 u32x4 *)(src + d * 2);
+        if constexpr (Q4) { // the pairs that Codes::pair gives: (0, 4), (1, 5), (2, 6), (3, 7)
+          qf[u][0] = __builtin_amdgcn_perm(x.z, x.x, 0x05040100u);
+          qf[u][1] = __builtin_amdgcn_perm(x.z, x.x, 0x07060302u);
+          qf[u][2] = __builtin_amdgcn_perm(x.w, x.y, 0x05040100u);
+          qf[u][3] = __builtin_amdgcn_perm(x.w, x.y, 0x07060302u);
+        } else {
+          qf[u][0] = x.x, qf[u][1] = x.y, qf[u][2] = x.z, qf[u][3] = x.w;
+        }
       }
     }
+
+    // ---- loads -------------------------------------------------------------------
+    constexpr int ES = Q4 ? 1 : 2; // bytes per stride unit
+    const uint32_t k_slot = (uint32_t)(c.k.slot * ES), v_slot = (uint32_t)(c.v.slot * ES);
+    const char *k_head = c.k.data + (int64_t)hk * c.k.head * ES;
+    const char *v_head = c.v.data + (int64_t)hk * c.v.head * ES;
+    const char *kp_head = (const char *)(c.k.params + (int64_t)hk * c.k.params_head);
+    const char *vp_head = (const char *)(c.v.params + (int64_t)hk * c.v.params_head);
+    // Of tile l & 1 of this wavefront's chunk (i & ~31) + (l >> 1): bytes to its first row in both pools and in
+    // the parameters', and whether it has a page.
+    struct Places {
+      int64_t k, v, kp, vp;
+      int bad;
+    } places{};
+    auto look_up = [&](int i) {
+      const int key = ((c0 + wave + kWaves * (i + (l >> 1))) * 2 + (l & 1)) * 16;
+      const uint32_t n = (uint32_t)key / (uint32_t)c.page_size;
+      int page = 0, slot = 0;
+      places.bad = 0;
+      if (key < keys) { // (and so n < table_pages)
+        slot = key - (int)n * c.page_size;
+        page = c.table[b * c.table_stride + n];
+        if ((uint32_t)page >= (uint32_t)c.pool_pages)
+          page = 0, places.bad = 1;
+      }
+      places.k = ((int64_t)page * c.k.page + (int64_t)slot * c.k.slot) * ES;
+      places.v = ((int64_t)page * c.v.page + (int64_t)slot * c.v.slot) * ES;
+      if constexpr (Q4) {
+        places.kp = ((int64_t)page * c.k.params_page + (int64_t)slot * c.k.params_slot) * 2;
+        places.vp = ((int64_t)page * c.v.params_page + (int64_t)slot * c.v.params_slot) * 2;
+      }
+    };
+    auto place = [&](int64_t x, int lane) {
+      return ((int64_t)pg_lane((int)(x >> 32), lane) << 32) | (uint32_t)pg_lane((int)x, lane);
+    };
+    // LDS, 4 bits: piece s of row r lies at piece s ^ swizzle(r), which spreads the rows of one read over the banks.
+    // LDS-DMA writes lane after lane: the lanes' own addresses are permuted.
+    auto swizzle = [](int r) { return r / (256 / ROW) & (SEGS - 1); };
+    // a lane's offsets from its tile's first row: 16 bits, its fragments; 4 bits, a piece of row l / SEGS (head dim 64: one
+    // load for both tiles)
+    const int piece = Q4 ? (l % SEGS ^ swizzle(l / SEGS)) * 16 : 0;
+    const uint32_t k_lane = Q4 ? (uint32_t)(l / SEGS % 16) * k_slot + (uint32_t)piece : (uint32_t)lq * k_slot + (uint32_t)(lg * 16);
+    const uint32_t v_lane = Q4 ? (uint32_t)(l / SEGS % 16) * v_slot + (uint32_t)piece : (uint32_t)(lg * 4) * v_slot + (uint32_t)(lq * T * 2);
+    // .. and a pair of row l % (16 NG) / NG of a tile: 16 lanes (of K, then V, both tiles) per load and group
+    const uint32_t pair_row = (uint32_t)(l % (16 * NG) / NG), pair_at = (uint32_t)(l % NG * 4);
+    const uint32_t kp_lane = pair_row * (uint32_t)(c.k.params_slot * 2) + pair_at;
+    const uint32_t vp_lane = pair_row * (uint32_t)(c.v.params_slot * 2) + pair_at;
+    struct Chunk { // 16 bits
+      u32x4 k[2 * KD], v[8];
+      int bad;
+    };
+    auto fetch = [&](Chunk &x, int i) {
+      if ((i & 31) == 0)
+        look_up(i);
+      const int lane = (i & 31) * 2;
+      x.bad = pg_lane(places.bad, lane) | pg_lane(places.bad, lane + 1) << 1;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const char *kt = k_head + place(places.k, lane + t), *vt = v_head + place(places.v, lane + t);
+#pragma unroll
+        for (int u = 0; u < KD; ++u)
+          x.k[t * KD + u] = *(const PG_AS1 u32x4 *)(kt + u * 64 + k_lane);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const char *p = vt + (uint64_t)r * v_slot + v_lane;
+          if constexpr (T == 8) {
+            x.v[t * 4 + r] = *(const PG_AS1 u32x4 *)p;
+          } else {
+            const u32x2 y = *(const PG_AS1 u32x2 *)p;
+            x.v[t * 4 + r].x = y.x, x.v[t * 4 + r].y = y.y;
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    constexpr int kDmas = SEGS + (NG == 4 ? 4 : NG); // 4 bits: LDS-DMA instructions of a chunk
+    uint32_t bads = 0; // of the last 16 chunks issued, the newest lowest
+    auto issue = [&](int i) { // chunk i, on its way to stage i % kStages
+      if constexpr (Q4) {
+        if ((i & 31) == 0)
+          look_up(i);
+        const int lane = (i & 31) * 2;
+        bads = bads << 2 | (uint32_t)(pg_lane(places.bad, lane) | pg_lane(places.bad, lane + 1) << 1);
+        const uint32_t stage = lds + (uint32_t)(i % S::kStages * S::kStage);
+        const char *kt[2], *vt[2], *kpt[2], *vpt[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          kt[t] = k_head + place(places.k, lane + t);
+          vt[t] = v_head + place(places.v, lane + t);
+          kpt[t] = kp_head + place(places.kp, lane + t);
+          vpt[t] = vp_head + place(places.vp, lane + t);
+        }
+        if constexpr (SEGS == 4) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            pg_dma16(kt[t] + k_lane, stage + t * 1024);
+            pg_dma16(vt[t] + v_lane, stage + 32 * ROW + t * 1024);
+          }
+        } else {
+          pg_dma16((l < 32 ? kt[0] : kt[1]) + k_lane, stage + 0);
+          pg_dma16((l < 32 ? vt[0] : vt[1]) + v_lane, stage + 32 * ROW);
+        }
+        if constexpr (NG == 1) {
+          const char *k = (l < 16 ? kpt[0] : kpt[1]) + kp_lane, *v = (l < 48 ? vpt[0] : vpt[1]) + vp_lane;
+          pg_dma4(l < 32 ? k : v, stage + S::kPairs);
+        } else if constexpr (NG == 2) {
+          pg_dma4((l < 32 ? kpt[0] : kpt[1]) + kp_lane, stage + S::kPairs);
+          pg_dma4((l < 32 ? vpt[0] : vpt[1]) + vp_lane, stage + S::kPairs + 256);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            pg_dma4(kpt[t] + kp_lane, stage + S::kPairs + t * 256);
+            pg_dma4(vpt[t] + vp_lane, stage + S::kPairs + 512 + t * 256);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    uint32_t k_at[NG], v_at[NG]; // of this lane's part of a group in a stage: K, row lq; V, row 4 lg
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const int kb = n * (GG / 2) + lg * (GG / 8), vb = n * (GG / 2) + lq * VB;
+      k_at[n] = lds + (uint32_t)(lq * ROW + ((kb / 16 ^ swizzle(lq)) << 4) + kb % 16);
+      v_at[n] = lds + (uint32_t)(32 * ROW + lg * 4 * ROW + ((vb / 16 ^ swizzle(lg * 4)) << 4) + vb % 16);
+    }
+    const uint32_t pairs_at = lds + (uint32_t)(S::kPairs + lg * 16 * NG);
+
+    f32x4 o[T];
+#pragma unroll
+    for (int j = 0; j < T; ++j)
+      o[j] = f32x4{0, 0, 0, 0};
+    f32x4 z[NG];    // 4 bits: sums of the rounded P scale
+    float lows[NG], scales[NG]; // and of P low and of P scale, over this lane's keys
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+      z[n] = f32x4{0, 0, 0, 0}, lows[n] = scales[n] = 0.f;
+    float m = kNegBig, sum = 0.f; // of row lq: maximum of Q . K over all lanes, sum over this lane's keys
+
+    auto spend = [&](Chunk &x, int i, int bad) {
+      const int key0 = (c0 + wave + kWaves * i) * kChunk;
+      const bool ends = key0 + kChunk > keys; // keys behind the last: nothing of theirs may reach a sum
+      const uint32_t stage = Q4 ? (uint32_t)(i % S::kStages * S::kStage) : 0;
+      // word r * NG + n of a tile: the pair of this lane's key r, group n
+      auto pair_of = [&](u32x4(&p)[2][NG], int t, int r, int n) {
+        // (through a scalar: bit-casting a vector's element in place reads element 0)
+        const uint32_t w = p[t][(r * NG + n) / 4][(r * NG + n) % 4];
+        return __builtin_bit_cast(f16x2, w);
+      };
+      auto read_pairs = [&](u32x4(&p)[2][NG], auto which) {
+        pg_static_for<2 * NG>([&](auto ic) {
+          constexpr int t = decltype(ic)::value / NG, n = decltype(ic)::value % NG;
+          pg_read<decltype(which)::value * 128 * NG + t * 64 * NG + n * 16>(p[t][n], pairs_at + stage);
+        });
+      };
+      auto pin_pairs = [&](u32x4(&p)[2][NG]) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int n = 0; n < NG; ++n)
+            pg_pin(p[t][n]);
+      };
+      float s[8];
+      if constexpr (Q4) {
+        typedef std::conditional_t<SG == 4, u32x4, std::conditional_t<SG == 2, u32x2, uint32_t>> KWords;
+        u32x4 kpar[2][NG];
+        KWords kw[2][NG];
+        pg_static_for<2 * NG>([&](auto ic) {
+          constexpr int t = decltype(ic)::value / NG, n = decltype(ic)::value % NG;
+          pg_read<t * 16 * ROW>(kw[t][n], k_at[n] + stage);
+        });
+        read_pairs(kpar, std::integral_constant<int, 0>{});
+        pg_lds_wait();
+        pin_pairs(kpar);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int n = 0; n < NG; ++n)
+            pg_pin(kw[t][n]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            uint32_t w[SG];
+            if constexpr (SG == 4)
+              w[0] = kw[t][n].x, w[1] = kw[t][n].y, w[2] = kw[t][n].z, w[3] = kw[t][n].w;
+            else if constexpr (SG == 2)
+              w[0] = kw[t][n].x, w[1] = kw[t][n].y;
+            else
+              w[0] = kw[t][n];
+            // bf16 starts at -128 sum(Q).  f16's 1024 would leave the score 2^-14 of sum |Q| scale:
+            // it is taken off the codes
+            const float start = BF16 ? -Codes<BF16>::kOffset * qsum[n] : 0.f;
+            f32x4 a{start, start, start, start};
+#pragma unroll
+            for (int u = 0; u < SG; ++u) {
+              uint32_t f[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                f[e] = codes.pair(w[u], e);
+                if constexpr (!BF16)
+                  f[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, f[e]) - f16x2{(_Float16)1024, (_Float16)1024});
+              }
+              a = pg_mfma<BF16>(f, qf[n * SG + u], a);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const f16x2 p = pair_of(kpar, t, r, n);
+              v[r] = __builtin_fmaf((float)p.x, a[r], __builtin_fmaf((float)p.y, qsum[n], v[r]));
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[t * 4 + r] = v[r];
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          f32x4 a{0, 0, 0, 0};
+#pragma unroll
+          for (int u = 0; u < KD; ++u) {
+            const u32x4 y = x.k[t * KD + u];
+            const uint32_t f[4] = {y.x, y.y, y.z, y.w};
+            a = pg_mfma<BF16>(f, qf[u], a);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[t * 4 + r] = a[r];
+        }
+      }
+      if (bad) { // (the asm keeps this a branch)
+        asm volatile("" : "+v"(s[0]));
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          s[e] = bad >> (e >> 2) & 1 ? __builtin_nanf("") : s[e];
+      }
+      if (key0 + kChunk > all_see)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          s[e] = key0 + (e >> 2) * 16 + lg * 4 + (e & 3) < seen ? s[e] : -INFINITY;
+      // V's part of the stage comes in beside the softmax
+      constexpr int kVReads = !Q4 ? 1 : 8 * NG;
+      uint32_t vw[kVReads]; // of group n, key e: word n * 8 + e
+      u32x4 vpar[2][NG];
+      if constexpr (Q4) {
+        pg_static_for<8 * NG>([&](auto ic) {
+          constexpr int n = decltype(ic)::value / 8, e = decltype(ic)::value % 8;
+          constexpr int off = ((e >> 2) * 16 + (e & 3)) * ROW;
+          if constexpr (VB == 4)
+            pg_read<off>(vw[n * 8 + e], v_at[n] + stage);
+          else if constexpr (VB == 2)
+            pg_read16<off>(vw[n * 8 + e], v_at[n] + stage);
+          else
+            pg_read8<off>(vw[n * 8 + e], v_at[n] + stage);
+        });
+        read_pairs(vpar, std::integral_constant<int, 1>{});
+      }
+      // The reference point m of the exponentials follows the maximum lazily: a chunk first runs against the one it
+      // inherits, with no maximum taken and nothing exchanged between lanes.  Only the first chunk, and one in which
+      // some lane's probabilities rise above kRedo, take the maximum and rescale; O = sum(P V) / sum(P) does
+      // not depend on m.
+      float p[8], psum;
+      auto exps = [&]() {
+        const float at_m = -(m * g.scale_log2e);
+        psum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], g.scale_log2e, at_m));
+          psum += p[e];
+        }
+      };
+      if (i > 0)
+        exps();
+      if (i == 0 || __builtin_amdgcn_ballot_w64(!(psum <= kRedo)) != 0) {
+        float top = s[0];
+        asm volatile("" : "+v"(top)); // (keeps the maximum in this branch)
+#pragma unroll
+        for (int e = 1; e < 8; ++e)
+          top = fmaxf(top, s[e]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mn = fmaxf(m, top);
+        const float alpha = __builtin_amdgcn_exp2f((m - mn) * g.scale_log2e);
+        m = mn;
+        sum *= alpha;
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+          o[j] *= alpha;
+        if constexpr (Q4)
+#pragma unroll
+          for (int n = 0; n < NG; ++n)
+            z[n] *= alpha, lows[n] *= alpha, scales[n] *= alpha;
+        exps();
+      }
+      sum += psum;
+      if constexpr (Q4) {
+        pg_lds_wait();
+        pin_pairs(vpar);
+#pragma unroll
+        for (int e = 0; e < kVReads; ++e)
+          pg_pin(vw[e]);
+        if (ends)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (key0 + t * 16 + lg * 4 + r >= keys)
+#pragma unroll
+                for (int n = 0; n < NG; ++n)
+                  vpar[t][(r * NG + n) / 4][(r * NG + n) % 4] = 0;
+        constexpr uint32_t kOne = BF16 ? 0x3f803f80u : 0x3c003c00u;
+        const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          float ps[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const f16x2 pr = pair_of(vpar, e >> 2, e & 3, n);
+            ps[e] = __builtin_fmaf(p[e], (float)pr.x, 0.f);
+            lows[n] = __builtin_fmaf(p[e], (float)pr.y, lows[n]);
+            scales[n] += ps[e];
+          }
+          const uint32_t pf[4] = {pg_pack<BF16>(ps[0], ps[1]), pg_pack<BF16>(ps[2], ps[3]),
+                                  pg_pack<BF16>(ps[4], ps[5]), pg_pack<BF16>(ps[6], ps[7])};
+          z[n] = pg_mfma<BF16>(ones, pf, z[n]);
+          uint32_t lo[4], hi[4]; // nibbles of the keys 2 e and 2 e + 1 in the halves
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t w0 = vw[n * 8 + 2 * e], w1 = vw[n * 8 + 2 * e + 1];
+            lo[e] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+            hi[e] = VB == 4 ? __builtin_amdgcn_perm(w1, w0, 0x07060302u) : 0;
+          }
+#pragma unroll
+          for (int j = 0; j < TG; ++j) {
+            uint32_t f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              f[e] = codes.pair(j < 4 ? lo[e] : hi[e], j & 3);
+            o[n * TG + j] = pg_mfma<BF16>(f, pf, o[n * TG + j]);
+          }
+        }
+      } else {
+        if (ends)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (key0 + (e >> 2) * 16 + lg * 4 + (e & 3) >= keys)
+              x.v[e] = u32x4{};
+        const uint32_t pf[4] = {pg_pack<BF16>(p[0], p[1]), pg_pack<BF16>(p[2], p[3]),
+                                pg_pack<BF16>(p[4], p[5]), pg_pack<BF16>(p[6], p[7])};
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+          uint32_t f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            f[e] = __builtin_amdgcn_perm(x.v[2 * e + 1][j / 2], x.v[2 * e][j / 2],
+                                         j & 1 ? 0x07060302u : 0x05040100u);
+          o[j] = pg_mfma<BF16>(f, pf, o[j]);
+        }
+      }
+    };
+    Chunk x0, x1;
     if constexpr (Q4) {
+      for (int i = 0; i < S::kStages - 1 && i < steps; ++i)
+        issue(i);
+    } else if (steps > 0) {
+      fetch(x0, 0);
+    }
+    if constexpr (Q4) { // (behind the first loads)
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         float s = 0.f;
@@ -252,379 +759,91 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
         qsum[n] = s;
       }
     }
-  }
-
-  // this workgroup's chunks, up to the last key that any of its rows sees
-  int chunks = seq.chunks;
-  if (g.causal) {
-    const int last = (qt * 16 + (left < 16 ? left : 16) - 1) / g.group;
-    int top = seq.length - seq.rows + last + 1;
-    top = top > keys ? keys : top < 1 ? 1 : top;
-    const int need = (top + kChunk - 1) / kChunk;
-    chunks = need < chunks ? need : chunks;
-  }
-  if (keys == 0)
-    chunks = 0;
-  const int c0 = (int)((int64_t)chunks * split / splits);
-  const int c1 = (int)((int64_t)chunks * (split + 1) / splits);
-  const int steps = (c1 - c0 - wave + kWaves - 1) / kWaves; // this wavefront's chunks c0 + wave + 4 i
-
-  // ---- loads -------------------------------------------------------------------
-  constexpr int ES = Q4 ? 1 : 2; // bytes per stride unit
-  const uint32_t k_slot = (uint32_t)(c.k.slot * ES), v_slot = (uint32_t)(c.v.slot * ES);
-  const char *k_head = c.k.data + (int64_t)hk * c.k.head * ES;
-  const char *v_head = c.v.data + (int64_t)hk * c.v.head * ES;
-  const _Float16 *kp_head = c.k.params + (int64_t)hk * c.k.params_head;
-  const _Float16 *vp_head = c.v.params + (int64_t)hk * c.v.params_head;
-  int pages = 0, slots = 0; // of tile l & 1 of this wavefront's chunk (i & ~31) + (l >> 1)
-  auto look_up = [&](int i) {
-    const int key = ((c0 + wave + kWaves * (i + (l >> 1))) * 2 + (l & 1)) * 16;
-    const uint32_t n = (uint32_t)key / (uint32_t)c.page_size;
-    pages = slots = 0;
-    if (key < keys) { // (and so n < table_pages)
-      slots = key - (int)n * c.page_size;
-      pages = c.table[b * c.table_stride + n];
-      pages = (uint32_t)pages < (uint32_t)c.pool_pages ? pages : -1;
-    }
-  };
-  // K: Q4 words of a lane's codes, group after group; V: pairs of keys (2 e, 2 e + 1)
-  struct Chunk {
-    u32x4 k[2][Q4 ? (KD + 3) / 4 : KD];
-    uint32_t v[Q4 ? 8 * NG : 1];
-    u32x4 v16[Q4 ? 1 : 8];
-    uint32_t kp[2], vp[2];
-    int bad;
-  };
-  constexpr int VB = Q4 ? GG / 32 : 4; // bytes of a V row and group per lane
-  static_assert(!Q4 || VB == 4 || VB == 2 || VB == 1, "groups of 32, 64 or 128");
-  auto fetch = [&](Chunk &x, int i) {
-    if ((i & 31) == 0)
-      look_up(i);
-    x.bad = 0;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      int page = __builtin_amdgcn_readlane(pages, (i & 31) * 2 + t);
-      const int slot = __builtin_amdgcn_readlane(slots, (i & 31) * 2 + t);
-      if (page < 0)
-        page = 0, x.bad |= 1 << t;
-      const char *kp = k_head + ((int64_t)page * c.k.page + (int64_t)slot * c.k.slot) * ES;
-      const char *vp = v_head + ((int64_t)page * c.v.page + (int64_t)slot * c.v.slot) * ES;
-      if constexpr (Q4) {
-        uint32_t w[KD];
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          const char *p = kp + (uint64_t)((uint32_t)lq * k_slot + (uint32_t)(lg * (GG / 8) + n * (GG / 2)));
-          if constexpr (SG == 4) {
-            const u32x4 y = *(const PG_AS1 u32x4 *)p;
-            w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
-          } else if constexpr (SG == 2) {
-            const u32x2 y = *(const PG_AS1 u32x2 *)p;
-            w[n * 2] = y.x, w[n * 2 + 1] = y.y;
-          } else {
-            w[n] = *(const PG_AS1 uint32_t *)p;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < KD; ++u)
-          x.k[t][u / 4][u % 4] = w[u];
-        const uint32_t row0 = (uint32_t)(lg * 4) * v_slot + (uint32_t)(lq * VB);
-#pragma unroll
-        for (int n = 0; n < NG; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) { // keys 4 lg + 2 e and + 1 of this tile
-            const char *p = vp + (uint64_t)(row0 + (uint32_t)(n * (GG / 2))) + (uint64_t)(2 * e) * v_slot;
-            if constexpr (VB == 4) {
-              x.v[(t * 2 + e) * 2] = *(const PG_AS1 uint32_t *)p;
-              x.v[(t * 2 + e) * 2 + 1] = *(const PG_AS1 uint32_t *)(p + v_slot);
-            } else {
-              typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-              us2 y;
-              if constexpr (VB == 2) {
-                y.x = *(const PG_AS1 unsigned short *)p;
-                y.y = *(const PG_AS1 unsigned short *)(p + v_slot);
-              } else {
-                y.x = *(const PG_AS1 unsigned char *)p;
-                y.y = *(const PG_AS1 unsigned char *)(p + v_slot);
-              }
-              x.v[n * 4 + t * 2 + e] = __builtin_bit_cast(uint32_t, y);
-            }
-          }
-        // parameters: this tile's 16 keys of K in lanes 0 .. 16 NG - 1 .., one pair per lane
-        // (NG 4: two tiles of pairs are 64 lanes each)
-        const _Float16 *kpp = kp_head + (int64_t)page * c.k.params_page + (int64_t)slot * c.k.params_slot;
-        const _Float16 *vpp = vp_head + (int64_t)page * c.v.params_page + (int64_t)slot * c.v.params_slot;
-        if (l < 16 * NG) {
-          x.kp[t] = *(const PG_AS1 uint32_t *)(kpp + (int64_t)(l / NG) * c.k.params_slot + l % NG * 2);
-          x.vp[t] = *(const PG_AS1 uint32_t *)(vpp + (int64_t)(l / NG) * c.v.params_slot + l % NG * 2);
-        }
-      } else {
-#pragma unroll
-        for (int u = 0; u < KD; ++u)
-          x.k[t][u] = *(const PG_AS1 u32x4 *)(kp + (uint64_t)((uint32_t)lq * k_slot + (uint32_t)(lg * 16 + u * 64)));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const char *p = vp + (uint64_t)((uint32_t)(lg * 4) * v_slot + (uint32_t)(lq * T * 2)) + (uint64_t)r * v_slot;
-          if constexpr (T == 8) {
-            x.v16[t * 4 + r] = *(const PG_AS1 u32x4 *)p;
-          } else {
-            const u32x2 y = *(const PG_AS1 u32x2 *)p;
-            x.v16[t * 4 + r].x = y.x, x.v16[t * 4 + r].y = y.y;
-          }
-        }
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-
-  f32x4 o[T];
-#pragma unroll
-  for (int j = 0; j < T; ++j)
-    o[j] = f32x4{0, 0, 0, 0};
-  f32x4 z[NG];    // 4 bits: sums of the rounded P scale
-  float lows[NG]; // and of P low, over this lane's keys
-#pragma unroll
-  for (int n = 0; n < NG; ++n)
-    z[n] = f32x4{0, 0, 0, 0}, lows[n] = 0.f;
-  float m = kNegBig, sum = 0.f; // of row lq: maximum over all lanes, sum over this lane's keys
-
-  auto spend = [&](Chunk &x, int i) {
-    const int key0 = (c0 + wave + kWaves * i) * kChunk;
-    const bool ends = key0 + kChunk > keys; // keys behind the last: nothing of theirs may reach a sum
-    u32x4 kpar[2][NG], vpar[2][NG]; // pairs of this lane's 4 keys of a tile: [t][..] is 4 NG words
     if constexpr (Q4) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (l < 16 * NG) {
-          params[wave][0][t * 16 * NG + l] = x.kp[t];
-          params[wave][1][t * 16 * NG + l] = x.vp[t];
-        }
-      // (one wavefront writes and reads: its LDS operations keep their order)
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          kpar[t][n] = *(const u32x4 *)&params[wave][0][(t * 16 + lg * 4) * NG + n * 4];
-          vpar[t][n] = *(const u32x4 *)&params[wave][1][(t * 16 + lg * 4) * NG + n * 4];
-        }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
-    // pair of key r of tile t, group n: word r * NG + n
-    auto pair_of = [&](u32x4(&p)[2][NG], int t, int r, int n) {
-      // (through a scalar: bit-casting a vector's element in place reads element 0)
-      const uint32_t w = p[t][(r * NG + n) / 4][(r * NG + n) % 4];
-      return __builtin_bit_cast(f16x2, w);
-    };
-    float s[8];
-    uint32_t live = 0;
-    float top = kNegBig;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float v[4];
-      if constexpr (Q4) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          v[r] = 0.f;
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          // bf16 starts at -128 sum(Q).  f16's 1024 would leave the score 2^-14 of sum |Q| scale:
-          // it is taken off the codes
-          const float start = BF16 ? -Codes<BF16>::kOffset * qsum[n] : 0.f;
-          f32x4 a{start, start, start, start};
-#pragma unroll
-          for (int u = n * SG; u < (n + 1) * SG; ++u) {
-            const uint32_t w = x.k[t][u / 4][u % 4];
-            uint32_t f[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              f[e] = Codes<BF16>::pair(w, e);
-              if constexpr (!BF16)
-                f[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, f[e]) - f16x2{(_Float16)1024, (_Float16)1024});
-            }
-            a = pg_mfma<BF16>(f, qf[u], a);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const f16x2 p = pair_of(kpar, t, r, n);
-            v[r] = __builtin_fmaf((float)p.x, a[r], __builtin_fmaf((float)p.y, qsum[n], v[r]));
-          }
-        }
-      } else {
-        f32x4 a{0, 0, 0, 0};
-#pragma unroll
-        for (int u = 0; u < KD; ++u) {
-          const u32x4 y = x.k[t][u];
-          const uint32_t f[4] = {y.x, y.y, y.z, y.w};
-          a = pg_mfma<BF16>(f, qf[u], a);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          v[r] = a[r];
+#pragma clang loop unroll(disable)
+      for (int i = 0; i < steps; ++i) {
+        // (stage (i - 1) % kStages, whose reads the last chunk has waited for)
+        if (i + S::kStages - 1 < steps)
+          issue(i + S::kStages - 1);
+        // chunk i is in LDS when no more than the younger chunks' loads are out
+        const int younger = steps - 1 - i < S::kStages - 1 ? steps - 1 - i : S::kStages - 1;
+        if (younger == 3)
+          __builtin_amdgcn_s_waitcnt(pg_wait_imm(3 * kDmas));
+        else if (younger == 2)
+          __builtin_amdgcn_s_waitcnt(pg_wait_imm(2 * kDmas));
+        else if (younger == 1)
+          __builtin_amdgcn_s_waitcnt(pg_wait_imm(kDmas));
+        else
+          __builtin_amdgcn_s_waitcnt(pg_wait_imm(0));
+        asm volatile("" ::: "memory");
+        spend(x0, i, (int)(bads >> (2 * younger)) & 3);
       }
-      if (x.bad & (1 << t))
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          v[r] = __builtin_nanf("");
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool in = key0 + t * 16 + lg * 4 + r < seen;
-        live |= (uint32_t)in << (t * 4 + r);
-        s[t * 4 + r] = v[r] * g.scale_log2e;
-        top = fmaxf(top, in ? s[t * 4 + r] : kNegBig);
+    } else {
+      for (int i = 0; i < steps;) {
+        if (i + 1 < steps)
+          fetch(x1, i + 1);
+        spend(x0, i, x0.bad);
+        if (++i >= steps)
+          break;
+        if (i + 1 < steps)
+          fetch(x0, i + 1);
+        spend(x1, i, x1.bad);
+        ++i;
       }
     }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float mn = fmaxf(m, top);
-    if (__builtin_amdgcn_ballot_w64(mn > m)) {
-      const float alpha = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      sum *= alpha;
-#pragma unroll
-      for (int j = 0; j < T; ++j)
-        o[j] *= alpha;
-      if constexpr (Q4)
-#pragma unroll
-        for (int n = 0; n < NG; ++n)
-          z[n] *= alpha, lows[n] *= alpha;
-    }
-    float p[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      p[e] = (live >> e) & 1 ? __builtin_amdgcn_exp2f(s[e] - m) : 0.f;
-      sum += p[e];
-    }
-    if constexpr (Q4) {
-      if (ends)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (key0 + t * 16 + lg * 4 + r >= keys)
-#pragma unroll
-              for (int n = 0; n < NG; ++n)
-                vpar[t][(r * NG + n) / 4][(r * NG + n) % 4] = 0;
-      constexpr uint32_t kOne = BF16 ? 0x3f803f80u : 0x3c003c00u;
-      const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
+
+    // ---- the wavefronts' parts meet: O^T value r of tile n * TG + j is column
+    // n * GG + (lg * 4 + r) * TG + j of row lq
+    if (beyond)
+      sum = __builtin_nanf("");
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if constexpr (Q4)
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        float ps[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const f16x2 pr = pair_of(vpar, e >> 2, e & 3, n);
-          ps[e] = p[e] * (float)pr.x;
-          lows[n] = __builtin_fmaf(p[e], (float)pr.y, lows[n]);
-        }
-        const uint32_t pf[4] = {pg_pack<BF16>(ps[0], ps[1]), pg_pack<BF16>(ps[2], ps[3]),
-                                pg_pack<BF16>(ps[4], ps[5]), pg_pack<BF16>(ps[6], ps[7])};
-        z[n] = pg_mfma<BF16>(ones, pf, z[n]);
-        uint32_t lo[4], hi[4]; // nibbles of the keys 2 e and 2 e + 1 in the halves
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (VB == 4) {
-            lo[e] = __builtin_amdgcn_perm(x.v[2 * e + 1], x.v[2 * e], 0x05040100u);
-            hi[e] = __builtin_amdgcn_perm(x.v[2 * e + 1], x.v[2 * e], 0x07060302u);
-          } else {
-            lo[e] = x.v[n * 4 + e];
-            hi[e] = 0;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < TG; ++j) {
-          uint32_t f[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            f[e] = Codes<BF16>::pair(j < 4 ? lo[e] : hi[e], j & 3);
-          o[n * TG + j] = pg_mfma<BF16>(f, pf, o[n * TG + j]);
-        }
+        lows[n] = __builtin_fmaf(8.f, scales[n], lows[n]);
+        lows[n] += __shfl_xor(lows[n], 16, 64);
+        lows[n] += __shfl_xor(lows[n], 32, 64);
       }
-    } else {
-      if (ends)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (key0 + (e >> 2) * 16 + lg * 4 + (e & 3) >= keys)
-            x.v16[e] = u32x4{};
-      const uint32_t pf[4] = {pg_pack<BF16>(p[0], p[1]), pg_pack<BF16>(p[2], p[3]),
-                              pg_pack<BF16>(p[4], p[5]), pg_pack<BF16>(p[6], p[7])};
+    for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int j = 0; j < T; ++j) {
-        uint32_t f[4];
+      for (int j = 0; j < TG; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          f[e] = __builtin_amdgcn_perm(x.v16[2 * e + 1][j / 2], x.v16[2 * e][j / 2],
-                                       j & 1 ? 0x07060302u : 0x05040100u);
-        o[j] = pg_mfma<BF16>(f, pf, o[j]);
+        for (int r = 0; r < 4; ++r) {
+          float v = o[n * TG + j][r];
+          if constexpr (Q4)
+            v = __builtin_fmaf(-(Codes<BF16>::kOffset + 8.f), z[n][r], v) + lows[n];
+          sums[(n * GG + (lg * 4 + r) * TG + j) * PITCH + lq] = v;
+        }
+    if (l < 16)
+      ml[wave][0][l] = m, ml[wave][1][l] = sum;
+    __syncthreads();
+    const int d = threadIdx.x % HD;
+    for (int q = threadIdx.x / HD; q < 16 && q < left; q += kWaves * 64 / HD) {
+      float top = ml[0][0][q];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w)
+        top = fmaxf(top, ml[w][0][q]);
+      float acc = 0.f, den = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f((ml[w][0][q] - top) * g.scale_log2e);
+        acc += ((const float *)(smem + w * S::kBytes))[d * PITCH + q] * f;
+        den += ml[w][1][q] * f;
+      }
+      if (!whole) {
+        const int64_t to = ((int64_t)blockIdx.x * 2 + slot) * 16 + q;
+        ((PG_AS1 float *)g.part)[to * HD + d] = acc;
+        if (d == 0)
+          ((PG_AS1 float *)g.part_ml)[to * 2] = top, ((PG_AS1 float *)g.part_ml)[to * 2 + 1] = den;
+      } else {
+        const int r = qt * 16 + q, p = r / g.group;
+        pg_store<BF16>(g.o, (int64_t)(seq.start + p) * g.o_st + (int64_t)(hk * g.group + r - p * g.group) * g.o_sh + d,
+                       den == 0.f ? 0.f : acc / den);
       }
     }
-  };
-  Chunk x0, x1;
-  int i = 0;
-  if (steps > 0)
-    fetch(x0, 0);
-  while (i < steps) {
-    if (i + 1 < steps)
-      fetch(x1, i + 1);
-    spend(x0, i);
-    if (++i >= steps)
-      break;
-    if (i + 1 < steps)
-      fetch(x0, i + 1);
-    spend(x1, i);
-    ++i;
-  }
-
-  // ---- the wavefronts' parts meet: O^T value r of tile n * TG + j is column
-  // n * GG + (lg * 4 + r) * TG + j of row lq
-  if (beyond)
-    sum = __builtin_nanf("");
-  sum += __shfl_xor(sum, 16, 64);
-  sum += __shfl_xor(sum, 32, 64);
-  if constexpr (Q4)
-#pragma unroll
-    for (int n = 0; n < NG; ++n) {
-      lows[n] += __shfl_xor(lows[n], 16, 64);
-      lows[n] += __shfl_xor(lows[n], 32, 64);
-    }
-#pragma unroll
-  for (int n = 0; n < NG; ++n)
-#pragma unroll
-    for (int j = 0; j < TG; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = o[n * TG + j][r];
-        if constexpr (Q4)
-          v = __builtin_fmaf(-Codes<BF16>::kOffset, z[n][r], v) + lows[n];
-        sums[wave][(n * GG + (lg * 4 + r) * TG + j) * PITCH + lq] = v;
-      }
-  if (l < 16)
-    ml[wave][0][l] = m, ml[wave][1][l] = sum;
-  __syncthreads();
-  const int d = threadIdx.x % HD;
-  for (int q = threadIdx.x / HD; q < 16 && q < left; q += kWaves * 64 / HD) {
-    float top = ml[0][0][q];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w)
-      top = fmaxf(top, ml[w][0][q]);
-    float acc = 0.f, den = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(ml[w][0][q] - top);
-      acc += sums[w][d * PITCH + q] * f;
-      den += ml[w][1][q] * f;
-    }
-    if (splits > 1) {
-      const int64_t at = (int64_t)(part + index) * 16 + q;
-      ((PG_AS1 float *)g.part)[at * HD + d] = acc;
-      if (d == 0)
-        ((PG_AS1 float *)g.part_ml)[at * 2] = top, ((PG_AS1 float *)g.part_ml)[at * 2 + 1] = den;
-    } else {
-      const int r = qt * 16 + q, p = r / g.group;
-      pg_store<BF16>(g.o, (int64_t)(seq.start + p) * g.o_st + (int64_t)(hk * g.group + r - p * g.group) * g.o_sh + d,
-                     den == 0.f ? 0.f : acc / den);
-    }
+    __syncthreads(); // (before the next segment's rows or sums)
   }
 }
 
@@ -639,13 +858,16 @@ __global__ __launch_bounds__(256) void sdpa_paged_join_kernel(PagedArgs g) {
   const int t = (int)(lin / heads), h = (int)(lin % heads);
   if (t < g.offsets[0] || t >= g.offsets[g.cache.batch])
     return;
-  const PG_AS1 int32_t *info = (const PG_AS1 int32_t *)g.info + (int64_t)t * 3;
-  const int first = info[0], splits = info[1], pos = info[2];
+  const PagedArgs::Info info = g.info[t];
   const int hk = h / g.group;
-  const int64_t row = (int64_t)pos * g.group + h - hk * g.group;
-  const int64_t piece = first + row / 16 * g.Hkv * splits + hk;
-  // (rows that offsets which overlap have left out hold anything)
-  if (splits <= 1 || pos < 0 || first < 0 || piece + (int64_t)(splits - 1) * g.Hkv >= g.parts)
+  const int64_t row = (int64_t)info.pos * g.group + h - hk * g.group, item = (int64_t)hk * info.tiles + row / 16;
+  if (info.per < 1 || info.chunks < 1 || info.pos < 0) // (rows that offsets which overlap have left out hold anything)
+    return;
+  // cuts that lie inside this segment and not near its ends
+  const int64_t from = info.first + item * info.chunks, near = info.per / kNear;
+  const int64_t cut0 = (from + near + info.per - 1) / info.per, cut1 = (from + info.chunks - near) / info.per;
+  const int64_t begin = cut0 - 1, pieces = cut1 - cut0 + 2;
+  if (info.chunks < 2 * near || pieces <= 1 || begin < 0 || begin + pieces > g.pieces)
     return;
   const PG_AS1 float *ml = (const PG_AS1 float *)g.part_ml;
   const PG_AS1 float *p = (const PG_AS1 float *)g.part;
@@ -653,14 +875,15 @@ __global__ __launch_bounds__(256) void sdpa_paged_join_kernel(PagedArgs g) {
     float m, l, o;
   };
   const auto load = [&](int s) {
-    const int64_t at = (piece + (int64_t)s * g.Hkv) * 16 + row % 16;
+    const int64_t at = ((begin + s) * 2 + (s == 0)) * 16 + row % 16;
     return Part{ml[at * 2], ml[at * 2 + 1], p[at * HD + d]};
   };
   constexpr int U = 8;
   float top = kNegBig, acc = 0.f, den = 0.f;
-  fhip_for_uniform_parts<U>(0, 1, splits, load, [&](const Part &x) {
+  fhip_for_uniform_parts<U>(0, 1, (int)pieces, load, [&](const Part &x) {
     const float m = fmaxf(top, x.m);
-    const float was = __builtin_amdgcn_exp2f(top - m), f = __builtin_amdgcn_exp2f(x.m - m);
+    const float was = __builtin_amdgcn_exp2f((top - m) * g.scale_log2e),
+                f = __builtin_amdgcn_exp2f((x.m - m) * g.scale_log2e);
     den = den * was + x.l * f;
     acc = acc * was + x.o * f;
     top = m;
@@ -668,8 +891,10 @@ __global__ __launch_bounds__(256) void sdpa_paged_join_kernel(PagedArgs g) {
   pg_store<BF16>(g.o, (int64_t)t * g.o_st + (int64_t)h * g.o_sh + d, den == 0.f ? 0.f : acc / den);
 }
 
-// Pieces that the work is cut into.
-constexpr int kTarget = 512;
+// Workgroups that share the line: two for each compute unit run at once.  In 4 bits, where a compute unit has more to
+// compute, two rounds of them are even: 64 chats of 16 to 16384 keys 113.6 us with 512, 117.3 with 768, 109.1 with 1024;
+// 32 chats in 16 bits 77.3, 78.3, 75.4, but 68.0 and 71.1 where 512 are one segment each.
+constexpr int kPieces16 = 512, kPieces4 = 1024;
 // Chunks that a piece has at least, and keys up to which no sequence is cut (the
 // launch that joins pieces takes longer than what it saves).
 constexpr int kLeast = 2 * kWaves;
@@ -679,7 +904,7 @@ struct PagedPlan {
   bool ok = false;
   int hd = 0, group = 0;
   bool bf16 = false, cut = false;
-  int64_t pieces = 0, parts = 0;
+  int64_t pieces = 0; // workgroups
   size_t bytes = 0, part_at = 0, ml_at = 0;
 };
 
@@ -688,6 +913,9 @@ PagedPlan make_plan(const fhip_sdpa_paged_desc *d) {
   const int dt = d->q.dtype;
   const int64_t T = d->q.dim[0], Hq = d->q.dim[1], D = d->q.dim[2], Hkv = d->cache.k.dim[1];
   if ((dt != FHIP_BFLOAT16 && dt != FHIP_HALF) || (D != 64 && D != 128) || d->o.dim[2] != D)
+    return p;
+  // the running maximum is taken over raw scores: needs a positive scale
+  if (d->has_scale && !(d->scale > 0.f && d->scale < INFINITY))
     return p;
   p.bf16 = dt == FHIP_BFLOAT16;
   p.hd = (int)D;
@@ -710,21 +938,23 @@ PagedPlan make_plan(const fhip_sdpa_paged_desc *d) {
       (q4 && (!fits(d->cache.k_params, 3, 2) || !fits(d->cache.v_params, 3, 2))))
     return p;
   // 32-bit offsets within a tile of 16 keys
-  if (d->cache.k.stride[2] * es >= (1 << 26) || d->cache.v.stride[2] * es >= (1 << 26))
+  if (d->cache.k.stride[2] * es >= (1 << 26) || d->cache.v.stride[2] * es >= (1 << 26) ||
+      (q4 && (d->cache.k_params.stride[2] >= (1 << 25) || d->cache.v_params.stride[2] >= (1 << 25))))
     return p;
   const int64_t group = Hq / Hkv, batch = d->cache.batch;
   // tiles of 16 rows, each sequence's last one short
   const int64_t tiles = Hkv * (T * group / 16 + (batch < T ? batch : T));
   if (T * group >= (1ll << 30) || tiles >= (1ll << 29))
     return p;
-  p.cut = d->cache.pages_per_sequence * d->cache.k.dim[2] > kWhole;
-  p.pieces = tiles + (p.cut ? kTarget + 8 : 0);
+  const int64_t keys = d->cache.pages_per_sequence * d->cache.k.dim[2];
+  // (the line's places are 32-bit numbers)
+  p.cut = keys > kWhole && tiles * ((keys + kChunk - 1) / kChunk) < (1ll << 31) - (1 << 24);
+  p.pieces = tiles;
   if (p.cut) {
-    // a sequence in several pieces has more chunks than a piece: at most twice kTarget of them
-    p.parts = 2 * kTarget + 64;
-    p.part_at = ((size_t)T * 12 + 255) / 256 * 256;
-    p.ml_at = p.part_at + (size_t)p.parts * 16 * (size_t)D * 4;
-    p.bytes = p.ml_at + (size_t)p.parts * 16 * 8;
+    p.pieces = q4 ? kPieces4 : kPieces16;
+    p.part_at = ((size_t)T * sizeof(PagedArgs::Info) + 255) / 256 * 256;
+    p.ml_at = p.part_at + (size_t)p.pieces * 2 * 16 * (size_t)D * 4;
+    p.bytes = p.ml_at + (size_t)p.pieces * 2 * 16 * 8;
   }
   p.ok = true;
   return p;
@@ -750,20 +980,26 @@ int fhip_fast_sdpa_paged(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d, const fhi
   g.cache = fhip_cache_view(d->cache, *cache);
   g.T = (int32_t)d->q.dim[0], g.Hkv = (int32_t)d->cache.k.dim[1], g.group = (int32_t)(d->q.dim[1] / g.Hkv);
   g.causal = d->is_causal != 0;
-  g.target = kTarget, g.least = p.cut ? kLeast : 1 << 26;
+  g.pieces = (int32_t)p.pieces, g.least = kLeast;
   const float scale = d->has_scale ? d->scale : 1.0f / sqrtf((float)p.hd);
   g.scale_log2e = scale * 1.4426950408889634f;
   if (p.cut) {
-    g.info = (int32_t *)workspace;
+    g.info = (PagedArgs::Info *)workspace;
     g.part = (float *)((char *)workspace + p.part_at);
     g.part_ml = (float *)((char *)workspace + p.ml_at);
-    g.parts = (int32_t)p.parts;
   }
   fhip_note_kernel(ctx, "sdpa_paged d=%d bits=%d group=%d cut=%d", p.hd, p.group ? 4 : 16, p.group, (int)p.cut);
   auto go = [&](auto bf, auto hd, auto grp) {
     constexpr bool BF = decltype(bf)::value;
     constexpr int HD = decltype(hd)::value, G = decltype(grp)::value;
-    hipLaunchKernelGGL((sdpa_paged_kernel<BF, HD, G>), dim3((unsigned)p.pieces), dim3(kWaves * 64), 0, ctx->stream, g);
+    constexpr int kLds = kWaves * PagedShape<HD, G>::kBytes;
+    static FhipOncePerDevice configured; // (one for each instance of this lambda)
+    if (kLds > 64 * 1024 && !configured.done(ctx->device)) {
+      FHIP_HIP_CHECK(ctx, hipFuncSetAttribute(reinterpret_cast<const void *>(sdpa_paged_kernel<BF, HD, G>),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+      configured.mark(ctx->device);
+    }
+    hipLaunchKernelGGL((sdpa_paged_kernel<BF, HD, G>), dim3((unsigned)p.pieces), dim3(kWaves * 64), kLds, ctx->stream, g);
     if (p.cut)
       hipLaunchKernelGGL((sdpa_paged_join_kernel<BF, HD>),
                          dim3((unsigned)(((int64_t)g.T * g.Hkv * g.group + 256 / HD - 1) / (256 / HD))), dim3(256), 0,
