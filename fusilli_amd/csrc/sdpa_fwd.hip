@@ -114,7 +114,94 @@ struct SdpaArgs {
   int32_t m_rows;   // rows of the mask: row r of a folded group reads row r % m_rows
   uint32_t m_bytes; // bytes of one (batch, head) slab
   int32_t m_dt;     // FHIP_BOOLEAN / FHIP_FLOAT / FHIP_BFLOAT16 / FHIP_HALF
+  // packed sequences (kernels with PACKED): rows of Q and of K, heads of K;
+  // 2^32 / group rounded up (0: groups of one)
+  const int32_t *offsets, *kv_offsets;
+  int32_t batch, T, Tk, Hkv;
+  uint32_t magic;
 };
+
+// ---- packed sequences ------------------------------------------------------
+// The rows of a sequence that share a key / value head are one matrix, position
+// after position (row r: position r / group, head r % group), cut into tiles of
+// ROWS.  No one but the device knows the lengths: every workgroup reads all of
+// them and finds its own tile.  Tiles come in classes of cost, keys of 2^k to
+// 2^(k + 1) - 1 tiles of 64, the most expensive first, so that the last ones to start are short;
+// the heads of a tile are neighbours, on one XCD each where there are 8.
+struct PackedSeq {
+  int start, n, kv_start, m; // rows and keys
+  int tiles;
+};
+template <int ROWS> __device__ __forceinline__ PackedSeq sd_packed_seq(const SdpaArgs &g, int b) {
+  PackedSeq s;
+  auto clamp = [](int x, int top) { return x < 0 ? 0 : x > top ? top : x; };
+  s.start = clamp(g.offsets[b], g.T);
+  s.n = clamp(g.offsets[b + 1], g.T) - s.start;
+  s.n = s.n < 0 ? 0 : s.n;
+  s.kv_start = clamp(g.kv_offsets[b], g.Tk);
+  s.m = clamp(g.kv_offsets[b + 1], g.Tk) - s.kv_start;
+  s.m = s.m < 0 ? 0 : s.m;
+  s.tiles = (s.n * g.group + ROWS - 1) / ROWS;
+  return s;
+}
+// Tiles of a sequence that take `cost` or more tiles of keys: the last ones, under a causal mask.
+template <int ROWS, bool CAUSAL>
+__device__ __forceinline__ int sd_packed_count(const SdpaArgs &g, const PackedSeq &s, int cost) {
+  if (cost <= 1)
+    return s.tiles;
+  const int64_t keys = (int64_t)(cost - 1) * kBKV; // a tile that sees more than these
+  if (keys >= s.m)
+    return 0;
+  if (!CAUSAL)
+    return s.tiles;
+  const int pos = (int)keys - (s.m - s.n); // the first position that does
+  return pos <= 0 ? s.tiles : pos >= s.n ? 0 : s.tiles - (int)((uint32_t)(pos * g.group) / ROWS);
+}
+__device__ __forceinline__ int sd_scan(int x) { // inclusive sums over the lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false); // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false); // row_bcast 15, 31
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+struct PackedItem {
+  int start, n, kv_start, m, hk, tile; // tile -1: none
+};
+template <int ROWS, bool CAUSAL>
+__device__ __forceinline__ PackedItem sd_packed_item(const SdpaArgs &g, int index) {
+  const int l = threadIdx.x & 63;
+  const PackedSeq front = l < g.batch ? sd_packed_seq<ROWS>(g, l) : PackedSeq{};
+  // (a class above every sequence's keys is passed over by its count of 0)
+  int keys = front.m;
+  for (int b = l + 64; b < g.batch; b += 64) {
+    const int m = sd_packed_seq<ROWS>(g, b).m;
+    keys = m > keys ? m : keys;
+  }
+  int k = 0;
+  while (__builtin_amdgcn_ballot_w64(keys > (kBKV << k)) != 0) // (keys < 2^30)
+    ++k;
+  int left = index;
+  for (; k >= 0; --k)
+    for (int b0 = 0; b0 < g.batch; b0 += 64) {
+      const PackedSeq s = b0 == 0 ? front : b0 + l < g.batch ? sd_packed_seq<ROWS>(g, b0 + l) : PackedSeq{};
+      const int above = sd_packed_count<ROWS, CAUSAL>(g, s, 2 << k);
+      const int mine = sd_packed_count<ROWS, CAUSAL>(g, s, 1 << k) - above;
+      const int upto = sd_scan(mine) * g.Hkv;
+      const uint64_t past = __builtin_amdgcn_ballot_w64(upto > left);
+      if (past) {
+        const int i = __builtin_ctzll(past);
+        const int r = left - __builtin_amdgcn_readlane(upto - mine * g.Hkv, i);
+        const int tile = __builtin_amdgcn_readlane(s.tiles - above, i) - 1 - r / g.Hkv;
+        return PackedItem{__builtin_amdgcn_readlane(s.start, i),    __builtin_amdgcn_readlane(s.n, i),
+                          __builtin_amdgcn_readlane(s.kv_start, i), __builtin_amdgcn_readlane(s.m, i),
+                          r % g.Hkv,                                tile};
+      }
+      left -= __builtin_amdgcn_readlane(upto, 63);
+    }
+  return PackedItem{0, 0, 0, 0, 0, -1};
+}
 
 template <int N, typename F> __device__ __forceinline__ void sd_static_for(F &&f) {
   if constexpr (N > 0) {
@@ -259,10 +346,12 @@ __device__ __forceinline__ void sd_barrier() {
 }
 
 // MASK: 0 no mask tensor, 1 mask read into registers, 2 mask staged in LDS
-template <bool BF16, bool CAUSAL, int HD, int MASK, bool SPLIT = false>
+// PACKED: packed sequences, a tile per workgroup
+template <bool BF16, bool CAUSAL, int HD, int MASK, bool SPLIT = false, bool PACKED = false>
 __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
   static_assert(!(CAUSAL && MASK), "a mask tensor excludes the causal flag");
   static_assert(!(SPLIT && MASK == 1), "split keys stage their mask");
+  static_assert(!(PACKED && MASK), "packed sequences have no mask tensor");
   using C = SdShape<HD>;
   constexpr int kD = HD;
   constexpr int kRowB = C::kRowB, kTileB = C::kTileB;
@@ -295,29 +384,66 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
     b = head / g.xcd_heads;
   }
   const int n_qtiles = (g.Sq + kRows - 1) / kRows;
-  const int passes = CAUSAL && n_qtiles - 1 - z != z ? 2 : 1;
+  const int passes = !PACKED && CAUSAL && n_qtiles - 1 - z != z ? 2 : 1;
   for (int pass = 0; pass < passes; ++pass) {
-  const int qtile = CAUSAL && pass == 0 ? n_qtiles - 1 - z : z;
+  PackedItem item{};
+  if constexpr (PACKED) {
+    item = sd_packed_item<kRows, CAUSAL>(g, (int)blockIdx.x);
+    if (item.tile < 0 || item.tile * kRows >= item.n * g.group) // (the latter where offsets overlap)
+      return;
+  }
+  const int qtile = PACKED ? item.tile : CAUSAL && pass == 0 ? n_qtiles - 1 - z : z;
+  const int Sq = PACKED ? item.n * g.group : g.Sq, Skv = PACKED ? item.m : g.Skv;
+  // a row's position (of PACKED's grouped heads), and the last key that it sees
+  auto pos_of = [&](int r) { return PACKED && g.magic ? (int)__umulhi((uint32_t)r, g.magic) : r; };
+  auto last_key = [&](int r) { return PACKED ? pos_of(r) + Skv - item.n : r; };
+  auto q_row = [&](int r) -> int64_t { // its elements from qp
+    if constexpr (PACKED) {
+      const int pos = pos_of(r);
+      return pos * g.q_ss + (int64_t)(r - pos * g.group) * g.q_sh;
+    } else {
+      return (int64_t)r * g.q_ss;
+    }
+  };
+  auto o_row = [&](int r) -> int64_t {
+    if constexpr (PACKED) {
+      const int pos = pos_of(r);
+      return pos * g.o_ss + (int64_t)(r - pos * g.group) * g.o_sh;
+    } else {
+      return (int64_t)r * g.o_ss;
+    }
+  };
   if (pass) // the first tile's output staging has been read
     __builtin_amdgcn_s_barrier();
-  const int hk = h / g.group;
+  const int hk = PACKED ? item.hk : h / g.group;
   const int q0 = qtile * kRows;
   const int qw0 = q0 + loader * 32; // first query row of this wavefront
   const int qrow = qw0 + lq;      // query this lane's scores belong to
 
-  const char *qp = g.q + (b * g.q_sb + h * g.q_sh) * 2;
-  const char *kp = g.k + (b * g.k_sb + hk * g.k_sh) * 2;
-  const char *vp = g.v + (b * g.v_sb + hk * g.v_sh) * 2;
+  const char *qp = PACKED ? g.q + (item.start * g.q_ss + (int64_t)(hk * g.group) * g.q_sh) * 2
+                          : g.q + (b * g.q_sb + h * g.q_sh) * 2;
+  const char *kp = g.k + ((PACKED ? item.kv_start * g.k_ss : b * g.k_sb) + hk * g.k_sh) * 2;
+  const char *vp = g.v + ((PACKED ? item.kv_start * g.v_ss : b * g.v_sb) + hk * g.v_sh) * 2;
+  auto o_base = [&] {
+    return PACKED ? g.o + (item.start * g.o_ss + (int64_t)(hk * g.group) * g.o_sh) * 2
+                  : g.o + (b * g.o_sb + h * g.o_sh) * 2;
+  };
   const int64_t k_rowb = g.k_ss * 2, v_rowb = g.v_ss * 2;
-  const int64_t k_bytes = (int64_t)(g.Skv - 1) * k_rowb + kRowB;
-  const int64_t v_bytes = (int64_t)(g.Skv - 1) * v_rowb + kRowB;
+  const int64_t k_bytes = (int64_t)(Skv - 1) * k_rowb + kRowB;
+  const int64_t v_bytes = (int64_t)(Skv - 1) * v_rowb + kRowB;
 
   // number of key tiles this workgroup visits
-  int kv_end = g.Skv;
+  int kv_end = Skv;
   if (CAUSAL) {
-    const int last_q = q0 + kRows - 1 < g.Sq - 1 ? q0 + kRows - 1 : g.Sq - 1;
-    kv_end = last_q + 1 < g.Skv ? last_q + 1 : g.Skv;
+    const int last_q = last_key(q0 + kRows - 1 < Sq - 1 ? q0 + kRows - 1 : Sq - 1);
+    kv_end = last_q + 1 < Skv ? last_q + 1 : Skv;
   }
+  if constexpr (PACKED)
+    if (kv_end <= 0) { // no row sees a key
+      for (int r = q0 + (int)threadIdx.x / C::kChunks; r < q0 + kRows && r < Sq; r += kWaves * 64 / C::kChunks)
+        *(SD_AS1 u32x4 *)(o_base() + o_row(r) * 2 + threadIdx.x % C::kChunks * 16) = u32x4{0, 0, 0, 0};
+      return;
+    }
   const int tiles = (kv_end + kBKV - 1) / kBKV;
   // the rounds they take, and the tile of this wavefront in round t
   const int rounds = SPLIT ? (tiles + 1) / 2 : tiles;
@@ -326,8 +452,8 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
   // ---- Q fragments (B operand of S^T = K Q^T): row lq, 8 d per register quad
   uint32_t qf[kD / 16][4];
   {
-    const int qr = qrow < g.Sq ? qrow : g.Sq - 1;
-    const char *src = qp + (int64_t)qr * g.q_ss * 2 + half * 16;
+    const int qr = qrow < Sq ? qrow : Sq - 1;
+    const char *src = qp + q_row(qr) * 2 + half * 16;
 #pragma unroll
     for (int ds = 0; ds < kD / 16; ++ds) {
       const u32x4 v = *(const SD_AS1 u32x4 *)(src + ds * 32);
@@ -551,8 +677,11 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
 
   uint32_t pf[4][4]; // probabilities as B-operand fragments, 16 keys each
   // a wavefront whose rows all lie above a tile has nothing to add
+  const int wave_first = PACKED ? last_key(qw0) : qw0; // last keys of its first and last row, and of this lane's
+  const int wave_last = PACKED ? last_key(qw0 + 31 < Sq ? qw0 + 31 : Sq - 1) : qw0 + 31;
+  const int row_last = PACKED ? last_key(qrow) : qrow;
   auto active = [&](int t) {
-    return !(CAUSAL && tile_of(t) * kBKV > qw0 + 31) && (!SPLIT || tile_of(t) < tiles);
+    return !(CAUSAL && tile_of(t) * kBKV > wave_last) && (!SPLIT || tile_of(t) < tiles);
   };
   // ring slots of tile t - 1, t, t + 1, t + 2 (slot of t + 2 == slot of t - 1, with two stages of t)
   int sl_prev = kStagesK - 1, sl_cur = 0, sl_next = 1;
@@ -800,7 +929,7 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
           fold(mraw);
         }
       }
-      const bool edge = (CAUSAL && kv0 + kBKV - 1 > qw0) || kv0 + kBKV > g.Skv;
+      const bool edge = (CAUSAL && kv0 + kBKV - 1 > wave_first) || kv0 + kBKV > Skv;
       if (edge) {
         // (masked kernels use -inf: a row may see dead keys before its first
         // live one, and exp2(-inf - reference) is 0 whatever the reference)
@@ -810,7 +939,7 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int key = kv0 + kb * 32 + (r >> 2) * 8 + half * 4 + (r & 3);
-            const bool dead = key >= g.Skv || (CAUSAL && key > qrow);
+            const bool dead = key >= Skv || (CAUSAL && key > row_last);
             s[kb][r] = dead ? gone : s[kb][r];
           }
       }
@@ -952,7 +1081,9 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-  char *op = g.o + (b * g.o_sb + h * g.o_sh) * 2;
+  char *op = o_base();
+  // (a row that sees no key is 0; a tile has some that do)
+  const bool sees = !PACKED || !CAUSAL || row_last >= 0;
   if constexpr (SPLIT) {
     // A wavefront keeps half of the features, its team's, and sends the others to the wavefront
     // that owns the same rows in the other team.
@@ -990,7 +1121,7 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          v[e] = (o[i][r + e] * mine + x[e] * theirs) * inv;
+          v[e] = sees ? (o[i][r + e] * mine + x[e] * theirs) * inv : 0.f;
         u32x2 w2;
         w2.x = sd_pack<BF16>(v[0], v[1]);
         w2.y = sd_pack<BF16>(v[2], v[3]);
@@ -1003,8 +1134,8 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
       const int cb = (l % kHalf) * 16;
       const u32x4 v = *(const SD_AS3 u32x4 *)(uintptr_t)(band + row * C::kSplitPitch + cb);
       const int qr = qw0 + row;
-      if (qr < g.Sq)
-        *(SD_AS1 u32x4 *)(op + (int64_t)qr * g.o_ss * 2 + team * (kRowB / 2) + cb) = v;
+      if (qr < Sq)
+        *(SD_AS1 u32x4 *)(op + o_row(qr) * 2 + team * (kRowB / 2) + cb) = v;
     }
   } else {
   const float inv = 1.0f / sd_half_sum(l_run);
@@ -1015,8 +1146,12 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       u32x2 w2;
-      w2.x = sd_pack<BF16>(o[dt][r4 * 4 + 0] * inv, o[dt][r4 * 4 + 1] * inv);
-      w2.y = sd_pack<BF16>(o[dt][r4 * 4 + 2] * inv, o[dt][r4 * 4 + 3] * inv);
+      if (sees) {
+        w2.x = sd_pack<BF16>(o[dt][r4 * 4 + 0] * inv, o[dt][r4 * 4 + 1] * inv);
+        w2.y = sd_pack<BF16>(o[dt][r4 * 4 + 2] * inv, o[dt][r4 * 4 + 3] * inv);
+      } else {
+        w2 = u32x2{0, 0};
+      }
       *(SD_AS3 u32x2 *)(uintptr_t)(band + lq * kOutPitch +
                                    (dt * 32 + r4 * 8 + half * 4) * 2) = w2;
     }
@@ -1028,8 +1163,8 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
     const u32x4 v =
         *(const SD_AS3 u32x4 *)(uintptr_t)(band + row * kOutPitch + cb);
     const int qr = qw0 + row;
-    if (qr < g.Sq)
-      *(SD_AS1 u32x4 *)(op + (int64_t)qr * g.o_ss * 2 + cb) = v;
+    if (qr < Sq)
+      *(SD_AS1 u32x4 *)(op + o_row(qr) * 2 + cb) = v;
   }
   }
   } // pass
@@ -1310,4 +1445,77 @@ int fhip_fast_sdpa(fhip_ctx *ctx, const fhip_sdpa_desc *d, const void *q,
   auto typed = [&](auto hd) { return p.bf16 ? pick(hd, std::true_type{}) : pick(hd, std::false_type{}); };
   return p.hd == 128 ? typed(std::integral_constant<int, 128>{})
                      : typed(std::integral_constant<int, 64>{});
+}
+
+// ---- packed sequences ------------------------------------------------------
+bool fhip_fast_sdpa_packed_applicable(const fhip_sdpa_packed_desc *d) {
+  const int dt = d->q.dtype;
+  const int64_t D = d->q.dim[2], T = d->q.dim[0], Tk = d->k.dim[0], group = d->q.dim[1] / d->k.dim[1];
+  if ((dt != FHIP_BFLOAT16 && dt != FHIP_HALF) || (D != 64 && D != 128) || d->v.dim[2] != D)
+    return false;
+  if (d->has_scale && !(d->scale > 0.f && d->scale < INFINITY)) // (maxima are taken over raw scores)
+    return false;
+  const fhip_tensor_desc *ts[4] = {&d->q, &d->k, &d->v, &d->o};
+  for (const fhip_tensor_desc *t : ts)
+    for (int i = 0; i < 2; ++i)
+      if (t->dim[i] > 1 && t->stride[i] % 8 != 0)
+        return false;
+  // 32-bit offsets within a sequence's K or V; rows by a multiplication (pos_of)
+  if (Tk * d->k.stride[0] * 2 >= (1ll << 31) || Tk * d->v.stride[0] * 2 >= (1ll << 31) || Tk >= (1 << 30))
+    return false;
+  return T * group < (1ll << 30) && T * group * group < (1ll << 32);
+}
+
+int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const void *q, const void *k, const void *v,
+                          const void *offsets, const void *kv_offsets, void *o, bool *handled) {
+  *handled = fhip_fast_sdpa_packed_applicable(d) &&
+             (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15) == 0;
+  if (!*handled)
+    return 0;
+  SdpaArgs g{};
+  g.q = (const char *)q, g.k = (const char *)k, g.v = (const char *)v, g.o = (char *)o;
+  g.q_ss = d->q.stride[0], g.q_sh = d->q.stride[1], g.k_ss = d->k.stride[0], g.k_sh = d->k.stride[1];
+  g.v_ss = d->v.stride[0], g.v_sh = d->v.stride[1], g.o_ss = d->o.stride[0], g.o_sh = d->o.stride[1];
+  g.offsets = (const int32_t *)offsets, g.kv_offsets = (const int32_t *)(kv_offsets ? kv_offsets : offsets);
+  g.batch = (int32_t)d->batch, g.T = (int32_t)d->q.dim[0], g.Tk = (int32_t)d->k.dim[0], g.Hkv = (int32_t)d->k.dim[1];
+  g.group = (int32_t)(d->q.dim[1] / g.Hkv);
+  g.magic = g.group > 1 ? (uint32_t)(((1ull << 32) + g.group - 1) / g.group) : 0;
+  g.causal = d->is_causal != 0;
+  const int hd = (int)d->q.dim[2];
+  const float scale = d->has_scale ? d->scale : 1.0f / sqrtf((float)hd);
+  g.scale = scale, g.scale_log2e = scale * 1.4426950408889634f;
+  const int64_t rows = (int64_t)g.T * g.group, seqs = d->batch < g.T ? d->batch : g.T;
+  static const char *force = getenv("PK_SPLIT");
+  const bool split = force ? atoi(force) != 0 : g.Hkv * (rows / kBQ + seqs / 2 + 1) < 256;
+  // tiles of all sequences, each one's last short
+  const int64_t tiles = g.Hkv * (rows / (split ? kBQ / 2 : kBQ) + seqs);
+  FHIP_REQUIRE(ctx, tiles < (1ll << 31), "fhip_sdpa_packed_fwd: more than 2^31 tiles");
+  auto launch = [&](auto kernel, int lds_bytes, FhipOncePerDevice &configured) {
+    if (!configured.done(ctx->device)) {
+      if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              lds_bytes) != hipSuccess)
+        return fhip_fail(ctx, "sdpa: cannot reserve LDS");
+      configured.mark(ctx->device);
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(kWaves * 64), lds_bytes, ctx->stream, g);
+    FHIP_HIP_CHECK(ctx, hipGetLastError());
+    return 0;
+  };
+  fhip_note_kernel(ctx, "sdpa_packed d=%d causal=%d%s", hd, (int)g.causal, split ? " split" : "");
+  static FhipOncePerDevice configured[2][2][4]; // one for each kernel instance
+  auto pick = [&](auto hdc, auto bf) {
+    constexpr int HD = decltype(hdc)::value;
+    constexpr bool BF = decltype(bf)::value;
+    using C = SdShape<HD>;
+    FhipOncePerDevice(&cfg)[4] = configured[HD == 128][BF];
+    if (split)
+      return g.causal ? launch(sdpa_fwd_kernel<BF, true, HD, 0, true, true>, C::split_lds(false), cfg[0])
+                      : launch(sdpa_fwd_kernel<BF, false, HD, 0, true, true>, C::split_lds(false), cfg[1]);
+    return g.causal ? launch(sdpa_fwd_kernel<BF, true, HD, 0, false, true>, C::kLdsB, cfg[2])
+                    : launch(sdpa_fwd_kernel<BF, false, HD, 0, false, true>, C::kLdsB, cfg[3]);
+  };
+  auto typed = [&](auto hdc) {
+    return d->q.dtype == FHIP_BFLOAT16 ? pick(hdc, std::true_type{}) : pick(hdc, std::false_type{});
+  };
+  return hd == 128 ? typed(std::integral_constant<int, 128>{}) : typed(std::integral_constant<int, 64>{});
 }

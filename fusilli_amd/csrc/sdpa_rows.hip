@@ -176,7 +176,7 @@ int fhip_sdpa_packed_fwd_workspace_size(const fhip_sdpa_packed_desc *d, size_t *
 int fhip_sdpa_packed_fwd_supported(const fhip_sdpa_packed_desc *d) {
   if (!d || packed_validate(nullptr, d) != 0)
     return 0;
-  return 1;
+  return fhip_fast_sdpa_packed_applicable(d) ? 2 : 1;
 }
 
 int fhip_sdpa_packed_fwd(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const void *q, const void *k, const void *v,
@@ -192,6 +192,10 @@ int fhip_sdpa_packed_fwd(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const vo
   (void)workspace;
   (void)workspace_bytes;
   FHIP_HIP_CHECK(ctx, hipSetDevice(ctx->device));
+  bool handled = false;
+  const int rc = fhip_fast_sdpa_packed(ctx, d, q, k, v, offsets, kv_offsets, o, &handled);
+  if (handled)
+    return rc;
   fhip_note_kernel(ctx, "sdpa_rows packed");
   RowsArgs g{};
   g.q = q, g.k = k, g.v = v, g.o = o;
