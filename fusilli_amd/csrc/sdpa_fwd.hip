@@ -346,19 +346,21 @@ __device__ __forceinline__ void sd_barrier() {
 }
 
 // MASK: 0 no mask tensor, 1 mask read into registers, 2 mask staged in LDS
-// PACKED: packed sequences, a tile per workgroup
-template <bool BF16, bool CAUSAL, int HD, int MASK, bool SPLIT = false, bool PACKED = false>
-__global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
+// PACKED: packed sequences, a tile per workgroup: 1 of 256 rows (128, SPLIT); 2 of 128 rows, a workgroup of
+// wavefronts 0 .. 3 alone with the rings of one team
+template <bool BF16, bool CAUSAL, int HD, int MASK, bool SPLIT = false, int PACKED = 0>
+__global__ __launch_bounds__(PACKED == 2 ? kWaves * 32 : kWaves * 64, 2) void sdpa_fwd_kernel(SdpaArgs g) {
+  constexpr bool HALF = PACKED == 2;
   static_assert(!(CAUSAL && MASK), "a mask tensor excludes the causal flag");
   static_assert(!(SPLIT && MASK == 1), "split keys stage their mask");
-  static_assert(!(PACKED && MASK), "packed sequences have no mask tensor");
+  static_assert(!(PACKED && MASK) && !(HALF && SPLIT), "packed sequences have no mask tensor, one team none to share with");
   using C = SdShape<HD>;
   constexpr int kD = HD;
   constexpr int kRowB = C::kRowB, kTileB = C::kTileB;
-  constexpr int kLoaders = SPLIT ? kWaves / 2 : kWaves; // wavefronts that bring a tile in
+  constexpr int kLoaders = SPLIT || HALF ? kWaves / 2 : kWaves; // wavefronts that bring a tile in
   constexpr int kLoadsPerTile = kTileB / 1024 / kLoaders, kOutPitch = C::kOutPitch;
-  constexpr int kRows = SPLIT ? kBQ / 2 : kBQ;
-  constexpr bool kTight = SPLIT && HD == 128; // two stages of V
+  constexpr int kRows = SPLIT || HALF ? kBQ / 2 : kBQ;
+  constexpr bool kTight = (SPLIT || HALF) && HD == 128; // two stages of V
   constexpr int kStagesK = kTight ? C::split_k(MASK != 0) : kStages;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
@@ -366,7 +368,7 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l = threadIdx.x & 63;
   const int half = l >> 5, lq = l & 31;
-  const int team = __builtin_amdgcn_readfirstlane(wave >> 2);
+  const int team = HALF ? 0 : __builtin_amdgcn_readfirstlane(wave >> 2);
   const int loader = SPLIT ? wave & 3 : wave;
   // Causal masks: a workgroup runs query tile (last - z) and then tile z, a
   // long and a short one, so all workgroups do the same work (tiles of one
@@ -440,7 +442,7 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
   }
   if constexpr (PACKED)
     if (kv_end <= 0) { // no row sees a key
-      for (int r = q0 + (int)threadIdx.x / C::kChunks; r < q0 + kRows && r < Sq; r += kWaves * 64 / C::kChunks)
+      for (int r = q0 + (int)threadIdx.x / C::kChunks; r < q0 + kRows && r < Sq; r += (HALF ? 32 : 64) * kWaves / C::kChunks)
         *(SD_AS1 u32x4 *)(o_base() + o_row(r) * 2 + threadIdx.x % C::kChunks * 16) = u32x4{0, 0, 0, 0};
       return;
     }
@@ -1073,7 +1075,7 @@ __global__ __launch_bounds__(kWaves * 64) void sdpa_fwd_kernel(SdpaArgs g) {
   for (int t = 1; t < rounds; ++t)
     round(t, std::integral_constant<int, 1>{});
   round(rounds, std::integral_constant<int, 2>{});
-  if (!team) // pairs with the last barrier of wavefronts 4..7
+  if (!HALF && !team) // pairs with the last barrier of wavefronts 4..7
     __builtin_amdgcn_s_barrier();
 
   // ---- epilogue: O = O^T / l, through LDS for row-contiguous stores -----------
@@ -1485,10 +1487,13 @@ int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const v
   const float scale = d->has_scale ? d->scale : 1.0f / sqrtf((float)hd);
   g.scale = scale, g.scale_log2e = scale * 1.4426950408889634f;
   const int64_t rows = (int64_t)g.T * g.group, seqs = d->batch < g.T ? d->batch : g.T;
-  static const char *force = getenv("PK_SPLIT");
-  const bool split = force ? atoi(force) != 0 : g.Hkv * (rows / kBQ + seqs / 2 + 1) < 256;
+  // Workgroups of one team (2) overlap one tile's loads and stores with another's products: 256 prompts of 64 tokens, 32
+  // heads on 8, D128 120.5 us whole (0), so 94.5; 64 of 512 296 / 257; 4 of 2048 155.3 / 155.4; 8192 tokens 459 / 479: whole
+  // from 4096 keys.  Few tiles of long sequences: both teams on the same rows (1), 1024 tokens 25.9 / 22.7, 2048 50.6 / 51.8.
+  const int64_t halves = g.Hkv * (rows / (kBQ / 2) + seqs / 2), keys = g.Tk / seqs;
+  const int cut = halves <= 256 && keys >= 512 ? 1 : hd == 128 && keys >= 4096 ? 0 : 2;
   // tiles of all sequences, each one's last short
-  const int64_t tiles = g.Hkv * (rows / (split ? kBQ / 2 : kBQ) + seqs);
+  const int64_t tiles = g.Hkv * (rows / (cut ? kBQ / 2 : kBQ) + seqs);
   FHIP_REQUIRE(ctx, tiles < (1ll << 31), "fhip_sdpa_packed_fwd: more than 2^31 tiles");
   auto launch = [&](auto kernel, int lds_bytes, FhipOncePerDevice &configured) {
     if (!configured.done(ctx->device)) {
@@ -1497,22 +1502,25 @@ int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const v
         return fhip_fail(ctx, "sdpa: cannot reserve LDS");
       configured.mark(ctx->device);
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(kWaves * 64), lds_bytes, ctx->stream, g);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(cut == 2 ? kWaves * 32 : kWaves * 64), lds_bytes, ctx->stream, g);
     FHIP_HIP_CHECK(ctx, hipGetLastError());
     return 0;
   };
-  fhip_note_kernel(ctx, "sdpa_packed d=%d causal=%d%s", hd, (int)g.causal, split ? " split" : "");
-  static FhipOncePerDevice configured[2][2][4]; // one for each kernel instance
+  fhip_note_kernel(ctx, "sdpa_packed d=%d causal=%d%s", hd, (int)g.causal, cut == 2 ? " half" : cut ? " split" : "");
+  static FhipOncePerDevice configured[2][2][6]; // one for each kernel instance
   auto pick = [&](auto hdc, auto bf) {
     constexpr int HD = decltype(hdc)::value;
     constexpr bool BF = decltype(bf)::value;
     using C = SdShape<HD>;
-    FhipOncePerDevice(&cfg)[4] = configured[HD == 128][BF];
-    if (split)
-      return g.causal ? launch(sdpa_fwd_kernel<BF, true, HD, 0, true, true>, C::split_lds(false), cfg[0])
-                      : launch(sdpa_fwd_kernel<BF, false, HD, 0, true, true>, C::split_lds(false), cfg[1]);
-    return g.causal ? launch(sdpa_fwd_kernel<BF, true, HD, 0, false, true>, C::kLdsB, cfg[2])
-                    : launch(sdpa_fwd_kernel<BF, false, HD, 0, false, true>, C::kLdsB, cfg[3]);
+    FhipOncePerDevice(&cfg)[6] = configured[HD == 128][BF];
+    if (cut == 2)
+      return g.causal ? launch(sdpa_fwd_kernel<BF, true, HD, 0, false, 2>, C::split_lds(false) / 2, cfg[4])
+                      : launch(sdpa_fwd_kernel<BF, false, HD, 0, false, 2>, C::split_lds(false) / 2, cfg[5]);
+    if (cut)
+      return g.causal ? launch(sdpa_fwd_kernel<BF, true, HD, 0, true, 1>, C::split_lds(false), cfg[0])
+                      : launch(sdpa_fwd_kernel<BF, false, HD, 0, true, 1>, C::split_lds(false), cfg[1]);
+    return g.causal ? launch(sdpa_fwd_kernel<BF, true, HD, 0, false, 1>, C::kLdsB, cfg[2])
+                    : launch(sdpa_fwd_kernel<BF, false, HD, 0, false, 1>, C::kLdsB, cfg[3]);
   };
   auto typed = [&](auto hdc) {
     return d->q.dtype == FHIP_BFLOAT16 ? pick(hdc, std::true_type{}) : pick(hdc, std::false_type{});
