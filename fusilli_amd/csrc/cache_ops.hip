@@ -438,7 +438,7 @@ int lanes_of(int64_t D, int64_t Dv) {
   return most <= 64 ? 8 : most <= 128 ? 16 : most <= 256 ? 32 : 64;
 }
 
-// Ranges of memory that a tensor of non-negative strides spans.
+// Whether every element of both lies at the same offset.
 bool same_tensor(const fhip_tensor_desc &a, const fhip_tensor_desc &b) {
   for (int i = 0; i < a.rank; ++i)
     if (a.dim[i] > 1 && a.stride[i] != b.stride[i])

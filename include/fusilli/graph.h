@@ -528,6 +528,93 @@ public:
     return o;
   }
 
+  // ---- packed sequences and paged caches (no counterpart in the reference) ----
+  // Attention of packed sequences on each other; kvOffsets null: K and V are
+  // packed like Q.
+  std::shared_ptr<TensorAttr>
+  sdpaPacked(const TensorPtr &q, const TensorPtr &k, const TensorPtr &v,
+             const TensorPtr &offsets, const TensorPtr &kvOffsets,
+             SdpaPackedAttr &attr) {
+    nameNode(attr, "sdpa_packed");
+    nameTensor(q, attr, "Q");
+    nameTensor(k, attr, "K");
+    nameTensor(v, attr, "V");
+    nameTensor(offsets, attr, "OFFSETS");
+    nameTensor(kvOffsets, attr, "KV_OFFSETS");
+    attr.setQ(q).setK(k).setV(v).setOFFSETS(offsets);
+    if (kvOffsets)
+      attr.setKV_OFFSETS(kvOffsets);
+    auto o = outputTensor(attr.getName() + "_O");
+    attr.setO(o);
+    subNodes_.emplace_back(
+        std::make_shared<SdpaPackedNode>(std::move(attr), context));
+    return o;
+  }
+
+  // Attention of each sequence's newest rows over its keys in a cache.
+  std::shared_ptr<TensorAttr> sdpaPaged(const TensorPtr &q,
+                                        const TensorPtr &offsets,
+                                        const CacheTensors &cache,
+                                        SdpaPagedAttr &attr) {
+    nameNode(attr, "sdpa_paged");
+    nameTensor(q, attr, "Q");
+    nameCache(offsets, cache, attr);
+    attr.setQ(q);
+    attr.setOFFSETS(offsets);
+    attr.setCache(cache);
+    auto o = outputTensor(attr.getName() + "_O");
+    attr.setO(o);
+    subNodes_.emplace_back(
+        std::make_shared<SdpaPagedNode>(std::move(attr), context));
+    return o;
+  }
+
+  // Puts K and V into the cache, whose tensors' buffers are updated in place:
+  // nodes added after this one see the new rows.  Returns {Q_OUT, K_OUT}, the
+  // turned rows; Q_OUT is null without Q, and K_OUT costs nothing where it is
+  // neither an output nor read.  q, rotation and positions may be null.
+  std::array<std::shared_ptr<TensorAttr>, 2>
+  cacheAppend(const TensorPtr &q, const TensorPtr &k, const TensorPtr &v,
+              const TensorPtr &rotation, const TensorPtr &positions,
+              const TensorPtr &offsets, const CacheTensors &cache,
+              CacheAppendAttr &attr) {
+    nameNode(attr, "cache_append");
+    nameTensor(q, attr, "Q");
+    nameTensor(k, attr, "K");
+    nameTensor(v, attr, "V");
+    nameTensor(rotation, attr, "ROTATION");
+    nameTensor(positions, attr, "POSITIONS");
+    nameCache(offsets, cache, attr);
+    attr.setQ(q).setK(k).setV(v).setROTATION(rotation).setPOSITIONS(positions);
+    attr.setOFFSETS(offsets);
+    attr.setCache(cache);
+    auto ko = outputTensor(attr.getName() + "_K_OUT");
+    std::shared_ptr<TensorAttr> qo;
+    if (q)
+      qo = outputTensor(attr.getName() + "_Q_OUT");
+    attr.setQ_OUT(qo).setK_OUT(ko);
+    subNodes_.emplace_back(
+        std::make_shared<CacheAppendNode>(std::move(attr), context));
+    return {qo, ko};
+  }
+
+  // Brings rows of a cache back to packed {K, V}, whose dims the caller sets
+  // on the returned tensors.
+  std::array<std::shared_ptr<TensorAttr>, 2>
+  cacheRead(const TensorPtr &offsets, const CacheTensors &cache,
+            CacheReadAttr &attr) {
+    nameNode(attr, "cache_read");
+    nameCache(offsets, cache, attr);
+    attr.setOFFSETS(offsets);
+    attr.setCache(cache);
+    auto k = outputTensor(attr.getName() + "_K");
+    auto v = outputTensor(attr.getName() + "_V");
+    attr.setK(k).setV(v);
+    subNodes_.emplace_back(
+        std::make_shared<CacheReadNode>(std::move(attr), context));
+    return {k, v};
+  }
+
   // Returns {Y, INV_RMS}; INV_RMS is null outside the training phase.
   std::array<std::shared_ptr<TensorAttr>, 2>
   rmsnorm(const TensorPtr &x, const TensorPtr &scale, RmsnormAttr &attr) {
@@ -624,6 +711,18 @@ private:
                          const char *suffix) {
     if (t && t->getName().empty())
       t->setName(attr.getName() + "_" + suffix);
+  }
+
+  template <typename Attr>
+  static void nameCache(const TensorPtr &offsets, const CacheTensors &c,
+                        const Attr &attr) {
+    nameTensor(offsets, attr, "OFFSETS");
+    nameTensor(c.k, attr, "CACHE_K");
+    nameTensor(c.v, attr, "CACHE_V");
+    nameTensor(c.kParams, attr, "CACHE_K_PARAMS");
+    nameTensor(c.vParams, attr, "CACHE_V_PARAMS");
+    nameTensor(c.pages, attr, "PAGES");
+    nameTensor(c.lengths, attr, "LENGTHS");
   }
 
   std::shared_ptr<TensorAttr>

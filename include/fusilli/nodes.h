@@ -31,6 +31,10 @@ public:
     Reduction,
     Custom,
     Sdpa,
+    SdpaPacked,
+    SdpaPaged,
+    CacheAppend,
+    CacheRead,
   };
 
   explicit INode(const Context &ctx) : context(ctx) {}
@@ -829,6 +833,255 @@ private:
     const auto &qd = sdpaAttr.getQ()->getDim();
     return {qd[0], qd[1], qd[2], sdpaAttr.getV()->getDim()[3]};
   }
+};
+
+// ---- packed sequences and paged caches ----------------------------------------
+// (no counterpart in the reference; what the kernels need beyond these checks
+// the planner asks the backend)
+namespace serving_utils {
+inline ErrorObject checkRows(const TensorPtr &t, const std::string &op,
+                             const std::string &which) {
+  FUSILLI_RETURN_ERROR_IF(!t, ErrorCode::AttributeNotSet,
+                          op + " tensor " + which + " not set");
+  FUSILLI_RETURN_ERROR_IF(t->getDim().size() != 3, ErrorCode::InvalidAttribute,
+                          op + " tensor " + which +
+                              " must be rank 3 [rows, heads, head_dim]");
+  return ok();
+}
+// A dense Int32 tensor of the given dims.
+inline ErrorObject checkIndices(const TensorPtr &t, const std::string &op,
+                                const std::string &which,
+                                const std::vector<int64_t> &dim) {
+  FUSILLI_RETURN_ERROR_IF(!t, ErrorCode::AttributeNotSet,
+                          op + " tensor " + which + " not set");
+  std::string text;
+  for (int64_t d : dim)
+    text += (text.empty() ? "" : ", ") + std::to_string(d);
+  FUSILLI_RETURN_ERROR_IF(t->getDim() != dim || !t->isContiguous(),
+                          ErrorCode::InvalidAttribute,
+                          op + " tensor " + which + " must be contiguous [" +
+                              text + "]");
+  FUSILLI_RETURN_ERROR_IF(t->getDataType() != DataType::Int32,
+                          ErrorCode::InvalidAttribute,
+                          op + " tensor " + which + " must be Int32");
+  return ok();
+}
+inline ErrorObject checkCache(const CacheTensors &c, const std::string &op) {
+  FUSILLI_RETURN_ERROR_IF(!c.k || !c.v || !c.pages || !c.lengths,
+                          ErrorCode::AttributeNotSet,
+                          op + " cache tensors CACHE_K, CACHE_V, PAGES and "
+                               "LENGTHS must be set");
+  FUSILLI_RETURN_ERROR_IF(!c.kParams != !c.vParams, ErrorCode::AttributeNotSet,
+                          op + " cache parameters go together");
+  for (const TensorPtr &t : {c.k, c.v, c.kParams, c.vParams})
+    FUSILLI_RETURN_ERROR_IF(t && t->getDim().size() != 4,
+                            ErrorCode::InvalidAttribute,
+                            op + " cache tensor '" + t->getName() +
+                                "' must be rank 4 [pages, heads, page_size, "
+                                "head_dim]");
+  FUSILLI_RETURN_ERROR_IF(c.pages->getDim().size() != 2,
+                          ErrorCode::InvalidAttribute,
+                          op + " tensor PAGES must be rank 2 [batch, pages]");
+  return ok();
+}
+inline ErrorObject checkCacheIndices(const CacheTensors &c,
+                                     const TensorPtr &offsets,
+                                     const std::string &op) {
+  const int64_t batch = c.pages->getDim()[0];
+  FUSILLI_CHECK_ERROR(checkIndices(offsets, op, "OFFSETS", {batch + 1}));
+  FUSILLI_CHECK_ERROR(
+      checkIndices(c.pages, op, "PAGES", {batch, c.pages->getDim()[1]}));
+  return checkIndices(c.lengths, op, "LENGTHS", {batch});
+}
+inline ErrorObject checkHeads(int64_t hq, int64_t hk, const std::string &op) {
+  FUSILLI_RETURN_ERROR_IF(hq % hk != 0, ErrorCode::InvalidAttribute,
+                          op + " requires Q heads (" + std::to_string(hq) +
+                              ") to be a multiple of K heads (" +
+                              std::to_string(hk) + ")");
+  return ok();
+}
+inline void inferRows(const TensorPtr &t, const std::vector<int64_t> &dim) {
+  if (t->getDim().empty())
+    t->setDim(dim);
+  if (t->getStride().empty())
+    t->setStride(
+        generateStrideFromDim(t->getDim(), getContiguousStrideOrder(3)));
+}
+} // namespace serving_utils
+
+class SdpaPackedNode : public NodeCRTP<SdpaPackedNode> {
+public:
+  SdpaPackedAttr sdpaPackedAttr;
+  SdpaPackedNode(SdpaPackedAttr &&attr, const Context &ctx)
+      : NodeCRTP(ctx), sdpaPackedAttr(std::move(attr)) {}
+  const std::string &getName() const override final {
+    return sdpaPackedAttr.getName();
+  }
+  Type getType() const override final { return Type::SdpaPacked; }
+
+  ErrorObject preValidateNode() const override final {
+    const auto &a = sdpaPackedAttr;
+    FUSILLI_CHECK_ERROR(serving_utils::checkRows(a.getQ(), kOp, "Q"));
+    FUSILLI_CHECK_ERROR(serving_utils::checkRows(a.getK(), kOp, "K"));
+    FUSILLI_CHECK_ERROR(serving_utils::checkRows(a.getV(), kOp, "V"));
+    FUSILLI_RETURN_ERROR_IF(!a.getOFFSETS(), ErrorCode::AttributeNotSet,
+                            std::string(kOp) + " tensor OFFSETS not set");
+    FUSILLI_RETURN_ERROR_IF(a.getOFFSETS()->getDim().size() != 1 ||
+                                a.getOFFSETS()->getDim()[0] < 2,
+                            ErrorCode::InvalidAttribute,
+                            std::string(kOp) +
+                                " tensor OFFSETS must be [batch + 1]");
+    return serving_utils::checkHeads(a.getQ()->getDim()[1],
+                                     a.getK()->getDim()[1], kOp);
+  }
+  ErrorObject inferPropertiesNode() override final {
+    sdpaPackedAttr.fillFromContext(context);
+    serving_utils::inferRows(sdpaPackedAttr.getO(), expectedOutputDim());
+    return ok();
+  }
+  ErrorObject postValidateNode() const override final {
+    const auto &a = sdpaPackedAttr;
+    const std::vector<int64_t> dim = a.getOFFSETS()->getDim();
+    FUSILLI_CHECK_ERROR(
+        serving_utils::checkIndices(a.getOFFSETS(), kOp, "OFFSETS", dim));
+    if (a.getKV_OFFSETS())
+      FUSILLI_CHECK_ERROR(serving_utils::checkIndices(a.getKV_OFFSETS(), kOp,
+                                                      "KV_OFFSETS", dim));
+    FUSILLI_RETURN_ERROR_IF(a.getO()->getDim() != expectedOutputDim(),
+                            ErrorCode::InvalidAttribute,
+                            std::string(kOp) +
+                                " output tensor O dimensions do not match "
+                                "expected shape [rows, headsQ, headDim]");
+    return ok();
+  }
+
+private:
+  static constexpr const char *kOp = "SDPA packed";
+  std::vector<int64_t> expectedOutputDim() const {
+    const auto &qd = sdpaPackedAttr.getQ()->getDim();
+    return {qd[0], qd[1], sdpaPackedAttr.getV()->getDim()[2]};
+  }
+};
+
+class SdpaPagedNode : public NodeCRTP<SdpaPagedNode> {
+public:
+  SdpaPagedAttr sdpaPagedAttr;
+  SdpaPagedNode(SdpaPagedAttr &&attr, const Context &ctx)
+      : NodeCRTP(ctx), sdpaPagedAttr(std::move(attr)) {}
+  const std::string &getName() const override final {
+    return sdpaPagedAttr.getName();
+  }
+  Type getType() const override final { return Type::SdpaPaged; }
+
+  ErrorObject preValidateNode() const override final {
+    const auto &a = sdpaPagedAttr;
+    FUSILLI_CHECK_ERROR(serving_utils::checkRows(a.getQ(), kOp, "Q"));
+    FUSILLI_CHECK_ERROR(serving_utils::checkCache(a.getCache(), kOp));
+    return serving_utils::checkHeads(a.getQ()->getDim()[1],
+                                     a.getCACHE_K()->getDim()[1], kOp);
+  }
+  ErrorObject inferPropertiesNode() override final {
+    sdpaPagedAttr.fillFromContext(context);
+    serving_utils::inferRows(sdpaPagedAttr.getO(), expectedOutputDim());
+    return ok();
+  }
+  ErrorObject postValidateNode() const override final {
+    const auto &a = sdpaPagedAttr;
+    FUSILLI_CHECK_ERROR(
+        serving_utils::checkCacheIndices(a.getCache(), a.getOFFSETS(), kOp));
+    FUSILLI_RETURN_ERROR_IF(a.getO()->getDim() != expectedOutputDim(),
+                            ErrorCode::InvalidAttribute,
+                            std::string(kOp) +
+                                " output tensor O dimensions do not match "
+                                "expected shape [rows, headsQ, headDim]");
+    return ok();
+  }
+
+private:
+  static constexpr const char *kOp = "SDPA paged";
+  std::vector<int64_t> expectedOutputDim() const {
+    const auto &qd = sdpaPagedAttr.getQ()->getDim();
+    const int64_t dv = sdpaPagedAttr.getCACHE_V()->getDim()[3];
+    return {qd[0], qd[1], sdpaPagedAttr.getCACHE_V_PARAMS() ? 2 * dv : dv};
+  }
+};
+
+class CacheAppendNode : public NodeCRTP<CacheAppendNode> {
+public:
+  CacheAppendAttr cacheAppendAttr;
+  CacheAppendNode(CacheAppendAttr &&attr, const Context &ctx)
+      : NodeCRTP(ctx), cacheAppendAttr(std::move(attr)) {}
+  const std::string &getName() const override final {
+    return cacheAppendAttr.getName();
+  }
+  Type getType() const override final { return Type::CacheAppend; }
+
+  ErrorObject preValidateNode() const override final {
+    const auto &a = cacheAppendAttr;
+    FUSILLI_CHECK_ERROR(serving_utils::checkRows(a.getK(), kOp, "K"));
+    FUSILLI_CHECK_ERROR(serving_utils::checkRows(a.getV(), kOp, "V"));
+    if (a.getQ())
+      FUSILLI_CHECK_ERROR(serving_utils::checkRows(a.getQ(), kOp, "Q"));
+    FUSILLI_RETURN_ERROR_IF(a.getROTATION() &&
+                                a.getROTATION()->getDim().size() != 2,
+                            ErrorCode::InvalidAttribute,
+                            std::string(kOp) + " tensor ROTATION must be rank "
+                                               "2 [positions, dims]");
+    return serving_utils::checkCache(a.getCache(), kOp);
+  }
+  ErrorObject inferPropertiesNode() override final {
+    cacheAppendAttr.fillFromContext(context);
+    serving_utils::inferRows(cacheAppendAttr.getK_OUT(),
+                             cacheAppendAttr.getK()->getDim());
+    if (cacheAppendAttr.getQ())
+      serving_utils::inferRows(cacheAppendAttr.getQ_OUT(),
+                               cacheAppendAttr.getQ()->getDim());
+    return ok();
+  }
+  ErrorObject postValidateNode() const override final {
+    const auto &a = cacheAppendAttr;
+    FUSILLI_CHECK_ERROR(
+        serving_utils::checkCacheIndices(a.getCache(), a.getOFFSETS(), kOp));
+    if (a.getPOSITIONS())
+      FUSILLI_CHECK_ERROR(serving_utils::checkIndices(
+          a.getPOSITIONS(), kOp, "POSITIONS", {a.getK()->getDim()[0]}));
+    return ok();
+  }
+
+private:
+  static constexpr const char *kOp = "Cache append";
+};
+
+class CacheReadNode : public NodeCRTP<CacheReadNode> {
+public:
+  CacheReadAttr cacheReadAttr;
+  CacheReadNode(CacheReadAttr &&attr, const Context &ctx)
+      : NodeCRTP(ctx), cacheReadAttr(std::move(attr)) {}
+  const std::string &getName() const override final {
+    return cacheReadAttr.getName();
+  }
+  Type getType() const override final { return Type::CacheRead; }
+
+  ErrorObject preValidateNode() const override final {
+    const auto &a = cacheReadAttr;
+    FUSILLI_CHECK_ERROR(serving_utils::checkCache(a.getCache(), kOp));
+    // how many rows there are the offsets say on the device only
+    FUSILLI_CHECK_ERROR(serving_utils::checkRows(a.getK(), kOp, "K"));
+    return serving_utils::checkRows(a.getV(), kOp, "V");
+  }
+  ErrorObject inferPropertiesNode() override final {
+    cacheReadAttr.fillFromContext(context);
+    serving_utils::inferRows(cacheReadAttr.getK(), {});
+    serving_utils::inferRows(cacheReadAttr.getV(), {});
+    return ok();
+  }
+  ErrorObject postValidateNode() const override final {
+    return serving_utils::checkCacheIndices(
+        cacheReadAttr.getCache(), cacheReadAttr.getOFFSETS(), kOp);
+  }
+
+private:
+  static constexpr const char *kOp = "Cache read";
 };
 
 // ---- norms ------------------------------------------------------------------

@@ -404,6 +404,155 @@ private:
   bool enableGqa_ = false;
 };
 
+// ---- packed sequences and paged caches (no counterpart in the reference) ------
+// Rows of all sequences lie packed in [rows, heads, head dim]; OFFSETS (Int32,
+// batch + 1) says where each sequence's are.  fusilli_hip.h has the layouts.
+class SdpaPackedAttr : public AttributesCRTP<SdpaPackedAttr> {
+public:
+  enum class InputNames : uint8_t { Q, K, V, OFFSETS, KV_OFFSETS };
+  enum class OutputNames : uint8_t { O };
+  FUSILLI_SLOT_MAPS
+  FUSILLI_IN_SLOT(SdpaPackedAttr, Q)
+  FUSILLI_IN_SLOT(SdpaPackedAttr, K)
+  FUSILLI_IN_SLOT(SdpaPackedAttr, V)
+  FUSILLI_IN_SLOT(SdpaPackedAttr, OFFSETS)
+  FUSILLI_IN_SLOT(SdpaPackedAttr, KV_OFFSETS)
+  FUSILLI_OUT_SLOT(SdpaPackedAttr, O)
+
+  SdpaPackedAttr &setIsCausal(bool v) {
+    isCausal_ = v;
+    return *this;
+  }
+  SdpaPackedAttr &setScale(std::optional<float> s) {
+    scale_ = s;
+    return *this;
+  }
+  bool getIsCausal() const { return isCausal_; }
+  std::optional<float> getScale() const { return scale_; }
+
+private:
+  bool isCausal_ = false;
+  std::optional<float> scale_;
+};
+
+// The tensors of a key / value cache: pools, with 4 bits their parameters
+// (null otherwise), the page table (Int32 [batch, pages of a sequence]) and each
+// sequence's length (Int32 [batch]).
+struct CacheTensors {
+  TensorPtr k, v, kParams, vParams, pages, lengths;
+};
+
+// Slots that every operation on a cache has.
+#define FUSILLI_CACHE_SLOTS(CLASS)                                             \
+  FUSILLI_IN_SLOT(CLASS, OFFSETS)                                              \
+  FUSILLI_IN_SLOT(CLASS, CACHE_K)                                              \
+  FUSILLI_IN_SLOT(CLASS, CACHE_V)                                              \
+  FUSILLI_IN_SLOT(CLASS, CACHE_K_PARAMS)                                       \
+  FUSILLI_IN_SLOT(CLASS, CACHE_V_PARAMS)                                       \
+  FUSILLI_IN_SLOT(CLASS, PAGES)                                                \
+  FUSILLI_IN_SLOT(CLASS, LENGTHS)                                              \
+  CLASS &setCache(const CacheTensors &c) {                                     \
+    return setCACHE_K(c.k)                                                     \
+        .setCACHE_V(c.v)                                                       \
+        .setCACHE_K_PARAMS(c.kParams)                                          \
+        .setCACHE_V_PARAMS(c.vParams)                                          \
+        .setPAGES(c.pages)                                                     \
+        .setLENGTHS(c.lengths);                                                \
+  }                                                                            \
+  CacheTensors getCache() const {                                              \
+    return {getCACHE_K(),        getCACHE_V(), getCACHE_K_PARAMS(),            \
+            getCACHE_V_PARAMS(), getPAGES(),   getLENGTHS()};                  \
+  }
+
+class SdpaPagedAttr : public AttributesCRTP<SdpaPagedAttr> {
+public:
+  enum class InputNames : uint8_t {
+    Q,
+    OFFSETS,
+    CACHE_K,
+    CACHE_V,
+    CACHE_K_PARAMS,
+    CACHE_V_PARAMS,
+    PAGES,
+    LENGTHS
+  };
+  enum class OutputNames : uint8_t { O };
+  FUSILLI_SLOT_MAPS
+  FUSILLI_IN_SLOT(SdpaPagedAttr, Q)
+  FUSILLI_CACHE_SLOTS(SdpaPagedAttr)
+  FUSILLI_OUT_SLOT(SdpaPagedAttr, O)
+
+  SdpaPagedAttr &setIsCausal(bool v) {
+    isCausal_ = v;
+    return *this;
+  }
+  SdpaPagedAttr &setScale(std::optional<float> s) {
+    scale_ = s;
+    return *this;
+  }
+  bool getIsCausal() const { return isCausal_; }
+  std::optional<float> getScale() const { return scale_; }
+
+private:
+  bool isCausal_ = true;
+  std::optional<float> scale_;
+};
+
+class CacheAppendAttr : public AttributesCRTP<CacheAppendAttr> {
+public:
+  enum class InputNames : uint8_t {
+    Q,
+    K,
+    V,
+    ROTATION,
+    POSITIONS,
+    OFFSETS,
+    CACHE_K,
+    CACHE_V,
+    CACHE_K_PARAMS,
+    CACHE_V_PARAMS,
+    PAGES,
+    LENGTHS
+  };
+  enum class OutputNames : uint8_t { Q_OUT, K_OUT };
+  FUSILLI_SLOT_MAPS
+  FUSILLI_IN_SLOT(CacheAppendAttr, Q)
+  FUSILLI_IN_SLOT(CacheAppendAttr, K)
+  FUSILLI_IN_SLOT(CacheAppendAttr, V)
+  FUSILLI_IN_SLOT(CacheAppendAttr, ROTATION)
+  FUSILLI_IN_SLOT(CacheAppendAttr, POSITIONS)
+  FUSILLI_CACHE_SLOTS(CacheAppendAttr)
+  FUSILLI_OUT_SLOT(CacheAppendAttr, Q_OUT)
+  FUSILLI_OUT_SLOT(CacheAppendAttr, K_OUT)
+
+  CacheAppendAttr &setInterleaved(bool v) {
+    interleaved_ = v;
+    return *this;
+  }
+  bool getInterleaved() const { return interleaved_; }
+
+private:
+  bool interleaved_ = false;
+};
+
+class CacheReadAttr : public AttributesCRTP<CacheReadAttr> {
+public:
+  enum class InputNames : uint8_t {
+    OFFSETS,
+    CACHE_K,
+    CACHE_V,
+    CACHE_K_PARAMS,
+    CACHE_V_PARAMS,
+    PAGES,
+    LENGTHS
+  };
+  enum class OutputNames : uint8_t { K, V };
+  FUSILLI_SLOT_MAPS
+  FUSILLI_CACHE_SLOTS(CacheReadAttr)
+  FUSILLI_OUT_SLOT(CacheReadAttr, K)
+  FUSILLI_OUT_SLOT(CacheReadAttr, V)
+};
+
 // ---- RMSNorm (attributes/rmsnorm_attributes.h) ------------------------------
 class RmsnormAttr : public AttributesCRTP<RmsnormAttr> {
 public:

@@ -42,6 +42,10 @@ enum class StepKind : uint32_t {
   ConvDGrad = 7,
   ConvWGrad = 8,
   BatchNorm = 9,
+  SdpaPacked = 10,
+  SdpaPaged = 11,
+  CacheAppend = 12,
+  CacheRead = 13,
 };
 
 constexpr int kMaxSlots = 12;
@@ -53,6 +57,12 @@ inline int32_t workspaceSlot(size_t index) {
   return -static_cast<int32_t>(index) - 2;
 }
 
+// (an append has more tensors than a step has slots)
+struct CacheAppendStep {
+  fhip_cache_append_desc d;
+  int32_t qOut, kOut; // slots
+};
+
 union StepDesc {
   fhip_matmul_desc matmul;
   fhip_conv_desc conv;
@@ -61,7 +71,13 @@ union StepDesc {
   fhip_reduce_desc reduce;
   fhip_pointwise_desc pointwise;
   fhip_batchnorm_desc batchnorm;
+  fhip_sdpa_packed_desc sdpaPacked;
+  fhip_sdpa_paged_desc sdpaPaged;
+  CacheAppendStep cacheAppend;
+  fhip_cache_read_desc cacheRead;
 };
+// A step's size is part of a saved plan's format.
+static_assert(sizeof(StepDesc) == sizeof(fhip_norm_desc));
 
 struct Step {
   uint32_t kind = 0;
@@ -104,6 +120,34 @@ enum : int {
   kBnY = 5,
   kBnSavedMean = 6,
   kBnSavedInvVar = 7
+};
+enum : int {
+  kSpQ = 0,
+  kSpK = 1,
+  kSpV = 2,
+  kSpOffsets = 3,
+  kSpKvOffsets = 4,
+  kSpO = 5,
+  kSpScratch = 6
+};
+enum : int { // the cache of the three operations on one: from kCa
+  kCaK = 0,
+  kCaV = 1,
+  kCaKParams = 2,
+  kCaVParams = 3,
+  kCaPages = 4,
+  kCaLengths = 5,
+  kCaOffsets = 6,
+  kSgQ = 7,
+  kSgO = 8,
+  kSgScratch = 9,
+  kAppQ = 7,
+  kAppK = 8,
+  kAppV = 9,
+  kAppRotation = 10,
+  kAppPositions = 11,
+  kReadK = 7,
+  kReadV = 8
 };
 enum : int { kRdX = 0, kRdY = 1 };
 enum : int { kPwIn0 = 0, kPwIn1 = 1, kPwIn2 = 2, kPwOut = 3 };
@@ -310,6 +354,22 @@ public:
         FUSILLI_CHECK_ERROR(planSdpa(i));
         ++i;
         break;
+      case INode::Type::SdpaPacked:
+        FUSILLI_CHECK_ERROR(planSdpaPacked(i));
+        ++i;
+        break;
+      case INode::Type::SdpaPaged:
+        FUSILLI_CHECK_ERROR(planSdpaPaged(i));
+        ++i;
+        break;
+      case INode::Type::CacheAppend:
+        FUSILLI_CHECK_ERROR(planCacheAppend(i));
+        ++i;
+        break;
+      case INode::Type::CacheRead:
+        FUSILLI_CHECK_ERROR(planCacheRead(i));
+        ++i;
+        break;
       case INode::Type::Reduction:
         FUSILLI_CHECK_ERROR(planReduction(i));
         ++i;
@@ -370,6 +430,18 @@ private:
       break;
     case INode::Type::Sdpa:
       each(static_cast<const SdpaNode &>(n).sdpaAttr);
+      break;
+    case INode::Type::SdpaPacked:
+      each(static_cast<const SdpaPackedNode &>(n).sdpaPackedAttr);
+      break;
+    case INode::Type::SdpaPaged:
+      each(static_cast<const SdpaPagedNode &>(n).sdpaPagedAttr);
+      break;
+    case INode::Type::CacheAppend:
+      each(static_cast<const CacheAppendNode &>(n).cacheAppendAttr);
+      break;
+    case INode::Type::CacheRead:
+      each(static_cast<const CacheReadNode &>(n).cacheReadAttr);
       break;
     case INode::Type::RmsNorm:
       each(static_cast<const RmsNormNode &>(n).rmsnormAttr);
@@ -703,6 +775,174 @@ private:
     return ok();
   }
 
+  // -- packed sequences and paged caches ------------------------------------------
+  // A workspace region of a step's own.
+  int32_t scratchSlot(size_t bytes) {
+    if (bytes == 0)
+      return kNoTensor;
+    WorkspaceTensor t;
+    t.offset = workspaceCursor_;
+    t.bytes = bytes;
+    workspaceCursor_ += (t.bytes + 255) / 256 * 256;
+    plan_.workspaceTensors.push_back(t);
+    return workspaceSlot(plan_.workspaceTensors.size() - 1);
+  }
+  // `executable`: what the backend's query said.
+  static ErrorObject mustRun(bool executable, const std::string &what,
+                             const std::string &name) {
+    FUSILLI_RETURN_ERROR_IF(!executable, ErrorCode::NotImplemented,
+                            what + " node '" + name +
+                                "' is not executable by this backend: " +
+                                fhip_last_error(nullptr));
+    return ok();
+  }
+  template <typename Attr>
+  ErrorObject planCache(const Attr &attr, fhip_cache_desc &c, Step &s) {
+    const CacheTensors t = attr.getCache();
+    FUSILLI_ASSIGN_OR_RETURN(c.k, toDesc(t.k));
+    FUSILLI_ASSIGN_OR_RETURN(c.v, toDesc(t.v));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kCaK], readSlot(t.k));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kCaV], readSlot(t.v));
+    if (t.kParams) {
+      FUSILLI_ASSIGN_OR_RETURN(c.k_params, toDesc(t.kParams));
+      FUSILLI_ASSIGN_OR_RETURN(c.v_params, toDesc(t.vParams));
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kCaKParams], readSlot(t.kParams));
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kCaVParams], readSlot(t.vParams));
+    }
+    c.batch = t.pages->getDim()[0];
+    c.pages_per_sequence = c.page_stride = t.pages->getDim()[1];
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kCaPages], readSlot(t.pages));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kCaLengths], readSlot(t.lengths));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kCaOffsets], readSlot(attr.getOFFSETS()));
+    return ok();
+  }
+
+  ErrorObject planSdpaPacked(size_t i) {
+    const auto &attr =
+        static_cast<const SdpaPackedNode &>(*nodes_[i]).sdpaPackedAttr;
+    Step s;
+    s.kind = static_cast<uint32_t>(StepKind::SdpaPacked);
+    fhip_sdpa_packed_desc &d = s.desc.sdpaPacked;
+    FUSILLI_ASSIGN_OR_RETURN(d.q, toDesc(attr.getQ()));
+    FUSILLI_ASSIGN_OR_RETURN(d.k, toDesc(attr.getK()));
+    FUSILLI_ASSIGN_OR_RETURN(d.v, toDesc(attr.getV()));
+    FUSILLI_ASSIGN_OR_RETURN(d.o, toDesc(attr.getO()));
+    d.batch = attr.getOFFSETS()->getDim()[0] - 1;
+    d.has_kv_offsets = attr.getKV_OFFSETS() ? 1 : 0;
+    d.is_causal = attr.getIsCausal() ? 1 : 0;
+    d.has_scale = attr.getScale().has_value() ? 1 : 0;
+    d.scale = attr.getScale().value_or(0.0f);
+    FUSILLI_CHECK_ERROR(mustRun(fhip_sdpa_packed_fwd_supported(&d) != 0,
+                                "SDPA packed", attr.getName()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSpQ], readSlot(attr.getQ()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSpK], readSlot(attr.getK()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSpV], readSlot(attr.getV()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSpOffsets], readSlot(attr.getOFFSETS()));
+    if (attr.getKV_OFFSETS()) {
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kSpKvOffsets],
+                               readSlot(attr.getKV_OFFSETS()));
+    }
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSpO], writeSlot(attr.getO()));
+    size_t scratch = 0;
+    FUSILLI_RETURN_ERROR_IF(
+        fhip_sdpa_packed_fwd_workspace_size(&d, &scratch) != 0,
+        ErrorCode::InternalError, std::string(fhip_last_error(nullptr)));
+    s.slot[kSpScratch] = scratchSlot(scratch);
+    plan_.steps.push_back(s);
+    return ok();
+  }
+
+  ErrorObject planSdpaPaged(size_t i) {
+    const auto &attr =
+        static_cast<const SdpaPagedNode &>(*nodes_[i]).sdpaPagedAttr;
+    Step s;
+    s.kind = static_cast<uint32_t>(StepKind::SdpaPaged);
+    fhip_sdpa_paged_desc &d = s.desc.sdpaPaged;
+    FUSILLI_ASSIGN_OR_RETURN(d.q, toDesc(attr.getQ()));
+    FUSILLI_ASSIGN_OR_RETURN(d.o, toDesc(attr.getO()));
+    FUSILLI_CHECK_ERROR(planCache(attr, d.cache, s));
+    d.is_causal = attr.getIsCausal() ? 1 : 0;
+    d.has_scale = attr.getScale().has_value() ? 1 : 0;
+    d.scale = attr.getScale().value_or(0.0f);
+    FUSILLI_CHECK_ERROR(mustRun(fhip_sdpa_paged_fwd_supported(&d) != 0,
+                                "SDPA paged", attr.getName()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSgQ], readSlot(attr.getQ()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSgO], writeSlot(attr.getO()));
+    size_t scratch = 0;
+    FUSILLI_RETURN_ERROR_IF(
+        fhip_sdpa_paged_fwd_workspace_size(&d, &scratch) != 0,
+        ErrorCode::InternalError, std::string(fhip_last_error(nullptr)));
+    s.slot[kSgScratch] = scratchSlot(scratch);
+    plan_.steps.push_back(s);
+    return ok();
+  }
+
+  ErrorObject planCacheAppend(size_t i) {
+    const auto &attr =
+        static_cast<const CacheAppendNode &>(*nodes_[i]).cacheAppendAttr;
+    Step s;
+    s.kind = static_cast<uint32_t>(StepKind::CacheAppend);
+    fhip_cache_append_desc &d = s.desc.cacheAppend.d;
+    s.desc.cacheAppend.qOut = s.desc.cacheAppend.kOut = kNoTensor;
+    FUSILLI_ASSIGN_OR_RETURN(d.k, toDesc(attr.getK()));
+    FUSILLI_ASSIGN_OR_RETURN(d.v, toDesc(attr.getV()));
+    if (attr.getQ()) {
+      FUSILLI_ASSIGN_OR_RETURN(d.q, toDesc(attr.getQ()));
+      FUSILLI_ASSIGN_OR_RETURN(d.q_out, toDesc(attr.getQ_OUT()));
+    }
+    // (a virtual K_OUT that no node reads is not written)
+    const TensorPtr kOut = attr.getK_OUT();
+    const bool wanted = !kOut->isVirtual() || consumers_.count(kOut.get()) > 0;
+    if (wanted) {
+      FUSILLI_ASSIGN_OR_RETURN(d.k_out, toDesc(kOut));
+    }
+    if (attr.getROTATION()) {
+      FUSILLI_ASSIGN_OR_RETURN(d.rotation, toDesc(attr.getROTATION()));
+    }
+    FUSILLI_CHECK_ERROR(planCache(attr, d.cache, s));
+    d.has_positions = attr.getPOSITIONS() ? 1 : 0;
+    d.interleaved = attr.getInterleaved() ? 1 : 0;
+    FUSILLI_CHECK_ERROR(mustRun(fhip_cache_append_supported(&d) != 0,
+                                "Cache append", attr.getName()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kAppK], readSlot(attr.getK()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kAppV], readSlot(attr.getV()));
+    if (attr.getROTATION()) {
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kAppRotation],
+                               readSlot(attr.getROTATION()));
+    }
+    if (attr.getPOSITIONS()) {
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kAppPositions],
+                               readSlot(attr.getPOSITIONS()));
+    }
+    if (attr.getQ()) {
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kAppQ], readSlot(attr.getQ()));
+      FUSILLI_ASSIGN_OR_RETURN(s.desc.cacheAppend.qOut,
+                               writeSlot(attr.getQ_OUT()));
+    }
+    if (wanted) {
+      FUSILLI_ASSIGN_OR_RETURN(s.desc.cacheAppend.kOut, writeSlot(kOut));
+    }
+    plan_.steps.push_back(s);
+    return ok();
+  }
+
+  ErrorObject planCacheRead(size_t i) {
+    const auto &attr =
+        static_cast<const CacheReadNode &>(*nodes_[i]).cacheReadAttr;
+    Step s;
+    s.kind = static_cast<uint32_t>(StepKind::CacheRead);
+    fhip_cache_read_desc &d = s.desc.cacheRead;
+    FUSILLI_ASSIGN_OR_RETURN(d.k, toDesc(attr.getK()));
+    FUSILLI_ASSIGN_OR_RETURN(d.v, toDesc(attr.getV()));
+    FUSILLI_CHECK_ERROR(planCache(attr, d.cache, s));
+    FUSILLI_CHECK_ERROR(mustRun(fhip_cache_read_supported(&d) != 0,
+                                "Cache read", attr.getName()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kReadK], writeSlot(attr.getK()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kReadV], writeSlot(attr.getV()));
+    plan_.steps.push_back(s);
+    return ok();
+  }
+
   ErrorObject planReduction(size_t i) {
     const auto &attr =
         static_cast<const ReductionNode &>(*nodes_[i]).reductionAttr;
@@ -917,6 +1157,11 @@ inline ErrorObject execute(fhip_ctx *ctx, const Plan &p,
                ? p.workspaceTensors[static_cast<size_t>(-slot - 2)].bytes
                : 0;
   };
+  auto cacheOf = [&](const Step &s) {
+    return fhip_cache_ptrs{ptr(s.slot[kCaK]),       ptr(s.slot[kCaV]),
+                           ptr(s.slot[kCaKParams]), ptr(s.slot[kCaVParams]),
+                           ptr(s.slot[kCaPages]),   ptr(s.slot[kCaLengths])};
+  };
   for (const Step &s : p.steps) {
     int rc = 0;
     const void *epi[FHIP_MAX_EPILOGUE] = {nullptr, nullptr, nullptr, nullptr};
@@ -964,6 +1209,38 @@ inline ErrorObject execute(fhip_ctx *ctx, const Plan &p,
                          ptr(s.slot[kNmOut]), ptr(s.slot[kNmMean]),
                          ptr(s.slot[kNmRstd]), nullptr, 0);
       break;
+    case StepKind::SdpaPacked:
+      rc = fhip_sdpa_packed_fwd(
+          ctx, &s.desc.sdpaPacked, ptr(s.slot[kSpQ]), ptr(s.slot[kSpK]),
+          ptr(s.slot[kSpV]), ptr(s.slot[kSpOffsets]),
+          ptr(s.slot[kSpKvOffsets]), ptr(s.slot[kSpO]),
+          ptr(s.slot[kSpScratch]), bytesOf(s.slot[kSpScratch]));
+      break;
+    case StepKind::SdpaPaged: {
+      const fhip_cache_ptrs cache = cacheOf(s);
+      rc = fhip_sdpa_paged_fwd(ctx, &s.desc.sdpaPaged, &cache,
+                               ptr(s.slot[kSgQ]), ptr(s.slot[kCaOffsets]),
+                               ptr(s.slot[kSgO]), ptr(s.slot[kSgScratch]),
+                               bytesOf(s.slot[kSgScratch]));
+      break;
+    }
+    case StepKind::CacheAppend: {
+      const fhip_cache_ptrs cache = cacheOf(s);
+      rc = fhip_cache_append(
+          ctx, &s.desc.cacheAppend.d, &cache, ptr(s.slot[kAppQ]),
+          ptr(s.slot[kAppK]), ptr(s.slot[kAppV]), ptr(s.slot[kAppRotation]),
+          ptr(s.slot[kCaOffsets]), ptr(s.slot[kAppPositions]),
+          ptr(s.desc.cacheAppend.qOut), ptr(s.desc.cacheAppend.kOut), nullptr,
+          0);
+      break;
+    }
+    case StepKind::CacheRead: {
+      const fhip_cache_ptrs cache = cacheOf(s);
+      rc = fhip_cache_read(ctx, &s.desc.cacheRead, &cache,
+                           ptr(s.slot[kCaOffsets]), ptr(s.slot[kReadK]),
+                           ptr(s.slot[kReadV]), nullptr, 0);
+      break;
+    }
     case StepKind::Reduce:
       rc = fhip_reduce(ctx, &s.desc.reduce, ptr(s.slot[kRdX]),
                        ptr(s.slot[kRdY]), nullptr, 0);

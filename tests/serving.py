@@ -2,6 +2,10 @@
 bits, and the bounds that their roundings allow."""
 from __future__ import annotations
 
+import os
+import subprocess
+import tempfile
+
 import numpy as np
 
 from fusilli_amd import capi
@@ -10,10 +14,6 @@ from helpers import HT
 
 # half a step of a type, relative to the value
 HALF_STEP = {capi.BFLOAT16: 2.0 ** -8, capi.HALF: 2.0 ** -11, capi.FLOAT: 2.0 ** -24}
-
-
-def rounded(x, dtype):
-    return np.asarray(oracle.dequantize(oracle.quantize(np.asarray(x), dtype), dtype), np.float64).reshape(np.shape(x))
 
 
 def starts(lens):
@@ -184,3 +184,15 @@ def check(got, ref, far, what=""):
     if bad.any():
         at = np.unravel_index(np.argmax(np.where(bad, np.nan_to_num(np.abs(got - ref) / far, nan=np.inf, posinf=1e30), -1)), got.shape)
         raise AssertionError(f"{what}: {bad.sum()} of {bad.size} outside, worst at {at}: {got[at]} for {ref[at]} +- {far[at]}")
+
+
+def cpp_binary(name, timeout, *only):
+    """Runs a graph-API test binary, whose cache files go to a directory of this run."""
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin", name)
+    with tempfile.TemporaryDirectory(prefix="fusilli_cache_") as where:
+        proc = subprocess.run([path, *only], capture_output=True, text=True, timeout=timeout,
+                              env=dict(os.environ, FUSILLI_CACHE_DIR=where))
+        left = [f for _, _, files in os.walk(where) for f in files]
+    assert proc.returncode == 0 and "cases, 0 failed checks" in proc.stdout, proc.stdout[-4000:] + proc.stderr[-2000:]
+    assert not left, left[:5]
+    return proc.stdout

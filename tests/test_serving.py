@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from fusilli_amd import capi
-from serving import from_groups, to_groups
+from serving import cpp_binary, from_groups, to_groups
 
 LIB = capi.load()
 
@@ -174,3 +174,8 @@ def test_the_formula_of_4_bits_keeps_within_half_a_scale():
     far = np.repeat(scale.astype(np.float64) * (0.5 + 15 * 2.0 ** -11) + np.abs(low.astype(np.float64)) * 2.0 ** -11, 32, -1)
     assert (np.abs(from_groups(code, scale, low) - x) <= far * (1 + 1e-5)).all()
     assert code.max() == 15 and code.min() == 0
+
+
+# -- the C++ graph API (tests/cpp/test_serving_api.cpp) -------------------------
+def test_graph_api_on_the_host():
+    cpp_binary("test_serving_api", 120, "host")

@@ -5,7 +5,8 @@ import pytest
 
 from fusilli_amd import capi
 from helpers import HT
-from serving import HALF_STEP, Cache, attend, check, rotation_table, starts, to_groups, turn, turn_bound
+from serving import (HALF_STEP, Cache, attend, check, cpp_binary, rotation_table, starts, to_groups, turn,
+                     turn_bound)
 
 pytestmark = pytest.mark.gpu
 SENTINEL = 77.0  # (exact in every type)
@@ -513,3 +514,8 @@ def test_a_conversation(ctx, group, d, dtype):
         got, _ = run_paged(ctx, cache, have, qo, at)
         check_paged(cache, have, qo, at, got)
     assert have == final
+
+
+def test_graph_api():
+    """Graphs that append and attend: a prompt, a chunk behind it, single tokens."""
+    cpp_binary("test_serving_api", 120)
