@@ -93,6 +93,7 @@ struct FhipKnobs {
   int wgrad_direct = -1;            // FUSILLI_HIP_WGRAD_DIRECT (-1: unset, 0: off)
   int sdpa_decode = -1;             // FUSILLI_HIP_SDPA_DECODE (-1: unset, 0: off, 1: wherever it can run)
   int sdpa_split = -1;              // FUSILLI_HIP_SDPA_SPLIT, of the tiled kernel (the same)
+  int sdpa_packed = -1;             // FUSILLI_HIP_SDPA_PACKED: teams of a packed tile on rows of their own (0), on the same (1), one (2)
   int dgrad_rf = -1;                // FUSILLI_HIP_DGRAD_ROWS (-1: unset, 0: off, n: rows per
                                     // tile, + 100 x column tiles per row of tiles)
 };

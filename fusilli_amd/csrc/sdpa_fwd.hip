@@ -933,9 +933,11 @@ __global__ __launch_bounds__(PACKED == 2 ? kWaves * 32 : kWaves * 64, 2) void sd
       }
       const bool edge = (CAUSAL && kv0 + kBKV - 1 > wave_first) || kv0 + kBKV > Skv;
       if (edge) {
-        // (masked kernels use -inf: a row may see dead keys before its first
-        // live one, and exp2(-inf - reference) is 0 whatever the reference)
-        const float gone = MASK ? -INFINITY : kNegBig;
+        // (-inf where a row may see dead keys before its first live one: with a
+        // mask, and packed, where a team's first tile may be one that only some
+        // rows of a wavefront reach; exp2(-inf - reference) is 0 whatever the
+        // reference, kNegBig against itself leaves its product's rounding, of 1e22)
+        const float gone = MASK || PACKED ? -INFINITY : kNegBig;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -1491,7 +1493,8 @@ int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const v
   // heads on 8, D128 120.5 us whole (0), so 94.5; 64 of 512 296 / 257; 4 of 2048 155.3 / 155.4; 8192 tokens 459 / 479: whole
   // from 4096 keys.  Few tiles of long sequences: both teams on the same rows (1), 1024 tokens 25.9 / 22.7, 2048 50.6 / 51.8.
   const int64_t halves = g.Hkv * (rows / (kBQ / 2) + seqs / 2), keys = g.Tk / seqs;
-  const int cut = halves <= 256 && keys >= 512 ? 1 : hd == 128 && keys >= 4096 ? 0 : 2;
+  const int forced = fhip_knobs().sdpa_packed;
+  const int cut = forced >= 0 && forced <= 2 ? forced : halves <= 256 && keys >= 512 ? 1 : hd == 128 && keys >= 4096 ? 0 : 2;
   // tiles of all sequences, each one's last short
   const int64_t tiles = g.Hkv * (rows / (cut ? kBQ / 2 : kBQ) + seqs);
   FHIP_REQUIRE(ctx, tiles < (1ll << 31), "fhip_sdpa_packed_fwd: more than 2^31 tiles");

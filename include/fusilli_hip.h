@@ -396,9 +396,12 @@ typedef struct {
  * kv_offsets[b + 1] - 1 of K and V, such as a prefix read back from a cache and
  * the rows themselves.  is_causal: row i of n sees the first m - n + i + 1 of m
  * keys (the last row sees all).  A row that sees no key is 0.  Heads are
- * grouped like fhip_sdpa_fwd's.  supported: 2 for bf16 / f16, D = Dv = 64 or
- * 128, positive scale, rows (heads, and tensors at the call) on 16 bytes and below
- * 2 GiB per K or V tensor; 1 for other sizes to 512 and f32. */
+ * grouped like fhip_sdpa_fwd's.  A key that some rows of a sequence may not see
+ * takes part in theirs with probability 0: 0 times an infinite or NaN value
+ * shows; other sequences' keys and values never do.  supported: 2 for bf16 / f16,
+ * D = Dv = 64 or 128, positive scale, rows (heads, and tensors at the call) on 16
+ * bytes, below 2 GiB per K or V tensor and T (Hq / Hkv)^2 below 2^32; 1 for other
+ * sizes to 512 and f32. */
 typedef struct {
   fhip_tensor_desc q; /* [T, Hq, D] */
   fhip_tensor_desc k; /* [Tk, Hkv, D]; Tk = T without kv_offsets */
@@ -422,11 +425,13 @@ int fhip_sdpa_packed_fwd(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d,
 /* Attention of each sequence's newest rows over its keys in a cache: single
  * tokens, drafts of several, chunks of a prompt.  is_causal: row i sees the
  * keys up to its own place; otherwise every row sees lengths[b] keys.  A row
- * that sees no key is 0.  Needs 256-byte aligned workspace of
+ * that sees no key is 0; what lies behind lengths[b] never matters, a key that
+ * only later rows see matters as above.  Needs 256-byte aligned workspace of
  * fhip_sdpa_paged_fwd_workspace_size bytes (parts of long sequences; it holds
  * nothing between calls, and calls that overlap need one each).  supported: 2 for
- * bf16 / f16, D = Dv = 64 or 128, pages of a multiple of 16 rows, groups of 32, 64
- * or 128, rows and parameters aligned to 16 and 4 bytes; otherwise 1. */
+ * bf16 / f16, D = Dv = 64 or 128, positive scale, pages of a multiple of 16 rows,
+ * groups of 32, 64 or 128, rows and parameters aligned to 16 and 4 bytes;
+ * otherwise 1. */
 typedef struct {
   fhip_tensor_desc q; /* [T, Hq, D] */
   fhip_tensor_desc o; /* [T, Hq, Dv] */
