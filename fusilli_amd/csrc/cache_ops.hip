@@ -47,7 +47,7 @@ __device__ void store_row(const FhipCacheView &c, const FhipPool &p, int page, i
       number &= __builtin_fabsf(of[i]) < INFINITY;
     }
     const FhipGroup g = fhip_group_of(number ? lo : INFINITY, hi);
-    ((uint8_t *)p.data)[at + e / 2] = (uint8_t)(fhip_code_of(g, x[e]) | fhip_code_of(g, x[e + 1]) << 4);
+    ((uint8_t *)p.data)[at + e / 2] = (uint8_t)((uint32_t)fhip_code_of(g, x[e]) | (uint32_t)fhip_code_of(g, x[e + 1]) << 4);
     if (e % c.group == 0)
       pairs[e / c.group * 2] = g.scale, pairs[e / c.group * 2 + 1] = g.low;
   }
@@ -232,10 +232,7 @@ __device__ __forceinline__ void hold(const FhipCacheView &c, const FhipPool &p, 
   const int lanes = c.group / 8;
   lo = over_group<false>(lo, lanes), hi = over_group<true>(hi, lanes);
   const FhipGroup g = fhip_group_of(lo, hi);
-  uint32_t codes = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    codes |= fhip_code_of(g, y[i]) << (4 * i);
+  const uint32_t codes = fhip_codes_of(g, y);
   if (!in)
     return;
   *(uint32_t *)(p.data + page * p.page + h * p.head + slot * p.slot + at / 2) = codes;
@@ -291,7 +288,7 @@ template <bool BF16, int LANES, int N> __global__ __launch_bounds__(kThreads) vo
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      c[i] = v[i / 4][i % 4], s[i] = v[2 + i / 4][i % 4];
+      c[i] = v[i / 4][i % 4], s[i] = g.interleaved || second ? v[2 + i / 4][i % 4] : -v[2 + i / 4][i % 4];
   }
   void *out = which == 0 ? g.q_out : which == 1 ? g.k_out : nullptr;
   const int64_t *os = which == 0 ? g.qo_s : g.ko_s;
@@ -318,8 +315,8 @@ template <bool BF16, int LANES, int N> __global__ __launch_bounds__(kThreads) vo
           widen<BF16>(other[i], w);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float a = y[e] * c[e], b = w[e] * s[e];
-            z[e] = second ? a + b : a - b;
+            const float a = y[e] * c[e], b = w[e] * s[e]; // (the first element's sine has its sign)
+            z[e] = a + b;
           }
         }
         bits = narrow<BF16>(z);
@@ -327,7 +324,8 @@ template <bool BF16, int LANES, int N> __global__ __launch_bounds__(kThreads) vo
       if (!turned)
         bits = BF16 ? u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u}
                     : u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
-      widen<BF16>(bits, y);
+      if (which != 0)
+        widen<BF16>(bits, y);
     }
     if (out && mine && r.b >= 0)
       *(u32x4 *)((char *)out + (t * os[0] + (h0 + i) * os[1] + at) * 2) = bits;
@@ -342,46 +340,48 @@ template <bool BF16, int LANES, int N> __global__ __launch_bounds__(kThreads) vo
   const int t = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, at = l % LANES * 8;
   const bool in = t < g.T;
   const int slices = (g.Hkv + N - 1) / N;
-  const bool is_k = (int)blockIdx.y < slices;
-  const int h0 = ((int)blockIdx.y - (is_k ? 0 : slices)) * N, D = is_k ? g.D : g.Dv;
-  const FhipPool &p = is_k ? g.cache.k : g.cache.v;
   const RowPlace r = place_of<LANES>(g.cache, g.offsets, t, in);
   const int page = r.b >= 0 && r.place >= 0 && r.place < kCacheMaxKeys ? fhip_page_of(g.cache, r.b, (int)r.place) : -1;
   const int slot = page < 0 ? 0 : (int)((uint32_t)r.place % (uint32_t)g.cache.page_size);
-  const bool mine = in && at < D && r.b >= 0, load = mine && page >= 0;
-  const int64_t from = page < 0 ? 0 : page * p.page + slot * p.slot, pair = page < 0 ? 0 : page * p.params_page + slot * p.params_slot;
-  char *out = (char *)(is_k ? g.k : g.v) + (t * (is_k ? g.k_s[0] : g.v_s[0]) + at) * 2;
-  const int64_t out_h = is_k ? g.k_s[1] : g.v_s[1];
   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-  u32x4 bits[N];
-  h2 scale[N];
+  for (int slice = blockIdx.y; slice < 2 * slices; slice += gridDim.y) {
+    const bool is_k = slice < slices;
+    const int h0 = (slice - (is_k ? 0 : slices)) * N, D = is_k ? g.D : g.Dv;
+    const FhipPool &p = is_k ? g.cache.k : g.cache.v;
+    const bool mine = in && at < D && r.b >= 0, load = mine && page >= 0;
+    const int64_t from = page < 0 ? 0 : page * p.page + slot * p.slot, pair = page < 0 ? 0 : page * p.params_page + slot * p.params_slot;
+    char *out = (char *)(is_k ? g.k : g.v) + (t * (is_k ? g.k_s[0] : g.v_s[0]) + at) * 2;
+    const int64_t out_h = is_k ? g.k_s[1] : g.v_s[1];
+    u32x4 bits[N];
+    h2 scale[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    bits[i] = BF16 ? u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u}
-                   : u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
-    if (load && h0 + i < g.Hkv) {
-      const int64_t row = from + (h0 + i) * p.head;
-      if (g.cache.group) {
-        bits[i].x = *(const uint32_t *)(p.data + row + at / 2);
-        scale[i] = *(const h2 *)(p.params + pair + (h0 + i) * p.params_head + at / g.cache.group * 2);
-      } else {
-        bits[i] = *(const u32x4 *)(p.data + (row + at) * 2);
+    for (int i = 0; i < N; ++i) {
+      bits[i] = BF16 ? u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u}
+                     : u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+      if (load && h0 + i < g.Hkv) {
+        const int64_t row = from + (h0 + i) * p.head;
+        if (g.cache.group) {
+          bits[i].x = *(const uint32_t *)(p.data + row + at / 2);
+          scale[i] = *(const h2 *)(p.params + pair + (h0 + i) * p.params_head + at / g.cache.group * 2);
+        } else {
+          bits[i] = *(const u32x4 *)(p.data + (row + at) * 2);
+        }
       }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (g.cache.group && load) {
-      const uint32_t w = bits[i].x;
-      const float a = (float)scale[i].x, b = (float)scale[i].y;
-      float y[8];
+    for (int i = 0; i < N; ++i) {
+      if (g.cache.group && load) {
+        const uint32_t w = bits[i].x;
+        const float a = (float)scale[i].x, b = (float)scale[i].y;
+        float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        y[e] = b + a * (float)(w >> (4 * e) & 15); // (the product is exact)
-      bits[i] = narrow<BF16>(y);
+        for (int e = 0; e < 8; ++e)
+          y[e] = b + a * (float)(w >> (4 * e) & 15); // (the product is exact)
+        bits[i] = narrow<BF16>(y);
+      }
+      if (mine && h0 + i < g.Hkv)
+        *(u32x4 *)(out + (h0 + i) * out_h * 2) = bits[i];
     }
-    if (mine && h0 + i < g.Hkv)
-      *(u32x4 *)(out + (h0 + i) * out_h * 2) = bits[i];
   }
 }
 
@@ -694,11 +694,14 @@ int fhip_cache_read(fhip_ctx *ctx, const fhip_cache_read_desc *d, const fhip_cac
     const int64_t rows = kThreads / lanes, blocks = (g.T + rows - 1) / rows;
     const int n = blocks * 2 * ((g.Hkv + 3) / 4) >= 1024 ? 4 : 1;
     const int64_t slices = 2 * (int64_t)((g.Hkv + n - 1) / n);
+    // a workgroup takes slices in turn, each behind the one search for its rows' pages, where a thousand workgroups
+    // are left: 24560 rows of 8 heads out of 4 bits 33.6 us with one workgroup for all, 36.0 with two, 39.0 with four
+    const int64_t beside = blocks >= 1024 ? 1 : blocks * slices <= 1024 ? slices : (1024 + blocks - 1) / blocks;
     if (slices <= 65535) {
       fhip_note_kernel(ctx, "cache_read bits=%d lanes=%d heads=%d", d->cache.k_params.rank ? 4 : 16, lanes, n);
       return with_lanes(d->k.dtype == FHIP_BFLOAT16, lanes, n, [&](auto bf, auto lc, auto nc) {
         hipLaunchKernelGGL((read_kernel<decltype(bf)::value, decltype(lc)::value, decltype(nc)::value>),
-                           dim3((unsigned)blocks, (unsigned)slices), dim3(kThreads), 0, ctx->stream, g);
+                           dim3((unsigned)blocks, (unsigned)beside), dim3(kThreads), 0, ctx->stream, g);
         FHIP_HIP_CHECK(ctx, hipGetLastError());
         return 0;
       });

@@ -93,21 +93,40 @@ __device__ __forceinline__ FhipGroup fhip_group_of(float lo, float hi) {
   const float l = (float)g.low;
   float wide = hi - l;
   wide = wide < 0.f ? 0.f : wide;
-  g.scale = (_Float16)(wide / 15.0f);
+  // wide / 15, correctly rounded: the quotient by the rounded reciprocal is within a step, and the exact remainder
+  // times the reciprocal takes it the rest of the way (infinite: NaN, refused below like infinity)
+  const float q = wide * (1.0f / 15.0f);
+  float part = __builtin_fmaf(__builtin_fmaf(-15.0f, q, wide), 1.0f / 15.0f, q);
+  asm("" : "+v"(part)); // (or the compiler rounds the sum to half at once)
+  g.scale = (_Float16)part;
   const float s = (float)g.scale;
   if (!(__builtin_fabsf(l) < INFINITY) || !(s < INFINITY)) {
     g.scale = g.low = (_Float16)__builtin_nanf("");
     g.by = 0.f;
   } else {
-    g.by = s > 0.f ? 1.0f / s : 0.f;
+    // 1 / s, correctly rounded: one step from the hardware's reciprocal, a unit off at most, leaves 2^-46, and the
+    // reciprocal of an 11-bit number lies 2^-36 or more from where rounding changes (or is a power of two, exact)
+    const float r = __builtin_amdgcn_rcpf(s);
+    g.by = s > 0.f ? __builtin_fmaf(__builtin_fmaf(-s, r, 1.0f), r, r) : 0.f;
   }
   return g;
 }
-__device__ __forceinline__ uint32_t fhip_code_of(const FhipGroup &g, float x) {
+// The code of x as a float, 0 for a NaN.
+__device__ __forceinline__ float fhip_code_of(const FhipGroup &g, float x) {
 #pragma clang fp contract(off)
-  const float c = __builtin_rintf((x - (float)g.low) * g.by);
-  // (a NaN's code is 0)
-  return (uint32_t)(c > 0.f ? (c < 15.f ? c : 15.f) : 0.f);
+  return __builtin_rintf(fminf(fmaxf((x - (float)g.low) * g.by, 0.f), 15.f));
+}
+// 8 codes of a word, the first in its lowest bits.  Added to 1.5 * 2^23 a number below 2^22 is rounded to an
+// integer, half to even, which lies in the sum's lowest bits; the rest is the same in every sum and comes off at the end.
+__device__ __forceinline__ uint32_t fhip_codes_of(const FhipGroup &g, const float (&x)[8]) {
+#pragma clang fp contract(off)
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    const float c = fminf(fmaxf((x[i] - (float)g.low) * g.by, 0.f), 15.f) + 12582912.0f;
+    w = (w << 4) + __builtin_bit_cast(uint32_t, c);
+  }
+  return w - 0x4b400000u * 0x11111111u;
 }
 
 #endif // __HIPCC__
