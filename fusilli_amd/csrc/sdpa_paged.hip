@@ -68,6 +68,7 @@ struct PagedArgs {
   int32_t T, Hkv, group; // group: query heads per key head
   int32_t causal;
   int32_t pieces, least; // workgroups that share the line, chunks that each has at least
+  int32_t few, small;    // workgroups where each would have fewer than `small` chunks
   float scale_log2e;
   // of sequences in several pieces (null: there are none)
   struct Info {
@@ -151,16 +152,21 @@ template <int N, typename F> __device__ __forceinline__ void pg_static_for(F &&f
 
 // 16 or 4 bytes per lane from memory to LDS, lane after lane from `to`.  (The builtin takes its size as
 // a literal, and 16 only for this device.)
+// ONCE: what nothing reads again (non-temporal).
 #if defined(__HIP_DEVICE_COMPILE__)
 #define PG_DMA(BYTES)                                                                            \
   __builtin_amdgcn_global_load_lds((const PG_AS1 void *)from,                                    \
                                    (PG_AS3 void *)(uintptr_t)__builtin_amdgcn_readfirstlane(to), \
-                                   BYTES, 0, 0)
+                                   BYTES, 0, ONCE ? 2 : 0)
 #else
 #define PG_DMA(BYTES)
 #endif
-__device__ __forceinline__ void pg_dma16(const char *from, uint32_t to) { PG_DMA(16); }
-__device__ __forceinline__ void pg_dma4(const char *from, uint32_t to) { PG_DMA(4); }
+template <bool ONCE> __device__ __forceinline__ void pg_dma16(const char *from, uint32_t to) { PG_DMA(16); }
+template <bool ONCE> __device__ __forceinline__ void pg_dma4(const char *from, uint32_t to) { PG_DMA(4); }
+template <bool ONCE, typename V> __device__ __forceinline__ V pg_load(const char *from) {
+  const PG_AS1 V *p = (const PG_AS1 V *)from;
+  return ONCE ? __builtin_nontemporal_load(p) : *p;
+}
 
 // s_waitcnt vmcnt(vm) alone.
 __device__ __forceinline__ constexpr int pg_wait_imm(int vm) {
@@ -221,7 +227,8 @@ __device__ __forceinline__ Sequence pg_sequence(const PagedArgs &g, int b) {
   return s;
 }
 
-template <bool BF16, int HD, int G>
+// ONCE: rows share no keys but within a tile: a key is read once (non-temporal).
+template <bool BF16, int HD, int G, bool ONCE>
 __global__ __launch_bounds__(kWaves * 64)
 __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
   constexpr bool Q4 = G != 0;
@@ -297,7 +304,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
   };
   int at = (int)blockIdx.x, stop = at + 1, per = 1;
   if (cut) {
-    per = (total - 1) / g.pieces + 1;
+    per = (total - 1) / (total < g.pieces * g.small ? g.few : g.pieces) + 1;
     per = per < g.least ? g.least : per;
     // the piece's ends, each at a segment's own where that is near
     const int64_t from = (int64_t)blockIdx.x * per;
@@ -439,14 +446,14 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
         const char *kt = k_head + place(places.k, lane + t), *vt = v_head + place(places.v, lane + t);
 #pragma unroll
         for (int u = 0; u < KD; ++u)
-          x.k[t * KD + u] = *(const PG_AS1 u32x4 *)(kt + u * 64 + k_lane);
+          x.k[t * KD + u] = pg_load<ONCE, u32x4>(kt + u * 64 + k_lane);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const char *p = vt + (uint64_t)r * v_slot + v_lane;
           if constexpr (T == 8) {
-            x.v[t * 4 + r] = *(const PG_AS1 u32x4 *)p;
+            x.v[t * 4 + r] = pg_load<ONCE, u32x4>(p);
           } else {
-            const u32x2 y = *(const PG_AS1 u32x2 *)p;
+            const u32x2 y = pg_load<ONCE, u32x2>(p);
             x.v[t * 4 + r].x = y.x, x.v[t * 4 + r].y = y.y;
           }
         }
@@ -473,24 +480,24 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
         if constexpr (SEGS == 4) {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            pg_dma16(kt[t] + k_lane, stage + t * 1024);
-            pg_dma16(vt[t] + v_lane, stage + 32 * ROW + t * 1024);
+            pg_dma16<ONCE>(kt[t] + k_lane, stage + t * 1024);
+            pg_dma16<ONCE>(vt[t] + v_lane, stage + 32 * ROW + t * 1024);
           }
         } else {
-          pg_dma16((l < 32 ? kt[0] : kt[1]) + k_lane, stage + 0);
-          pg_dma16((l < 32 ? vt[0] : vt[1]) + v_lane, stage + 32 * ROW);
+          pg_dma16<ONCE>((l < 32 ? kt[0] : kt[1]) + k_lane, stage + 0);
+          pg_dma16<ONCE>((l < 32 ? vt[0] : vt[1]) + v_lane, stage + 32 * ROW);
         }
         if constexpr (NG == 1) {
           const char *k = (l < 16 ? kpt[0] : kpt[1]) + kp_lane, *v = (l < 48 ? vpt[0] : vpt[1]) + vp_lane;
-          pg_dma4(l < 32 ? k : v, stage + S::kPairs);
+          pg_dma4<ONCE>(l < 32 ? k : v, stage + S::kPairs);
         } else if constexpr (NG == 2) {
-          pg_dma4((l < 32 ? kpt[0] : kpt[1]) + kp_lane, stage + S::kPairs);
-          pg_dma4((l < 32 ? vpt[0] : vpt[1]) + vp_lane, stage + S::kPairs + 256);
+          pg_dma4<ONCE>((l < 32 ? kpt[0] : kpt[1]) + kp_lane, stage + S::kPairs);
+          pg_dma4<ONCE>((l < 32 ? vpt[0] : vpt[1]) + vp_lane, stage + S::kPairs + 256);
         } else {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            pg_dma4(kpt[t] + kp_lane, stage + S::kPairs + t * 256);
-            pg_dma4(vpt[t] + vp_lane, stage + S::kPairs + 512 + t * 256);
+            pg_dma4<ONCE>(kpt[t] + kp_lane, stage + S::kPairs + t * 256);
+            pg_dma4<ONCE>(vpt[t] + vp_lane, stage + S::kPairs + 512 + t * 256);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -516,49 +523,76 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
       z[n] = f32x4{0, 0, 0, 0}, lows[n] = scales[n] = 0.f;
     float m = kNegBig, sum = 0.f; // of row lq: maximum of Q . K over all lanes, sum over this lane's keys
 
-    auto spend = [&](Chunk &x, int i, int bad) {
-      const int key0 = (c0 + wave + kWaves * i) * kChunk;
-      const bool ends = key0 + kChunk > keys; // keys behind the last: nothing of theirs may reach a sum
-      const uint32_t stage = Q4 ? (uint32_t)(i % S::kStages * S::kStage) : 0;
-      // word r * NG + n of a tile: the pair of this lane's key r, group n
-      auto pair_of = [&](u32x4(&p)[2][NG], int t, int r, int n) {
-        // (through a scalar: bit-casting a vector's element in place reads element 0)
-        const uint32_t w = p[t][(r * NG + n) / 4][(r * NG + n) % 4];
-        return __builtin_bit_cast(f16x2, w);
-      };
-      auto read_pairs = [&](u32x4(&p)[2][NG], auto which) {
-        pg_static_for<2 * NG>([&](auto ic) {
-          constexpr int t = decltype(ic)::value / NG, n = decltype(ic)::value % NG;
-          pg_read<decltype(which)::value * 128 * NG + t * 64 * NG + n * 16>(p[t][n], pairs_at + stage);
-        });
-      };
-      auto pin_pairs = [&](u32x4(&p)[2][NG]) {
+    // ---- a chunk's steps: scores, probabilities p, their product with V ---------------------
+    float s[8], p[8];
+    // in 4 bits the words and pairs of K and V that LDS holds; of group n: tile t's row lq, and key e
+    typedef std::conditional_t<SG == 4, u32x4, std::conditional_t<SG == 2, u32x2, uint32_t>> KWords;
+    constexpr int kVReads = 8 * NG;
+    KWords kw[2][NG];
+    uint32_t vw[kVReads];
+    u32x4 kpar[2][NG], vpar[2][NG];
+    // word r * NG + n of a tile: the pair of this lane's key r, group n
+    auto pair_of = [&](u32x4(&x)[2][NG], int t, int r, int n) {
+      // (through a scalar: bit-casting a vector's element in place reads element 0)
+      const uint32_t w = x[t][(r * NG + n) / 4][(r * NG + n) % 4];
+      return __builtin_bit_cast(f16x2, w);
+    };
+    auto read_pairs = [&](u32x4(&x)[2][NG], uint32_t stage, auto which) {
+      pg_static_for<2 * NG>([&](auto ic) {
+        constexpr int t = decltype(ic)::value / NG, n = decltype(ic)::value % NG;
+        pg_read<decltype(which)::value * 128 * NG + t * 64 * NG + n * 16>(x[t][n], pairs_at + stage);
+      });
+    };
+    auto pin_pairs = [&](u32x4(&x)[2][NG]) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int n = 0; n < NG; ++n)
-            pg_pin(p[t][n]);
-      };
-      float s[8];
+        for (int n = 0; n < NG; ++n)
+          pg_pin(x[t][n]);
+    };
+    auto read_k = [&](int i) {
+      const uint32_t stage = (uint32_t)(i % S::kStages * S::kStage);
+      pg_static_for<2 * NG>([&](auto ic) {
+        constexpr int t = decltype(ic)::value / NG, n = decltype(ic)::value % NG;
+        pg_read<t * 16 * ROW>(kw[t][n], k_at[n] + stage);
+      });
+      read_pairs(kpar, stage, std::integral_constant<int, 0>{});
+    };
+    auto read_v = [&](int i) {
+      const uint32_t stage = (uint32_t)(i % S::kStages * S::kStage);
+      pg_static_for<8 * NG>([&](auto ic) {
+        constexpr int n = decltype(ic)::value / 8, e = decltype(ic)::value % 8;
+        constexpr int off = ((e >> 2) * 16 + (e & 3)) * ROW;
+        if constexpr (VB == 4)
+          pg_read<off>(vw[n * 8 + e], v_at[n] + stage);
+        else if constexpr (VB == 2)
+          pg_read16<off>(vw[n * 8 + e], v_at[n] + stage);
+        else
+          pg_read8<off>(vw[n * 8 + e], v_at[n] + stage);
+      });
+      read_pairs(vpar, stage, std::integral_constant<int, 1>{});
+    };
+    auto wait_k = [&]() {
+      pg_lds_wait();
+      pin_pairs(kpar);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+          pg_pin(kw[t][n]);
+    };
+    auto wait_v = [&]() {
+      pg_lds_wait();
+      pin_pairs(vpar);
+#pragma unroll
+      for (int e = 0; e < kVReads; ++e)
+        pg_pin(vw[e]);
+    };
+    auto scores = [&](Chunk &x) {
       if constexpr (Q4) {
-        typedef std::conditional_t<SG == 4, u32x4, std::conditional_t<SG == 2, u32x2, uint32_t>> KWords;
-        u32x4 kpar[2][NG];
-        KWords kw[2][NG];
-        pg_static_for<2 * NG>([&](auto ic) {
-          constexpr int t = decltype(ic)::value / NG, n = decltype(ic)::value % NG;
-          pg_read<t * 16 * ROW>(kw[t][n], k_at[n] + stage);
-        });
-        read_pairs(kpar, std::integral_constant<int, 0>{});
-        pg_lds_wait();
-        pin_pairs(kpar);
+        f32x4 a[2][NG]; // (products first: a sum waits for its last one)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int n = 0; n < NG; ++n)
-            pg_pin(kw[t][n]);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int n = 0; n < NG; ++n) {
             uint32_t w[SG];
@@ -571,7 +605,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
             // bf16 starts at -128 sum(Q).  f16's 1024 would leave the score 2^-14 of sum |Q| scale:
             // it is taken off the codes
             const float start = BF16 ? -Codes<BF16>::kOffset * qsum[n] : 0.f;
-            f32x4 a{start, start, start, start};
+            a[t][n] = f32x4{start, start, start, start};
 #pragma unroll
             for (int u = 0; u < SG; ++u) {
               uint32_t f[4];
@@ -581,18 +615,22 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
                 if constexpr (!BF16)
                   f[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, f[e]) - f16x2{(_Float16)1024, (_Float16)1024});
               }
-              a = pg_mfma<BF16>(f, qf[n * SG + u], a);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const f16x2 p = pair_of(kpar, t, r, n);
-              v[r] = __builtin_fmaf((float)p.x, a[r], __builtin_fmaf((float)p.y, qsum[n], v[r]));
+              a[t][n] = pg_mfma<BF16>(f, qf[n * SG + u], a[t][n]);
             }
           }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            s[t * 4 + r] = v[r];
-        }
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float v = 0.f;
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+              const f16x2 c = pair_of(kpar, t, r, n);
+              v = __builtin_fmaf((float)c.x, a[t][n][r], __builtin_fmaf((float)c.y, qsum[n], v));
+            }
+            s[t * 4 + r] = v;
+          }
       } else {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -608,38 +646,27 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
             s[t * 4 + r] = a[r];
         }
       }
+    };
+    // The reference point m of the exponentials follows the maximum lazily: a chunk first runs against the one it
+    // inherits, with no maximum taken and nothing exchanged between lanes.  Only the first chunk, and one in which
+    // some lane's probabilities rise above kRedo, take the maximum and rescale; O = sum(P V) / sum(P) does
+    // not depend on m.
+    auto softmax = [&](int i, int bad) {
+      const int key0 = (c0 + wave + kWaves * i) * kChunk;
       if (bad) { // (the asm keeps this a branch)
         asm volatile("" : "+v"(s[0]));
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           s[e] = bad >> (e >> 2) & 1 ? __builtin_nanf("") : s[e];
       }
-      if (key0 + kChunk > all_see)
+      if (key0 + kChunk > all_see) {
+        int key = key0 + lg * 4;
+        asm volatile("" : "+v"(key)); // (and its sums in here)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          s[e] = key0 + (e >> 2) * 16 + lg * 4 + (e & 3) < seen ? s[e] : -INFINITY;
-      // V's part of the stage comes in beside the softmax
-      constexpr int kVReads = !Q4 ? 1 : 8 * NG;
-      uint32_t vw[kVReads]; // of group n, key e: word n * 8 + e
-      u32x4 vpar[2][NG];
-      if constexpr (Q4) {
-        pg_static_for<8 * NG>([&](auto ic) {
-          constexpr int n = decltype(ic)::value / 8, e = decltype(ic)::value % 8;
-          constexpr int off = ((e >> 2) * 16 + (e & 3)) * ROW;
-          if constexpr (VB == 4)
-            pg_read<off>(vw[n * 8 + e], v_at[n] + stage);
-          else if constexpr (VB == 2)
-            pg_read16<off>(vw[n * 8 + e], v_at[n] + stage);
-          else
-            pg_read8<off>(vw[n * 8 + e], v_at[n] + stage);
-        });
-        read_pairs(vpar, std::integral_constant<int, 1>{});
+          s[e] = key + (e >> 2) * 16 + (e & 3) < seen ? s[e] : -INFINITY;
       }
-      // The reference point m of the exponentials follows the maximum lazily: a chunk first runs against the one it
-      // inherits, with no maximum taken and nothing exchanged between lanes.  Only the first chunk, and one in which
-      // some lane's probabilities rise above kRedo, take the maximum and rescale; O = sum(P V) / sum(P) does
-      // not depend on m.
-      float p[8], psum;
+      float psum;
       auto exps = [&]() {
         const float at_m = -(m * g.scale_log2e);
         psum = 0.f;
@@ -673,21 +700,27 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
         exps();
       }
       sum += psum;
+    };
+    // keys behind the last: nothing of theirs may reach a sum
+    auto clear_behind = [&](Chunk &x, int i) {
+      const int key0 = (c0 + wave + kWaves * i) * kChunk;
+      if (key0 + kChunk > keys) {
+        int key = key0 + lg * 4;
+        asm volatile("" : "+v"(key));
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (key + (e >> 2) * 16 + (e & 3) >= keys) {
+            if constexpr (Q4)
+#pragma unroll
+              for (int n = 0; n < NG; ++n)
+                vpar[e >> 2][((e & 3) * NG + n) / 4][((e & 3) * NG + n) % 4] = 0;
+            else
+              x.v[e] = u32x4{};
+          }
+      }
+    };
+    auto values = [&](Chunk &x) {
       if constexpr (Q4) {
-        pg_lds_wait();
-        pin_pairs(vpar);
-#pragma unroll
-        for (int e = 0; e < kVReads; ++e)
-          pg_pin(vw[e]);
-        if (ends)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (key0 + t * 16 + lg * 4 + r >= keys)
-#pragma unroll
-                for (int n = 0; n < NG; ++n)
-                  vpar[t][(r * NG + n) / 4][(r * NG + n) % 4] = 0;
         constexpr uint32_t kOne = BF16 ? 0x3f803f80u : 0x3c003c00u;
         const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
 #pragma unroll
@@ -720,11 +753,6 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
           }
         }
       } else {
-        if (ends)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (key0 + (e >> 2) * 16 + lg * 4 + (e & 3) >= keys)
-              x.v[e] = u32x4{};
         const uint32_t pf[4] = {pg_pack<BF16>(p[0], p[1]), pg_pack<BF16>(p[2], p[3]),
                                 pg_pack<BF16>(p[4], p[5]), pg_pack<BF16>(p[6], p[7])};
 #pragma unroll
@@ -760,6 +788,9 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
       }
     }
     if constexpr (Q4) {
+      // A chunk's words come out of LDS while the step in front of the one that takes them runs: K's beside the last
+      // chunk's product with V, V's beside its own scores.  (Four groups' words are too many registers for that.)
+      constexpr bool kAhead = NG < 4;
 #pragma clang loop unroll(disable)
       for (int i = 0; i < steps; ++i) {
         // (stage (i - 1) % kStages, whose reads the last chunk has waited for)
@@ -776,18 +807,43 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
         else
           __builtin_amdgcn_s_waitcnt(pg_wait_imm(0));
         asm volatile("" ::: "memory");
-        spend(x0, i, (int)(bads >> (2 * younger)) & 3);
+        const int bad = (int)(bads >> (2 * younger)) & 3;
+        read_k(i);
+        __builtin_amdgcn_sched_barrier(0);
+        if (kAhead && i > 0)
+          values(x0);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_k();
+        if (kAhead)
+          read_v(i);
+        __builtin_amdgcn_sched_barrier(0);
+        scores(x0);
+        if (!kAhead)
+          read_v(i);
+        softmax(i, bad);
+        wait_v();
+        clear_behind(x0, i);
+        if (!kAhead)
+          values(x0);
       }
+      if (kAhead && steps > 0)
+        values(x0);
     } else {
+      auto spend = [&](Chunk &x, int i) {
+        scores(x);
+        softmax(i, x.bad);
+        clear_behind(x, i);
+        values(x);
+      };
       for (int i = 0; i < steps;) {
         if (i + 1 < steps)
           fetch(x1, i + 1);
-        spend(x0, i, x0.bad);
+        spend(x0, i);
         if (++i >= steps)
           break;
         if (i + 1 < steps)
           fetch(x0, i + 1);
-        spend(x1, i, x1.bad);
+        spend(x1, i);
         ++i;
       }
     }
@@ -847,18 +903,27 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
   }
 }
 
-// Joins the pieces of one row of a query head per HD threads.
-template <bool BF16, int HD>
-__global__ __launch_bounds__(256) void sdpa_paged_join_kernel(PagedArgs g) {
+// Joins the pieces of one row of a query head, which TEAMS of HD threads take in turn: several where there are few rows
+// (up to kJoinRows), which may have many pieces each.  One chat of 30000 keys in 4 bits, 117 pieces: 38.8 us with one team, 33.2
+// with four; 192 rows of 32 heads, few of which have more than three, 110 and 122.
+constexpr int kJoinWide = 512, kJoinRows = 512;
+template <int HD, int TEAMS> struct JoinShape {
+  static constexpr int kThreads = TEAMS > 1 ? TEAMS * HD : 256;
+  static constexpr int kRows = kThreads / (TEAMS * HD); // rows of a workgroup
+};
+template <bool BF16, int HD, int TEAMS>
+__global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_join_kernel(PagedArgs g) {
+  __shared__ float parts[TEAMS][HD], tops[TEAMS], dens[TEAMS];
   const uint32_t heads = (uint32_t)(g.Hkv * g.group);
-  const uint32_t lin = blockIdx.x * (256 / HD) + threadIdx.x / HD;
-  const int d = threadIdx.x % HD;
+  const uint32_t lin = blockIdx.x * JoinShape<HD, TEAMS>::kRows + (TEAMS > 1 ? 0 : threadIdx.x / HD);
   if (lin >= (uint32_t)g.T * heads)
     return;
+  const int d = threadIdx.x % HD, team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / HD) : 0;
   const int t = (int)(lin / heads), h = (int)(lin % heads);
-  if (t < g.offsets[0] || t >= g.offsets[g.cache.batch])
-    return;
+  const int begins = g.offsets[0], ends = g.offsets[g.cache.batch];
   const PagedArgs::Info info = g.info[t];
+  if (t < begins || t >= ends)
+    return;
   const int hk = h / g.group;
   const int64_t row = (int64_t)info.pos * g.group + h - hk * g.group, item = (int64_t)hk * info.tiles + row / 16;
   if (info.per < 1 || info.chunks < 1 || info.pos < 0) // (rows that offsets which overlap have left out hold anything)
@@ -878,16 +943,27 @@ __global__ __launch_bounds__(256) void sdpa_paged_join_kernel(PagedArgs g) {
     const int64_t at = ((begin + s) * 2 + (s == 0)) * 16 + row % 16;
     return Part{ml[at * 2], ml[at * 2 + 1], p[at * HD + d]};
   };
-  constexpr int U = 8;
   float top = kNegBig, acc = 0.f, den = 0.f;
-  fhip_for_uniform_parts<U>(0, 1, (int)pieces, load, [&](const Part &x) {
+  const auto take = [&](const Part &x) {
     const float m = fmaxf(top, x.m);
     const float was = __builtin_amdgcn_exp2f((top - m) * g.scale_log2e),
                 f = __builtin_amdgcn_exp2f((x.m - m) * g.scale_log2e);
     den = den * was + x.l * f;
     acc = acc * was + x.o * f;
     top = m;
-  });
+  };
+  fhip_for_uniform_parts<(TEAMS > 1 ? 4 : 8)>(team, TEAMS, (int)pieces, load, take);
+  if constexpr (TEAMS > 1) { // (all of a workgroup's threads have the same row, and come here or none)
+    parts[team][d] = acc;
+    if (d == 0)
+      tops[team] = top, dens[team] = den;
+    __syncthreads();
+    if (team != 0)
+      return;
+#pragma unroll
+    for (int i = 1; i < TEAMS; ++i)
+      take(Part{tops[i], dens[i], parts[i][d]});
+  }
   pg_store<BF16>(g.o, (int64_t)t * g.o_st + (int64_t)h * g.o_sh + d, den == 0.f ? 0.f : acc / den);
 }
 
@@ -895,6 +971,12 @@ __global__ __launch_bounds__(256) void sdpa_paged_join_kernel(PagedArgs g) {
 // compute, two rounds of them are even: 64 chats of 16 to 16384 keys 113.6 us with 512, 117.3 with 768, 109.1 with 1024;
 // 32 chats in 16 bits 77.3, 78.3, 75.4, but 68.0 and 71.1 where 512 are one segment each.
 constexpr int kPieces16 = 512, kPieces4 = 1024;
+// One round where the second would have pieces of fewer chunks than this: 8 chats of 8192 keys 31.2 us in two, 25.5 in one.
+constexpr int kSmall = 64;
+// Bytes of K and V that the page table has room for from which they are read as non-temporal: half of what the memory-side
+// cache holds.  64 chats of 8192 keys 364 us without, 322 with (4 bits 131.7, 126.1); one of 30000, which the cache keeps from
+// call to call, 31.3 and 33.0.
+constexpr double kOnce = 128 << 20;
 // Chunks that a piece has at least, and keys up to which no sequence is cut (the
 // launch that joins pieces takes longer than what it saves).
 constexpr int kLeast = 2 * kWaves;
@@ -903,7 +985,7 @@ constexpr int64_t kWhole = 1024;
 struct PagedPlan {
   bool ok = false;
   int hd = 0, group = 0;
-  bool bf16 = false, cut = false;
+  bool bf16 = false, cut = false, once = false;
   int64_t pieces = 0; // workgroups
   size_t bytes = 0, part_at = 0, ml_at = 0;
 };
@@ -948,6 +1030,8 @@ PagedPlan make_plan(const fhip_sdpa_paged_desc *d) {
     return p;
   const int64_t keys = d->cache.pages_per_sequence * d->cache.k.dim[2];
   // (the line's places are 32-bit numbers)
+  const int64_t row = q4 ? d->cache.k.dim[3] + 2 * d->cache.k_params.dim[3] : 2 * D;
+  p.once = T * group <= 16 * batch && 2.0 * (double)(row * Hkv) * (double)batch * (double)keys >= kOnce;
   p.cut = keys > kWhole && tiles * ((keys + kChunk - 1) / kChunk) < (1ll << 31) - (1 << 24);
   p.pieces = tiles;
   if (p.cut) {
@@ -981,6 +1065,7 @@ int fhip_fast_sdpa_paged(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d, const fhi
   g.T = (int32_t)d->q.dim[0], g.Hkv = (int32_t)d->cache.k.dim[1], g.group = (int32_t)(d->q.dim[1] / g.Hkv);
   g.causal = d->is_causal != 0;
   g.pieces = (int32_t)p.pieces, g.least = kLeast;
+  g.few = kPieces16, g.small = kSmall;
   const float scale = d->has_scale ? d->scale : 1.0f / sqrtf((float)p.hd);
   g.scale_log2e = scale * 1.4426950408889634f;
   if (p.cut) {
@@ -993,17 +1078,31 @@ int fhip_fast_sdpa_paged(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d, const fhi
     constexpr bool BF = decltype(bf)::value;
     constexpr int HD = decltype(hd)::value, G = decltype(grp)::value;
     constexpr int kLds = kWaves * PagedShape<HD, G>::kBytes;
-    static FhipOncePerDevice configured; // (one for each instance of this lambda)
-    if (kLds > 64 * 1024 && !configured.done(ctx->device)) {
-      FHIP_HIP_CHECK(ctx, hipFuncSetAttribute(reinterpret_cast<const void *>(sdpa_paged_kernel<BF, HD, G>),
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-      configured.mark(ctx->device);
+    auto launch = [&](auto kernel, FhipOncePerDevice &configured) {
+      if (kLds > 64 * 1024 && !configured.done(ctx->device)) {
+        FHIP_HIP_CHECK(ctx, hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+        configured.mark(ctx->device);
+      }
+      hipLaunchKernelGGL(kernel, dim3((unsigned)p.pieces), dim3(kWaves * 64), kLds, ctx->stream, g);
+      return 0;
+    };
+    static FhipOncePerDevice configured[2]; // (two for each instance of this lambda)
+    if (p.once ? launch(sdpa_paged_kernel<BF, HD, G, true>, configured[0])
+               : launch(sdpa_paged_kernel<BF, HD, G, false>, configured[1]))
+      return 1;
+    if (p.cut) {
+      auto join = [&](auto teams) {
+        constexpr int TEAMS = decltype(teams)::value, kRows = JoinShape<HD, TEAMS>::kRows;
+        const int64_t rows = (int64_t)g.T * g.Hkv * g.group;
+        hipLaunchKernelGGL((sdpa_paged_join_kernel<BF, HD, TEAMS>), dim3((unsigned)((rows + kRows - 1) / kRows)),
+                           dim3(JoinShape<HD, TEAMS>::kThreads), 0, ctx->stream, g);
+      };
+      if ((int64_t)g.T * g.Hkv * g.group <= kJoinRows)
+        join(std::integral_constant<int, kJoinWide / HD>{});
+      else
+        join(std::integral_constant<int, 1>{});
     }
-    hipLaunchKernelGGL((sdpa_paged_kernel<BF, HD, G>), dim3((unsigned)p.pieces), dim3(kWaves * 64), kLds, ctx->stream, g);
-    if (p.cut)
-      hipLaunchKernelGGL((sdpa_paged_join_kernel<BF, HD>),
-                         dim3((unsigned)(((int64_t)g.T * g.Hkv * g.group + 256 / HD - 1) / (256 / HD))), dim3(256), 0,
-                         ctx->stream, g);
     FHIP_HIP_CHECK(ctx, hipGetLastError());
     return 0;
   };
