@@ -57,7 +57,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kChunk = 32; // keys of a step
 constexpr float kNegBig = -1.0e30f;
-constexpr int kNear = 4; // a cut moves by up to a quarter of a piece
+// A cut moves by up to a piece / kNear: 5 batches of 32 chats in 16 bits took 73 .. 90 us with 4, 66 .. 87 with 8, 66 .. 85 with
+// 16, of 64 in 4 bits with drafts 102 .. 126, 99 .. 122 and 100 .. 123.
+constexpr int kNear = 8;
 
 struct PagedArgs {
   const char *q;
@@ -968,8 +970,8 @@ __global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_j
 }
 
 // Workgroups that share the line: two for each compute unit run at once.  In 4 bits, where a compute unit has more to
-// compute, two rounds of them are even: 64 chats of 16 to 16384 keys 113.6 us with 512, 117.3 with 768, 109.1 with 1024;
-// 32 chats in 16 bits 77.3, 78.3, 75.4, but 68.0 and 71.1 where 512 are one segment each.
+// compute, two rounds of them are even: 64 chats of 16 to 16384 keys 110.3 us with 512, 114.6 with 768, 105.4 with 1024, 110.2
+// with 1536; 32 chats in 16 bits 72.1 with 512, 72.3 with 1024.
 constexpr int kPieces16 = 512, kPieces4 = 1024;
 // One round where the second would have pieces of fewer chunks than this: 8 chats of 8192 keys 31.2 us in two, 25.5 in one.
 constexpr int kSmall = 64;
