@@ -799,6 +799,9 @@ private:
   template <typename Attr>
   ErrorObject planCache(const Attr &attr, fhip_cache_desc &c, Step &s) {
     const CacheTensors t = attr.getCache();
+    // (again: buffers may have given dynamic dims other extents)
+    FUSILLI_CHECK_ERROR(serving_utils::checkCacheIndices(
+        t, attr.getOFFSETS(), "Node '" + attr.getName() + "':"));
     FUSILLI_ASSIGN_OR_RETURN(c.k, toDesc(t.k));
     FUSILLI_ASSIGN_OR_RETURN(c.v, toDesc(t.v));
     FUSILLI_ASSIGN_OR_RETURN(s.slot[kCaK], readSlot(t.k));
@@ -827,6 +830,10 @@ private:
     FUSILLI_ASSIGN_OR_RETURN(d.k, toDesc(attr.getK()));
     FUSILLI_ASSIGN_OR_RETURN(d.v, toDesc(attr.getV()));
     FUSILLI_ASSIGN_OR_RETURN(d.o, toDesc(attr.getO()));
+    if (attr.getKV_OFFSETS()) // (again: of dynamic dims)
+      FUSILLI_CHECK_ERROR(serving_utils::checkIndices(
+          attr.getKV_OFFSETS(), "Node '" + attr.getName() + "':", "KV_OFFSETS",
+          attr.getOFFSETS()->getDim()));
     d.batch = attr.getOFFSETS()->getDim()[0] - 1;
     d.has_kv_offsets = attr.getKV_OFFSETS() ? 1 : 0;
     d.is_causal = attr.getIsCausal() ? 1 : 0;
@@ -900,6 +907,10 @@ private:
       FUSILLI_ASSIGN_OR_RETURN(d.rotation, toDesc(attr.getROTATION()));
     }
     FUSILLI_CHECK_ERROR(planCache(attr, d.cache, s));
+    if (attr.getPOSITIONS()) // (again: of dynamic dims)
+      FUSILLI_CHECK_ERROR(serving_utils::checkIndices(
+          attr.getPOSITIONS(), "Node '" + attr.getName() + "':", "POSITIONS",
+          {attr.getK()->getDim()[0]}));
     d.has_positions = attr.getPOSITIONS() ? 1 : 0;
     d.interleaved = attr.getInterleaved() ? 1 : 0;
     FUSILLI_CHECK_ERROR(mustRun(fhip_cache_append_supported(&d) != 0,

@@ -125,6 +125,25 @@ TEST("host: a step of decoding is two kernels, its rows between them in the work
   CHECK(ko->isVirtual());
 }
 
+TEST("host: keys alone go into a cache; their turned rows are an output where they are marked as one") {
+  for (bool out : {false, true}) {
+    Graph g = newGraph("prefill");
+    Rows r = rowsOf(g, 20);
+    CacheTensors c = cacheOf(g);
+    CacheAppendAttr aa;
+    aa.setName("a");
+    auto [qo, ko] = g.cacheAppend(nullptr, r.k, r.v, r.rotation, nullptr, r.offsets, c, aa);
+    CHECK(!qo);
+    ko->setOutput(out);
+    REQUIRE_OK(g.validate());
+    REQUIRE_ASSIGN(Handle cpu, Handle::create(Backend::CPU));
+    REQUIRE_OK(g.compile(cpu, true));
+    CHECK(g.getKernelCount() == std::optional<size_t>(1));
+    CHECK(ko->getDim() == (Dims{20, kHk, kD}));
+    CHECK(ko->isVirtual() == !out);
+  }
+}
+
 TEST("host: what no kernel takes is refused by compile") {
   Graph g = newGraph("refused");
   Rows r = rowsOf(g, 2);
@@ -295,6 +314,47 @@ TEST("a prompt, a chunk behind it and single tokens through graphs that share a 
     std::printf("  step %zu: worst error %.3f of its bound\n", step, worst);
     CHECK(worst <= 1.0);
   }
+}
+
+TEST("buffers that give dynamic dims extents which do not belong together are refused") {
+  Graph g = newGraph("dynamic");
+  auto q = g.tensor(mk("q", {2, kHq, kD}, DataType::BFloat16));
+  auto offsets = g.tensor(mk("offsets", {kBatch + 1}, DataType::Int32).setDynamicDims({0}));
+  CacheTensors c = cacheOf(g);
+  c.lengths->setDynamicDims({0});
+  c.pages->setDynamicDims({0, 1});
+  SdpaPagedAttr a;
+  a.setName("p");
+  auto o = g.sdpaPaged(q, offsets, c, a);
+  o->setOutput(true);
+  REQUIRE_OK(g.validate());
+  REQUIRE_OK(g.compile(gpu(), true));
+  auto need = g.getWorkspaceSize();
+  REQUIRE(!isError(need) && **need == 0);
+  const Dims pool = {kPool, kHk, kPage, kD};
+  const std::vector<bf16> rows(kPool * kHk * kPage * kD, (bf16)1.f);
+  auto run = [&](int64_t batch, int64_t table, int64_t nOffsets, int64_t nLengths) {
+    Pack pack;
+    pack[q] = bufOf(std::vector<bf16>(2 * kHq * kD, (bf16)1.f), {2, kHq, kD});
+    pack[o] = bufOf(std::vector<bf16>(2 * kHq * kD, (bf16)7.f), {2, kHq, kD});
+    pack[c.k] = bufOf(rows, pool);
+    pack[c.v] = bufOf(rows, pool);
+    pack[c.pages] = bufOf(std::vector<int32_t>(batch * table, 1), {batch, table});
+    pack[c.lengths] = bufOf(std::vector<int32_t>(nLengths, 20), {nLengths});
+    std::vector<int32_t> at(nOffsets, 2);
+    at[0] = 0;
+    pack[offsets] = bufOf(at, {nOffsets});
+    auto st = g.execute(gpu(), pack, nullptr);
+    if (!st.isError())
+      for (float x : floats(pack[o]))
+        CHECK(x == 1.f);
+    return st;
+  };
+  REQUIRE_OK(run(2, 4, 3, 2));
+  REQUIRE_OK(run(1, 3, 2, 1)); // both rows to one sequence
+  CHECK_ERROR(run(2, 4, 2, 2), ErrorCode::InvalidAttribute, "Node 'p': tensor OFFSETS must be contiguous [3]");
+  CHECK_ERROR(run(2, 4, 3, 1), ErrorCode::InvalidAttribute, "Node 'p': tensor LENGTHS must be contiguous [2]");
+  CHECK_ERROR(run(1, 4, 3, 2), ErrorCode::InvalidAttribute, "Node 'p': tensor OFFSETS must be contiguous [2]");
 }
 
 int main(int argc, char **argv) { return mini::run(argc, argv); }
