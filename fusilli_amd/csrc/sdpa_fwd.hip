@@ -193,6 +193,9 @@ __device__ __forceinline__ PackedItem sd_packed_item(const SdpaArgs &g, int inde
       if (past) {
         const int i = __builtin_ctzll(past);
         const int r = left - __builtin_amdgcn_readlane(upto - mine * g.Hkv, i);
+        // (what offsets that overlap, and so hold more tiles than a number counts, could lead to)
+        if ((uint32_t)r >= (uint32_t)(__builtin_amdgcn_readlane(mine, i) * g.Hkv))
+          return PackedItem{0, 0, 0, 0, 0, -1};
         const int tile = __builtin_amdgcn_readlane(s.tiles - above, i) - 1 - r / g.Hkv;
         return PackedItem{__builtin_amdgcn_readlane(s.start, i),    __builtin_amdgcn_readlane(s.n, i),
                           __builtin_amdgcn_readlane(s.kv_start, i), __builtin_amdgcn_readlane(s.m, i),

@@ -404,3 +404,62 @@ def test_packed_from_a_graph(d):
             assert torch.equal(*outs) and bool((outs[0][sum(lens):] == 3).all())
         del graph
         one.close(), two.close()
+
+
+# ---- metadata that does not fit the tensors ------------------------------------------
+@pytest.mark.parametrize("d", [64, 80])
+def test_offsets_behind_the_rows(ctx, d):
+    """The last sequence claims more rows than there are: the others, and memory behind the tensors, do not notice."""
+    rng = np.random.default_rng([41, d])
+    q, k, v = rows_of(rng, [90, 4, d], BF16), rows_of(rng, [90, 2, d], BF16), rows_of(rng, [90, 2, d], BF16)
+    dims = [90 + 64, 4, d]
+    o = HT.from_logical(np.full(dims, 3.0), BF16)
+    desc = capi.SdpaPackedDesc()
+    desc.q, desc.k, desc.v = q.desc(), k.desc(), v.desc()
+    desc.o = capi.TensorDesc.make([90, 4, d], [4 * d, d, 1], BF16)
+    desc.batch, desc.is_causal = 3, 1
+    buf = o.upload(ctx)
+    ctx.sdpa_packed_fwd(desc, q.upload(ctx), k.upload(ctx), v.upload(ctx), ints(ctx, [0, 40, 50, 5000]), buf)
+    got = o.fetch(ctx, buf).logical()
+    assert (got[90:] == 3).all()
+    got[50:] = 77.0  # (rows of the third sequence, which the checks take for rows of none)
+    check_packed(q, k, v, [0, 40, 50], True, got[:90])
+
+    cache = Cache(rng, [40, 30, 20], 2, d, 16, BF16)
+    desc = capi.SdpaPagedDesc()
+    desc.q, desc.cache, desc.is_causal = q.desc(), cache.desc(), 1
+    desc.o = capi.TensorDesc.make([90, 4, d], [4 * d, d, 1], BF16)
+    buf = HT.from_logical(np.full(dims, 3.0), BF16).upload(ctx)
+    ctx.sdpa_paged_fwd(desc, cache.upload(ctx), q.upload(ctx), ints(ctx, [0, 1, 3, 5000]), buf)
+    got = o.fetch(ctx, buf).logical()
+    assert (got[90:] == 3).all()
+    got[3:] = 77.0
+    check_paged(cache, [40, 30], q, [0, 1, 3], got[:90])
+
+    read = capi.CacheReadDesc()
+    read.k = read.v = capi.TensorDesc.make([60, 2, d], [2 * d, d, 1], BF16)
+    read.cache = cache.desc()
+    bufs = [HT.from_logical(np.full([100, 2, d], 3.0), BF16) for _ in "kv"]
+    at = [b.upload(ctx) for b in bufs]
+    ctx.cache_read(read, cache.upload(ctx), ints(ctx, [0, 40, 50, 5000]), *at)
+    for x, host, b in zip("kv", bufs, at):
+        out = host.fetch(ctx, b).logical()
+        assert np.array_equal(out[:40], cache.rows(x, 0)) and np.array_equal(out[40:50], cache.rows(x, 1)[20:])
+        assert np.isnan(out[50:60]).all() and (out[60:] == 3).all()  # (places in front of the first)
+
+
+@pytest.mark.parametrize("lengths", [[-5, 20, 30], [40, 20, 2 ** 30]])
+def test_lengths_that_no_cache_has(ctx, lengths):
+    rng = np.random.default_rng([42])
+    cache = Cache(rng, [40, 20, 30], 2, 128, 16, BF16)
+    q = rows_of(rng, [3, 8, 128], BF16)
+    got, _ = run_paged(ctx, cache, lengths, q, [0, 1, 2, 3])
+    ok = [b for b in range(3) if 0 <= lengths[b] <= 40]
+    for b in ok:
+        one = np.full_like(got, 77.0)
+        one[b] = got[b]
+        check_paged(cache, [0] * b + [lengths[b]], q, [b] * (b + 1) + [b + 1], one)
+    if lengths[0] < 0:
+        assert not got[0].any()  # no key: 0
+    else:
+        assert np.isnan(got[2]).all()  # keys that the table has no places for
