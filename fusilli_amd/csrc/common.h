@@ -291,6 +291,23 @@ __device__ __forceinline__ void fhip_for_uniform_parts(int first, int step, int 
   }
 }
 
+// The first of `count` ascending values that is above `x` (-1: none), found by a wavefront with 64 of them at a time.
+__device__ __forceinline__ int fhip_first_above(const int32_t *values, int count, int x) {
+  const int l = threadIdx.x & 63;
+  int lo = 0, n = count;
+  while (n > 64) {
+    const int step = (n + 63) / 64, end = (l + 1) * step < n ? (l + 1) * step : n;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(l * step < n && values[lo + end - 1] > x);
+    if (past == 0)
+      return -1;
+    const int at = __builtin_ctzll(past) * step;
+    lo += at;
+    n = n - at < step ? n - at : step;
+  }
+  const uint64_t past = __builtin_amdgcn_ballot_w64(l < n && values[lo + l] > x);
+  return past ? lo + __builtin_ctzll(past) : -1;
+}
+
 // Load element `idx` of a tensor of runtime dtype as CT (float or double).
 template <typename CT>
 __device__ __forceinline__ CT fhip_load(const void *p, int dt, int64_t idx) {

@@ -126,8 +126,10 @@ int fhip_decode_sdpa(fhip_ctx *ctx, const fhip_sdpa_desc *d, const void *q,
 // Packed sequences on the tiled kernel: 16-bit rows, head dim 64 or 128, positive
 // scale, K and V below 2 GiB.  `handled` false where a pointer's alignment does not fit.
 bool fhip_fast_sdpa_packed_applicable(const fhip_sdpa_packed_desc *d);
+size_t fhip_fast_sdpa_packed_workspace(const fhip_sdpa_packed_desc *d);
 int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const void *q, const void *k,
-                          const void *v, const void *offsets, const void *kv_offsets, void *o, bool *handled);
+                          const void *v, const void *offsets, const void *kv_offsets, void *o, void *workspace,
+                          bool *handled);
 
 // Attention over a paged cache on MFMA: 16-bit rows, head dim 64 or 128, pages of a
 // multiple of 16 rows.  `handled` false where a pointer's alignment does not fit.

@@ -117,6 +117,8 @@ struct SdpaArgs {
   // packed sequences (kernels with PACKED): rows of Q and of K, heads of K;
   // 2^32 / group rounded up (0: groups of one)
   const int32_t *offsets, *kv_offsets;
+  const int32_t *index; // of many sequences (sd_packed_index_kernel); null: none
+  int32_t classes;      // of cost
   int32_t batch, T, Tk, Hkv;
   uint32_t magic;
 };
@@ -124,8 +126,8 @@ struct SdpaArgs {
 // ---- packed sequences ------------------------------------------------------
 // The rows of a sequence that share a key / value head are one matrix, position
 // after position (row r: position r / group, head r % group), cut into tiles of
-// ROWS.  No one but the device knows the lengths: every workgroup reads all of
-// them and finds its own tile.  Tiles come in classes of cost, keys of 2^k to
+// ROWS.  No one but the device knows the lengths: every workgroup finds its own
+// tile from them.  Tiles come in classes of cost, keys of 2^k to
 // 2^(k + 1) - 1 tiles of 64, the most expensive first, so that the last ones to start are short;
 // the heads of a tile are neighbours, on one XCD each where there are 8.
 struct PackedSeq {
@@ -169,40 +171,81 @@ __device__ __forceinline__ int sd_scan(int x) { // inclusive sums over the lanes
 struct PackedItem {
   int start, n, kv_start, m, hk, tile; // tile -1: none
 };
+
+// More sequences than a wavefront has lanes: a walk over all of them in every workgroup, for each class, would take
+// longer than its tile (1024 prompts of 300 tokens 4469 us, 2113 like this; 64 of 64 24.4 and 27.2).  A first kernel, with a
+// workgroup for each class, writes how many tiles (of all heads) the classes above it have, how many it has itself, and
+// their sums up to each sequence, in which the others search 64 at a time.
+constexpr int kPackedLanes = 64;
+constexpr int kPackedClasses = 25; // (fewer than 2^30 keys)
+template <int ROWS, bool CAUSAL> __global__ __launch_bounds__(1024) void sd_packed_index_kernel(SdpaArgs g, int32_t *index) {
+  __shared__ int sums[2][16];
+  const int k = blockIdx.x, l = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t *const upto = index + 64 + (int64_t)k * g.batch;
+  int own = 0, above = 0;
+  for (int b0 = 0; b0 < g.batch; b0 += 1024) {
+    const int b = b0 + (int)threadIdx.x;
+    const PackedSeq s = b < g.batch ? sd_packed_seq<ROWS>(g, b) : PackedSeq{};
+    const int more = sd_packed_count<ROWS, CAUSAL>(g, s, 2 << k);
+    const int x = sd_scan(sd_packed_count<ROWS, CAUSAL>(g, s, 1 << k) - more), y = sd_scan(more);
+    if (l == 63)
+      sums[0][wave] = x, sums[1][wave] = y;
+    __syncthreads();
+    int front = own;
+    for (int w = 0; w < 16; ++w) {
+      front += w < wave ? sums[0][w] : 0;
+      own += sums[0][w], above += sums[1][w];
+    }
+    if (b < g.batch)
+      upto[b] = (front + x) * g.Hkv;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0)
+    index[k] = above * g.Hkv, index[32 + k] = own * g.Hkv;
+}
+template <int ROWS, bool CAUSAL> __device__ __forceinline__ PackedItem sd_packed_lookup(const SdpaArgs &g, int index) {
+  const int l = threadIdx.x & 63;
+  const int above = l < g.classes ? g.index[l] : 0, own = l < g.classes ? g.index[32 + l] : 0;
+  const uint64_t in = __builtin_amdgcn_ballot_w64(index >= above && index - above < own);
+  const PackedItem none{0, 0, 0, 0, 0, -1};
+  if (in == 0)
+    return none;
+  const int k = __builtin_ctzll(in), left = index - __builtin_amdgcn_readlane(above, k);
+  const int32_t *const upto = g.index + 64 + (int64_t)k * g.batch;
+  const int b = fhip_first_above(upto, g.batch, left);
+  if (b < 0)
+    return none;
+  const PackedSeq s = sd_packed_seq<ROWS>(g, b);
+  const int more = sd_packed_count<ROWS, CAUSAL>(g, s, 2 << k);
+  const int mine = (sd_packed_count<ROWS, CAUSAL>(g, s, 1 << k) - more) * g.Hkv, r = left - (upto[b] - mine);
+  if ((uint32_t)r >= (uint32_t)mine) // (what offsets that overlap could lead to)
+    return none;
+  return PackedItem{s.start, s.n, s.kv_start, s.m, r % g.Hkv, s.tiles - more - 1 - r / g.Hkv};
+}
 template <int ROWS, bool CAUSAL>
 __device__ __forceinline__ PackedItem sd_packed_item(const SdpaArgs &g, int index) {
+  if (g.index)
+    return sd_packed_lookup<ROWS, CAUSAL>(g, index);
   const int l = threadIdx.x & 63;
-  const PackedSeq front = l < g.batch ? sd_packed_seq<ROWS>(g, l) : PackedSeq{};
-  // (a class above every sequence's keys is passed over by its count of 0)
-  int keys = front.m;
-  for (int b = l + 64; b < g.batch; b += 64) {
-    const int m = sd_packed_seq<ROWS>(g, b).m;
-    keys = m > keys ? m : keys;
-  }
+  const PackedSeq s = l < g.batch ? sd_packed_seq<ROWS>(g, l) : PackedSeq{};
   int k = 0;
-  while (__builtin_amdgcn_ballot_w64(keys > (kBKV << k)) != 0) // (keys < 2^30)
+  while (__builtin_amdgcn_ballot_w64(s.m > (kBKV << k)) != 0) // (keys < 2^30)
     ++k;
   int left = index;
-  for (; k >= 0; --k)
-    for (int b0 = 0; b0 < g.batch; b0 += 64) {
-      const PackedSeq s = b0 == 0 ? front : b0 + l < g.batch ? sd_packed_seq<ROWS>(g, b0 + l) : PackedSeq{};
-      const int above = sd_packed_count<ROWS, CAUSAL>(g, s, 2 << k);
-      const int mine = sd_packed_count<ROWS, CAUSAL>(g, s, 1 << k) - above;
-      const int upto = sd_scan(mine) * g.Hkv;
-      const uint64_t past = __builtin_amdgcn_ballot_w64(upto > left);
-      if (past) {
-        const int i = __builtin_ctzll(past);
-        const int r = left - __builtin_amdgcn_readlane(upto - mine * g.Hkv, i);
-        // (what offsets that overlap, and so hold more tiles than a number counts, could lead to)
-        if ((uint32_t)r >= (uint32_t)(__builtin_amdgcn_readlane(mine, i) * g.Hkv))
-          return PackedItem{0, 0, 0, 0, 0, -1};
-        const int tile = __builtin_amdgcn_readlane(s.tiles - above, i) - 1 - r / g.Hkv;
-        return PackedItem{__builtin_amdgcn_readlane(s.start, i),    __builtin_amdgcn_readlane(s.n, i),
-                          __builtin_amdgcn_readlane(s.kv_start, i), __builtin_amdgcn_readlane(s.m, i),
-                          r % g.Hkv,                                tile};
-      }
-      left -= __builtin_amdgcn_readlane(upto, 63);
+  for (; k >= 0; --k) {
+    const int more = sd_packed_count<ROWS, CAUSAL>(g, s, 2 << k);
+    const int mine = (sd_packed_count<ROWS, CAUSAL>(g, s, 1 << k) - more) * g.Hkv, upto = sd_scan(mine);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > left);
+    if (past) {
+      const int i = __builtin_ctzll(past), r = left - __builtin_amdgcn_readlane(upto - mine, i);
+      if ((uint32_t)r >= (uint32_t)__builtin_amdgcn_readlane(mine, i)) // (as in the lookup)
+        break;
+      return PackedItem{__builtin_amdgcn_readlane(s.start, i),    __builtin_amdgcn_readlane(s.n, i),
+                        __builtin_amdgcn_readlane(s.kv_start, i), __builtin_amdgcn_readlane(s.m, i),
+                        r % g.Hkv, __builtin_amdgcn_readlane(s.tiles - more, i) - 1 - r / g.Hkv};
     }
+    left -= __builtin_amdgcn_readlane(upto, 63);
+  }
   return PackedItem{0, 0, 0, 0, 0, -1};
 }
 
@@ -1473,8 +1516,19 @@ bool fhip_fast_sdpa_packed_applicable(const fhip_sdpa_packed_desc *d) {
   return T * group < (1ll << 30) && T * group * group < (1ll << 32);
 }
 
+static int packed_classes(const fhip_sdpa_packed_desc *d) {
+  int n = 1;
+  while (n < kPackedClasses && ((int64_t)kBKV << (n - 1)) < d->k.dim[0])
+    ++n;
+  return n;
+}
+
+size_t fhip_fast_sdpa_packed_workspace(const fhip_sdpa_packed_desc *d) {
+  return d->batch <= kPackedLanes ? 0 : 4 * (64 + (size_t)packed_classes(d) * (size_t)d->batch);
+}
+
 int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const void *q, const void *k, const void *v,
-                          const void *offsets, const void *kv_offsets, void *o, bool *handled) {
+                          const void *offsets, const void *kv_offsets, void *o, void *workspace, bool *handled) {
   *handled = fhip_fast_sdpa_packed_applicable(d) &&
              (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15) == 0;
   if (!*handled)
@@ -1501,6 +1555,17 @@ int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const v
   // tiles of all sequences, each one's last short
   const int64_t tiles = g.Hkv * (rows / (cut ? kBQ / 2 : kBQ) + seqs);
   FHIP_REQUIRE(ctx, tiles < (1ll << 31), "fhip_sdpa_packed_fwd: more than 2^31 tiles");
+  if (fhip_fast_sdpa_packed_workspace(d)) {
+    g.index = (const int32_t *)workspace, g.classes = packed_classes(d);
+    auto index = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)g.classes), dim3(1024), 0, ctx->stream, g, (int32_t *)workspace);
+    };
+    if (cut)
+      g.causal ? index(sd_packed_index_kernel<kBQ / 2, true>) : index(sd_packed_index_kernel<kBQ / 2, false>);
+    else
+      g.causal ? index(sd_packed_index_kernel<kBQ, true>) : index(sd_packed_index_kernel<kBQ, false>);
+    FHIP_HIP_CHECK(ctx, hipGetLastError());
+  }
   auto launch = [&](auto kernel, int lds_bytes, FhipOncePerDevice &configured) {
     if (!configured.done(ctx->device)) {
       if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,

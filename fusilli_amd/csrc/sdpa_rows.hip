@@ -164,6 +164,12 @@ static int check_q_o(fhip_ctx *ctx, const char *who, const fhip_tensor_desc &q, 
   return 0;
 }
 
+static int check_workspace(fhip_ctx *ctx, const char *who, size_t need, const void *workspace, size_t bytes) {
+  FHIP_REQUIRE(ctx, need == 0 || (workspace && bytes >= need && ((uintptr_t)workspace & 255) == 0),
+               "%s: needs %zu bytes of 256-byte aligned workspace, got %zu", who, need, bytes);
+  return 0;
+}
+
 static int packed_validate(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d) {
   static const char who[] = "fhip_sdpa_packed_fwd";
   FHIP_REQUIRE(ctx, d != nullptr, "%s: null descriptor", who);
@@ -195,6 +201,10 @@ extern "C" {
 int fhip_sdpa_packed_fwd_workspace_size(const fhip_sdpa_packed_desc *d, size_t *bytes) {
   FHIP_REQUIRE(nullptr, d && bytes, "fhip_sdpa_packed_fwd_workspace_size: null");
   *bytes = 0;
+  if (packed_validate(nullptr, d) != 0)
+    return 1;
+  if (fhip_fast_sdpa_packed_applicable(d))
+    *bytes = fhip_fast_sdpa_packed_workspace(d);
   return 0;
 }
 
@@ -214,13 +224,15 @@ int fhip_sdpa_packed_fwd(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const vo
   FHIP_REQUIRE(ctx, q && k && v && offsets && o, "%s: null tensor pointer", who);
   FHIP_REQUIRE(ctx, (d->has_kv_offsets != 0) == (kv_offsets != nullptr), "%s: kv_offsets and has_kv_offsets disagree",
                who);
-  (void)workspace;
-  (void)workspace_bytes;
   FHIP_HIP_CHECK(ctx, hipSetDevice(ctx->device));
-  bool handled = false;
-  const int rc = fhip_fast_sdpa_packed(ctx, d, q, k, v, offsets, kv_offsets, o, &handled);
-  if (handled)
-    return rc;
+  if (fhip_fast_sdpa_packed_applicable(d)) {
+    if (check_workspace(ctx, who, fhip_fast_sdpa_packed_workspace(d), workspace, workspace_bytes))
+      return 1;
+    bool handled = false;
+    const int rc = fhip_fast_sdpa_packed(ctx, d, q, k, v, offsets, kv_offsets, o, workspace, &handled);
+    if (handled)
+      return rc;
+  }
   fhip_note_kernel(ctx, "sdpa_rows packed");
   RowsArgs g{};
   g.q = q, g.k = k, g.v = v, g.o = o;
@@ -255,9 +267,8 @@ int fhip_sdpa_paged_fwd(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d, const fhip
   FHIP_REQUIRE(ctx, q && offsets && o, "%s: null tensor pointer", who);
   FHIP_HIP_CHECK(ctx, hipSetDevice(ctx->device));
   if (fhip_fast_sdpa_paged_applicable(d)) {
-    const size_t need = fhip_fast_sdpa_paged_workspace(d);
-    FHIP_REQUIRE(ctx, need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0),
-                 "%s: needs %zu bytes of 256-byte aligned workspace, got %zu", who, need, workspace_bytes);
+    if (check_workspace(ctx, who, fhip_fast_sdpa_paged_workspace(d), workspace, workspace_bytes))
+      return 1;
     bool handled = false;
     const int rc = fhip_fast_sdpa_paged(ctx, d, cache, q, offsets, o, workspace, &handled);
     if (handled)

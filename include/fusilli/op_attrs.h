@@ -464,6 +464,7 @@ struct CacheTensors {
             getCACHE_V_PARAMS(), getPAGES(),   getLENGTHS()};                  \
   }
 
+// (causal unless told otherwise: a row sees the keys up to its own place)
 class SdpaPagedAttr : public AttributesCRTP<SdpaPagedAttr> {
 public:
   enum class InputNames : uint8_t {

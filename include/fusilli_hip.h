@@ -398,7 +398,9 @@ typedef struct {
  * keys (the last row sees all).  A row that sees no key is 0.  Heads are
  * grouped like fhip_sdpa_fwd's.  A key that some rows of a sequence may not see
  * takes part in theirs with probability 0: 0 times an infinite or NaN value
- * shows; other sequences' keys and values never do.  supported: 2 for bf16 / f16,
+ * shows; other sequences' keys and values never do.  More than 64 sequences need
+ * 256-byte aligned workspace of fhip_sdpa_packed_fwd_workspace_size bytes (what
+ * fhip_sdpa_paged_fwd says about its own holds here).  supported: 2 for bf16 / f16,
  * D = Dv = 64 or 128, positive scale, rows (heads, and tensors at the call) on 16
  * bytes, below 2 GiB per K or V tensor and T (Hq / Hkv)^2 below 2^32; 1 for other
  * sizes to 512 and f32. */
@@ -427,7 +429,7 @@ int fhip_sdpa_packed_fwd(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d,
  * keys up to its own place; otherwise every row sees lengths[b] keys.  A row
  * that sees no key is 0; what lies behind lengths[b] never matters, a key that
  * only later rows see matters as above.  Needs 256-byte aligned workspace of
- * fhip_sdpa_paged_fwd_workspace_size bytes (parts of long sequences; it holds
+ * fhip_sdpa_paged_fwd_workspace_size bytes (parts of long sequences, sums over many; it holds
  * nothing between calls, and calls that overlap need one each).  supported: 2 for
  * bf16 / f16, D = Dv = 64 or 128, positive scale, pages of a multiple of 16 rows,
  * groups of 32, 64 or 128, rows and parameters aligned to 16 and 4 bytes;
@@ -483,7 +485,8 @@ int fhip_cache_append(fhip_ctx *ctx, const fhip_cache_append_desc *d,
 
 /* Brings the last offsets[b + 1] - offsets[b] keys and values of each sequence
  * back to packed rows (f32, bf16 or f16; values in 4 bits are rounded to it once;
- * 16-bit and f32 caches are read in their own type). */
+ * 16-bit and f32 caches are read in their own type).  supported: 2 for 16-bit rows of
+ * a multiple of 8 dims on 16 bytes, groups of 32, 64, 128 or 256 dims; otherwise 1. */
 typedef struct {
   fhip_tensor_desc k; /* [T, Hkv, D]  */
   fhip_tensor_desc v; /* [T, Hkv, Dv] */

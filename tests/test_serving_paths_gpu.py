@@ -8,7 +8,7 @@ import torch  # (before the library, which then shares its runtime)
 
 from fusilli_amd import capi
 from helpers import HT
-from serving import Cache, check, rotation_table, starts
+from serving import Cache, attend, check, rotation_table, starts
 from test_serving_gpu import (check_packed, check_paged, ints, one_step, rows_of, run_append, run_packed, run_paged, run_read)
 
 pytestmark = pytest.mark.gpu
@@ -118,6 +118,33 @@ def test_many_sequences(ctx, group, batch):
         ref = np.concatenate([cache.rows(x, b) for b in range(batch)])
         far = 2.0 ** -24 * np.abs(ref) + 0.5 * one_step(np.abs(ref) * (1 + 2.0 ** -24), BF16) if group else 0 * ref
         check(out[:-1], ref, far)
+
+
+@pytest.mark.parametrize("batch,most,past", [(65, 200, 0), (300, 90, 400), (1025, 9, 0), (5000, 3, 5)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_packed_sequences(ctx, batch, most, past, causal):
+    rng = np.random.default_rng([43, batch])
+    new = [int(x) for x in rng.integers(0, most, batch)]
+    keys = [n + int(x) for n, x in zip(new, rng.integers(0, past + 1, batch))]
+    q, k, v = rows_of(rng, [sum(new), 2, 64], BF16), rows_of(rng, [sum(keys), 1, 64], BF16), rows_of(rng, [sum(keys), 1, 64], BF16)
+    got, level = run_packed(ctx, q, k, v, starts(new), causal, starts(keys))
+    assert level == 2
+    check_packed(q, k, v, starts(new), causal, got, starts(keys))
+
+
+def test_many_paged_sequences(ctx):
+    rng = np.random.default_rng([44])
+    keys, rows = [int(x) for x in rng.integers(0, 20, 5000)], [int(x) for x in rng.integers(0, 3, 5000)]
+    cache = Cache(rng, keys, 1, 64, 16, BF16)
+    q = rows_of(rng, [sum(rows), 2, 64], BF16)
+    got, level = run_paged(ctx, cache, keys, q, starts(rows))
+    assert level == 2
+    for x in range(0, 5000, 61):  # (some of them: each takes the whole cache's values)
+        a, b = starts(rows)[x], starts(rows)[x + 1]
+        ref, far = attend(q.logical().astype(np.float64)[a:b], cache.rows("k", x), cache.rows("v", x),
+                          np.clip(keys[x] - (b - a) + 1 + np.arange(b - a), 0, keys[x]), BF16)
+        check(got[a:b], ref, far, f"sequence {x}")
+    assert (got != 77).all()
 
 
 def test_many_long_sequences(ctx):
@@ -245,6 +272,28 @@ def test_workspaces(ctx):
         assert (space.download(np.uint8, need + 256)[need:] == fill).all()
     assert np.array_equal(got[0], got[0xff])
     check_paged(cache, keys, q, [0, 1, 2], got[0])
+
+
+def test_workspace_of_many_packed_sequences(ctx):
+    rng = np.random.default_rng([45])
+    lens = [int(x) for x in rng.integers(0, 30, 100)]
+    q, k, v = (rows_of(rng, [sum(lens), h, 64], BF16) for h in (4, 2, 2))
+    d = capi.SdpaPackedDesc()
+    d.q = d.o = q.desc()
+    d.k, d.v, d.batch, d.is_causal = k.desc(), v.desc(), 64, 1
+    assert ctx.sdpa_packed_workspace(d) == 0
+    d.batch = 100
+    need = ctx.sdpa_packed_workspace(d)
+    assert need > 0
+    bufs, bo, offsets, space = [t.upload(ctx) for t in (q, k, v)], q.upload(ctx), ints(ctx, starts(lens)), ctx.alloc(need + 256)
+    for where, size in ((space.ptr, need - 1), (space.ptr + 64, need), (None, need)):
+        assert ctx.lib.fhip_sdpa_packed_fwd(ctx.handle, ctypes.byref(d), *(b.ptr for b in bufs), offsets.ptr, None, bo.ptr, where, size) != 0
+        assert f"needs {need} bytes of 256-byte aligned workspace" in ctx.lib.fhip_last_error(ctx.handle).decode()
+    for fill in (0x00, 0xff):
+        space.upload(np.full(need + 256, fill, np.uint8))
+        ctx.sdpa_packed_fwd(d, *bufs, offsets, bo, workspace=space)
+        assert (space.download(np.uint8, need + 256)[need:] == fill).all()
+        check_packed(q, k, v, starts(lens), True, HT.from_logical(np.zeros(q.dims), BF16).fetch(ctx, bo).logical())
 
 
 # ---- recorded ----------------------------------------------------------------------
