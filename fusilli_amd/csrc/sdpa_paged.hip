@@ -877,12 +877,18 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
       sum = __builtin_nanf("");
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
+    // The codes' part times the sum of P scale over that of its rounded values: their mean rounding is gone, and with it all
+    // of it where one key has (nearly) all of P.
+    float even[NG];
     if constexpr (Q4)
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         lows[n] = __builtin_fmaf(8.f, scales[n], lows[n]);
         lows[n] += __shfl_xor(lows[n], 16, 64);
         lows[n] += __shfl_xor(lows[n], 32, 64);
+        scales[n] += __shfl_xor(scales[n], 16, 64);
+        scales[n] += __shfl_xor(scales[n], 32, 64);
+        even[n] = z[n][0] > 0.f ? scales[n] / z[n][0] : 1.f;
       }
 #pragma unroll
     for (int n = 0; n < NG; ++n)
@@ -892,7 +898,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
         for (int r = 0; r < 4; ++r) {
           float v = o[n * TG + j][r];
           if constexpr (Q4)
-            v = __builtin_fmaf(-(Codes<BF16>::kOffset + 8.f), z[n][r], v) + lows[n];
+            v = __builtin_fmaf(__builtin_fmaf(-(Codes<BF16>::kOffset + 8.f), z[n][r], v), even[n], lows[n]);
           sums[(n * GG + (lg * 4 + r) * TG + j) * PITCH + lq] = v;
         }
     if (l < 16)

@@ -247,6 +247,23 @@ def test_a_pool_beyond_32_bits(group):
     c.close()
 
 
+@pytest.mark.parametrize("dtype", [BF16, capi.HALF])
+@pytest.mark.parametrize("d,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+def test_one_key_in_4_bits_is_its_value(ctx, dtype, d, group):
+    """No probability is rounded where there is one key; of what acts on the codes, some eight roundings in f32 of at most
+    143 scale + |low| are left, and the result's own."""
+    rng = np.random.default_rng([46, d, group])
+    cache = Cache(rng, [1] * 20, 2, d, 16, dtype, group)
+    q = rows_of(rng, [20, 6, d], dtype)
+    got, level = run_paged(ctx, cache, [1] * 20, q, np.arange(21))
+    assert level == 2
+    pair = np.abs(cache.v[1].logical().astype(np.float64))[cache.table[:, 0], :, 0]
+    size = np.repeat(np.repeat(143 * pair[..., ::2] + pair[..., 1::2], group, -1), 3, 1)
+    ref = np.repeat(np.stack([cache.rows("v", b)[0] for b in range(20)]), 3, 1)
+    f32 = 8 * 2.0 ** -24 * size
+    check(got, ref, f32 + 0.5 * one_step(np.abs(ref) + f32, dtype))
+
+
 # ---- workspaces ------------------------------------------------------------------
 def test_workspaces(ctx):
     rng = np.random.default_rng([39])
