@@ -23,15 +23,16 @@
 // taken off, V's comes from a product with ones), scales and lows act on sums and
 // probabilities in f32.  P scale is rounded where P would be; so that its rounding
 // meets no larger numbers than in 16 bits, the codes count from the middle, as
-// c - 8, and 8 (P . scale) goes with the lows.  Each product's 32 dims (K) or 16 columns (V) lie within a group.
+// c - 8, and 8 (P . scale) goes with the lows; in the end the codes' part is scaled
+// by the sum of P scale over that of its rounded values.  Each product's 32 dims (K) or 16 columns (V) lie within a group.
 //
 // In 4 bits a chunk is 4 KB, and more of them have to be on their way: rows and parameters go
 // to a ring of stages in the wavefront's own LDS by LDS-DMA, from which each lane takes
 // what its fragments need.
 //
 // Work: no one but the device knows the lengths.  All sequences' chunks, one
-// tile and head after another, are one line that is cut into equal pieces, one per
-// workgroup; each reads all lengths and finds its own.  What a workgroup does of
+// tile and head after another, are one line that is cut into pieces, one per
+// workgroup; each finds its own from the lengths.  What a workgroup does of
 // a (sequence, tile, head) is a segment: whole ones it stores, parts meet in the
 // workspace, in a fixed order, in a second kernel.  A cut near a segment's end moves
 // there: a new segment waits for its first loads, 3 us in which its workgroup reads nothing.
@@ -39,9 +40,9 @@
 // takes one whole (sequence, tile, head).
 //
 // bf16, 32 heads on 8 of 128: one token of each of 32 sequences of 16 to 8192 keys (354 MB) 66.9 us, 5.3 TB/s; of 64 with
-// 8192 keys each 319 us, 6.7 TB/s, a reading stream's rate.  4 bits, groups of 64: three tokens of 64 sequences of 16 to 16384
-// keys (391 MB) 104 us, 3.8 TB/s, one of 64 with 8192 122 us, 4.9 TB/s: the vector ALU works 67 % of the time on codes, scales
-// and probabilities (315 instructions a chunk), and a sixth goes into the last pieces' ends.
+// 8192 keys each 320 us, 6.7 TB/s, a reading stream's rate.  4 bits, groups of 64: three tokens of 64 sequences of 16 to 16384
+// keys (391 MB) 95.5 us, 4.1 TB/s, one of 64 with 8192 124 us, 4.9 TB/s: the vector ALU works 67 % of the time on codes, scales
+// and probabilities (315 instructions a chunk).
 #include "paged_cache.h"
 #include "fast_paths.h"
 
@@ -62,9 +63,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kChunk = 32; // keys of a step
 constexpr float kNegBig = -1.0e30f;
-// A cut moves by up to a piece / kNear: 5 batches of 32 chats in 16 bits took 73 .. 90 us with 4, 66 .. 87 with 8, 66 .. 85 with
-// 16, of 64 in 4 bits with drafts 102 .. 126, 99 .. 122 and 100 .. 123.
-constexpr int kNear = 8;
 
 struct PagedArgs {
   const char *q;
@@ -74,17 +72,55 @@ struct PagedArgs {
   FhipCacheView cache;
   int32_t T, Hkv, group; // group: query heads per key head
   int32_t causal;
-  int32_t pieces, least; // workgroups that share the line, chunks that each has at least
-  int32_t few, small;    // workgroups where each would have fewer than `small` chunks
+  int32_t pieces; // workgroups that share the line
   int32_t *upto;         // of many sequences, their work summed up to each (null: walked over)
   float scale_log2e;
   // of sequences in several pieces (null: there are none)
   struct Info {
     int32_t first; // the sequence's place on the line
-    int32_t chunks, pos, tiles, per;
+    int32_t chunks, pos, tiles;
+    int32_t large, small; // chunks of the pieces
   } *info;        // [T]
   float *part;    // [piece][2][16][HD] sums: of a segment that another piece began, and of one that it goes on with
   float *part_ml; // [piece][2][16] (m, l)
+};
+
+// Workgroups that share the line: two for each compute unit run at once.  In 4 bits, where a compute unit has more to
+// compute, their ends lie further apart, and 256 more with pieces of a quarter go where one is done: 6 batches of 64 chats
+// with drafts 112.3 us in the mean with 512 equal pieces, 112.1 with 1024, 107.0 with 512 and 512 quarters, 107.6 like this.
+constexpr int kLarge = 512, kPieces16 = kLarge, kPieces4 = kLarge + 256;
+constexpr int kQuarter = 4;
+// One round where pieces are fewer chunks than this: 8 chats of 8192 keys 31.2 us in two equal rounds, 25.5 in one.
+constexpr int kSmall = 64;
+// Chunks that a piece has at least, and keys up to which no sequence is cut (the
+// launch that joins pieces takes longer than what it saves).
+constexpr int kLeast = 2 * kWaves;
+constexpr int64_t kWhole = 1024;
+// A cut moves by up to a piece / kNear: 5 batches of 32 chats in 16 bits took 73 .. 90 us with 4, 66 .. 87 with 8, 66 .. 85 with
+// 16, of 64 in 4 bits with drafts 102 .. 126, 99 .. 122 and 100 .. 123.
+constexpr int kNear = 8;
+static_assert(kLeast >= kNear, "a cut at a segment's end is always near");
+
+// The pieces' places on the line: kLarge large ones, then small ones.
+struct Pieces {
+  int32_t large, small; // chunks of each
+  static __device__ __forceinline__ Pieces of(int total, int pieces) {
+    const int rest = total < pieces * kSmall ? 0 : pieces - kLarge;
+    Pieces p;
+    p.large = (int)(((int64_t)total * kQuarter - 1) / (kLarge * kQuarter + rest)) + 1;
+    p.large = p.large < kLeast ? kLeast : p.large;
+    p.small = (p.large + kQuarter - 1) / kQuarter;
+    p.small = p.small < kLeast ? kLeast : p.small;
+    return p;
+  }
+  __device__ __forceinline__ int64_t at(uint32_t i) const {
+    return i <= kLarge ? (int64_t)i * large : (int64_t)kLarge * large + (int64_t)(i - kLarge) * small;
+  }
+  // the last piece that begins at x or in front of it
+  __device__ __forceinline__ int64_t last(int64_t x) const {
+    const int64_t bend = (int64_t)kLarge * large;
+    return x < bend ? x / large : kLarge + (x - bend) / small;
+  }
 };
 
 template <bool BF16>
@@ -326,23 +362,23 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
       seq = Sequence{pg_lane(s.start, b), pg_lane(s.rows, b), pg_lane(s.length, b), pg_lane(s.tiles, b), pg_lane(s.chunks, b)};
     }
   };
-  int at = (int)blockIdx.x, stop = at + 1, per = 1;
+  int at = (int)blockIdx.x, stop = at + 1;
+  Pieces pieces{};
   if (cut) {
-    per = (total - 1) / (total < g.pieces * g.small ? g.few : g.pieces) + 1;
-    per = per < g.least ? g.least : per;
+    pieces = Pieces::of(total, g.pieces);
     // the piece's ends, each at a segment's own where that is near
-    const int64_t from = (int64_t)blockIdx.x * per;
+    const int64_t from = pieces.at(blockIdx.x);
     auto snapped = [&](int64_t x) {
       if (x >= total)
         return total;
       find((int)x);
       if (b < 0)
         return total;
-      const int near = per / kNear, inside = ((int)x - first) % seq.chunks;
+      const int near = pieces.large / kNear, inside = ((int)x - first) % seq.chunks;
       return inside < near ? (int)x - inside : seq.chunks - inside < near ? (int)x - inside + seq.chunks : (int)x;
     };
     at = snapped(from);
-    stop = snapped(from + per);
+    stop = snapped(pieces.at(blockIdx.x + 1));
   }
   if (at >= total)
     return;
@@ -381,7 +417,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
     }
     all_see = __builtin_amdgcn_readfirstlane(all_see);
     if (cut && hk == 0 && slot == 1 && threadIdx.x < 16)
-      g.info[seq.start + pos] = PagedArgs::Info{first, seq.chunks, pos, seq.tiles, per};
+      g.info[seq.start + pos] = PagedArgs::Info{first, seq.chunks, pos, seq.tiles, pieces.large, pieces.small};
     // chunks behind the last key that any row sees have nothing
     const int need = (__builtin_amdgcn_readfirstlane(any_sees) + kChunk - 1) / kChunk;
     c1 = c1 < need ? c1 : need;
@@ -955,11 +991,12 @@ __global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_j
     return;
   const int hk = h / g.group;
   const int64_t row = (int64_t)info.pos * g.group + h - hk * g.group, item = (int64_t)hk * info.tiles + row / 16;
-  if (info.per < 1 || info.chunks < 1 || info.pos < 0) // (rows that offsets which overlap have left out hold anything)
+  if (info.large < 1 || info.small < 1 || info.chunks < 1 || info.pos < 0) // (rows that offsets which overlap have left out hold anything)
     return;
   // cuts that lie inside this segment and not near its ends
-  const int64_t from = info.first + item * info.chunks, near = info.per / kNear;
-  const int64_t cut0 = (from + near + info.per - 1) / info.per, cut1 = (from + info.chunks - near) / info.per;
+  const Pieces cuts{info.large, info.small};
+  const int64_t from = info.first + item * info.chunks, near = info.large / kNear;
+  const int64_t cut0 = cuts.last(from + near - 1) + 1, cut1 = cuts.last(from + info.chunks - near);
   const int64_t begin = cut0 - 1, pieces = cut1 - cut0 + 2;
   if (info.chunks < 2 * near || pieces <= 1 || begin < 0 || begin + pieces > g.pieces)
     return;
@@ -996,21 +1033,10 @@ __global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_j
   pg_store<BF16>(g.o, (int64_t)t * g.o_st + (int64_t)h * g.o_sh + d, den == 0.f ? 0.f : acc / den);
 }
 
-// Workgroups that share the line: two for each compute unit run at once.  In 4 bits, where a compute unit has more to
-// compute, two rounds of them are even: 64 chats of 16 to 16384 keys 110.3 us with 512, 114.6 with 768, 105.4 with 1024, 110.2
-// with 1536; 32 chats in 16 bits 72.1 with 512, 72.3 with 1024.
-constexpr int kPieces16 = 512, kPieces4 = 1024;
-// One round where the second would have pieces of fewer chunks than this: 8 chats of 8192 keys 31.2 us in two, 25.5 in one.
-constexpr int kSmall = 64;
 // Bytes of K and V that the page table has room for from which they are read as non-temporal: half of what the memory-side
 // cache holds.  64 chats of 8192 keys 364 us without, 322 with (4 bits 131.7, 126.1); one of 30000, which the cache keeps from
 // call to call, 31.3 and 33.0.
 constexpr double kOnce = 128 << 20;
-// Chunks that a piece has at least, and keys up to which no sequence is cut (the
-// launch that joins pieces takes longer than what it saves).
-constexpr int kLeast = 2 * kWaves;
-constexpr int64_t kWhole = 1024;
-
 struct PagedPlan {
   bool ok = false;
   int hd = 0, group = 0;
@@ -1098,8 +1124,7 @@ int fhip_fast_sdpa_paged(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d, const fhi
   g.cache = fhip_cache_view(d->cache, *cache);
   g.T = (int32_t)d->q.dim[0], g.Hkv = (int32_t)d->cache.k.dim[1], g.group = (int32_t)(d->q.dim[1] / g.Hkv);
   g.causal = d->is_causal != 0;
-  g.pieces = (int32_t)p.pieces, g.least = kLeast;
-  g.few = kPieces16, g.small = kSmall;
+  g.pieces = (int32_t)p.pieces;
   const float scale = d->has_scale ? d->scale : 1.0f / sqrtf((float)p.hd);
   g.scale_log2e = scale * 1.4426950408889634f;
   if (p.cut) {
