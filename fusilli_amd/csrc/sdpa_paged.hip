@@ -116,10 +116,10 @@ struct Pieces {
   __device__ __forceinline__ int64_t at(uint32_t i) const {
     return i <= kLarge ? (int64_t)i * large : (int64_t)kLarge * large + (int64_t)(i - kLarge) * small;
   }
-  // the last piece that begins at x or in front of it
-  __device__ __forceinline__ int64_t last(int64_t x) const {
-    const int64_t bend = (int64_t)kLarge * large;
-    return x < bend ? x / large : kLarge + (x - bend) / small;
+  // the last piece that begins at x or in front of it (places on the line are 31-bit numbers)
+  __device__ __forceinline__ int last(uint32_t x) const {
+    const uint32_t bend = (uint32_t)kLarge * (uint32_t)large;
+    return (int)(x < bend ? x / (uint32_t)large : kLarge + (x - bend) / (uint32_t)small);
   }
 };
 
@@ -969,47 +969,53 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
 }
 
 // Joins the pieces of one row of a query head, which TEAMS of HD threads take in turn: several where there are few rows
-// (up to kJoinRows), which may have many pieces each.  One chat of 30000 keys in 4 bits, 117 pieces: 38.8 us with one team, 33.2
-// with four; 192 rows of 32 heads, few of which have more than three, 110 and 122.
+// (up to kJoinRows), which may have many pieces each; otherwise one, of 4 columns a thread.  One chat of 30000 keys in 4 bits,
+// 117 pieces: 38.8 us with one team, 33.2 with four; 192 rows of 32 heads, few of which have more than three, 110 and 122.
 constexpr int kJoinWide = 512, kJoinRows = 512;
 template <int HD, int TEAMS> struct JoinShape {
+  static constexpr int kVec = TEAMS > 1 ? 1 : 4; // columns of a thread
   static constexpr int kThreads = TEAMS > 1 ? TEAMS * HD : 256;
-  static constexpr int kRows = kThreads / (TEAMS * HD); // rows of a workgroup
+  static constexpr int kRows = kThreads * kVec / (TEAMS * HD); // rows of a workgroup
 };
 template <bool BF16, int HD, int TEAMS>
 __global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_join_kernel(PagedArgs g) {
+  constexpr int VEC = JoinShape<HD, TEAMS>::kVec, ROWS = JoinShape<HD, TEAMS>::kRows;
   __shared__ float parts[TEAMS][HD], tops[TEAMS], dens[TEAMS];
   const uint32_t heads = (uint32_t)(g.Hkv * g.group);
-  const uint32_t lin = blockIdx.x * JoinShape<HD, TEAMS>::kRows + (TEAMS > 1 ? 0 : threadIdx.x / HD);
+  const uint32_t lin = blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / (HD / VEC) : 0);
   if (lin >= (uint32_t)g.T * heads)
     return;
-  const int d = threadIdx.x % HD, team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / HD) : 0;
+  const int d = threadIdx.x % (HD / VEC) * VEC, team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / HD) : 0;
   const int t = (int)(lin / heads), h = (int)(lin % heads);
   const int begins = g.offsets[0], ends = g.offsets[g.cache.batch];
   const PagedArgs::Info info = g.info[t];
   if (t < begins || t >= ends)
     return;
   const int hk = h / g.group;
-  const int64_t row = (int64_t)info.pos * g.group + h - hk * g.group, item = (int64_t)hk * info.tiles + row / 16;
   if (info.large < 1 || info.small < 1 || info.chunks < 1 || info.pos < 0) // (rows that offsets which overlap have left out hold anything)
     return;
   // cuts that lie inside this segment and not near its ends
+  const uint32_t row = (uint32_t)info.pos * (uint32_t)g.group + (uint32_t)(h - hk * g.group);
+  const uint32_t item = (uint32_t)hk * (uint32_t)info.tiles + row / 16;
   const Pieces cuts{info.large, info.small};
-  const int64_t from = info.first + item * info.chunks, near = info.large / kNear;
-  const int64_t cut0 = cuts.last(from + near - 1) + 1, cut1 = cuts.last(from + info.chunks - near);
-  const int64_t begin = cut0 - 1, pieces = cut1 - cut0 + 2;
-  if (info.chunks < 2 * near || pieces <= 1 || begin < 0 || begin + pieces > g.pieces)
+  const uint32_t from = (uint32_t)info.first + item * (uint32_t)info.chunks, near = (uint32_t)info.large / kNear;
+  const int cut0 = cuts.last(from + near - 1) + 1, cut1 = cuts.last(from + (uint32_t)info.chunks - near);
+  const int begin = cut0 - 1, pieces = cut1 - cut0 + 2;
+  if ((uint32_t)info.chunks < 2 * near || pieces <= 1 || begin < 0 || pieces > g.pieces || begin > g.pieces - pieces)
     return;
+  typedef float Vec __attribute__((ext_vector_type(VEC)));
   const PG_AS1 float *ml = (const PG_AS1 float *)g.part_ml;
   const PG_AS1 float *p = (const PG_AS1 float *)g.part;
   struct Part {
-    float m, l, o;
+    float m, l;
+    Vec o;
   };
   const auto load = [&](int s) {
-    const int64_t at = ((begin + s) * 2 + (s == 0)) * 16 + row % 16;
-    return Part{ml[at * 2], ml[at * 2 + 1], p[at * HD + d]};
+    const int64_t at = ((int64_t)(begin + s) * 2 + (s == 0)) * 16 + row % 16;
+    return Part{ml[at * 2], ml[at * 2 + 1], *(const PG_AS1 Vec *)(p + at * HD + d)};
   };
-  float top = kNegBig, acc = 0.f, den = 0.f;
+  float top = kNegBig, den = 0.f;
+  Vec acc = 0.f;
   const auto take = [&](const Part &x) {
     const float m = fmaxf(top, x.m);
     const float was = __builtin_amdgcn_exp2f((top - m) * g.scale_log2e),
@@ -1018,9 +1024,9 @@ __global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_j
     acc = acc * was + x.o * f;
     top = m;
   };
-  fhip_for_uniform_parts<(TEAMS > 1 ? 4 : 8)>(team, TEAMS, (int)pieces, load, take);
+  fhip_for_uniform_parts<(TEAMS > 1 ? 4 : 8)>(team, TEAMS, pieces, load, take);
   if constexpr (TEAMS > 1) { // (all of a workgroup's threads have the same row, and come here or none)
-    parts[team][d] = acc;
+    parts[team][d] = acc[0];
     if (d == 0)
       tops[team] = top, dens[team] = den;
     __syncthreads();
@@ -1028,9 +1034,11 @@ __global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_j
       return;
 #pragma unroll
     for (int i = 1; i < TEAMS; ++i)
-      take(Part{tops[i], dens[i], parts[i][d]});
+      take(Part{tops[i], dens[i], Vec{parts[i][d]}});
   }
-  pg_store<BF16>(g.o, (int64_t)t * g.o_st + (int64_t)h * g.o_sh + d, den == 0.f ? 0.f : acc / den);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    pg_store<BF16>(g.o, (int64_t)t * g.o_st + (int64_t)h * g.o_sh + d + i, den == 0.f ? 0.f : acc[i] / den);
 }
 
 // Bytes of K and V that the page table has room for from which they are read as non-temporal: half of what the memory-side
