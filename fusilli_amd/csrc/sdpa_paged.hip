@@ -41,8 +41,8 @@
 //
 // bf16, 32 heads on 8 of 128: one token of each of 32 sequences of 16 to 8192 keys (354 MB) 66.9 us, 5.3 TB/s; of 64 with
 // 8192 keys each 320 us, 6.7 TB/s, a reading stream's rate.  4 bits, groups of 64: three tokens of 64 sequences of 16 to 16384
-// keys (391 MB) 95.5 us, 4.1 TB/s, one of 64 with 8192 124 us, 4.9 TB/s: the vector ALU works 67 % of the time on codes, scales
-// and probabilities (315 instructions a chunk).
+// keys (391 MB) 91.5 us, 4.3 TB/s, one of 64 with 8192 124 us, 4.9 TB/s: the vector ALU works 71 % of the time on codes, scales
+// and probabilities (315 instructions a chunk), for two wavefronts a SIMD about what it can.
 #include "paged_cache.h"
 #include "fast_paths.h"
 
