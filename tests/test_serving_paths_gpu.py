@@ -529,3 +529,72 @@ def test_lengths_that_no_cache_has(ctx, lengths):
         assert not got[0].any()  # no key: 0
     else:
         assert np.isnan(got[2]).all()  # keys that the table has no places for
+
+
+# ---- heads and pointers ------------------------------------------------------------
+@pytest.mark.parametrize("hq,hk", [(40, 1), (66, 2), (17, 17)])
+@pytest.mark.parametrize("group", [0, 64])
+def test_many_heads(ctx, hq, hk, group):
+    rng = np.random.default_rng([47, hq, group])
+    lens, past = [9, 1, 0, 30], [70, 0, 5, 2]
+    keys = [a + b for a, b in zip(lens, past)]
+    cache = Cache(rng, keys, hk, 64, 16, BF16, group)
+    q = rows_of(rng, [40, hq, 64], BF16)
+    got, level = run_paged(ctx, cache, keys, q, starts(lens))
+    assert level == 2
+    check_paged(cache, keys, q, starts(lens), got)
+    k, v = rows_of(rng, [sum(keys), hk, 64], BF16), rows_of(rng, [sum(keys), hk, 64], BF16)
+    got, level = run_packed(ctx, q, k, v, starts(lens), True, starts(keys))
+    assert level == 2
+    check_packed(q, k, v, starts(lens), True, got, starts(keys))
+
+
+@pytest.mark.parametrize("group", [0, 32])
+def test_tensors_on_odd_addresses(ctx, group):
+    """One element behind where the vector kernels can load: the general ones take the call."""
+    rng = np.random.default_rng([48, group])
+    keys, new, d = [30, 7], [3, 2], 64
+    at = starts(new)
+    cache = Cache(rng, keys, 2, d, 16, BF16, group)
+    tensors = {n: rows_of(rng, [5, h, d], BF16) for n, h in (("q", 4), ("k", 2), ("v", 2))}
+
+    def shifted(t):
+        raw = np.concatenate([np.zeros(1, t.storage.dtype), t.storage.reshape(-1)])
+        buf = ctx.to_device(raw)
+        return buf, buf.ptr + raw.itemsize
+
+    bufs = {n: shifted(t) for n, t in tensors.items()}
+    offsets, pointers = ints(ctx, at), cache.upload(ctx)
+    a = capi.CacheAppendDesc()
+    a.k, a.v, a.cache = tensors["k"].desc(), tensors["v"].desc(), cache.desc()
+    ctx.cache_append(a, pointers, bufs["k"][1], bufs["v"][1], offsets)
+    assert ctx.last_kernel() == "cache_append_rows"
+    cache.fetch(ctx)
+    if not group:
+        for b, n in enumerate(keys):
+            assert np.array_equal(cache.rows("k", b)[n - new[b]:], tensors["k"].logical()[at[b]:at[b + 1]])
+    out = HT.from_logical(np.full([5, 4, d], 77.0), BF16)
+    p = capi.SdpaPagedDesc()
+    p.q, p.o, p.cache, p.is_causal = tensors["q"].desc(), out.desc(), cache.desc(), 1
+    bo = out.upload(ctx)
+    ctx.sdpa_paged_fwd(p, pointers, bufs["q"][1], offsets, bo)
+    assert ctx.last_kernel() == "sdpa_rows paged"
+    check_paged(cache, keys, tensors["q"], at, out.fetch(ctx, bo).logical())
+    s = capi.SdpaPackedDesc()
+    s.q, s.k, s.v, s.o = (tensors[n].desc() for n in "qkvq")
+    s.batch, s.is_causal = 2, 1
+    bo = HT.from_logical(np.full([5, 4, d], 77.0), BF16).upload(ctx)
+    ctx.sdpa_packed_fwd(s, *(bufs[n][1] for n in "qkv"), offsets, bo)
+    assert ctx.last_kernel() == "sdpa_rows packed"
+    check_packed(tensors["q"], tensors["k"], tensors["v"], at, True, out.fetch(ctx, bo).logical())
+    r = capi.CacheReadDesc()
+    r.k = r.v = capi.TensorDesc.make([37, 2, d], [2 * d, d, 1], BF16)
+    r.cache = cache.desc()
+    room = [ctx.alloc(2 * (37 * 2 * d + 1)) for _ in "kv"]
+    ctx.cache_read(r, pointers, ints(ctx, starts(keys)), *(b.ptr + 2 for b in room))
+    assert ctx.last_kernel() == "cache_read_rows"
+    for x, b in zip("kv", room):
+        back = HT([37, 2, d], [2 * d, d, 1], BF16, b.download(np.uint16)[1:].copy()).logical()
+        ref = np.concatenate([cache.rows(x, i) for i in range(2)])
+        far = 2.0 ** -24 * np.abs(ref) + 0.5 * one_step(np.abs(ref) * (1 + 2.0 ** -24), BF16) if group else 0 * ref
+        check(back, ref, far)
