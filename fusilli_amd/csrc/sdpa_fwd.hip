@@ -1548,10 +1548,15 @@ int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const v
   const int64_t rows = (int64_t)g.T * g.group, seqs = d->batch < g.T ? d->batch : g.T;
   // Workgroups of one team (2) overlap one tile's loads and stores with another's products: 256 prompts of 64 tokens, 32
   // heads on 8, D128 120.5 us whole (0), so 94.5; 64 of 512 296 / 257; 4 of 2048 155.3 / 155.4; 8192 tokens 459 / 479: whole
-  // from 4096 keys.  Few tiles of long sequences: both teams on the same rows (1), 1024 tokens 25.9 / 22.7, 2048 50.6 / 51.8.
+  // from 4096 keys.  Few tiles of long sequences: both teams on the same rows (1).  Under a causal mask the longest
+  // tile, which sees all keys, is then what takes the time, up to two tiles of 128 rows per compute unit: (tiles, keys) on one
+  // team / on both, D64 (260, 1040) 19.9 / 16.3 us, (500, 2000) 33.5 / 33.0, (500, 4000) 61.5 / 53.5, but (260, 693) 15.2 /
+  // 17.6, (500, 1333) 25.1 / 34.1, (600, 4800) 77 / 79; D128 (260, 1040) 27.5 / 22.4.  Without a mask, up to one per
+  // compute unit: (150, 600) 12.2 / 11.7, (260, 2080) 38.3 / 46.9.
   const int64_t halves = g.Hkv * (rows / (kBQ / 2) + seqs / 2), keys = g.Tk / seqs;
   const int forced = fhip_knobs().sdpa_packed;
-  const int cut = forced >= 0 && forced <= 2 ? forced : halves <= 256 && keys >= 512 ? 1 : hd == 128 && keys >= 4096 ? 0 : 2;
+  const bool both = keys >= 512 && (g.causal ? halves <= 512 && keys >= 4 * halves : halves <= 256);
+  const int cut = forced >= 0 && forced <= 2 ? forced : both ? 1 : hd == 128 && keys >= 4096 ? 0 : 2;
   // tiles of all sequences, each one's last short
   const int64_t tiles = g.Hkv * (rows / (cut ? kBQ / 2 : kBQ) + seqs);
   FHIP_REQUIRE(ctx, tiles < (1ll << 31), "fhip_sdpa_packed_fwd: more than 2^31 tiles");

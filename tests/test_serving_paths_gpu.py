@@ -19,8 +19,10 @@ BF16 = capi.BFLOAT16
 @pytest.mark.parametrize("lens,hq,hkv,d,name", [
     ([40, 9], 4, 2, 64, "sdpa_packed d=64 causal=1 half"),
     ([1100], 4, 4, 128, "sdpa_packed d=128 causal=1 split"),
-    ([4100], 16, 8, 128, "sdpa_packed d=128 causal=1"),
-    ([4100], 16, 8, 64, "sdpa_packed d=64 causal=1 half"),
+    ([4100], 32, 8, 128, "sdpa_packed d=128 causal=1"),
+    ([4100], 32, 8, 64, "sdpa_packed d=64 causal=1 half"),
+    ([4090], 16, 8, 64, "sdpa_packed d=64 causal=1 split"),
+    ([700, 700, 700], 16, 8, 128, "sdpa_packed d=128 causal=1 half"),
     ([40, 9], 4, 2, 80, "sdpa_rows packed"),
 ])
 def test_packed_route(ctx, lens, hq, hkv, d, name):
