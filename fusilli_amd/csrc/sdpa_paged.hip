@@ -73,7 +73,7 @@ struct PagedArgs {
   int32_t T, Hkv, group; // group: query heads per key head
   int32_t causal;
   int32_t pieces; // workgroups that share the line
-  int32_t *upto;         // of many sequences, their work summed up to each (null: walked over)
+  int32_t *upto;  // of many sequences, their work summed up to each (null: few)
   float scale_log2e;
   // of sequences in several pieces (null: there are none)
   struct Info {
@@ -1092,9 +1092,9 @@ PagedPlan make_plan(const fhip_sdpa_paged_desc *d) {
   if (T * group >= (1ll << 30) || tiles >= (1ll << 29))
     return p;
   const int64_t keys = d->cache.pages_per_sequence * d->cache.k.dim[2];
-  // (the line's places are 32-bit numbers)
   const int64_t row = q4 ? d->cache.k.dim[3] + 2 * d->cache.k_params.dim[3] : 2 * D;
   p.once = T * group <= 16 * batch && 2.0 * (double)(row * Hkv) * (double)batch * (double)keys >= kOnce;
+  // (the line's places are 31-bit numbers; the second launch has a thread for each 4 columns of a row)
   p.cut = keys > kWhole && T * Hq <= (1 << 24) && tiles * ((keys + kChunk - 1) / kChunk) < (1ll << 31) - (1 << 24);
   p.pieces = tiles;
   if (p.cut) {
