@@ -6,6 +6,7 @@
 #define FUSILLI_AMD_CSRC_PAGED_CACHE_H
 
 #include "common.h"
+#include "serving_split.h"
 
 constexpr int kCacheMaxDim = 512; // of a head
 constexpr int64_t kCacheMaxKeys = (1ll << 30); // of a sequence: places stay 32-bit numbers

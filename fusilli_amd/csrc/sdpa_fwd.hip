@@ -44,6 +44,7 @@
 // node/sdpa_node.h:138-176 (rank 4, every dim 1 or the full extent).
 #include "common.h"
 #include "fast_paths.h"
+#include "serving_split.h"
 
 #include <cstdlib>
 #include <type_traits>
@@ -136,13 +137,9 @@ struct PackedSeq {
 };
 template <int ROWS> __device__ __forceinline__ PackedSeq sd_packed_seq(const SdpaArgs &g, int b) {
   PackedSeq s;
-  auto clamp = [](int x, int top) { return x < 0 ? 0 : x > top ? top : x; };
-  s.start = clamp(g.offsets[b], g.T);
-  s.n = clamp(g.offsets[b + 1], g.T) - s.start;
-  s.n = s.n < 0 ? 0 : s.n;
-  s.kv_start = clamp(g.kv_offsets[b], g.Tk);
-  s.m = clamp(g.kv_offsets[b + 1], g.Tk) - s.kv_start;
-  s.m = s.m < 0 ? 0 : s.m;
+  const FhipRows q = fhip_rows_between(g.offsets[b], g.offsets[b + 1], g.T),
+                 k = fhip_rows_between(g.kv_offsets[b], g.kv_offsets[b + 1], g.Tk);
+  s.start = q.first, s.n = q.count, s.kv_start = k.first, s.m = k.count;
   s.tiles = (s.n * g.group + ROWS - 1) / ROWS;
   return s;
 }

@@ -258,10 +258,8 @@ struct Sequence {
 };
 __device__ __forceinline__ Sequence pg_sequence(const PagedArgs &g, int b) {
   Sequence s;
-  const int a = g.offsets[b], e = g.offsets[b + 1];
-  s.start = a < 0 ? 0 : a > g.T ? g.T : a;
-  s.rows = (e > g.T ? g.T : e) - s.start;
-  s.rows = s.rows < 0 ? 0 : s.rows;
+  const FhipRows r = fhip_rows_between(g.offsets[b], g.offsets[b + 1], g.T);
+  s.start = r.first, s.rows = r.count;
   const int len = g.cache.lengths[b];
   s.length = len < 0 ? 0 : len;
   const int room = g.cache.table_pages * g.cache.page_size; // <= 2^30

@@ -47,7 +47,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void sdpa_rows_kernel(RowsArgs g) {
   const int b = fhip_sequence_of(g.offsets, g.batch, t);
   if (b < 0)
     return;
-  const int n = g.offsets[b + 1] - g.offsets[b], i = t - g.offsets[b];
+  const int64_t behind = (int64_t)g.offsets[b + 1] - t; // rows of the sequence from this one on
   int64_t first = 0, keys; // the sequence's keys; the first one's packed row
   int64_t stored; // keys that the page table has places for
   if (g.k) {
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void sdpa_rows_kernel(RowsArgs g) {
     keys = g.cache.lengths[b];
     stored = (int64_t)g.cache.table_pages * g.cache.page_size;
   }
-  int64_t seen = g.causal ? keys - n + i + 1 : keys;
+  int64_t seen = g.causal ? keys - behind + 1 : keys;
   bool bad = seen > stored;
   seen = seen < 0 ? 0 : bad ? stored : seen;
   for (int e = threadIdx.x; e < g.D; e += blockDim.x)

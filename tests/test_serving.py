@@ -179,3 +179,7 @@ def test_the_formula_of_4_bits_keeps_within_half_a_scale():
 # -- the C++ graph API (tests/cpp/test_serving_api.cpp) -------------------------
 def test_graph_api_on_the_host():
     cpp_binary("test_serving_api", 120, "host")
+
+
+def test_rows_of_any_offsets_on_the_host():
+    cpp_binary("test_serving_split", 60)
