@@ -59,8 +59,11 @@ __global__ __launch_bounds__(64) void append_rows_kernel(AppendArgs g) {
 #pragma clang fp contract(off)
   __shared__ float row[kCacheMaxDim];
   const int heads = g.Hq + 2 * g.Hkv;
-  const int t = (int)(blockIdx.x / (uint32_t)heads), which = (int)(blockIdx.x % (uint32_t)heads);
+  const uint32_t at_line = fhip_line_index(blockIdx.y);
+  const int t = (int)(at_line / (uint32_t)heads), which = (int)(at_line % (uint32_t)heads);
   const int lane = threadIdx.x;
+  if (t >= g.T)
+    return;
   const int b = fhip_sequence_of(g.offsets, g.cache.batch, t);
   if (b < 0)
     return;
@@ -121,7 +124,10 @@ struct ReadArgs {
 };
 
 __global__ __launch_bounds__(64) void read_rows_kernel(ReadArgs g) {
-  const int t = (int)(blockIdx.x / (uint32_t)(2 * g.Hkv)), which = (int)(blockIdx.x % (uint32_t)(2 * g.Hkv));
+  const uint32_t at_line = fhip_line_index(blockIdx.y);
+  const int t = (int)(at_line / (uint32_t)(2 * g.Hkv)), which = (int)(at_line % (uint32_t)(2 * g.Hkv));
+  if (t >= g.T)
+    return;
   const int b = fhip_sequence_of(g.offsets, g.cache.batch, t);
   if (b < 0)
     return;
@@ -248,7 +254,7 @@ __device__ __forceinline__ void hold(const FhipCacheView &c, const FhipPool &p, 
 template <bool BF16, int LANES, int N> __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g) {
 #pragma clang fp contract(off)
   const int l = threadIdx.x & 63;
-  const int t = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, at = l % LANES * 8;
+  const int t = (int)fhip_line_index(blockIdx.z) * (kThreads / LANES) + threadIdx.x / LANES, at = l % LANES * 8;
   const bool in = t < g.T;
   // heads of Q, of K, of V in slices of N
   const int q_slices = (g.Hq + N - 1) / N, k_slices = (g.Hkv + N - 1) / N;
@@ -339,7 +345,7 @@ template <bool BF16, int LANES, int N> __global__ __launch_bounds__(kThreads) vo
 template <bool BF16, int LANES, int N> __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs g) {
 #pragma clang fp contract(off)
   const int l = threadIdx.x & 63;
-  const int t = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, at = l % LANES * 8;
+  const int t = (int)fhip_line_index(blockIdx.z) * (kThreads / LANES) + threadIdx.x / LANES, at = l % LANES * 8;
   const bool in = t < g.T;
   const int slices = (g.Hkv + N - 1) / N;
   const RowPlace r = place_of<LANES>(g.cache, g.offsets, t, in);
@@ -650,15 +656,14 @@ int fhip_cache_append(fhip_ctx *ctx, const fhip_cache_append_desc *d, const fhip
       fhip_note_kernel(ctx, "cache_append bits=%d lanes=%d heads=%d", d->cache.k_params.rank ? 4 : 16, lanes, n);
       return with_lanes(d->k.dtype == FHIP_BFLOAT16, lanes, n, [&](auto bf, auto lc, auto nc) {
         hipLaunchKernelGGL((append_kernel<decltype(bf)::value, decltype(lc)::value, decltype(nc)::value>),
-                           dim3((unsigned)blocks, (unsigned)slices), dim3(kThreads), 0, ctx->stream, g);
+                           fhip_line_grid(blocks, (unsigned)slices), dim3(kThreads), 0, ctx->stream, g);
         FHIP_HIP_CHECK(ctx, hipGetLastError());
         return 0;
       });
     }
   }
   fhip_note_kernel(ctx, "cache_append_rows");
-  hipLaunchKernelGGL(append_rows_kernel, dim3((unsigned)((int64_t)g.T * (g.Hq + 2 * g.Hkv))), dim3(64), 0, ctx->stream,
-                     g);
+  hipLaunchKernelGGL(append_rows_kernel, fhip_line_grid((int64_t)g.T * (g.Hq + 2 * g.Hkv)), dim3(64), 0, ctx->stream, g);
   FHIP_HIP_CHECK(ctx, hipGetLastError());
   return 0;
 }
@@ -703,14 +708,14 @@ int fhip_cache_read(fhip_ctx *ctx, const fhip_cache_read_desc *d, const fhip_cac
       fhip_note_kernel(ctx, "cache_read bits=%d lanes=%d heads=%d", d->cache.k_params.rank ? 4 : 16, lanes, n);
       return with_lanes(d->k.dtype == FHIP_BFLOAT16, lanes, n, [&](auto bf, auto lc, auto nc) {
         hipLaunchKernelGGL((read_kernel<decltype(bf)::value, decltype(lc)::value, decltype(nc)::value>),
-                           dim3((unsigned)blocks, (unsigned)beside), dim3(kThreads), 0, ctx->stream, g);
+                           fhip_line_grid(blocks, (unsigned)beside), dim3(kThreads), 0, ctx->stream, g);
         FHIP_HIP_CHECK(ctx, hipGetLastError());
         return 0;
       });
     }
   }
   fhip_note_kernel(ctx, "cache_read_rows");
-  hipLaunchKernelGGL(read_rows_kernel, dim3((unsigned)((int64_t)g.T * 2 * g.Hkv)), dim3(64), 0, ctx->stream, g);
+  hipLaunchKernelGGL(read_rows_kernel, fhip_line_grid((int64_t)g.T * 2 * g.Hkv), dim3(64), 0, ctx->stream, g);
   FHIP_HIP_CHECK(ctx, hipGetLastError());
   return 0;
 }

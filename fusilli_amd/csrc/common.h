@@ -291,6 +291,16 @@ __device__ __forceinline__ void fhip_for_uniform_parts(int first, int step, int 
   }
 }
 
+// A line of workgroups that one dimension of a grid may not hold (its threads are a number below 2^32): rows of 2^22 in
+// two dimensions.  The last row has some behind the line's end, which a kernel leaves at once.
+constexpr int kFhipLineBits = 22;
+inline dim3 fhip_line_grid(int64_t workgroups, unsigned other = 0) {
+  constexpr int64_t row = 1ll << kFhipLineBits;
+  const unsigned x = (unsigned)(workgroups < row ? workgroups : row), y = (unsigned)((workgroups + row - 1) / row);
+  return other ? dim3(x, other, y) : dim3(x, y); // (`other`: the grid's second dimension is in use)
+}
+__device__ __forceinline__ uint32_t fhip_line_index(uint32_t row) { return (row << kFhipLineBits) + blockIdx.x; }
+
 // The first of `count` ascending values that is above `x` (-1: none), found by a wavefront with 64 of them at a time.
 __device__ __forceinline__ int fhip_first_above(const int32_t *values, int count, int x) {
   const int l = threadIdx.x & 63;

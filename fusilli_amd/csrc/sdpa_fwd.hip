@@ -433,7 +433,7 @@ __global__ __launch_bounds__(PACKED == 2 ? kWaves * 32 : kWaves * 64, 2) void sd
   for (int pass = 0; pass < passes; ++pass) {
   PackedItem item{};
   if constexpr (PACKED) {
-    item = sd_packed_item<kRows, CAUSAL>(g, (int)blockIdx.x);
+    item = sd_packed_item<kRows, CAUSAL>(g, (int)fhip_line_index(blockIdx.y));
     if (item.tile < 0 || item.tile * kRows >= item.n * g.group) // (the latter where offsets overlap)
       return;
   }
@@ -1575,7 +1575,7 @@ int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const v
         return fhip_fail(ctx, "sdpa: cannot reserve LDS");
       configured.mark(ctx->device);
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(cut == 2 ? kWaves * 32 : kWaves * 64), lds_bytes, ctx->stream, g);
+    hipLaunchKernelGGL(kernel, fhip_line_grid(tiles), dim3(cut == 2 ? kWaves * 32 : kWaves * 64), lds_bytes, ctx->stream, g);
     FHIP_HIP_CHECK(ctx, hipGetLastError());
     return 0;
   };

@@ -360,7 +360,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
       seq = Sequence{pg_lane(s.start, b), pg_lane(s.rows, b), pg_lane(s.length, b), pg_lane(s.tiles, b), pg_lane(s.chunks, b)};
     }
   };
-  int at = (int)blockIdx.x, stop = at + 1;
+  int at = (int)fhip_line_index(blockIdx.y), stop = at + 1;
   Pieces pieces{};
   if (cut) {
     pieces = Pieces::of(total, g.pieces);
@@ -1154,7 +1154,7 @@ int fhip_fast_sdpa_paged(fhip_ctx *ctx, const fhip_sdpa_paged_desc *d, const fhi
                                                 hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
         configured.mark(ctx->device);
       }
-      hipLaunchKernelGGL(kernel, dim3((unsigned)p.pieces), dim3(kWaves * 64), kLds, ctx->stream, g);
+      hipLaunchKernelGGL(kernel, fhip_line_grid(p.pieces), dim3(kWaves * 64), kLds, ctx->stream, g);
       return 0;
     };
     static FhipOncePerDevice configured[2]; // (two for each instance of this lambda)

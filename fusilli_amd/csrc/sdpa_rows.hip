@@ -41,7 +41,10 @@ constexpr int kRowWaves = 8;
 
 __global__ __launch_bounds__(64 * kRowWaves) void sdpa_rows_kernel(RowsArgs g) {
   extern __shared__ float query[]; // [D], then for each wavefront its maximum and sum, and [Dv] parts
-  const int t = (int)(blockIdx.x / (uint32_t)g.Hq), h = (int)(blockIdx.x % (uint32_t)g.Hq), hk = h / g.group;
+  const uint32_t line = fhip_line_index(blockIdx.y);
+  const int t = (int)(line / (uint32_t)g.Hq), h = (int)(line % (uint32_t)g.Hq), hk = h / g.group;
+  if (t >= g.T)
+    return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   float *const tops = query + g.D, *const sums = tops + waves, *const part = sums + waves;
   const int b = fhip_sequence_of(g.offsets, g.batch, t);
@@ -146,7 +149,7 @@ int launch_rows(fhip_ctx *ctx, RowsArgs &g, const fhip_tensor_desc &q, const fhi
   int waves = 1;
   while (waves < kRowWaves && rows * waves * 2 <= 8192)
     waves *= 2;
-  hipLaunchKernelGGL(sdpa_rows_kernel, dim3((unsigned)rows), dim3(64 * waves),
+  hipLaunchKernelGGL(sdpa_rows_kernel, fhip_line_grid(rows), dim3(64 * waves),
                      sizeof(float) * (g.D + waves * (g.Dv + 2)), ctx->stream, g);
   FHIP_HIP_CHECK(ctx, hipGetLastError());
   return 0;

@@ -2,6 +2,7 @@
 lines of pieces, small and infinite values."""
 import numpy as np
 import pytest
+import torch  # (before the library, which then shares its runtime)
 
 from fusilli_amd import capi
 from helpers import HT
@@ -85,3 +86,128 @@ def test_offsets_of_any_value(ctx, d, more, room, offsets, alone):
     cache.fetch(ctx)
     if alone:
         assert np.array_equal(cache.rows("v", b)[keys[b] - (hi - lo):], vl[lo:hi])
+
+
+# ---- more workgroups than one dimension of a grid holds ---------------------------------
+def desc_of(t, strides=None):
+    types = {torch.bfloat16: BF16, torch.float32: capi.FLOAT, torch.float16: capi.HALF}
+    return capi.TensorDesc.make(list(t.shape), list(t.stride() if strides is None else strides), types[t.dtype])
+
+
+def pages_of(k, v, table, lengths):
+    c = capi.CacheDesc()
+    c.k, c.v = desc_of(k), desc_of(v)
+    c.batch, c.pages_per_sequence = table.shape
+    c.page_stride = table.shape[1]
+    return c, capi.CachePointers.make(*(t.data_ptr() for t in (k, v, table, lengths)))
+
+
+def cuda_ints(values):
+    return torch.tensor(values, device="cuda", dtype=torch.int32)
+
+
+@pytest.fixture
+def own_stream():
+    """A context on the stream that torch's work of the test is on as well (of the null stream it would make its own)."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        c = capi.Context(0, stream.cuda_stream)
+        yield c
+        stream.synchronize()
+        c.close()
+    torch.cuda.empty_cache()
+
+
+def test_append_and_read_of_2_to_the_26_rows_of_heads(own_stream):
+    """The general kernels: one wavefront per row of a head, 2^32 threads and some more."""
+    c, t, page = own_stream, (1 << 25) + 3, 1 << 16
+    k, v = (torch.randn(t, 1, 2, device="cuda") for _ in "kv")
+    pools = [torch.zeros(t // page + 1, 1, page, 2, device="cuda") for _ in "kv"]
+    table = torch.arange(t // page + 1, device="cuda", dtype=torch.int32)[None]
+    lengths, offsets = cuda_ints([t]), cuda_ints([0, t])
+    cache, at = pages_of(*pools, table, lengths)
+    a = capi.CacheAppendDesc()
+    a.k, a.v, a.cache = desc_of(k), desc_of(v), cache
+    c.cache_append(a, at, k.data_ptr(), v.data_ptr(), offsets.data_ptr())
+    assert c.last_kernel() == "cache_append_rows"
+    for x, pool in zip((k, v), pools):
+        assert torch.equal(pool.view(-1, 1, 2)[:t], x) and not pool.view(-1, 2)[t:].any()
+    back = [torch.zeros_like(x) for x in (k, v)]
+    r = capi.CacheReadDesc()
+    r.k, r.v, r.cache = desc_of(k), desc_of(v), cache
+    c.cache_read(r, at, offsets.data_ptr(), *(x.data_ptr() for x in back))
+    assert c.last_kernel() == "cache_read_rows"
+    assert torch.equal(back[0], k) and torch.equal(back[1], v)
+
+
+def test_append_of_many_wide_rows(own_stream):
+    """The kernel of 16-bit rows, 64 lanes a row: every row is the same (a stride of 0) and goes to one page, but for the
+    last, which alone lies in another one."""
+    c, t, page, d = own_stream, (1 << 26) + 1, 1 << 14, 512
+    k, v = (torch.randn(1, 1, d, device="cuda").bfloat16() for _ in "kv")
+    pools = [torch.zeros(2, 1, page, d, device="cuda", dtype=torch.bfloat16) for _ in "kv"]
+    table = torch.zeros(1, t // page + 1, device="cuda", dtype=torch.int32)
+    table[0, -1] = 1
+    lengths, offsets = cuda_ints([t]), cuda_ints([0, t])
+    cache, at = pages_of(*pools, table, lengths)
+    a = capi.CacheAppendDesc()
+    a.k = a.v = capi.TensorDesc.make([t, 1, d], [0, d, 1], BF16)
+    a.cache = cache
+    c.cache_append(a, at, k.data_ptr(), v.data_ptr(), offsets.data_ptr())
+    assert c.last_kernel().startswith("cache_append bits=16 lanes=64")
+    for x, pool in zip((k, v), pools):
+        assert torch.equal(pool[0, 0], x[0].expand(page, d))
+        assert torch.equal(pool[1, 0, :1], x[0]) and not pool[1, 0, 1:].any()
+
+
+def test_read_of_2_to_the_29_rows(own_stream):
+    """The kernel of 16-bit rows, 8 lanes a row.  All pages but the last are one."""
+    c, t, page, d = own_stream, (1 << 29) + 1, 1 << 16, 8
+    pools = [torch.randn(2, 1, page, d, device="cuda").bfloat16() for _ in "kv"]
+    table = torch.zeros(1, t // page + 1, device="cuda", dtype=torch.int32)
+    table[0, -1] = 1
+    lengths, offsets = cuda_ints([t]), cuda_ints([0, t])
+    cache, at = pages_of(*pools, table, lengths)
+    outs = [torch.zeros(t, 1, d, device="cuda", dtype=torch.bfloat16) for _ in "kv"]
+    r = capi.CacheReadDesc()
+    r.k, r.v, r.cache = desc_of(outs[0]), desc_of(outs[1]), cache
+    c.cache_read(r, at, offsets.data_ptr(), *(x.data_ptr() for x in outs))
+    assert c.last_kernel().startswith("cache_read bits=16 lanes=8")
+    for pool, out in zip(pools, outs):
+        assert bool((out[:-1].view(-1, page, d) == pool[0, 0]).all()) and torch.equal(out[-1], pool[1, :, 0])
+
+
+@pytest.mark.parametrize("d,level", [(2, 1), (64, 2)])
+def test_packed_rows_of_2_to_the_24_tiles(own_stream, d, level):
+    """Sequences of one row each: what they see is their own V.  (K and V of all heads are one, by a stride of 0.)"""
+    c, heads = own_stream, 64
+    t = (1 << 20) + 1 if level == 1 else (1 << 18) + 1
+    kind = torch.float32 if level == 1 else torch.bfloat16
+    q, o = torch.randn(t, heads, d, device="cuda", dtype=kind), torch.zeros(t, heads, d, device="cuda", dtype=kind)
+    k, v = (torch.randn(t, 1, d, device="cuda", dtype=kind) for _ in "kv")
+    offsets = torch.arange(t + 1, device="cuda", dtype=torch.int32)
+    p = capi.SdpaPackedDesc()
+    p.q, p.o, p.batch, p.is_causal = desc_of(q), desc_of(o), t, 1
+    p.k = p.v = capi.TensorDesc.make([t, heads, d], [d, 0, 1], p.q.dtype)
+    assert c.lib.fhip_sdpa_packed_fwd_supported(p) == level
+    space = torch.empty(c.sdpa_packed_workspace(p) + 256, device="cuda", dtype=torch.uint8)
+    c.sdpa_packed_fwd(p, q.data_ptr(), k.data_ptr(), v.data_ptr(), offsets.data_ptr(), o.data_ptr(), workspace=(space.data_ptr() + 255) // 256 * 256)
+    assert c.last_kernel().startswith("sdpa_packed" if level == 2 else "sdpa_rows")
+    assert bool((o == v).all())
+
+
+def test_paged_rows_of_2_to_the_24_tiles(own_stream):
+    """Sequences of one row and one key, all in the same page."""
+    c, heads, t, d = own_stream, 64, (1 << 18) + 1, 64
+    q, o = (torch.randn(t, heads, d, device="cuda", dtype=torch.bfloat16) for _ in "qo")
+    pools = [torch.randn(1, heads, 16, d, device="cuda").bfloat16() for _ in "kv"]
+    table, lengths = torch.zeros(t, 1, device="cuda", dtype=torch.int32), torch.ones(t, device="cuda", dtype=torch.int32)
+    offsets = torch.arange(t + 1, device="cuda", dtype=torch.int32)
+    p = capi.SdpaPagedDesc()
+    p.q, p.o, p.is_causal = desc_of(q), desc_of(o), 1
+    p.cache, at = pages_of(*pools, table, lengths)
+    assert c.lib.fhip_sdpa_paged_fwd_supported(p) == 2
+    space = torch.empty(c.sdpa_paged_workspace(p) + 256, device="cuda", dtype=torch.uint8)
+    c.sdpa_paged_fwd(p, at, q.data_ptr(), offsets.data_ptr(), o.data_ptr(), (space.data_ptr() + 255) // 256 * 256)
+    assert c.last_kernel().startswith("sdpa_paged d=64")
+    assert bool((o == pools[1][0, :, 0]).all())
