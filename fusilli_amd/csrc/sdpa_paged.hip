@@ -310,8 +310,14 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
   constexpr int KD = HD / 32;      // MFMA steps of a score tile
   constexpr int SG = GG / 32;      // of them per group
   constexpr int PITCH = 17;        // floats per column of O in LDS
-  // (f16: P scale stays a number for scales up to half's range / 15)
-  constexpr float kRedo = Q4 && !BF16 ? 7.0f : 8192.0f;
+  constexpr float kRedo = 8192.0f;
+  // 4 bits under f16: P scale goes into the product, and scales are halves of any size.  So that it neither loses bits
+  // below f16's normal numbers nor passes its largest, a row's probabilities carry a factor 2^lift, which begins (with
+  // each new maximum) where the smallest half comes to 2^12, and falls to what brings the sum of a lane's products
+  // below kMost.
+  constexpr bool LIFT = Q4 && !BF16;
+  constexpr int kLift = 36;
+  constexpr float kMost = 32768.0f;
   using S = PagedShape<HD, G>;
   constexpr int ROW = S::kRow, SEGS = ROW / 16; // 4 bits: bytes of a row, 16-byte pieces of it
   constexpr int VB = GG / 32;      // bytes of a V row and group per lane
@@ -579,6 +585,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
     for (int n = 0; n < NG; ++n)
       z[n] = f32x4{0, 0, 0, 0}, lows[n] = scales[n] = 0.f;
     float m = kNegBig, sum = 0.f; // of row lq: maximum of Q . K over all lanes, sum over this lane's keys
+    int lift = LIFT ? kLift : 0;  // of row lq, in all of its lanes
 
     // ---- a chunk's steps: scores, probabilities p, their product with V ---------------------
     float s[8], p[8];
@@ -708,6 +715,16 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
     // inherits, with no maximum taken and nothing exchanged between lanes.  Only the first chunk, and one in which
     // some lane's probabilities rise above kRedo, take the maximum and rescale; O = sum(P V) / sum(P) does
     // not depend on m.
+    auto rescale = [&](float by) {
+      sum *= by;
+#pragma unroll
+      for (int j = 0; j < T; ++j)
+        o[j] *= by;
+      if constexpr (Q4)
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+          z[n] *= by, lows[n] *= by, scales[n] *= by;
+    };
     auto softmax = [&](int i, int bad) {
       const int key0 = (c0 + wave + kWaves * i) * kChunk;
       if (bad) { // (the asm keeps this a branch)
@@ -725,7 +742,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
       }
       float psum;
       auto exps = [&]() {
-        const float at_m = -(m * g.scale_log2e);
+        const float at_m = LIFT ? __builtin_fmaf(-m, g.scale_log2e, (float)lift) : -(m * g.scale_log2e);
         psum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -735,7 +752,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
       };
       if (i > 0)
         exps();
-      if (i == 0 || __builtin_amdgcn_ballot_w64(!(psum <= kRedo)) != 0) {
+      if (i == 0 || __builtin_amdgcn_ballot_w64(!(psum <= (LIFT ? __builtin_ldexpf(kRedo, lift) : kRedo))) != 0) {
         float top = s[0];
         asm volatile("" : "+v"(top)); // (keeps the maximum in this branch)
 #pragma unroll
@@ -744,16 +761,10 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float mn = fmaxf(m, top);
-        const float alpha = __builtin_amdgcn_exp2f((m - mn) * g.scale_log2e);
-        m = mn;
-        sum *= alpha;
-#pragma unroll
-        for (int j = 0; j < T; ++j)
-          o[j] *= alpha;
-        if constexpr (Q4)
-#pragma unroll
-          for (int n = 0; n < NG; ++n)
-            z[n] *= alpha, lows[n] *= alpha, scales[n] *= alpha;
+        const int raised = LIFT && mn > m ? kLift - lift : 0;
+        const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m - mn, g.scale_log2e, (float)raised));
+        m = mn, lift += raised;
+        rescale(alpha);
         exps();
       }
       sum += psum;
@@ -782,13 +793,34 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
         const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-          float ps[8];
+          float ps[8], part = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const f16x2 pr = pair_of(vpar, e >> 2, e & 3, n);
             ps[e] = __builtin_fmaf(p[e], (float)pr.x, 0.f);
             lows[n] = __builtin_fmaf(p[e], (float)pr.y, lows[n]);
-            scales[n] += ps[e];
+            if constexpr (LIFT)
+              part += ps[e];
+            else
+              scales[n] += ps[e];
+          }
+          if constexpr (LIFT) {
+            if (__builtin_amdgcn_ballot_w64(!(part <= kMost)) != 0) {
+              float most = part;
+              asm volatile("" : "+v"(most)); // (keeps this a branch)
+              most = fmaxf(most, __shfl_xor(most, 16, 64));
+              most = fmaxf(most, __shfl_xor(most, 32, 64));
+              // to between 2^14 and kMost; groups in front of this one have this chunk in their sums already
+              const int down = most > kMost && most < INFINITY ? (int)(__builtin_bit_cast(uint32_t, most) >> 23) - (127 + 14) : 0;
+              const float by = __builtin_ldexpf(1.0f, -down);
+              lift -= down;
+              part *= by;
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                p[e] *= by, ps[e] *= by;
+              rescale(by);
+            }
+            scales[n] += part;
           }
           const uint32_t pf[4] = {pg_pack<BF16>(ps[0], ps[1]), pg_pack<BF16>(ps[2], ps[3]),
                                   pg_pack<BF16>(ps[4], ps[5]), pg_pack<BF16>(ps[6], ps[7])};
@@ -907,6 +939,9 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
 
     // ---- the wavefronts' parts meet: O^T value r of tile n * TG + j is column
     // n * GG + (lg * 4 + r) * TG + j of row lq
+    const float drop = LIFT ? __builtin_ldexpf(1.0f, -lift) : 1.0f;
+    if constexpr (LIFT)
+      sum *= drop;
     if (beyond)
       sum = __builtin_nanf("");
     sum += __shfl_xor(sum, 16, 64);
@@ -923,6 +958,8 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
         scales[n] += __shfl_xor(scales[n], 16, 64);
         scales[n] += __shfl_xor(scales[n], 32, 64);
         even[n] = z[n][0] > 0.f ? scales[n] / z[n][0] : 1.f;
+        if constexpr (LIFT)
+          even[n] *= drop, lows[n] *= drop;
       }
 #pragma unroll
     for (int n = 0; n < NG; ++n)

@@ -7,7 +7,7 @@ import torch  # (before the library, which then shares its runtime)
 from fusilli_amd import capi
 from helpers import HT
 from serving import Cache, attend, check
-from test_serving_gpu import ints, rows_of
+from test_serving_gpu import check_paged, ints, rows_of, run_paged
 
 pytestmark = pytest.mark.gpu
 BF16 = capi.BFLOAT16
@@ -211,3 +211,45 @@ def test_paged_rows_of_2_to_the_24_tiles(own_stream):
     c.sdpa_paged_fwd(p, at, q.data_ptr(), offsets.data_ptr(), o.data_ptr(), (space.data_ptr() + 255) // 256 * 256)
     assert c.last_kernel().startswith("sdpa_paged d=64")
     assert bool((o == pools[1][0, :, 0]).all())
+
+
+# ---- 4 bits of any size -----------------------------------------------------------
+class Given:
+    """The values that a pool is made of, in the place of a generator."""
+
+    def __init__(self, values):
+        self.values = values
+
+    def standard_normal(self, dims):
+        return np.broadcast_to(self.values, dims)
+
+
+@pytest.mark.parametrize("dtype", [capi.HALF, BF16])
+@pytest.mark.parametrize("d,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("keys,room", [([700, 3, 90], 0), ([3000, 40], 4096)])
+@pytest.mark.parametrize("how", ["1e-3", "1e-4", "1e-5", "3e3", "rows", "groups", "rising", "falling", "constant"])
+def test_values_in_4_bits_of_any_size(ctx, dtype, d, group, keys, room, how):
+    """P times V's scale is rounded to the rows' type: it has to keep that type's bits for scales from half's smallest to
+    its largest, also where they change along the keys while the maximum moves, or from group to group."""
+    rng = np.random.default_rng([51, d, group, sum(keys)])
+    cache = Cache(rng, keys, 2, d, 16, dtype, group)
+    at = np.zeros([cache.pool, 1, 16, 1])  # each place's part of its sequence
+    for b, n in enumerate(keys):
+        j = np.arange(n)
+        at[cache.table[b, j // 16], 0, j % 16, 0] = j / n
+    size = {"rows": 10.0 ** rng.uniform(-5, 2, at.shape), "rising": 10.0 ** (-5 + 8 * at), "falling": 10.0 ** (3 - 8 * at),
+            "groups": np.repeat(10.0 ** rng.uniform(-3, 1, [1, 2, 1, d // group]), group, -1), "constant": 0.0}.get(how)
+    v = rng.standard_normal([cache.pool, 2, 16, d]) * (float(how) if size is None else size) + (0.3 if how == "constant" else 0)
+    cache.v = cache._pool(Given(v), d, None)
+    if how in ("rising", "falling"):  # scores that rise along the keys by e^40, so that the last ones count
+        k = rng.standard_normal([cache.pool, 2, 16, d]) * 0.2 + 40 * at / np.sqrt(d)
+        cache.k = cache._pool(Given(k), d, None)
+    if room:
+        cache.table = np.concatenate([cache.table, np.full([len(keys), room // 16 - cache.table.shape[1]], -7, np.int32)], 1)
+    q = rows_of(rng, [2 * len(keys), 4, d], dtype, std=1.0)
+    if how in ("rising", "falling"):
+        q = HT.from_logical(1.0 + 0.01 * q.logical(), dtype)
+    offsets = 2 * np.arange(len(keys) + 1)
+    got, level = run_paged(ctx, cache, keys, q, offsets)
+    assert level == 2
+    check_paged(cache, keys, q, offsets, got)
