@@ -427,8 +427,8 @@ int fhip_sdpa_packed_fwd(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d,
 /* Attention of each sequence's newest rows over its keys in a cache: single
  * tokens, drafts of several, chunks of a prompt.  is_causal: row i sees the
  * keys up to its own place; otherwise every row sees lengths[b] keys.  A row
- * that sees no key is 0; what lies behind lengths[b] never matters, a key that
- * only later rows see matters as above.  Needs 256-byte aligned workspace of
+ * that sees no key is 0 (one that sees only scores of -inf is NaN); what lies behind
+ * lengths[b] never matters, a key that only later rows see matters as above.  Needs 256-byte aligned workspace of
  * fhip_sdpa_paged_fwd_workspace_size bytes (parts of long sequences, sums over many; it holds
  * nothing between calls, and calls that overlap need one each).  supported: 2 for
  * bf16 / f16, D = Dv = 64 or 128, positive scale, pages of a multiple of 16 rows,

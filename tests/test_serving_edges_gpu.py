@@ -7,11 +7,19 @@ import torch  # (before the library, which then shares its runtime)
 from fusilli_amd import capi
 from helpers import HT
 from serving import Cache, attend, check
-from test_serving_gpu import check_paged, ints, rows_of, run_paged
+from test_serving_gpu import check_paged, ints, rows_of, run_packed, run_paged
 
 pytestmark = pytest.mark.gpu
 BF16 = capi.BFLOAT16
 INT_MIN = -2 ** 31
+
+
+def widened(cache, room):
+    """The cache's table with room for `room` keys, whose further entries are never read."""
+    more = room // cache.page - cache.table.shape[1]
+    if more > 0:
+        cache.table = np.concatenate([cache.table, np.full([len(cache.keys), more], -7, np.int32)], 1)
+    return cache
 
 
 # ---- metadata of any value -------------------------------------------------------
@@ -44,9 +52,7 @@ def test_offsets_of_any_value(ctx, d, more, room, offsets, alone):
     offsets = offsets + offsets[-1:] * more
     t, batch = 90, len(offsets) - 1
     keys = [int(x) for x in rng.integers(40, 60, batch)]
-    cache = Cache(rng, keys, 2, d, 16, BF16)
-    if room > cache.table.shape[1] * 16:
-        cache.table = np.concatenate([cache.table, np.full([batch, room // 16 - cache.table.shape[1]], -7, np.int32)], 1)
+    cache = widened(Cache(rng, keys, 2, d, 16, BF16), room)
     q, k, v = (rows_of(rng, [t, h, d], BF16) for h in (4, 2, 2))
     bufs, at, cached = [x.upload(ctx) for x in (q, k, v)], ints(ctx, offsets), cache.upload(ctx)
     p = capi.SdpaPagedDesc()
@@ -244,8 +250,7 @@ def test_values_in_4_bits_of_any_size(ctx, dtype, d, group, keys, room, how):
     if how in ("rising", "falling"):  # scores that rise along the keys by e^40, so that the last ones count
         k = rng.standard_normal([cache.pool, 2, 16, d]) * 0.2 + 40 * at / np.sqrt(d)
         cache.k = cache._pool(Given(k), d, None)
-    if room:
-        cache.table = np.concatenate([cache.table, np.full([len(keys), room // 16 - cache.table.shape[1]], -7, np.int32)], 1)
+    widened(cache, room)
     q = rows_of(rng, [2 * len(keys), 4, d], dtype, std=1.0)
     if how in ("rising", "falling"):
         q = HT.from_logical(1.0 + 0.01 * q.logical(), dtype)
@@ -253,3 +258,35 @@ def test_values_in_4_bits_of_any_size(ctx, dtype, d, group, keys, room, how):
     got, level = run_paged(ctx, cache, keys, q, offsets)
     assert level == 2
     check_paged(cache, keys, q, offsets, got)
+
+
+# ---- scores of -inf ---------------------------------------------------------------
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("room", [64, 4096])
+def test_keys_of_minus_infinity(ctx, d, room):
+    """A key with a score of -inf has no part; where a row sees no other one, the quotient is 0 / 0, not that of no key."""
+    rng = np.random.default_rng([52, d, room])
+    keys, offsets = [1, 40, 0, 33, 1500 if room > 1500 else 60], [0, 1, 2, 3, 5, 6]
+    cache = Cache(rng, keys, 2, d, 16, BF16)
+    k = cache.k[0].logical()
+    gone = [[0], [3, 39], [], range(33), range(keys[4])]
+    for b, js in enumerate(gone):
+        for j in js:
+            k[cache.table[b, j // 16], :, j % 16] = -np.inf
+    cache.k[0] = HT.from_logical(k, BF16)
+    widened(cache, room)
+    q = HT.from_logical(0.1 + np.abs(rng.standard_normal([6, 4, d])), BF16)
+    got, _ = run_paged(ctx, cache, keys, q, offsets)
+    assert np.isnan(got[0]).all() and np.isnan(got[3:]).all() and not got[2].any()
+    left = np.delete(np.arange(40), gone[1])
+    ref, far = attend(q.logical()[1:2].astype(np.float64), cache.rows("k", 1)[left], cache.rows("v", 1)[left], [38], BF16)
+    check(got[1:2], ref, far)
+    # the same through packed rows
+    k, v = (rows_of(rng, [sum(keys), 2, d], BF16) for _ in "kv")
+    kl, at = k.logical(), np.concatenate([[0], np.cumsum(keys)])
+    for b, js in enumerate(gone):
+        kl[[at[b] + j for j in js]] = -np.inf
+    got, _ = run_packed(ctx, q, HT.from_logical(kl, BF16), v, offsets, True, kv_offsets=at)
+    assert np.isnan(got[0]).all() and np.isnan(got[3:]).all() and not got[2].any()
+    ref, far = attend(q.logical()[1:2].astype(np.float64), kl[1:41][left], v.logical()[1:41][left].astype(np.float64), [38], BF16)
+    check(got[1:2], ref, far)
