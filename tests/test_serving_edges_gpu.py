@@ -290,3 +290,20 @@ def test_keys_of_minus_infinity(ctx, d, room):
     assert np.isnan(got[0]).all() and np.isnan(got[3:]).all() and not got[2].any()
     ref, far = attend(q.logical()[1:2].astype(np.float64), kl[1:41][left], v.logical()[1:41][left].astype(np.float64), [38], BF16)
     check(got[1:2], ref, far)
+
+
+# ---- layouts on the tuned kernel ----------------------------------------------------
+@pytest.mark.parametrize("d,group", [(64, 0), (128, 0), (64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("order,page,dtype", [((0, 2, 1, 3), 16, BF16), ((1, 0, 2, 3), 32, capi.HALF), ((2, 1, 0, 3), 48, BF16)])
+@pytest.mark.parametrize("keys,room", [([90, 1, 400], 0), ([90, 1, 2100], 4096)])
+def test_paged_layouts(ctx, d, group, causal, order, page, dtype, keys, room):
+    """Any order of a pool's dims, heads of Q outermost, rows of O apart, a scale, rows in front of the first sequence and
+    behind the last, in one workgroup for each tile and cut into pieces."""
+    rng = np.random.default_rng([53, d, group, page])
+    cache = widened(Cache(rng, keys, 2, d, page, dtype, group, order=order), room)
+    offsets = [2, 5, 6, 8]
+    q = rows_of(rng, [11, 6, d], dtype, "heads")
+    got, level = run_paged(ctx, cache, keys, q, offsets, causal, scale=0.11, o_how="wide")
+    assert level == 2 and ctx.last_kernel().startswith(f"sdpa_paged d={d} bits={4 if group else 16} group={group} cut={int(room > 0)}")
+    check_paged(cache, keys, q, offsets, got, causal, scale=0.11)
