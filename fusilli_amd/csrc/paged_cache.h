@@ -9,6 +9,12 @@
 #include "serving_split.h"
 
 constexpr int kCacheMaxDim = 512; // of a head
+// Scales that the tuned attention kernels take: their maxima are those of raw scores and begin at -1e30, whose multiple by
+// the scale has to stay a number (above, a row that sees nothing of a chunk would be exp2(-inf + inf)).
+constexpr float kCacheMaxScale = 1e8f;
+inline bool fhip_tuned_scale(bool has_scale, float scale) {
+  return !has_scale || (scale > 0.f && scale <= kCacheMaxScale);
+}
 constexpr int64_t kCacheMaxKeys = (1ll << 30); // of a sequence: places stay 32-bit numbers
 
 // One pool of a cache: K or V.  Strides in elements (bytes, in 4 bits).

@@ -44,7 +44,7 @@
 // node/sdpa_node.h:138-176 (rank 4, every dim 1 or the full extent).
 #include "common.h"
 #include "fast_paths.h"
-#include "serving_split.h"
+#include "paged_cache.h"
 
 #include <cstdlib>
 #include <type_traits>
@@ -1500,7 +1500,7 @@ bool fhip_fast_sdpa_packed_applicable(const fhip_sdpa_packed_desc *d) {
   const int64_t D = d->q.dim[2], T = d->q.dim[0], Tk = d->k.dim[0], group = d->q.dim[1] / d->k.dim[1];
   if ((dt != FHIP_BFLOAT16 && dt != FHIP_HALF) || (D != 64 && D != 128) || d->v.dim[2] != D)
     return false;
-  if (d->has_scale && !(d->scale > 0.f && d->scale < INFINITY)) // (maxima are taken over raw scores)
+  if (!fhip_tuned_scale(d->has_scale, d->scale))
     return false;
   const fhip_tensor_desc *ts[4] = {&d->q, &d->k, &d->v, &d->o};
   for (const fhip_tensor_desc *t : ts)

@@ -1094,8 +1094,7 @@ PagedPlan make_plan(const fhip_sdpa_paged_desc *d) {
   const int64_t T = d->q.dim[0], Hq = d->q.dim[1], D = d->q.dim[2], Hkv = d->cache.k.dim[1];
   if ((dt != FHIP_BFLOAT16 && dt != FHIP_HALF) || (D != 64 && D != 128) || d->o.dim[2] != D)
     return p;
-  // the running maximum is taken over raw scores: needs a positive scale
-  if (d->has_scale && !(d->scale > 0.f && d->scale < INFINITY))
+  if (!fhip_tuned_scale(d->has_scale, d->scale))
     return p;
   p.bf16 = dt == FHIP_BFLOAT16;
   p.hd = (int)D;

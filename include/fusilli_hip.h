@@ -401,7 +401,7 @@ typedef struct {
  * shows; other sequences' keys and values never do.  More than 64 sequences need
  * 256-byte aligned workspace of fhip_sdpa_packed_fwd_workspace_size bytes (what
  * fhip_sdpa_paged_fwd says about its own holds here).  supported: 2 for bf16 / f16,
- * D = Dv = 64 or 128, positive scale, rows (heads, and tensors at the call) on 16
+ * D = Dv = 64 or 128, scale in (0, 1e8], rows (heads, and tensors at the call) on 16
  * bytes, below 2 GiB per K or V tensor and T (Hq / Hkv)^2 below 2^32; 1 for other
  * sizes to 512 and f32. */
 typedef struct {
@@ -431,7 +431,7 @@ int fhip_sdpa_packed_fwd(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d,
  * lengths[b] never matters, a key that only later rows see matters as above.  Needs 256-byte aligned workspace of
  * fhip_sdpa_paged_fwd_workspace_size bytes (parts of long sequences, sums over many; it holds
  * nothing between calls, and calls that overlap need one each).  supported: 2 for
- * bf16 / f16, D = Dv = 64 or 128, positive scale, pages of a multiple of 16 rows,
+ * bf16 / f16, D = Dv = 64 or 128, scale in (0, 1e8], pages of a multiple of 16 rows,
  * groups of 32, 64 or 128, rows and parameters aligned to 16 and 4 bytes;
  * otherwise 1. */
 typedef struct {

@@ -144,6 +144,16 @@ def test_taken(what, d, dtype):
     assert SUPPORTED[what](None) == 0
 
 
+@pytest.mark.parametrize("what", ["packed", "paged"])
+@pytest.mark.parametrize("scale,level", [(1e8, 2), (1e-30, 2), (1.1e8, 1), (3e38, 1), (np.inf, 1), (np.nan, 1), (0.0, 1), (-1.0, 1)])
+def test_scales_of_the_tuned_kernels(what, scale, level):
+    x = MAKE[what]()
+    x.has_scale, x.scale = 1, scale
+    assert SUPPORTED[what](x) == level
+    x.has_scale = 0  # (then it is not read)
+    assert SUPPORTED[what](x) == 2
+
+
 def test_null_arguments():
     n = ctypes.c_size_t(1)
     for name, make in (("sdpa_packed_fwd", packed), ("sdpa_paged_fwd", paged), ("cache_append", append), ("cache_read", read)):

@@ -307,3 +307,36 @@ def test_paged_layouts(ctx, d, group, causal, order, page, dtype, keys, room):
     got, level = run_paged(ctx, cache, keys, q, offsets, causal, scale=0.11, o_how="wide")
     assert level == 2 and ctx.last_kernel().startswith(f"sdpa_paged d={d} bits={4 if group else 16} group={group} cut={int(room > 0)}")
     check_paged(cache, keys, q, offsets, got, causal, scale=0.11)
+
+
+# ---- scales -------------------------------------------------------------------------
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale,tuned", [(1e4, True), (1e9, False), (1e30, False)])
+def test_scales_that_leave_one_key(ctx, d, scale, tuned):
+    """Scores that differ by at least 1: the largest one has all of the probability, whatever a chunk's other rows see.  It
+    is rounded to bf16, and so is the result."""
+    rng = np.random.default_rng([54, d])
+    keys, lens = [70, 0, 33, 1100], [40, 2, 33, 3]
+    offsets = np.concatenate([[0], np.cumsum(lens)])
+    cache = widened(Cache(rng, keys, 1, d, 16, BF16), 2048)
+    kl = np.zeros(cache.k[0].logical().shape, np.float32)
+    for b, n in enumerate(keys):
+        j = np.arange(n)
+        order = rng.permutation(n)
+        kl[cache.table[b, j // 16], 0, j % 16, 0], kl[cache.table[b, j // 16], 0, j % 16, 1] = order // 128, order % 128
+    cache.k[0] = HT.from_logical(kl, BF16)
+    ql = np.zeros([offsets[-1], 2, d])
+    ql[:, :, 0], ql[:, :, 1] = 128, 1  # (q . k is the key's number in the permutation)
+    q = HT.from_logical(ql, BF16)
+    got, level = run_paged(ctx, cache, keys, q, offsets, scale=scale)
+    assert level == (2 if tuned else 1)
+    at = np.concatenate([[0], np.cumsum(keys)])
+    k, v = (HT.from_logical(np.concatenate([cache.rows(x, b) for b in range(4)]), BF16) for x in "kv")
+    packed, _ = run_packed(ctx, q, k, v, offsets, True, kv_offsets=at, scale=scale)
+    for b, (n, m) in enumerate(zip(lens, keys)):
+        score = k.logical()[at[b]:at[b + 1], 0, :2] @ [128, 1]
+        for i in range(n):
+            seen = max(m - n + i + 1, 0)
+            want = v.logical()[at[b] + np.argmax(score[:seen]), 0] if seen else np.zeros(d)
+            for out in (got, packed):
+                check(out[offsets[b] + i], np.broadcast_to(want, [2, d]), np.abs(want) * 2.01 * 2.0 ** -8, f"{b} {i}")
