@@ -1495,6 +1495,10 @@ int fhip_fast_sdpa(fhip_ctx *ctx, const fhip_sdpa_desc *d, const void *q,
 }
 
 // ---- packed sequences ------------------------------------------------------
+// Elements from a row of K or V to the next.  One row alone may come with any stride: the rows that a tile has behind it lie
+// outside the buffer with this one, and read as zeros.
+static int64_t packed_kv_stride(const fhip_tensor_desc &t) { return t.dim[0] > 1 ? t.stride[0] : t.dim[2]; }
+
 bool fhip_fast_sdpa_packed_applicable(const fhip_sdpa_packed_desc *d) {
   const int dt = d->q.dtype;
   const int64_t D = d->q.dim[2], T = d->q.dim[0], Tk = d->k.dim[0], group = d->q.dim[1] / d->k.dim[1];
@@ -1508,7 +1512,8 @@ bool fhip_fast_sdpa_packed_applicable(const fhip_sdpa_packed_desc *d) {
       if (t->dim[i] > 1 && t->stride[i] % 8 != 0)
         return false;
   // 32-bit offsets within a sequence's K or V; rows by a multiplication (pos_of)
-  if (Tk * d->k.stride[0] * 2 >= (1ll << 31) || Tk * d->v.stride[0] * 2 >= (1ll << 31) || Tk >= (1 << 30))
+  constexpr int64_t room = (1ll << 30) - 1; // elements
+  if (Tk > room || packed_kv_stride(d->k) > room / Tk || packed_kv_stride(d->v) > room / Tk)
     return false;
   return T * group < (1ll << 30) && T * group * group < (1ll << 32);
 }
@@ -1532,8 +1537,8 @@ int fhip_fast_sdpa_packed(fhip_ctx *ctx, const fhip_sdpa_packed_desc *d, const v
     return 0;
   SdpaArgs g{};
   g.q = (const char *)q, g.k = (const char *)k, g.v = (const char *)v, g.o = (char *)o;
-  g.q_ss = d->q.stride[0], g.q_sh = d->q.stride[1], g.k_ss = d->k.stride[0], g.k_sh = d->k.stride[1];
-  g.v_ss = d->v.stride[0], g.v_sh = d->v.stride[1], g.o_ss = d->o.stride[0], g.o_sh = d->o.stride[1];
+  g.q_ss = d->q.stride[0], g.q_sh = d->q.stride[1], g.k_ss = packed_kv_stride(d->k), g.k_sh = d->k.stride[1];
+  g.v_ss = packed_kv_stride(d->v), g.v_sh = d->v.stride[1], g.o_ss = d->o.stride[0], g.o_sh = d->o.stride[1];
   g.offsets = (const int32_t *)offsets, g.kv_offsets = (const int32_t *)(kv_offsets ? kv_offsets : offsets);
   g.batch = (int32_t)d->batch, g.T = (int32_t)d->q.dim[0], g.Tk = (int32_t)d->k.dim[0], g.Hkv = (int32_t)d->k.dim[1];
   g.group = (int32_t)(d->q.dim[1] / g.Hkv);

@@ -340,3 +340,42 @@ def test_scales_that_leave_one_key(ctx, d, scale, tuned):
             want = v.logical()[at[b] + np.argmax(score[:seen]), 0] if seen else np.zeros(d)
             for out in (got, packed):
                 check(out[offsets[b] + i], np.broadcast_to(want, [2, d]), np.abs(want) * 2.01 * 2.0 ** -8, f"{b} {i}")
+
+
+# ---- strides of dims of one -----------------------------------------------------------
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("stride", [0, 3, 8, 1 << 40])
+def test_one_row_of_any_stride(ctx, d, stride):
+    """The strides of dims of 1 are not used: neither their alignment nor their size matters, and what lies a stride behind
+    the row is not taken for another one."""
+    rng = np.random.default_rng([55, d])
+    v = rng.standard_normal([1, 1, d])
+    v[0, 0, d - 9] = np.inf
+    q, k, v = HT.from_logical(rng.standard_normal([1, 4, d]), BF16), rows_of(rng, [1, 1, d], BF16), HT.from_logical(v, BF16)
+    o = HT.from_logical(np.full([1, 4, d], 77.0), BF16)
+    p = capi.SdpaPackedDesc()
+    p.q, p.o = (capi.TensorDesc.make([1, 4, d], [stride, d, 1], BF16) for _ in "qo")
+    p.k, p.v = (capi.TensorDesc.make([1, 1, d], [stride, stride, 1], BF16) for _ in "kv")
+    p.batch, p.is_causal = 1, 1
+    bufs, bo = [x.upload(ctx) for x in (q, k, v)], o.upload(ctx)
+    assert ctx.lib.fhip_sdpa_packed_fwd_supported(p) == (1 if d == 80 else 2)
+    ctx.sdpa_packed_fwd(p, *bufs, ints(ctx, [0, 1]), bo)
+    assert np.array_equal(o.fetch(ctx, bo).logical(), np.broadcast_to(v.logical(), [1, 4, d]))
+    cache = Cache(rng, [7], 1, d, 16, BF16)
+    a = capi.CacheAppendDesc()
+    a.q, a.q_out, a.k, a.v, a.cache = p.q, p.o, p.k, p.v, cache.desc()
+    at = cache.upload(ctx)
+    ctx.cache_append(a, at, bufs[1], bufs[2], ints(ctx, [0, 1]), q=bufs[0], q_out=bo)
+    cache.fetch(ctx)
+    assert np.array_equal(o.fetch(ctx, bo).logical(), q.logical()) and np.array_equal(cache.rows("v", 0)[6], v.logical()[0])
+    r = capi.CacheReadDesc()
+    r.k, r.v, r.cache = p.k, p.v, cache.desc()
+    back = [HT.from_logical(np.full([1, 1, d], 77.0), BF16) for _ in "kv"]
+    outs = [x.upload(ctx) for x in back]
+    ctx.cache_read(r, at, ints(ctx, [0, 1]), *outs)
+    assert np.array_equal(back[1].fetch(ctx, outs[1]).logical(), v.logical())
+    g = capi.SdpaPagedDesc()
+    g.q, g.o, g.cache, g.is_causal = p.q, p.o, cache.desc(), 0
+    cache.v[0] = HT.from_logical(rng.standard_normal(cache.v[0].dims), BF16)
+    ctx.sdpa_paged_fwd(g, cache.upload(ctx), bufs[0], ints(ctx, [0, 1]), bo)
+    check_paged(cache, [7], q, [0, 1], o.fetch(ctx, bo).logical(), causal=False)
