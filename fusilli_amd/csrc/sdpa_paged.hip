@@ -85,43 +85,8 @@ struct PagedArgs {
   float *part_ml; // [piece][2][16] (m, l)
 };
 
-// Workgroups that share the line: two for each compute unit run at once.  In 4 bits, where a compute unit has more to
-// compute, their ends lie further apart, and 256 more with pieces of a quarter go where one is done: 6 batches of 64 chats
-// with drafts 112.3 us in the mean with 512 equal pieces, 112.1 with 1024, 107.0 with 512 and 512 quarters, 107.6 like this.
-constexpr int kLarge = 512, kPieces16 = kLarge, kPieces4 = kLarge + 256;
-constexpr int kQuarter = 4;
-// One round where pieces are fewer chunks than this: 8 chats of 8192 keys 31.2 us in two equal rounds, 25.5 in one.
-constexpr int kSmall = 64;
-// Chunks that a piece has at least, and keys up to which no sequence is cut (the
-// launch that joins pieces takes longer than what it saves).
-constexpr int kLeast = 2 * kWaves;
+// Keys up to which no sequence is cut (the launch that joins pieces takes longer than what it saves).
 constexpr int64_t kWhole = 1024;
-// A cut moves by up to a piece / kNear: 5 batches of 32 chats in 16 bits took 73 .. 90 us with 4, 66 .. 87 with 8, 66 .. 85 with
-// 16, of 64 in 4 bits with drafts 102 .. 126, 99 .. 122 and 100 .. 123.
-constexpr int kNear = 8;
-static_assert(kLeast >= kNear, "a cut at a segment's end is always near");
-
-// The pieces' places on the line: kLarge large ones, then small ones.
-struct Pieces {
-  int32_t large, small; // chunks of each
-  static __device__ __forceinline__ Pieces of(int total, int pieces) {
-    const int rest = total < pieces * kSmall ? 0 : pieces - kLarge;
-    Pieces p;
-    p.large = (int)(((int64_t)total * kQuarter - 1) / (kLarge * kQuarter + rest)) + 1;
-    p.large = p.large < kLeast ? kLeast : p.large;
-    p.small = (p.large + kQuarter - 1) / kQuarter;
-    p.small = p.small < kLeast ? kLeast : p.small;
-    return p;
-  }
-  __device__ __forceinline__ int64_t at(uint32_t i) const {
-    return i <= kLarge ? (int64_t)i * large : (int64_t)kLarge * large + (int64_t)(i - kLarge) * small;
-  }
-  // the last piece that begins at x or in front of it (places on the line are 31-bit numbers)
-  __device__ __forceinline__ int last(uint32_t x) const {
-    const uint32_t bend = (uint32_t)kLarge * (uint32_t)large;
-    return (int)(x < bend ? x / (uint32_t)large : kLarge + (x - bend) / (uint32_t)small);
-  }
-};
 
 template <bool BF16>
 __device__ __forceinline__ f32x4 pg_mfma(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4 c) {
@@ -367,9 +332,9 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
     }
   };
   int at = (int)fhip_line_index(blockIdx.y), stop = at + 1;
-  Pieces pieces{};
+  FhipPieces pieces{};
   if (cut) {
-    pieces = Pieces::of(total, g.pieces);
+    pieces = FhipPieces::of(total, g.pieces);
     // the piece's ends, each at a segment's own where that is near
     const int64_t from = pieces.at(blockIdx.x);
     auto snapped = [&](int64_t x) {
@@ -378,8 +343,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
       find((int)x);
       if (b < 0)
         return total;
-      const int near = pieces.large / kNear, inside = ((int)x - first) % seq.chunks;
-      return inside < near ? (int)x - inside : seq.chunks - inside < near ? (int)x - inside + seq.chunks : (int)x;
+      return pieces.moved((int)x, first, seq.chunks);
     };
     at = snapped(from);
     stop = snapped(pieces.at(blockIdx.x + 1));
@@ -1029,14 +993,12 @@ __global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_j
   const int hk = h / g.group;
   if (info.large < 1 || info.small < 1 || info.chunks < 1 || info.pos < 0) // (rows that offsets which overlap have left out hold anything)
     return;
-  // cuts that lie inside this segment and not near its ends
   const uint32_t row = (uint32_t)info.pos * (uint32_t)g.group + (uint32_t)(h - hk * g.group);
   const uint32_t item = (uint32_t)hk * (uint32_t)info.tiles + row / 16;
-  const Pieces cuts{info.large, info.small};
-  const uint32_t from = (uint32_t)info.first + item * (uint32_t)info.chunks, near = (uint32_t)info.large / kNear;
-  const int cut0 = cuts.last(from + near - 1) + 1, cut1 = cuts.last(from + (uint32_t)info.chunks - near);
-  const int begin = cut0 - 1, pieces = cut1 - cut0 + 2;
-  if ((uint32_t)info.chunks < 2 * near || pieces <= 1 || begin < 0 || pieces > g.pieces || begin > g.pieces - pieces)
+  const FhipParts parts_of = FhipPieces{info.large, info.small}.parts((uint32_t)info.first + item * (uint32_t)info.chunks,
+                                                                      (uint32_t)info.chunks, g.pieces);
+  const int begin = parts_of.begin, pieces = parts_of.count;
+  if (pieces == 0) // (its one workgroup has stored it)
     return;
   typedef float Vec __attribute__((ext_vector_type(VEC)));
   const PG_AS1 float *ml = (const PG_AS1 float *)g.part_ml;
@@ -1132,7 +1094,7 @@ PagedPlan make_plan(const fhip_sdpa_paged_desc *d) {
   p.cut = keys > kWhole && T * Hq <= (1 << 24) && tiles * ((keys + kChunk - 1) / kChunk) < (1ll << 31) - (1 << 24);
   p.pieces = tiles;
   if (p.cut) {
-    p.pieces = q4 ? kPieces4 : kPieces16;
+    p.pieces = q4 ? kFhipPieces4 : kFhipPieces16;
     p.part_at = ((size_t)T * sizeof(PagedArgs::Info) + 255) / 256 * 256;
     p.ml_at = p.part_at + (size_t)p.pieces * 2 * 16 * (size_t)D * 4;
     p.bytes = p.ml_at + (size_t)p.pieces * 2 * 16 * 8;

@@ -7,7 +7,7 @@ import torch  # (before the library, which then shares its runtime)
 from fusilli_amd import capi
 from helpers import HT
 from serving import Cache, attend, check
-from test_serving_gpu import check_paged, ints, rows_of, run_packed, run_paged
+from test_serving_gpu import check_paged, ints, rows_of, run_packed, run_paged, steps_of
 
 pytestmark = pytest.mark.gpu
 BF16 = capi.BFLOAT16
@@ -379,3 +379,35 @@ def test_one_row_of_any_stride(ctx, d, stride):
     cache.v[0] = HT.from_logical(rng.standard_normal(cache.v[0].dims), BF16)
     ctx.sdpa_paged_fwd(g, cache.upload(ctx), bufs[0], ints(ctx, [0, 1]), bo)
     check_paged(cache, [7], q, [0, 1], o.fetch(ctx, bo).logical(), causal=False)
+
+
+# ---- long lines of pieces -------------------------------------------------------------
+@pytest.mark.parametrize("d,group,dtype", [(64, 0, BF16), (64, 64, capi.HALF)])
+@pytest.mark.parametrize("what", ["many rows", "few rows"])
+def test_long_lines(ctx, d, group, dtype, what):
+    """Pieces of more than 64 chunks: their cuts move to the ends of segments that are near, and in 4 bits smaller ones follow
+    the large ones.  Sequences from shorter than a move to longer than many pieces, joined by one team a row and by several."""
+    rng = np.random.default_rng([56, d, group])
+    if what == "many rows":
+        hq, hk = 16, 2
+        keys, rows = [9000, 5, 120, 20000, 640, 3333, 1, 300, 14000, 7000, 250, 4444], [32, 3, 32, 31, 32, 32, 1, 17, 32, 32, 32, 30]
+    else:
+        hq, hk = 32, 2
+        keys, rows = [9000, 58500, 40], [1, 14, 1]
+    line = sum(-(-n // 32) * -(-r * (hq // hk) // 16) * hk for n, r in zip(keys, rows))
+    assert line > 768 * 64 and (sum(rows) * hq <= 512) == (what == "few rows")
+    cache = Cache(rng, keys, hk, d, 64, dtype, group)
+    offsets = np.concatenate([[0], np.cumsum(rows)])
+    q = rows_of(rng, [sum(rows), hq, d], dtype)
+    got, level = run_paged(ctx, cache, keys, q, offsets)
+    assert level == 2 and ctx.last_kernel().endswith("cut=1")
+    ql = q.logical().astype(np.float64)
+    values = {x: cache.values(x) for x in "kv"}
+    for b, (n, m) in enumerate(zip(rows, keys)):
+        j = np.arange(m)
+        k, v = (values[x][cache.table[b, j // 64], :, j % 64] for x in "kv")
+        some = np.arange(n) if n < 16 else np.arange(b % 2, n, 2)  # (a row of each tile of 16: 2 positions of 8 heads)
+        ref, far = attend(ql[offsets[b] + some], k, v, np.clip(m - n + 1 + some, 0, m), dtype, **steps_of(cache, b, m))
+        check(got[offsets[b] + some], ref, far, f"sequence {b}")
+    again, _ = run_paged(ctx, cache, keys, q, offsets)
+    assert np.array_equal(got, again)
