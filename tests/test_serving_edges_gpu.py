@@ -7,7 +7,7 @@ import torch  # (before the library, which then shares its runtime)
 from fusilli_amd import capi
 from helpers import HT
 from serving import Cache, attend, check
-from test_serving_gpu import check_paged, ints, rows_of, run_packed, run_paged, steps_of
+from test_serving_gpu import check_held, check_paged, ints, rows_of, run_packed, run_paged, steps_of
 
 pytestmark = pytest.mark.gpu
 BF16 = capi.BFLOAT16
@@ -411,3 +411,26 @@ def test_long_lines(ctx, d, group, dtype, what):
         check(got[offsets[b] + some], ref, far, f"sequence {b}")
     again, _ = run_paged(ctx, cache, keys, q, offsets)
     assert np.array_equal(got, again)
+
+
+# ---- appended from odd addresses --------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, capi.HALF])
+@pytest.mark.parametrize("group", [0, 32, 64])
+def test_append_from_odd_addresses_stores_what_it_should(ctx, dtype, group):
+    """The general kernel at the sizes of the vector one: both pools, codes and parameters, and nothing else of them."""
+    rng = np.random.default_rng([57, group])
+    keys, new, d = [30, 7], [3, 2], 64
+    at = np.concatenate([[0], np.cumsum(new)])
+    cache = Cache(rng, keys, 2, d, 16, dtype, group)
+    before = [[t.logical() for t in x] for x in (cache.k, cache.v)]
+    k, v = (rows_of(rng, [5, 2, d], dtype) for _ in "kv")
+    bufs = [ctx.to_device(np.concatenate([np.zeros(1, x.storage.dtype), x.storage.reshape(-1)])) for x in (k, v)]
+    a = capi.CacheAppendDesc()
+    a.k, a.v, a.cache = k.desc(), v.desc(), cache.desc()
+    ctx.cache_append(a, cache.upload(ctx), *(b.ptr + 2 for b in bufs), ints(ctx, at))
+    assert ctx.last_kernel() == "cache_append_rows"
+    cache.fetch(ctx)
+    place = np.concatenate([np.arange(m - n, m) for n, m in zip(new, keys)])
+    where = cache.table[np.repeat([0, 1], new), place // 16], place % 16
+    check_held(cache, before[0], [t.logical() for t in cache.k], where, k.logical(), group, dtype, "K")
+    check_held(cache, before[1], [t.logical() for t in cache.v], where, v.logical(), group, dtype, "V")
