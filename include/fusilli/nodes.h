@@ -894,7 +894,7 @@ inline ErrorObject checkCacheIndices(const CacheTensors &c,
   return checkIndices(c.lengths, op, "LENGTHS", {batch});
 }
 inline ErrorObject checkHeads(int64_t hq, int64_t hk, const std::string &op) {
-  FUSILLI_RETURN_ERROR_IF(hq % hk != 0, ErrorCode::InvalidAttribute,
+  FUSILLI_RETURN_ERROR_IF(hk <= 0 || hq % hk != 0, ErrorCode::InvalidAttribute,
                           op + " requires Q heads (" + std::to_string(hq) +
                               ") to be a multiple of K heads (" +
                               std::to_string(hk) + ")");

@@ -159,6 +159,27 @@ TEST("host: what no kernel takes is refused by compile") {
               "in type");
 }
 
+TEST("host: K and caches without heads are refused") {
+  for (int64_t heads : {0, -1}) {
+    Graph g = newGraph("headless");
+    Rows r = rowsOf(g, 20);
+    SdpaPackedAttr a;
+    a.setName("p");
+    g.sdpaPacked(r.q, g.tensor(mk("k0", {20, heads, kD}, DataType::BFloat16)), r.v, r.offsets, nullptr, a)->setOutput(true);
+    CHECK_ERROR(g.validate(), ErrorCode::InvalidAttribute,
+                "SDPA packed requires Q heads (4) to be a multiple of K heads (" + std::to_string(heads) + ")");
+    Graph h = newGraph("headless_cache");
+    Rows s = rowsOf(h, 2);
+    CacheTensors c = cacheOf(h);
+    c.k = h.tensor(mk("cache_k0", {kPool, heads, kPage, kD}, DataType::BFloat16));
+    SdpaPagedAttr b;
+    b.setName("a");
+    h.sdpaPaged(s.q, s.offsets, c, b)->setOutput(true);
+    CHECK_ERROR(h.validate(), ErrorCode::InvalidAttribute,
+                "SDPA paged requires Q heads (4) to be a multiple of K heads (" + std::to_string(heads) + ")");
+  }
+}
+
 // ---- on the GPU ----------------------------------------------------------------
 static Handle &gpu() {
   static Handle h = [] {
