@@ -42,7 +42,7 @@
 // bf16, 32 heads on 8 of 128: one token of each of 32 sequences of 16 to 8192 keys (354 MB) 66.9 us, 5.3 TB/s; of 64 with
 // 8192 keys each 320 us, 6.7 TB/s, a reading stream's rate.  4 bits, groups of 64: three tokens of 64 sequences of 16 to 16384
 // keys (391 MB) 91.5 us, 4.3 TB/s, one of 64 with 8192 124 us, 4.9 TB/s: the vector ALU works 71 % of the time on codes, scales
-// and probabilities (315 instructions a chunk), for two wavefronts a SIMD about what it can.
+// and probabilities (309 instructions a chunk), for two wavefronts a SIMD about what it can.
 #include "paged_cache.h"
 #include "fast_paths.h"
 
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(1024) void sdpa_paged_index_kernel(PagedArgs g) {
   }
 }
 
-// ONCE: rows share no keys but within a tile: a key is read once (non-temporal).
+// ONCE: rows share no keys but within a tile, as far as the host knows: a key is read once (non-temporal).
 template <bool BF16, int HD, int G, bool ONCE>
 __global__ __launch_bounds__(kWaves * 64)
 __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
@@ -1040,7 +1040,8 @@ __global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_j
 
 // Bytes of K and V that the page table has room for from which they are read as non-temporal: half of what the memory-side
 // cache holds.  64 chats of 8192 keys 364 us without, 322 with (4 bits 131.7, 126.1); one of 30000, which the cache keeps from
-// call to call, 31.3 and 33.0.
+// call to call, 31.3 and 33.0.  Sequences whose pages are the same, which only the device knows, lose by it: 64 of 4288 keys, 4096 of
+// them shared, 84 and 104 us (4 bits 68 and 72); with nothing shared 194 and 172, 32 of 8192 with 1024 shared 169 and 155.
 constexpr double kOnce = 128 << 20;
 struct PagedPlan {
   bool ok = false;

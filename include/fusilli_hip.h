@@ -402,7 +402,7 @@ typedef struct {
  * 256-byte aligned workspace of fhip_sdpa_packed_fwd_workspace_size bytes (what
  * fhip_sdpa_paged_fwd says about its own holds here).  supported: 2 for bf16 / f16,
  * D = Dv = 64 or 128, scale in (0, 1e8], rows (heads, and tensors at the call) on 16
- * bytes, below 2 GiB per K or V tensor and T (Hq / Hkv)^2 below 2^32; 1 for other
+ * bytes, Tk times the stride of K's and of V's rows below 2 GiB and T (Hq / Hkv)^2 below 2^32; 1 for other
  * sizes to 512 and f32. */
 typedef struct {
   fhip_tensor_desc q; /* [T, Hq, D] */
