@@ -365,7 +365,8 @@ int fhip_sdpa_fwd(fhip_ctx *ctx, const fhip_sdpa_desc *d, const void *q,
  *      group of G neighbouring elements.  Code c stands for low + scale * c:
  *        low = half(min), scale = half((max - low) / 15) (at least 0),
  *        c = round((x - low) * (1 / scale)) within 0 .. 15, 0 where scale is 0,
- *      in f32 with ties to even.  A group that holds an infinity or a NaN, or
+ *      in f32 with ties to even (a cache that the caller fills by other means has
+ *      scales of at least 0 as well).  A group that holds an infinity or a NaN, or
  *      whose low or scale is beyond half's range, is kept as (NaN, NaN).
  *
  *      Offsets, lengths and page numbers are device data and are not checked

@@ -6,6 +6,7 @@ import torch  # (before the library, which then shares its runtime)
 
 from fusilli_amd import capi
 from helpers import HT
+import test_serving_paths_gpu
 from serving import Cache, attend, check
 from test_serving_gpu import check_held, check_paged, ints, rows_of, run_packed, run_paged, steps_of
 
@@ -434,3 +435,37 @@ def test_append_from_odd_addresses_stores_what_it_should(ctx, dtype, group):
     where = cache.table[np.repeat([0, 1], new), place // 16], place % 16
     check_held(cache, before[0], [t.logical() for t in cache.k], where, k.logical(), group, dtype, "K")
     check_held(cache, before[1], [t.logical() for t in cache.v], where, v.logical(), group, dtype, "V")
+
+
+# ---- large pools, every step on one stream -----------------------------------------------
+@pytest.mark.parametrize("group", [0, 64])
+def test_a_pool_beyond_32_bits_on_one_stream(group):
+    """test_serving_paths_gpu's steps with torch's current stream not the null one, of which a context makes a stream of its
+    own: the copies into the pools and the calls are in order."""
+    with torch.cuda.stream(torch.cuda.Stream()):
+        test_serving_paths_gpu.test_a_pool_beyond_32_bits(group)
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("group", [32, 64])
+def test_missing_pages_and_keys_behind_the_table_in_f16(ctx, group):
+    """Rows that see them are NaN, the others of their tile and sequence are not, in the kernel that follows the products'
+    size too."""
+    rng = np.random.default_rng([59, group])
+    keys, rows = [40, 600, 20], [1, 300, 1]
+    cache = widened(Cache(rng, keys, 1, 64, 16, capi.HALF, group), 2048)
+    cache.table[1, 30] = cache.pool + 5  # (keys 480 .. 495)
+    lengths = [40, 600, 2049]
+    cache.table[2, :] = cache.table[0, 0]
+    q = rows_of(rng, [302, 2, 64], capi.HALF)
+    offsets = [0, 1, 301, 302]
+    got, level = run_paged(ctx, cache, lengths, q, offsets)
+    assert level == 2 and np.isnan(got[301]).all()
+    seen = 301 + np.arange(300)
+    assert np.isnan(got[1:301][seen > 480]).all() and np.isfinite(got[1:301][seen <= 480]).all()
+    ql = q.logical().astype(np.float64)
+    ref, far = attend(ql[:1], cache.rows("k", 0), cache.rows("v", 0), [40], capi.HALF, **steps_of(cache, 0, 40))
+    check(got[:1], ref, far)
+    cache.table[1, 30] = 0
+    ref, far = attend(ql[1:181], cache.rows("k", 1, 480), cache.rows("v", 1, 480), seen[:180], capi.HALF, **steps_of(cache, 1, 480))
+    check(got[1:181], ref, far)
