@@ -906,8 +906,9 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
     const float drop = LIFT ? __builtin_ldexpf(1.0f, -lift) : 1.0f;
     if constexpr (LIFT)
       sum *= drop;
-    // (0 / 1 where a row sees no key; 0 / 0 stays where all scores that it sees are -inf)
-    sum = beyond ? __builtin_nanf("") : seen == 0 ? 1.f : sum;
+    // (a row that sees no key has a sum below 0, and is 0 whatever values met its probabilities of 0; 0 / 0 stays where all
+    // scores that a row sees are -inf)
+    sum = beyond ? __builtin_nanf("") : seen == 0 ? -1.f : sum;
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     // The codes' part times the sum of P scale over that of its rounded values: their mean rounding is gone, and with it all
@@ -960,7 +961,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void sdpa_paged_kernel(PagedArgs g) {
       } else {
         const int r = qt * 16 + q, p = r / g.group;
         pg_store<BF16>(g.o, (int64_t)(seq.start + p) * g.o_st + (int64_t)(hk * g.group + r - p * g.group) * g.o_sh + d,
-                       acc / den);
+                       den < 0.f ? 0.f : acc / den);
       }
     }
     __syncthreads(); // (before the next segment's rows or sums)
@@ -1035,7 +1036,7 @@ __global__ __launch_bounds__((JoinShape<HD, TEAMS>::kThreads)) void sdpa_paged_j
   }
 #pragma unroll
   for (int i = 0; i < VEC; ++i)
-    pg_store<BF16>(g.o, (int64_t)t * g.o_st + (int64_t)h * g.o_sh + d + i, acc[i] / den);
+    pg_store<BF16>(g.o, (int64_t)t * g.o_st + (int64_t)h * g.o_sh + d + i, den < 0.f ? 0.f : acc[i] / den);
 }
 
 // Bytes of K and V that the page table has room for from which they are read as non-temporal: half of what the memory-side

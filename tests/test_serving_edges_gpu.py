@@ -469,3 +469,32 @@ def test_missing_pages_and_keys_behind_the_table_in_f16(ctx, group):
     cache.table[1, 30] = 0
     ref, far = attend(ql[1:181], cache.rows("k", 1, 480), cache.rows("v", 1, 480), seen[:180], capi.HALF, **steps_of(cache, 1, 480))
     check(got[1:181], ref, far)
+
+
+@pytest.mark.parametrize("d,group", [(64, 0), (128, 0), (128, 64), (80, 0)])
+@pytest.mark.parametrize("dtype", [BF16, capi.HALF])
+@pytest.mark.parametrize("room", [0, 2048])
+def test_rows_without_keys_beside_values_that_are_no_numbers(ctx, d, group, dtype, room):
+    """More rows than keys, whose values are NaN or infinite: the first rows see none of them and are 0."""
+    rng = np.random.default_rng([60, d, group])
+    keys, rows = [2, 30, 1200 if room else 70], [5, 41, 3]
+    offsets = np.concatenate([[0], np.cumsum(rows)])
+    cache = widened(Cache(rng, keys, 1, d, 16, dtype, group), room)
+    pool = cache.v[-1].logical()  # (values, or in 4 bits their parameters)
+    for b in range(2):
+        pool[cache.table[b, 0]] = np.nan if b else np.inf
+    cache.v[-1] = HT.from_logical(pool, cache.v[-1].dtype)
+    q = rows_of(rng, [offsets[-1], 2, d], dtype)
+    got, _ = run_paged(ctx, cache, keys, q, offsets)
+    assert not got[:3].any() and not got[5:16].any()
+    assert not np.isfinite(got[3:5]).any() and not np.isfinite(got[16:46]).any()
+    j = np.arange(keys[2])
+    with np.errstate(invalid="ignore"):
+        k, v = (cache.values(x)[cache.table[2, j // 16], :, j % 16] for x in "kv")
+    ref, far = attend(q.logical()[46:].astype(np.float64), k, v, keys[2] - 2 + np.arange(3), dtype, **steps_of(cache, 2, keys[2]))
+    check(got[46:], ref, far)
+    if not group:
+        at = np.concatenate([[0], np.cumsum(keys)])
+        kp, vp = (HT.from_logical(np.concatenate([cache.rows(x, b) for b in range(3)]), dtype) for x in "kv")
+        got, _ = run_packed(ctx, q, kp, vp, offsets, True, kv_offsets=at)
+        assert not got[:3].any() and not got[5:16].any() and not np.isfinite(got[16:46]).any()
