@@ -43,6 +43,8 @@ RED_NAMES = ["NOT_SET", "ADD", "SUM", "MUL", "MIN", "MAX", "AMAX", "AVG",
 RED = {n: i for i, n in enumerate(RED_NAMES)}
 
 OPERAND_NONE, OPERAND_TENSOR, OPERAND_SCALAR = 0, 1, 2
+# fhip_quantize_front
+QUANTIZE_FRONT = {"NONE": 0, "RMSNORM": 1, "SWISH_GATE": 2}
 
 
 class TensorDesc(Structure):
@@ -111,6 +113,28 @@ class NormDesc(Structure):
                 ("is_layernorm", c_int32), ("emit_stats", c_int32),
                 ("stats_dtype", c_int32), ("epilogue", Epilogue),
                 ("out_dtype", c_int32), ("out", TensorDesc)]
+
+
+class QuantizeRowsDesc(Structure):
+    _fields_ = [("x", TensorDesc), ("up", TensorDesc), ("q", TensorDesc),
+                ("scale_stride", c_int64), ("weight_stride", c_int64),
+                ("front", c_int32), ("has_weight", c_int32),
+                ("weight_dtype", c_int32), ("epsilon", c_float)]
+
+
+class MatmulQuantizedDesc(Structure):
+    _fields_ = [("a", TensorDesc), ("b", TensorDesc), ("c", TensorDesc),
+                ("epilogue", Epilogue), ("out_dtype", c_int32),
+                ("out", TensorDesc), ("a_scale_stride", c_int64),
+                ("b_scale_stride", c_int64), ("bias_stride", c_int64),
+                ("has_bias", c_int32), ("bias_dtype", c_int32)]
+
+
+class SampleDesc(Structure):
+    _fields_ = [("logits", TensorDesc), ("has_temperature", c_int32),
+                ("has_top_k", c_int32), ("has_top_p", c_int32),
+                ("has_min_p", c_int32), ("temperature", c_float),
+                ("top_k", c_int32), ("top_p", c_float), ("min_p", c_float)]
 
 
 class BatchNormDesc(Structure):
@@ -260,6 +284,16 @@ SYMBOLS = {
     "fhip_cache_read_workspace_size": (c_int, [POINTER(CacheReadDesc), POINTER(c_size_t)]),
     "fhip_cache_read_supported": (c_int, [POINTER(CacheReadDesc)]),
     "fhip_cache_read": (c_int, [_P, POINTER(CacheReadDesc), POINTER(CachePointers), _P, _P, _P, _P, c_size_t]),
+    "fhip_quantize_rows_workspace_size": (c_int, [POINTER(QuantizeRowsDesc), POINTER(c_size_t)]),
+    "fhip_quantize_rows_supported": (c_int, [POINTER(QuantizeRowsDesc)]),
+    "fhip_quantize_rows": (c_int, [_P, POINTER(QuantizeRowsDesc), _P, _P, _P, _P, _P, _P, c_size_t]),
+    "fhip_matmul_quantized_workspace_size": (c_int, [POINTER(MatmulQuantizedDesc), POINTER(c_size_t)]),
+    "fhip_matmul_quantized_supported": (c_int, [POINTER(MatmulQuantizedDesc)]),
+    "fhip_matmul_quantized": (c_int, [_P, POINTER(MatmulQuantizedDesc), _P, _P, _P, _P, _P, POINTER(_P), _P, _P,
+                                      c_size_t]),
+    "fhip_sample_workspace_size": (c_int, [POINTER(SampleDesc), POINTER(c_size_t)]),
+    "fhip_sample_supported": (c_int, [POINTER(SampleDesc)]),
+    "fhip_sample": (c_int, [_P, POINTER(SampleDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t]),
     "fhip_norm_fwd_workspace_size": (c_int, [POINTER(NormDesc), POINTER(c_size_t)]),
     "fhip_norm_fwd_supported": (c_int, [POINTER(NormDesc)]),
     "fhip_norm_fwd": (c_int, [_P, POINTER(NormDesc), _P, _P, _P, POINTER(_P), _P, _P, _P, _P, c_size_t]),
@@ -538,6 +572,36 @@ class Context:
         self._check(self.lib.fhip_cache_read(
             self.handle, byref(d), byref(cache), _p(offsets), _p(k), _p(v),
             None, 0))
+
+    def quantize_rows(self, d: QuantizeRowsDesc, x, q, scale, up=None, weight=None):
+        self._check(self.lib.fhip_quantize_rows(
+            self.handle, byref(d), _p(x), _p(up), _p(weight), _p(q), _p(scale),
+            None, 0))
+
+    def matmul_quantized(self, d: MatmulQuantizedDesc, a, b, a_scale, b_scale, out,
+                         bias=None, epilogue_operands=()):
+        self._check(self.lib.fhip_matmul_quantized(
+            self.handle, byref(d), _p(a), _p(b), _p(a_scale), _p(b_scale),
+            _p(bias), _epi_ptrs(epilogue_operands), _p(out), None, 0))
+
+    def sample_workspace(self, d: SampleDesc) -> int:
+        n = c_size_t(0)
+        if self.lib.fhip_sample_workspace_size(byref(d), byref(n)) != 0:
+            raise FusilliHipError(self.lib.fhip_last_error(None).decode())
+        return n.value
+
+    def sample(self, d: SampleDesc, logits, uniform, token, temperature=None,
+               top_k=None, top_p=None, min_p=None, probability=None,
+               workspace=None):
+        """`workspace`: a DeviceBuffer or address of at least
+        sample_workspace(d) bytes; allocated here when omitted."""
+        need = self.sample_workspace(d)
+        if need and workspace is None:
+            workspace = self.alloc(need)
+        self._check(self.lib.fhip_sample(
+            self.handle, byref(d), _p(logits), _p(uniform), _p(temperature),
+            _p(top_k), _p(top_p), _p(min_p), _p(token), _p(probability),
+            _p(workspace), need))
 
     def norm_fwd(self, d: NormDesc, x, scale, bias, out, mean=None, rstd=None,
                  epilogue_operands=()):

@@ -351,6 +351,13 @@ __device__ __forceinline__ CT fhip_load(const void *p, int dt, int64_t idx) {
   }
 }
 
+// The same of a tensor of f32, bf16 or f16.
+__device__ __forceinline__ float fhip_load_float(const void *p, int dt, int64_t idx) {
+  return dt == FHIP_FLOAT      ? ((const float *)p)[idx]
+         : dt == FHIP_BFLOAT16 ? (float)((const __bf16 *)p)[idx]
+                               : (float)((const _Float16 *)p)[idx];
+}
+
 // N values `step` apart in a tensor of f32, bf16 or f16: one choice for all.  A launch of a few
 // workgroups waits for its code as it does for its data; four calls of fhip_store
 // are 7 KB, of which each executes a line of its own.
@@ -413,6 +420,22 @@ __device__ __forceinline__ void fhip_store(void *p, int dt, int64_t idx, CT v) {
   default:
     break;
   }
+}
+
+// Scales of a product of 8-bit codes, one for each row of A and each column of B, and its bias.
+struct FhipProductScales {
+  const float *a, *b;
+  const void *bias; // or null
+  int64_t a_s, b_s, bias_s; // 0: one for all
+  int32_t bias_dt;
+  __device__ __forceinline__ float row(int64_t m) const { return a[m * a_s]; }
+  __device__ __forceinline__ float column(int64_t n) const { return b[n * b_s]; }
+  __device__ __forceinline__ float bias_of(int64_t n) const { return bias ? fhip_load_float(bias, bias_dt, n * bias_s) : -0.f; }
+};
+// One form for all kernels, so that results do not depend on which of them ran (x * y + -0 is
+// x * y: without a bias the product is what is rounded).
+__device__ __forceinline__ float fhip_scaled(int sum, float row, float column, float bias) {
+  return __builtin_fmaf((float)sum * row, column, bias);
 }
 
 // Round a compute-type value through a storage dtype (the rounding point of a

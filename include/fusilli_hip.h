@@ -501,6 +501,121 @@ int fhip_cache_read(fhip_ctx *ctx, const fhip_cache_read_desc *d,
                     const fhip_cache_ptrs *cache, const void *offsets, void *k,
                     void *v, void *workspace, size_t workspace_bytes);
 
+/* ---- models served in 8 bits.  The reference has none of the following; they
+ *      stand beside fhip_matmul and fhip_norm_fwd and share their conventions.
+ *
+ *      fhip_quantize_rows brings rows to 8-bit codes, with the operation that
+ *      stands in front of a linear layer: y = f(x) in f32,
+ *        FHIP_QUANTIZE_NONE        x
+ *        FHIP_QUANTIZE_RMSNORM     x / sqrt(mean(x^2) + epsilon) * weight
+ *                                  (weight: optional vector of K elements)
+ *        FHIP_QUANTIZE_SWISH_GATE  x / (1 + exp(-x)) * up
+ *      and of each row, with a = max |y|,
+ *        scale = a / 127, code = rint(y * (127 / a)) within -127 .. 127,
+ *      so that a code stands for code * scale.  A row of zeros has scale 0 and
+ *      codes 0, a row whose y holds a NaN or an infinity scale NaN and codes 0.
+ *      (Where a is below 2^-100 both factors of the product are taken 2^64
+ *      times as large; scales below 2^-126 are subnormal and lose bits.)
+ *      X's type: f32, bf16 or f16; strides are free.  supported: 2 for rows and
+ *      codes with a last stride of 1 whose starts and K lie on 16 bytes of X (and UP) and 8
+ *      codes, K at most 16384, X and weight of one type; otherwise 1. ------- */
+typedef enum {
+  FHIP_QUANTIZE_NONE = 0,
+  FHIP_QUANTIZE_RMSNORM = 1,
+  FHIP_QUANTIZE_SWISH_GATE = 2
+} fhip_quantize_front;
+
+typedef struct {
+  fhip_tensor_desc x;    /* [rows, K] */
+  fhip_tensor_desc up;   /* [rows, K], X's type (swish gate); rank 0 otherwise */
+  fhip_tensor_desc q;    /* [rows, K] Int8 */
+  int64_t scale_stride;  /* elements between the rows' scales (Float) */
+  int64_t weight_stride; /* and between the weight's elements */
+  int32_t front;         /* fhip_quantize_front */
+  int32_t has_weight;    /* RMS norm */
+  int32_t weight_dtype;  /* f32, bf16 or f16 */
+  float epsilon;
+} fhip_quantize_rows_desc;
+
+int fhip_quantize_rows_workspace_size(const fhip_quantize_rows_desc *d,
+                                      size_t *bytes);
+int fhip_quantize_rows_supported(const fhip_quantize_rows_desc *d);
+int fhip_quantize_rows(fhip_ctx *ctx, const fhip_quantize_rows_desc *d,
+                       const void *x, const void *up, const void *weight,
+                       void *q, void *scale, void *workspace,
+                       size_t workspace_bytes);
+
+/* Product of 8-bit codes with a scale for each row of A and each column of B:
+ *   C[m][n] = round((sum over k of A[m][k] B[k][n]) * a_scale[m] * b_scale[n] + bias[n])
+ * with whole sums (K is at most 131071, so that they stay below 2^31) brought to
+ * f32, products from left to right and one rounding to C's type; then the fused
+ * chain, as for fhip_matmul.  A stride of 0 between scales: one for all.
+ * Whatever way the work is cut, the results are the same.  Needs no workspace;
+ * where few tiles share a long K it uses the context's scratch like fhip_matmul.
+ * supported: 2 where fhip_matmul takes Int8 operands of this layout on its tiled
+ * kernels and C, OUT and the chain are what it takes of float products;
+ * otherwise 1 (the direct kernels, or for any strides one thread per result). */
+typedef struct {
+  fhip_tensor_desc a; /* [M, K] Int8 */
+  fhip_tensor_desc b; /* [K, N] Int8 */
+  fhip_tensor_desc c; /* [M, N] f32, bf16 or f16 */
+  fhip_epilogue epilogue;
+  int32_t out_dtype;
+  fhip_tensor_desc out;
+  int64_t a_scale_stride, b_scale_stride; /* between scales (Float) */
+  int64_t bias_stride;
+  int32_t has_bias;
+  int32_t bias_dtype; /* f32, bf16 or f16 */
+} fhip_matmul_quantized_desc;
+
+int fhip_matmul_quantized_workspace_size(const fhip_matmul_quantized_desc *d,
+                                         size_t *bytes);
+int fhip_matmul_quantized_supported(const fhip_matmul_quantized_desc *d);
+int fhip_matmul_quantized(fhip_ctx *ctx, const fhip_matmul_quantized_desc *d,
+                          const void *a, const void *b, const void *a_scale,
+                          const void *b_scale, const void *bias,
+                          const void *const *epilogue_operands, void *out,
+                          void *workspace, size_t workspace_bytes);
+
+/* A token for each row of logits, drawn with the caller's random numbers.  With m
+ * a row's largest logit and T its temperature, word i has the weight
+ *   w_i = exp((logit_i - m) / T), 1 for the largest,
+ * in f64, held as a whole multiple of 2^-40.  Words are ordered by their logits, the
+ * largest first, equal ones by their index, and the first so many are kept as the
+ * strictest of these says:
+ *   top_k   the first top_k (0 or less: all);
+ *   top_p   of what top_k keeps, the fewest whose weights' sum reaches top_p of
+ *           all of it (1 or more, or NaN: all; 0 or less: the first);
+ *   min_p   those whose weight is at least min_p (NaN: all);
+ * one at least.  TOKEN is the first word in that order up to which the kept weights'
+ * sum exceeds uniform times all of it (uniform in [0, 1); values outside count as
+ * the nearest inside, NaN as 0), PROBABILITY its weight over that sum.  T that is
+ * not above 0: the first word, with probability 1.  Logits that are NaN or -inf are
+ * never drawn; a row of nothing else has token -1 and probability 0.  The settings
+ * are vectors of `rows` elements on the device or, where there is none, the
+ * descriptor's.  At most 2^24 words.  Needs 256-byte aligned workspace of
+ * fhip_sample_workspace_size bytes; it holds nothing between calls, and calls that
+ * overlap need one each.  supported: 2 for a last stride of 1; otherwise 1. */
+typedef struct {
+  fhip_tensor_desc logits; /* [rows, words] f32, bf16 or f16 */
+  int32_t has_temperature, has_top_k, has_top_p, has_min_p;
+  float temperature; /* without a vector */
+  int32_t top_k;
+  float top_p, min_p;
+} fhip_sample_desc;
+
+int fhip_sample_workspace_size(const fhip_sample_desc *d, size_t *bytes);
+int fhip_sample_supported(const fhip_sample_desc *d);
+int fhip_sample(fhip_ctx *ctx, const fhip_sample_desc *d, const void *logits,
+                const void *uniform,     /* Float [rows] */
+                const void *temperature, /* Float [rows] or null */
+                const void *top_k,       /* Int32 [rows] or null */
+                const void *top_p,       /* Float [rows] or null */
+                const void *min_p,       /* Float [rows] or null */
+                void *token,             /* Int32 [rows] */
+                void *probability,       /* Float [rows] or null */
+                void *workspace, size_t workspace_bytes);
+
 /* ---- RMSNorm / LayerNorm forward (node/rmsnorm_node.h:38-219,
  *      node/layernorm_node.h:38-264, node/norm_utils.h:27-99;
  *      aten.rms_norm / aten.(native_)layer_norm,
