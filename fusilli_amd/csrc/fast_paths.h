@@ -6,7 +6,8 @@
 
 #include "common.h"
 
-bool fhip_fast_matmul_applicable(const fhip_matmul_desc *d);
+// `scaled`, `scales`: int8 operands whose sums are scaled (the descriptor's C and chain are floats).
+bool fhip_fast_matmul_applicable(const fhip_matmul_desc *d, bool scaled = false);
 int fhip_fast_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a,
                      const void *b, const DevEpilogue &epi, void *out);
 
@@ -14,7 +15,8 @@ int fhip_fast_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a,
 // a 128-byte slice, or those below.  `handled` false where none takes the descriptor, `short_k`
 // true where that is for the speed of the general path's f32 tiles over a short K.
 int fhip_tuned_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a, const void *b,
-                      const DevEpilogue &epi, void *out, bool *handled, bool *short_k);
+                      const DevEpilogue &epi, void *out, bool *handled, bool *short_k,
+                      const FhipProductScales *scales = nullptr);
 
 // Few rows or columns, K or row starts that do not fit that contract, f32, and few tiles, on
 // kernels that load MFMA fragments straight from global memory or stage tiles through
@@ -22,7 +24,7 @@ int fhip_tuned_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a, c
 // `other_us` (0: there is no other).  `whole`: the contract holds.
 int fhip_direct_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a, const void *b,
                        const DevEpilogue &epi, void *out, double other_us, bool whole, bool *handled,
-                       bool *short_k);
+                       bool *short_k, const FhipProductScales *scales = nullptr);
 
 // `allow_scratch` false: only plans that leave the context's scratch alone
 // (no zero-padded channel copies, no split reduction) -- for the entry point

@@ -58,7 +58,7 @@ bool short_k(const DirectPlan &p, const DirectArgs &g, int64_t M, int64_t N, int
   return K < (tiles <= 256 ? (p.b_kc ? 20 : 12) : (p.b_kc ? 50 : 40) + (tiles >= 1024 ? 8 : 0));
 }
 
-bool direct_plan(const fhip_matmul_desc *d, DirectPlan *p, DirectArgs *g, int64_t *batch, double *us,
+bool direct_plan(const fhip_matmul_desc *d, bool scaled, DirectPlan *p, DirectArgs *g, int64_t *batch, double *us,
                  bool *too_short) {
   const int r = d->a.rank;
   if ((r != 2 && r != 3) || d->a.dtype != d->b.dtype)
@@ -66,7 +66,7 @@ bool direct_plan(const fhip_matmul_desc *d, DirectPlan *p, DirectArgs *g, int64_
   switch (d->a.dtype) {
   case FHIP_BFLOAT16: p->kind = GK_BF16; break;
   case FHIP_HALF: p->kind = GK_F16; break;
-  case FHIP_INT8: p->kind = GK_I8; break;
+  case FHIP_INT8: p->kind = scaled ? GK_I8S : GK_I8; break;
   case FHIP_FP8E4M3: p->kind = GK_FP8E4M3; break;
   case FHIP_FP8E5M2: p->kind = GK_FP8E5M2; break;
   case FHIP_FLOAT: p->kind = GK_F32; break;
@@ -139,7 +139,7 @@ bool direct_plan(const fhip_matmul_desc *d, DirectPlan *p, DirectArgs *g, int64_
   *us = best;
   // (16-bit operands into f32: the f32 tiles would be further from the exact sums, f16 K24
   // 1.3 units of 2^-24 against 0.7)
-  const bool f32_of_16 = p->kind != GK_F32 && d->c.dtype == FHIP_FLOAT && d->out.dtype == FHIP_FLOAT;
+  const bool f32_of_16 = p->kind != GK_F32 && p->kind != GK_I8S && d->c.dtype == FHIP_FLOAT && d->out.dtype == FHIP_FLOAT;
   *too_short = !f32_of_16 && short_k(*p, *g, M, N, K, *batch);
   if (*too_short)
     return false;
@@ -258,13 +258,13 @@ double tile_plan(const DirectPlan &dp, const DirectArgs &g, int elem, bool gelu,
 
 int fhip_direct_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a, const void *b,
                        const DevEpilogue &epi, void *out, double other_us, bool whole, bool *handled,
-                       bool *short_k) {
+                       bool *short_k, const FhipProductScales *scales) {
   *handled = *short_k = false;
   DirectPlan p;
   DirectArgs g{};
   int64_t batch = 1;
   double us = 0;
-  if (!direct_plan(d, &p, &g, &batch, &us, short_k))
+  if (!direct_plan(d, scales != nullptr, &p, &g, &batch, &us, short_k))
     return 0;
   // operands at their own alignment
   const uintptr_t am = fhip_dtype_size(d->a.dtype) - 1;
@@ -273,6 +273,8 @@ int fhip_direct_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a, 
   g.a = (const char *)a;
   g.b = (const char *)b;
   g.out = (char *)out;
+  if (scales)
+    g.scales = *scales;
   g.epi = epi;
   g.epi.rank = 3;
   const int r = d->a.rank;
@@ -295,7 +297,7 @@ int fhip_direct_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a, 
   }
   // f32 results of 16-bit or fp8 operands keep the kernel they had: the length of the chains
   // that the sums are taken in shows there.
-  const bool f32_out = p.kind != GK_I8 && d->c.dtype == FHIP_FLOAT && d->out.dtype == FHIP_FLOAT;
+  const bool f32_out = p.kind != GK_I8 && !scales && d->c.dtype == FHIP_FLOAT && d->out.dtype == FHIP_FLOAT;
   // Split products over a long K stay on the tiled GEMM, and so do those over one whole slice (bf16
   // 5696 x 5184 x 64 in four batches 59 us, here 416; 1536 x 448 x 64 5.7 / 9.5); those over less
   // than a slice stay here.
@@ -329,12 +331,13 @@ int fhip_direct_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a, 
       return 1;
   }
   if (p.tile) {
-    static const char *const kKindName[] = {"bf16", "f16", "i8", "fp8e4m3", "fp8e5m2"};
+    static const char *const kKindName[] = {"bf16", "f16", "i8", "fp8e4m3", "fp8e5m2", "f32", "i8s"};
     fhip_note_kernel(ctx, "gemm_mfma %s %dx%d waves=%d split=%d", kKindName[p.kind], 16 * p.mt, 16 * p.nt, p.waves, g.splits);
     switch (p.kind) {
     case GK_BF16: return tile_launch_bf16(ctx, p, g, batch);
     case GK_F16: return tile_launch_f16(ctx, p, g, batch);
     case GK_I8: return tile_launch_i8(ctx, p, g, batch);
+    case GK_I8S: return tile_launch_i8s(ctx, p, g, batch);
     case GK_FP8E4M3: return tile_launch_fp8e4m3(ctx, p, g, batch);
     default: return tile_launch_fp8e5m2(ctx, p, g, batch);
     }
@@ -344,6 +347,7 @@ int fhip_direct_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a, 
   case GK_BF16: return direct_launch_bf16(ctx, p, g, batch);
   case GK_F16: return direct_launch_f16(ctx, p, g, batch);
   case GK_I8: return direct_launch_i8(ctx, p, g, batch);
+  case GK_I8S: return direct_launch_i8s(ctx, p, g, batch);
   case GK_FP8E4M3: return direct_launch_fp8e4m3(ctx, p, g, batch);
   case GK_FP8E5M2: return direct_launch_fp8e5m2(ctx, p, g, batch);
   default: return direct_launch_f32(ctx, p, g, batch);

@@ -52,6 +52,7 @@ struct DirectArgs {
   // none), which depends on the column alone
   int32_t lean, lean_op;
   DevEpilogue epi; // strides over (batch, m, n)
+  FhipProductScales scales; // GK_I8S
 };
 
 template <int KIND> struct DirectKind {
@@ -62,7 +63,7 @@ template <int KIND> struct DirectKind {
   static constexpr int KS = 4 * CE;            // K of a step (one MFMA, f32: four)
   static constexpr int SK = 128 / ELEM;        // K of a slice
   static constexpr int STEPS = SK / KS;        // steps of a slice: 2 (fp8: 1)
-  using Acc = std::conditional_t<KIND == GK_I8, int, float>;
+  using Acc = std::conditional_t<KIND == GK_I8 || KIND == GK_I8S, int, float>;
   typedef Acc Acc4 __attribute__((ext_vector_type(4)));
 };
 
@@ -308,7 +309,7 @@ __device__ __forceinline__ void direct_coord(int q, int *m, int *dm, int *n) {
 // Finishes and stores N values of column n, value i at row rows[i] (all values of
 // a thread together: a fused operand's loads are then one round trip, not one per
 // four values -- a bias on 64 x 64 tiles cost 6 us).
-template <typename Acc, int N>
+template <typename Acc, int N, bool SCALED = false>
 __device__ __forceinline__ void direct_store(const DirectArgs &g, int64_t batch, const int (&row)[N], int n,
                                              const Acc (&acc)[N]) {
   if (n >= g.N)
@@ -321,16 +322,26 @@ __device__ __forceinline__ void direct_store(const DirectArgs &g, int64_t batch,
     at[r] = batch * g.o_batch + (int64_t)n * g.o_sn + rows[r] * g.o_sm;
     live |= (uint32_t)(row[r] < g.M) << r;
   }
-  if constexpr (std::is_same<Acc, int>::value) {
+  if constexpr (std::is_same<Acc, int>::value && !SCALED) {
 #pragma unroll
     for (int r = 0; r < N; ++r)
       if ((live >> r) & 1)
         ((GEMM_AS1 int32_t *)g.out)[at[r]] = acc[r];
   } else {
     float v[N];
+    if constexpr (SCALED) {
+      const float column = g.scales.column(n), bias = g.scales.bias_of(n);
 #pragma unroll
-    for (int r = 0; r < N; ++r)
-      v[r] = acc[r];
+      for (int r = 0; r < N; ++r)
+        v[r] = g.scales.row(rows[r]);
+#pragma unroll
+      for (int r = 0; r < N; ++r)
+        v[r] = fhip_scaled(acc[r], v[r], column, bias);
+    } else {
+#pragma unroll
+      for (int r = 0; r < N; ++r)
+        v[r] = acc[r];
+    }
     fhip_round_fast_vec<N>(g.c_dt, v);
     if (g.epi.count > 0) {
       const int64_t coord[3] = {batch, 0, n};
@@ -486,11 +497,11 @@ __attribute__((amdgpu_waves_per_eu(
       row[e * 4 + r] = m0 + m + r * dm, vals[e * 4 + r] = v[r];
   }
   if (!g.partial)
-    direct_store<Acc, PER * 4>(g, batch, row, n0 + n, vals);
+    direct_store<Acc, PER * 4, KIND == GK_I8S>(g, batch, row, n0 + n, vals);
 }
 
 // Adds the split parts of every tile in order and finishes as above.
-template <typename Acc, bool A_KC, bool B_KC, int MT, int NT>
+template <typename Acc, bool A_KC, bool B_KC, int MT, int NT, bool SCALED = false>
 __global__ __launch_bounds__(64) void gemm_direct_finish_kernel(DirectArgs g) {
   typedef Acc Acc4 __attribute__((ext_vector_type(4)));
   constexpr int Q = MT * NT * 64;
@@ -506,7 +517,7 @@ __global__ __launch_bounds__(64) void gemm_direct_finish_kernel(DirectArgs g) {
   m += tile_m * 16 * MT;
   const int row[4] = {m, m + dm, m + 2 * dm, m + 3 * dm};
   const Acc vals[4] = {v.x, v.y, v.z, v.w};
-  direct_store<Acc, 4>(g, batch, row, tile_n * 16 * NT + n, vals);
+  direct_store<Acc, 4, SCALED>(g, batch, row, tile_n * 16 * NT + n, vals);
 }
 
 // What the host decided about one call.
@@ -528,7 +539,7 @@ int direct_launch(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64
   hipLaunchKernelGGL((gemm_direct_kernel<KIND, A_KC, B_KC, MT, NT, U, MAXW>), grid, dim3(p.waves * 64),
                      p.waves * PRIVATE, ctx->stream, g);
   if (g.splits > 1)
-    hipLaunchKernelGGL((gemm_direct_finish_kernel<Acc, A_KC, B_KC, MT, NT>),
+    hipLaunchKernelGGL((gemm_direct_finish_kernel<Acc, A_KC, B_KC, MT, NT, KIND == GK_I8S>),
                        dim3(grid.x, MT * NT, grid.z), dim3(64), 0, ctx->stream, g);
   FHIP_HIP_CHECK(ctx, hipGetLastError());
   return 0;
@@ -565,6 +576,7 @@ int direct_launch_kind(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, 
 int direct_launch_bf16(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 int direct_launch_f16(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 int direct_launch_i8(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
+int direct_launch_i8s(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 int direct_launch_fp8e4m3(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 int direct_launch_fp8e5m2(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 int direct_launch_f32(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);

@@ -48,7 +48,9 @@ typedef float gemm_f32x4 __attribute__((ext_vector_type(4)));
       char __attribute__((address_space(3))) *)(uint32_t)(uintptr_t)(base) +   \
       (byte_off)))
 
-enum GemmKind { GK_BF16 = 0, GK_F16 = 1, GK_I8 = 2, GK_FP8E4M3 = 3, GK_FP8E5M2 = 4 };
+// GK_I8S: int8 operands whose whole sums are scaled by row and column (5: f32, see
+// gemm_direct_kernel.h).
+enum GemmKind { GK_BF16 = 0, GK_F16 = 1, GK_I8 = 2, GK_FP8E4M3 = 3, GK_FP8E5M2 = 4, GK_I8S = 6 };
 
 template <int KIND> struct KindTraits;
 template <> struct KindTraits<GK_BF16> {
@@ -72,6 +74,7 @@ template <> struct KindTraits<GK_I8> {
   using AccVec = i32x16;
   using AccVec4 = i32x4;
 };
+template <> struct KindTraits<GK_I8S> : KindTraits<GK_I8> {};
 template <> struct KindTraits<GK_FP8E4M3> {
   static constexpr int kElemBytes = 1;
   static constexpr int kStepBytes = 64;
@@ -176,6 +179,7 @@ struct GemmArgs {
   float lin_a[FHIP_MAX_EPILOGUE], lin_b[FHIP_MAX_EPILOGUE];
   int32_t lin_mul[FHIP_MAX_EPILOGUE], lin_relu[FHIP_MAX_EPILOGUE];
   DevEpilogue epi;            // strides refer to (batch, m, n)
+  FhipProductScales scales;   // GK_I8S
 };
 
 // Fragment (per-lane MFMA operand) holder: FRAG_REGS 32-bit registers.
@@ -196,7 +200,7 @@ __device__ __forceinline__ void mfma32(typename KindTraits<KIND>::AccVec &c,
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(
         __builtin_bit_cast(f16x8, a.r), __builtin_bit_cast(f16x8, b.r), c, 0, 0,
         0);
-  } else if constexpr (KIND == GK_I8) {
+  } else if constexpr (KIND == GK_I8 || KIND == GK_I8S) {
     c = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a.r),
                                               __builtin_bit_cast(i32x4, b.r), c,
                                               0, 0, 0);
@@ -225,7 +229,7 @@ __device__ __forceinline__ void mfma16(typename KindTraits<KIND>::AccVec4 &c,
   } else if constexpr (KIND == GK_F16) {
     c = __builtin_amdgcn_mfma_f32_16x16x32_f16(
         __builtin_bit_cast(f16x8, a.r), __builtin_bit_cast(f16x8, b.r), c, 0, 0, 0);
-  } else if constexpr (KIND == GK_I8) {
+  } else if constexpr (KIND == GK_I8 || KIND == GK_I8S) {
     c = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a.r),
                                               __builtin_bit_cast(i32x4, b.r), c, 0, 0, 0);
   } else {
@@ -667,6 +671,8 @@ __global__ __launch_bounds__(NW * 64)
 __attribute__((amdgpu_waves_per_eu(A_MODE == A_HALO ? 2 : 1, 8))) void
 gemm_kernel(GemmArgs g) {
   using Acc = typename KindTraits<KIND>::Acc;
+  // what the epilogue finds in the accumulators (scaled sums: f32 in the registers of the int32)
+  constexpr bool INTS = KIND == GK_I8, SCALED = KIND == GK_I8S;
   constexpr bool A_KC = A_MODE != A_MCONTIG;
   constexpr int ELEM = KindTraits<KIND>::kElemBytes;
   constexpr int STEPB = KindTraits<KIND>::kStepBytes;
@@ -1324,11 +1330,45 @@ gemm_kernel(GemmArgs g) {
   const int64_t gM = m_end, gN = n_store; // rows and columns that are stored
   const int o_dt = g.o_dt;
 
+  auto val_get = [&](int i, int j, int r) __attribute__((always_inline)) -> float {
+    return __builtin_bit_cast(float, acc_get(i, j, r));
+  };
+  auto val_set = [&](int i, int j, int r, float v) __attribute__((always_inline)) {
+    acc_set(i, j, r, __builtin_bit_cast(Acc, v));
+  };
+  if constexpr (SCALED) {
+    // A lane's sums of a 16 x 16 tile are four rows of one column.
+    static_assert(M16, "scales by 16 x 16 tiles");
+    float cs[TN16], cb[TN16];
+#pragma unroll
+    for (int j = 0; j < TN16; ++j) {
+      int64_t n = n0 + wn * WN + j * 16 + c16;
+      n = n < g.N ? n : g.N - 1;
+      cs[j] = g.scales.column(n);
+      cb[j] = g.scales.bias_of(n);
+    }
+    float rs[TM16][4];
+#pragma unroll
+    for (int i = 0; i < TM16; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t m = m0 + wm * WM + i * 16 + g16 * 4 + q;
+        rs[i][q] = g.scales.row(m < g.M ? m : g.M - 1);
+      }
+#pragma unroll
+    for (int i = 0; i < TM16; ++i)
+#pragma unroll
+      for (int j = 0; j < TN16; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          acc16[i][j][q] = __builtin_bit_cast(int, fhip_scaled(acc16[i][j][q], rs[i][q], cs[j], cb[j]));
+  }
+
   // Lean path, step 1: the chain runs on the accumulators where they are.  A
   // lane's accumulators of column tile j all belong to one output column, so
   // an op is y <- y * S + T with one (S, T) pair of registers per (op, j):
   // (operand, -0) for MUL, (a, b * operand) for the additive modes.
-  if constexpr (!std::is_same<Acc, int>::value) {
+  if constexpr (!INTS) {
     if (lean && nops > 0) {
       // (column tiles of 16 with the 16 x 16 shapes)
       constexpr int CT = M16 ? TN16 : TN, CW = M16 ? 16 : 32;
@@ -1370,7 +1410,7 @@ gemm_kernel(GemmArgs g) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int c = M16 ? j * 2 + ((r >> 2) & 1) : j;
-              acc_set(i, j, r, __builtin_fmaf(acc_get(i, j, r), S[e][c], T[e][c]));
+              val_set(i, j, r, __builtin_fmaf(val_get(i, j, r), S[e][c], T[e][c]));
             }
         if (lin_relu[e]) {
           // one instruction per value (fmaxf would first quiet its input);
@@ -1381,9 +1421,9 @@ gemm_kernel(GemmArgs g) {
             for (int j = 0; j < TN; ++j)
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
-                float y = acc_get(i, j, r);
+                float y = val_get(i, j, r);
                 asm("v_max_f32 %0, 0, %0" : "+v"(y));
-                acc_set(i, j, r, y);
+                val_set(i, j, r, y);
               }
         }
       });
@@ -1391,7 +1431,7 @@ gemm_kernel(GemmArgs g) {
   }
   // Step 2, 16-bit outputs: the values are rounded here and leave through LDS
   // as packed pairs of consecutive rows (half the LDS traffic and passes).
-  const bool packed = !std::is_same<Acc, int>::value && lean &&
+  const bool packed = !INTS && lean &&
                       (o_dt == FHIP_BFLOAT16 || o_dt == FHIP_HALF);
   const uint32_t wr2 =
       band + (uint32_t)(M16 ? g16 * 2 * PITCH + c16 * 4
@@ -1402,7 +1442,7 @@ gemm_kernel(GemmArgs g) {
 
   gemm_static_for<TM / BANDS>([&](auto rc) {
     constexpr int round = decltype(rc)::value;
-    if constexpr (!std::is_same<Acc, int>::value) {
+    if constexpr (!INTS) {
       if (packed) {
         // pair-row k of a band holds rows 2k and 2k + 1 as (low, high) halves
         auto run = [&](auto ot_c) {
@@ -1413,8 +1453,8 @@ gemm_kernel(GemmArgs g) {
             for (int j = 0; j < TN; ++j)
 #pragma unroll
               for (int r = 0; r < 16; r += 2) {
-                const float lo = acc_get(round * BANDS + bi, j, r);
-                const float hi = acc_get(round * BANDS + bi, j, r + 1);
+                const float lo = val_get(round * BANDS + bi, j, r);
+                const float hi = val_get(round * BANDS + bi, j, r + 1);
                 uint32_t pk;
                 if constexpr (OT == 1) {
                   typedef __bf16 b2 __attribute__((ext_vector_type(2)));
@@ -1503,7 +1543,7 @@ gemm_kernel(GemmArgs g) {
         continue;
       const bool full = ncol + 8 <= n_store;
       const int64_t o0 = ob + m * g.o_sm + ncol * g.o_sn;
-      if constexpr (std::is_same<Acc, int>::value) {
+      if constexpr (INTS) {
         GEMM_AS1 int32_t *out = (GEMM_AS1 int32_t *)g.out;
         if (full && g.o_vec) {
           *(GEMM_AS1 u32x4 *)(out + o0) = v0;
@@ -1778,6 +1818,7 @@ int conv_launch_halo(fhip_ctx *ctx, const GemmArgs &g) {
 int gemm_launch_bf16(fhip_ctx *ctx, const GemmPlan &p, const GemmArgs &g);
 int gemm_launch_f16(fhip_ctx *ctx, const GemmPlan &p, const GemmArgs &g);
 int gemm_launch_i8(fhip_ctx *ctx, const GemmPlan &p, const GemmArgs &g);
+int gemm_launch_i8s(fhip_ctx *ctx, const GemmPlan &p, const GemmArgs &g);
 int gemm_launch_fp8e4m3(fhip_ctx *ctx, const GemmPlan &p, const GemmArgs &g);
 int gemm_launch_fp8e5m2(fhip_ctx *ctx, const GemmPlan &p, const GemmArgs &g);
 

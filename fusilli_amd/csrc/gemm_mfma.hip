@@ -56,13 +56,17 @@ bool kind_for(int a_dt, int b_dt, int *kind) {
 }
 
 // `ragged`: K may end inside a 128-byte slice.
-GemmPlan make_plan(const fhip_matmul_desc *d, bool ragged) {
+// `scaled`: sums of int8 operands are scaled, so that results are floats with a chain.
+GemmPlan make_plan(const fhip_matmul_desc *d, bool ragged, bool scaled = false) {
   GemmPlan p;
   const int r = d->a.rank;
   if (r != 2 && r != 3)
     return p;
   if (!kind_for(d->a.dtype, d->b.dtype, &p.kind))
     return p;
+  if (scaled)
+    p.kind = GK_I8S;
+  const bool i8 = p.kind == GK_I8 || scaled;
   const int elem = fhip_dtype_size(d->a.dtype);
   p.M = d->a.dim[r - 2];
   p.K = d->a.dim[r - 1];
@@ -159,8 +163,8 @@ GemmPlan make_plan(const fhip_matmul_desc *d, bool ragged) {
                         pace8i[3] = {1.38, 0.95, 0.66};
     static const double fixed16[3] = {11.0, 6.7, 6.4}, fixed8f[3] = {11.0, 5.7, 3.3},
                         fixed8i[3] = {18.0, 9.0, 7.7};
-    const double pace = (k16 ? pace16 : p.kind == GK_I8 ? pace8i : pace8f)[shape];
-    const double fixed = (k16 ? fixed16 : p.kind == GK_I8 ? fixed8i : fixed8f)[shape];
+    const double pace = (k16 ? pace16 : i8 ? pace8i : pace8f)[shape];
+    const double fixed = (k16 ? fixed16 : i8 ? fixed8i : fixed8f)[shape];
     const double t = tiles(bm, bn) * sk;
     const double full = floor(t / 256.0), rest = t - 256.0 * full;
     const double rounds = full + (rest > 0 ? 1 : 0);
@@ -168,7 +172,7 @@ GemmPlan make_plan(const fhip_matmul_desc *d, bool ragged) {
     const double run = (double)((slices + sk - 1) / sk); // slices of a part
     double us = run * pace * work +
                 (shape != 2 ? fixed * rounds
-                 : p.kind == GK_I8 ? fixed * (1.0 + 0.5 * (rounds - 1)) // (int32 stores)
+                 : i8 ? fixed * (1.0 + 0.5 * (rounds - 1)) // (int32 stores)
                                    // (a partner with under 4.25 us of K slices does not cover it:
                                    // fp8 4096 x 4096 x 512 18.9 us against 16.1 on 256 x 256)
                                    : fixed + (rounds - 1) * fmax(0.0, 4.25 - run * pace));
@@ -251,6 +255,8 @@ struct GemmSumArgs {
   int32_t N, pitch, parts, rank;
   int32_t c_dt, o_dt;
   int32_t ints;    // the parts are int32 sums (int8 operands): added exactly, no epilogue
+  int32_t scaled;  // ... and then scaled
+  FhipProductScales scales;
   DevEpilogue epi; // strides over the matmul's result dims
 };
 
@@ -264,23 +270,32 @@ __global__ void gemm_splitk_sum_kernel(GemmSumArgs a) {
   const int64_t m = e / a.N;
   const int64_t n0 = e - m * a.N;
   const float *src = a.part + m * a.pitch + n0;
+  float v[4];
   if (a.ints) {
     uint4 sum = *(const uint4 *)src; // (unsigned: wraps like the kernel's int32 accumulators)
     fhip_for_uniform_parts<4>(
         1, 1, a.parts, [&](int z) { return *(const uint4 *)(src + (int64_t)z * a.part_stride); },
-        [&](uint4 v) { sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w; });
-    uint32_t *o = (uint32_t *)a.out + m * a.o_sm + n0;
-    o[0] = sum.x, o[1] = sum.y, o[2] = sum.z, o[3] = sum.w;
-    return;
+        [&](uint4 x) { sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w; });
+    if (!a.scaled) {
+      uint32_t *o = (uint32_t *)a.out + m * a.o_sm + n0;
+      o[0] = sum.x, o[1] = sum.y, o[2] = sum.z, o[3] = sum.w;
+      return;
+    }
+    const uint32_t w[4] = {sum.x, sum.y, sum.z, sum.w};
+    const float row = a.scales.row(m);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = fhip_scaled((int)w[i], row, a.scales.column(n0 + i), a.scales.bias_of(n0 + i));
+  } else {
+    float4 acc = *(const float4 *)src;
+    fhip_for_uniform_parts<4>(
+        1, 1, a.parts, [&](int z) { return *(const float4 *)(src + (int64_t)z * a.part_stride); },
+        [&](float4 x) { acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w; });
+    v[0] = acc.x, v[1] = acc.y, v[2] = acc.z, v[3] = acc.w;
   }
-  float4 acc = *(const float4 *)src;
-  fhip_for_uniform_parts<4>(
-      1, 1, a.parts, [&](int z) { return *(const float4 *)(src + (int64_t)z * a.part_stride); },
-      [&](float4 v) { acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w; });
   int64_t coord[FHIP_MAX_RANK];
   coord[0] = 0;
   coord[a.rank - 2] = m;
-  float v[4] = {acc.x, acc.y, acc.z, acc.w};
   int64_t cols[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -295,10 +310,10 @@ __global__ void gemm_splitk_sum_kernel(GemmSumArgs a) {
 } // namespace
 
 static int run_plan(fhip_ctx *ctx, GemmPlan p, const fhip_matmul_desc *d, const void *a,
-                    const void *b, const DevEpilogue &epi, void *out);
+                    const void *b, const DevEpilogue &epi, void *out, const FhipProductScales *scales = nullptr);
 
-bool fhip_fast_matmul_applicable(const fhip_matmul_desc *d) {
-  return make_plan(d, false).ok;
+bool fhip_fast_matmul_applicable(const fhip_matmul_desc *d, bool scaled) {
+  return make_plan(d, false, scaled).ok;
 }
 
 int fhip_fast_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a,
@@ -309,36 +324,38 @@ int fhip_fast_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a,
 }
 
 int fhip_tuned_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a,
-                      const void *b, const DevEpilogue &epi, void *out, bool *handled, bool *short_k) {
+                      const void *b, const DevEpilogue &epi, void *out, bool *handled, bool *short_k,
+                      const FhipProductScales *scales) {
   *handled = true;
   *short_k = false;
-  const GemmPlan p = make_plan(d, true);
-  const bool whole = p.ok && p.K * fhip_dtype_size(d->a.dtype) % kTileKBytes == 0;
+  const GemmPlan p = make_plan(d, true, scales != nullptr);
   const bool aligned = (((uintptr_t)a | (uintptr_t)b) & 15) == 0;
+  // (scaled products off 16 bytes go to the other kernels)
+  const bool whole = p.ok && p.K * fhip_dtype_size(d->a.dtype) % kTileKBytes == 0 && (aligned || !scales);
   if (whole && (!aligned || fhip_knobs().gemm_tile_bm || fhip_knobs().gemm_split))
-    return run_plan(ctx, p, d, a, b, epi, out); // (misaligned operands of the contract are refused)
+    return run_plan(ctx, p, d, a, b, epi, out, scales); // (misaligned operands of the contract are refused)
   double us = 0;
   // (f32 results of a K inside one 16-byte chunk, which the direct kernels leave to the general
   // path, stay there: an fp8 MFMA aligns its products to the largest, 5e-6 of the result at K 13)
-  const bool f32_out = p.kind != GK_I8 && d->c.dtype == FHIP_FLOAT && d->out.dtype == FHIP_FLOAT;
+  const bool f32_out = p.kind != GK_I8 && !scales && d->c.dtype == FHIP_FLOAT && d->out.dtype == FHIP_FLOAT;
   if (p.ok && aligned && (whole || !f32_out)) {
     // (the planner's estimate against 154 products of 128 to 4096 rows and 256 to 8192 columns:
     // 14 % rms for 16 bits, 5 for fp8, 11 for int8; GELU over whole 128-wide tiles 6 us)
     const bool gelu = fhip_epilogue_is_transcendental(d->epilogue);
-    us = p.kind == GK_I8 ? 0.95 * p.us - 1.0
+    us = p.kind == GK_I8 || scales ? 0.95 * p.us - 1.0 + (gelu ? 6.0 : 0.0)
          : p.kind == GK_BF16 || p.kind == GK_F16 ? 1.1 * p.us - 1.0 + (gelu ? 6.0 : 0.0)
                                                  : 1.05 * p.us + 1.6 + (gelu ? 6.0 : 0.0);
     us = us > 1.0 ? us : 1.0;
   }
-  const int rc = fhip_direct_matmul(ctx, d, a, b, epi, out, us, whole, handled, short_k);
+  const int rc = fhip_direct_matmul(ctx, d, a, b, epi, out, us, whole, handled, short_k, scales);
   if (*handled || us == 0 || *short_k)
     return rc;
   *handled = true;
-  return run_plan(ctx, p, d, a, b, epi, out);
+  return run_plan(ctx, p, d, a, b, epi, out, scales);
 }
 
 static int run_plan(fhip_ctx *ctx, GemmPlan p, const fhip_matmul_desc *d, const void *a,
-                    const void *b, const DevEpilogue &epi, void *out) {
+                    const void *b, const DevEpilogue &epi, void *out, const FhipProductScales *scales) {
   const int64_t pitch = (p.N + p.bn - 1) / p.bn * p.bn; // of the parts of a split reduction
   const size_t part_bytes = (size_t)p.ksplit * (size_t)(p.M * pitch) * sizeof(float);
   if (p.ksplit > 1 && !fhip_ctx_scratch_ready(ctx, part_bytes))
@@ -370,6 +387,8 @@ static int run_plan(fhip_ctx *ctx, GemmPlan p, const fhip_matmul_desc *d, const 
               (p.o_batch * oe) % 16 == 0 &&
               ((uintptr_t)out & 15) == 0;
   }
+  if (scales)
+    g.scales = *scales;
   // epilogue strides on (batch, m, n)
   g.epi = epi;
   g.epi.rank = 3;
@@ -381,7 +400,7 @@ static int run_plan(fhip_ctx *ctx, GemmPlan p, const fhip_matmul_desc *d, const 
     o.stride[1] = s.stride[r - 2];
     o.stride[2] = s.stride[r - 1];
   }
-  static const char *const kKindName[] = {"bf16", "f16", "i8", "fp8e4m3", "fp8e5m2"};
+  static const char *const kKindName[] = {"bf16", "f16", "i8", "fp8e4m3", "fp8e5m2", "f32", "i8s"};
   fhip_note_kernel(ctx, "gemm_mfma %s %dx%d waves=8 split=%d", kKindName[p.kind], p.bm, p.bn,
                    p.ksplit);
   auto launch = [&]() {
@@ -392,6 +411,8 @@ static int run_plan(fhip_ctx *ctx, GemmPlan p, const fhip_matmul_desc *d, const 
       return gemm_launch_f16(ctx, p, g);
     case GK_I8:
       return gemm_launch_i8(ctx, p, g);
+    case GK_I8S: // (parts of a split reduction are plain sums)
+      return p.ksplit > 1 ? gemm_launch_i8(ctx, p, g) : gemm_launch_i8s(ctx, p, g);
     case GK_FP8E4M3:
       return gemm_launch_fp8e4m3(ctx, p, g);
     default:
@@ -408,7 +429,8 @@ static int run_plan(fhip_ctx *ctx, GemmPlan p, const fhip_matmul_desc *d, const 
     if (fhip_ctx_scratch(ctx, part_bytes, &sp) != 0)
       return 1;
     g.out = (char *)sp;
-    g.c_dt = g.o_dt = p.kind == GK_I8 ? FHIP_INT32 : FHIP_FLOAT;
+    const bool ints = p.kind == GK_I8 || p.kind == GK_I8S;
+    g.c_dt = g.o_dt = ints ? FHIP_INT32 : FHIP_FLOAT;
     g.o_sm = pitch;
     g.n_store = pitch;
     g.o_sn = 1;
@@ -437,7 +459,10 @@ static int run_plan(fhip_ctx *ctx, GemmPlan p, const fhip_matmul_desc *d, const 
     sa.rank = r;
     sa.c_dt = d->c.dtype;
     sa.o_dt = d->out.dtype;
-    sa.ints = p.kind == GK_I8;
+    sa.ints = ints;
+    sa.scaled = scales != nullptr;
+    if (scales)
+      sa.scales = *scales;
     sa.epi = epi;
     hipLaunchKernelGGL(gemm_splitk_sum_kernel, dim3((unsigned)((sa.mn4 + 255) / 256)),
                        dim3(256), 0, ctx->stream, sa);
@@ -445,16 +470,5 @@ static int run_plan(fhip_ctx *ctx, GemmPlan p, const fhip_matmul_desc *d, const 
     return 0;
   }
   gemm_fill_linear(d->epilogue, g);
-  switch (p.kind) {
-  case GK_BF16:
-    return gemm_launch_bf16(ctx, p, g);
-  case GK_F16:
-    return gemm_launch_f16(ctx, p, g);
-  case GK_I8:
-    return gemm_launch_i8(ctx, p, g);
-  case GK_FP8E4M3:
-    return gemm_launch_fp8e4m3(ctx, p, g);
-  default:
-    return gemm_launch_fp8e5m2(ctx, p, g);
-  }
+  return launch();
 }

@@ -238,16 +238,33 @@ template <int V> struct TileColumns {
   }
 };
 
+// The same of the columns' scales and bias.
+template <int V, bool SCALED> struct TileScales {
+  __device__ __forceinline__ void request(const DirectArgs &, int) {}
+};
+template <int V> struct TileScales<V, true> {
+  float scale[V], bias[V];
+  __device__ __forceinline__ void request(const DirectArgs &g, int n) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int64_t at = n + i < g.N ? n + i : g.N - 1;
+      scale[i] = g.scales.column(at);
+      bias[i] = g.scales.bias_of(at);
+    }
+  }
+};
+
 // Finishes and stores the V values of columns n .. of row m, which starts at element `row` of
 // OUT (-1: there is no such row).
-template <typename Acc, int V, bool PLAIN = false>
+template <typename Acc, int V, bool PLAIN = false, bool SCALED = false>
 __device__ __forceinline__ void tile_store(const DirectArgs &g, int64_t batch, int m, int64_t row, int n,
-                                           const Acc (&acc)[V], const TileColumns<V> *lean = nullptr) {
+                                           const Acc (&acc)[V], const TileColumns<V> *lean,
+                                           const TileScales<V, SCALED> &scales) {
   if (row < 0 || n >= g.N)
     return;
   const int live = g.N - n < V ? g.N - n : V;
   const int64_t at = row + (int64_t)n * g.o_sn;
-  if constexpr (std::is_same<Acc, int>::value) {
+  if constexpr (std::is_same<Acc, int>::value && !SCALED) {
     typedef int loose __attribute__((ext_vector_type(4), aligned(4)));
     GEMM_AS1 int32_t *out = (GEMM_AS1 int32_t *)g.out + at;
 #pragma unroll
@@ -263,9 +280,16 @@ __device__ __forceinline__ void tile_store(const DirectArgs &g, int64_t batch, i
     }
   } else {
     float v[V];
+    if constexpr (SCALED) {
+      const float by = g.scales.row(m);
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      v[i] = acc[i];
+      for (int i = 0; i < V; ++i)
+        v[i] = fhip_scaled(acc[i], by, scales.scale[i], scales.bias[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        v[i] = acc[i];
+    }
     fhip_round_fast_vec<V>(g.c_dt, v);
     if (PLAIN) { // (no fused chain)
     } else if (lean && g.lean) {
@@ -334,9 +358,10 @@ __device__ __forceinline__ void tile_store(const DirectArgs &g, int64_t batch, i
 }
 
 // Adds a tile's SUMS shares of K in LDS, finishes and stores it.
-template <typename Acc, int V, int BM, int BN, int SUMS, int PITCH, int SUM, int THREADS, bool PLAIN, class Row>
+template <typename Acc, int V, int BM, int BN, int SUMS, int PITCH, int SUM, int THREADS, bool PLAIN, bool SCALED, class Row>
 __device__ __forceinline__ void tile_finish(const DirectArgs &g, uint32_t lds, uint32_t id, int64_t batch, int m0, int n0,
-                                            const TileColumns<V> &columns, const Row &at_row) {
+                                            const TileColumns<V> &columns, const TileScales<V, SCALED> &scales,
+                                            const Row &at_row) {
   typedef Acc Acc4 __attribute__((ext_vector_type(4)));
   constexpr int RUNS = BN / V; // runs of V columns in a row
 #pragma clang loop unroll(disable)
@@ -352,7 +377,7 @@ __device__ __forceinline__ void tile_finish(const DirectArgs &g, uint32_t lds, u
         x += p[h * (SUM / 16)];
       v[q] = x.x, v[q + 1] = x.y, v[q + 2] = x.z, v[q + 3] = x.w;
     }
-    tile_store<Acc, V, PLAIN>(g, batch, m0 + row, at_row(m0 + row), n0 + col, v, &columns);
+    tile_store<Acc, V, PLAIN, SCALED>(g, batch, m0 + row, at_row(m0 + row), n0 + col, v, &columns, scales);
   }
 }
 
@@ -558,6 +583,9 @@ __device__ __forceinline__ void tile_run(const DirectArgs &g, uint32_t smem, con
   TileColumns<S::V> columns;
   if (!PLAIN && g.lean && g.lean_op >= 0 && !g.partial)
     columns.request(g, n0 + (int)(threadIdx.x % (BN / S::V)) * S::V);
+  TileScales<S::V, KIND == GK_I8S> scales;
+  if (!g.partial)
+    scales.request(g, n0 + (int)(threadIdx.x % (BN / S::V)) * S::V);
   gemm_static_for<U>([&](auto uc) {
     constexpr int u = decltype(uc)::value, n = (u + 2) % U;
     constexpr int last = ((u + 1) * S::STEPS - 1) & 1;
@@ -594,8 +622,8 @@ __device__ __forceinline__ void tile_run(const DirectArgs &g, uint32_t smem, con
     tile_part<Acc, BM, BN, S::kSums, S::kPitch, S::kSum, 256 * TEAMS>(g, smem, id, batch);
     return;
   }
-  tile_finish<Acc, S::V, BM, BN, S::kSums, S::kPitch, S::kSum, 256 * TEAMS, PLAIN>(g, smem, id, batch, m0, n0, columns,
-                                                                                  at_row);
+  tile_finish<Acc, S::V, BM, BN, S::kSums, S::kPitch, S::kSum, 256 * TEAMS, PLAIN, KIND == GK_I8S>(
+      g, smem, id, batch, m0, n0, columns, scales, at_row);
 }
 
 template <int KIND, bool A_KC, bool B_KC, int MT, int NT, int TEAMS, int U>
@@ -625,7 +653,7 @@ __attribute__((amdgpu_waves_per_eu(2, 8))) void gemm_tile_kernel(DirectArgs g) {
 }
 
 // Adds the split parts of every tile in order and finishes as above: four columns a thread.
-template <typename Acc, int BM, int BN, bool BY_ROWS = false>
+template <typename Acc, int BM, int BN, bool BY_ROWS = false, bool SCALED = false>
 __global__ __launch_bounds__(256) void gemm_tile_finish_kernel(DirectArgs g) {
   typedef Acc Acc4 __attribute__((ext_vector_type(4)));
   const uint32_t run = (uint32_t)(BY_ROWS ? g.tiles_n : g.tiles_m); // tiles one after another, row by row or down a column
@@ -636,14 +664,16 @@ __global__ __launch_bounds__(256) void gemm_tile_finish_kernel(DirectArgs g) {
   TileColumns<4> columns;
   if (g.lean && g.lean_op >= 0)
     columns.request(g, tile_n * BN + q % (BN / 4) * 4);
+  TileScales<4, SCALED> scales;
+  scales.request(g, tile_n * BN + q % (BN / 4) * 4);
   const GEMM_AS1 Acc4 *p = (const GEMM_AS1 Acc4 *)g.partial + (batch * gridDim.x + blockIdx.x) * (BM * BN / 4) + q;
   const int64_t stride = (int64_t)gridDim.z * gridDim.x * (BM * BN / 4);
   Acc4 x = p[0];
   fhip_for_uniform_parts<4>(1, 1, g.splits, [&](int s) { return p[s * stride]; }, [&](Acc4 v) { x += v; });
   const Acc v[4] = {x.x, x.y, x.z, x.w};
   const int m = tile_m * BM + q / (BN / 4);
-  tile_store<Acc, 4>(g, batch, m, m < g.M ? batch * g.o_batch + (int64_t)m * g.o_sm : -1, tile_n * BN + q % (BN / 4) * 4, v,
-                   &columns);
+  tile_store<Acc, 4, false, SCALED>(g, batch, m, m < g.M ? batch * g.o_batch + (int64_t)m * g.o_sm : -1,
+                                    tile_n * BN + q % (BN / 4) * 4, v, &columns, scales);
 }
 
 template <int KIND, bool A_KC, bool B_KC, int MT, int NT, int TEAMS, int U>
@@ -659,7 +689,7 @@ int tile_launch(fhip_ctx *ctx, const DirectArgs &g, int64_t batch) {
   const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)batch);
   hipLaunchKernelGGL(kernel, grid, dim3(256 * TEAMS), S::kLds, ctx->stream, g);
   if (g.splits > 1)
-    hipLaunchKernelGGL((gemm_tile_finish_kernel<typename DirectKind<KIND>::Acc, S::BM, S::BN>),
+    hipLaunchKernelGGL((gemm_tile_finish_kernel<typename DirectKind<KIND>::Acc, S::BM, S::BN, false, KIND == GK_I8S>),
                        dim3(grid.x, S::BM * S::BN / 1024, grid.z), dim3(256), 0, ctx->stream, g);
   FHIP_HIP_CHECK(ctx, hipGetLastError());
   return 0;
@@ -693,6 +723,7 @@ int tile_launch_kind(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, in
 int tile_launch_bf16(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 int tile_launch_f16(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 int tile_launch_i8(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
+int tile_launch_i8s(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 int tile_launch_fp8e4m3(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 int tile_launch_fp8e5m2(fhip_ctx *ctx, const DirectPlan &p, const DirectArgs &g, int64_t batch);
 

@@ -35,6 +35,15 @@ bool is_float(int dt) { return dt == FHIP_FLOAT || dt == FHIP_BFLOAT16 || dt == 
 
 } // namespace
 
+// The product as fhip_matmul's kernels have it.
+static fhip_matmul_desc matmul_of(const fhip_matmul_quantized_desc &d) {
+  fhip_matmul_desc m;
+  m.a = d.a, m.b = d.b, m.c = d.c, m.out = d.out;
+  m.epilogue = d.epilogue;
+  m.out_dtype = d.out_dtype;
+  return m;
+}
+
 static int validate(fhip_ctx *ctx, const fhip_matmul_quantized_desc *d) {
   static const char who[] = "fhip_matmul_quantized";
   FHIP_REQUIRE(ctx, d != nullptr, "%s: null descriptor", who);
@@ -72,7 +81,8 @@ int fhip_matmul_quantized_workspace_size(const fhip_matmul_quantized_desc *d, si
 int fhip_matmul_quantized_supported(const fhip_matmul_quantized_desc *d) {
   if (!d || validate(nullptr, d) != 0)
     return 0;
-  return 1;
+  const fhip_matmul_desc m = matmul_of(*d);
+  return fhip_fast_matmul_applicable(&m, true) ? 2 : 1;
 }
 
 int fhip_matmul_quantized(fhip_ctx *ctx, const fhip_matmul_quantized_desc *d, const void *a, const void *b,
@@ -93,6 +103,11 @@ int fhip_matmul_quantized(fhip_ctx *ctx, const fhip_matmul_quantized_desc *d, co
   FhipProductScales s{};
   s.a = (const float *)a_scale, s.b = (const float *)b_scale, s.bias = bias;
   s.a_s = d->a_scale_stride, s.b_s = d->b_scale_stride, s.bias_s = d->bias_stride, s.bias_dt = d->bias_dtype;
+  const fhip_matmul_desc md = matmul_of(*d);
+  bool handled = false, short_k = false;
+  const int rc = fhip_tuned_matmul(ctx, &md, a, b, epi, out, &handled, &short_k, &s);
+  if (handled)
+    return rc;
   fhip_note_kernel(ctx, "matmul_quantized_generic");
   ScaledArgs g{};
   g.a = (const int8_t *)a, g.b = (const int8_t *)b, g.out = out, g.scales = s;

@@ -615,6 +615,68 @@ public:
     return {k, v};
   }
 
+  // Rows to 8-bit codes: {Q, SCALE}.  up (swish gate) and weight (RMS norm) may
+  // be null.
+  std::array<std::shared_ptr<TensorAttr>, 2>
+  quantizeRows(const TensorPtr &x, const TensorPtr &up, const TensorPtr &weight,
+               QuantizeRowsAttr &attr) {
+    nameNode(attr, "quantize_rows");
+    nameTensor(x, attr, "X");
+    nameTensor(up, attr, "UP");
+    nameTensor(weight, attr, "WEIGHT");
+    nameTensor(attr.getEpsilon(), attr, "EPSILON");
+    attr.setX(x).setUP(up).setWEIGHT(weight);
+    auto q = outputTensor(attr.getName() + "_Q");
+    auto scale = outputTensor(attr.getName() + "_SCALE");
+    attr.setQ(q).setSCALE(scale);
+    subNodes_.emplace_back(
+        std::make_shared<QuantizeRowsNode>(std::move(attr), context));
+    return {q, scale};
+  }
+
+  // Product of 8-bit codes with scales per row and column; bias may be null.
+  std::shared_ptr<TensorAttr>
+  matmulQuantized(const TensorPtr &a, const TensorPtr &aScale,
+                  const TensorPtr &b, const TensorPtr &bScale,
+                  const TensorPtr &bias, MatmulQuantizedAttr &attr) {
+    nameNode(attr, "matmul_quantized");
+    nameTensor(a, attr, "A");
+    nameTensor(aScale, attr, "A_SCALE");
+    nameTensor(b, attr, "B");
+    nameTensor(bScale, attr, "B_SCALE");
+    nameTensor(bias, attr, "BIAS");
+    attr.setA(a).setA_SCALE(aScale).setB(b).setB_SCALE(bScale).setBIAS(bias);
+    auto c = outputTensor(attr.getName() + "_C");
+    attr.setC(c);
+    subNodes_.emplace_back(
+        std::make_shared<MatmulQuantizedNode>(std::move(attr), context));
+    return c;
+  }
+
+  // Tokens from logits: {TOKEN, PROBABILITY}.  A setting is a vector, a scalar
+  // constant, or null where it is off; PROBABILITY costs nothing where it is
+  // neither an output nor read.
+  std::array<std::shared_ptr<TensorAttr>, 2>
+  sample(const TensorPtr &logits, const TensorPtr &uniform,
+         const TensorPtr &temperature, const TensorPtr &topK,
+         const TensorPtr &topP, const TensorPtr &minP, SampleAttr &attr) {
+    nameNode(attr, "sample");
+    nameTensor(logits, attr, "LOGITS");
+    nameTensor(uniform, attr, "UNIFORM");
+    nameTensor(temperature, attr, "TEMPERATURE");
+    nameTensor(topK, attr, "TOP_K");
+    nameTensor(topP, attr, "TOP_P");
+    nameTensor(minP, attr, "MIN_P");
+    attr.setLOGITS(logits).setUNIFORM(uniform).setTEMPERATURE(temperature);
+    attr.setTOP_K(topK).setTOP_P(topP).setMIN_P(minP);
+    auto token = outputTensor(attr.getName() + "_TOKEN");
+    auto probability = outputTensor(attr.getName() + "_PROBABILITY");
+    attr.setTOKEN(token).setPROBABILITY(probability);
+    subNodes_.emplace_back(
+        std::make_shared<SampleNode>(std::move(attr), context));
+    return {token, probability};
+  }
+
   // Returns {Y, INV_RMS}; INV_RMS is null outside the training phase.
   std::array<std::shared_ptr<TensorAttr>, 2>
   rmsnorm(const TensorPtr &x, const TensorPtr &scale, RmsnormAttr &attr) {

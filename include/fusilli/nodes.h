@@ -35,6 +35,9 @@ public:
     SdpaPaged,
     CacheAppend,
     CacheRead,
+    QuantizeRows,
+    MatmulQuantized,
+    Sample,
   };
 
   explicit INode(const Context &ctx) : context(ctx) {}
@@ -1082,6 +1085,243 @@ public:
 
 private:
   static constexpr const char *kOp = "Cache read";
+};
+
+// ---- models served in 8 bits ----------------------------------------------------
+// (no counterpart in the reference; what the kernels need beyond these checks
+// the planner asks the backend)
+namespace quantized_utils {
+inline ErrorObject checkMatrix(const TensorPtr &t, const std::string &op,
+                               const std::string &which) {
+  FUSILLI_RETURN_ERROR_IF(!t, ErrorCode::AttributeNotSet,
+                          op + " tensor " + which + " not set");
+  FUSILLI_RETURN_ERROR_IF(t->getDim().size() != 2, ErrorCode::InvalidAttribute,
+                          op + " tensor " + which + " must be rank 2");
+  return ok();
+}
+// A vector along one dim of a matrix: `dim`, or one value for all of it.
+inline ErrorObject checkAlong(const TensorPtr &t, const std::string &op,
+                              const std::string &which,
+                              const std::vector<int64_t> &dim, bool float32) {
+  FUSILLI_RETURN_ERROR_IF(!t, ErrorCode::AttributeNotSet,
+                          op + " tensor " + which + " not set");
+  FUSILLI_RETURN_ERROR_IF(
+      t->getDim() != dim && t->getDim() != (std::vector<int64_t>{1, 1}),
+      ErrorCode::InvalidAttribute,
+      op + " tensor " + which + " must be [" + std::to_string(dim[0]) + ", " +
+          std::to_string(dim[1]) + "] or [1, 1]");
+  FUSILLI_RETURN_ERROR_IF(float32 && t->getDataType() != DataType::Float,
+                          ErrorCode::InvalidAttribute,
+                          op + " tensor " + which + " must be Float");
+  return ok();
+}
+// A dense vector [rows].
+inline ErrorObject checkVector(const TensorPtr &t, const std::string &op,
+                               const std::string &which, int64_t rows,
+                               DataType type) {
+  FUSILLI_RETURN_ERROR_IF(t->getDim() != std::vector<int64_t>{rows} ||
+                              !t->isContiguous(),
+                          ErrorCode::InvalidAttribute,
+                          op + " tensor " + which + " must be contiguous [" +
+                              std::to_string(rows) + "]");
+  FUSILLI_RETURN_ERROR_IF(t->getDataType() != type,
+                          ErrorCode::InvalidAttribute,
+                          op + " tensor " + which + " must be " +
+                              (type == DataType::Int32 ? "Int32" : "Float"));
+  return ok();
+}
+inline void infer(const TensorPtr &t, const std::vector<int64_t> &dim,
+                  DataType type) {
+  if (t->getDim().empty())
+    t->setDim(dim);
+  if (t->getStride().empty())
+    t->setStride(generateStrideFromDim(
+        t->getDim(), getContiguousStrideOrder(t->getDim().size())));
+  if (type != DataType::NotSet && t->getDataType() == DataType::NotSet)
+    t->setDataType(type);
+}
+} // namespace quantized_utils
+
+class QuantizeRowsNode : public NodeCRTP<QuantizeRowsNode> {
+public:
+  QuantizeRowsAttr quantizeRowsAttr;
+  QuantizeRowsNode(QuantizeRowsAttr &&attr, const Context &ctx)
+      : NodeCRTP(ctx), quantizeRowsAttr(std::move(attr)) {}
+  const std::string &getName() const override final {
+    return quantizeRowsAttr.getName();
+  }
+  Type getType() const override final { return Type::QuantizeRows; }
+
+  ErrorObject preValidateNode() const override final {
+    using Front = QuantizeRowsAttr::Front;
+    const auto &a = quantizeRowsAttr;
+    const std::string op = kOp;
+    FUSILLI_CHECK_ERROR(quantized_utils::checkMatrix(a.getX(), op, "X"));
+    FUSILLI_RETURN_ERROR_IF(
+        (a.getUP() != nullptr) != (a.getFront() == Front::SWISH_GATE),
+        ErrorCode::InvalidAttribute,
+        op + " tensor UP and the swish gate go together");
+    if (a.getUP())
+      FUSILLI_CHECK_ERROR(quantized_utils::checkMatrix(a.getUP(), op, "UP"));
+    FUSILLI_RETURN_ERROR_IF(a.getWEIGHT() && a.getFront() != Front::RMSNORM,
+                            ErrorCode::InvalidAttribute,
+                            op + " tensor WEIGHT needs the RMS norm");
+    if (a.getFront() == Front::RMSNORM) {
+      FUSILLI_RETURN_ERROR_IF(!a.getEpsilon(), ErrorCode::AttributeNotSet,
+                              op + " epsilon not set");
+      FUSILLI_RETURN_ERROR_IF(!a.getEpsilon()->isScalar(),
+                              ErrorCode::InvalidAttribute,
+                              op + " epsilon must be a scalar constant");
+    }
+    return ok();
+  }
+  ErrorObject inferPropertiesNode() override final {
+    const auto &a = quantizeRowsAttr;
+    const auto &x = a.getX()->getDim();
+    quantized_utils::infer(a.getQ(), x, DataType::Int8);
+    quantized_utils::infer(a.getSCALE(), {x[0], 1}, DataType::Float);
+    quantizeRowsAttr.fillFromContext(context);
+    return ok();
+  }
+  ErrorObject postValidateNode() const override final {
+    return checkShapes(quantizeRowsAttr, kOp);
+  }
+  // (the planner checks them again: buffers may give dynamic dims other extents)
+  static ErrorObject checkShapes(const QuantizeRowsAttr &a,
+                                 const std::string &op) {
+    const auto &x = a.getX()->getDim();
+    FUSILLI_RETURN_ERROR_IF(a.getQ()->getDim() != x,
+                            ErrorCode::InvalidAttribute,
+                            op + " output tensor Q must have X's shape");
+    FUSILLI_RETURN_ERROR_IF(
+        a.getSCALE()->getDim() != (std::vector<int64_t>{x[0], 1}) ||
+            a.getSCALE()->getDataType() != DataType::Float,
+        ErrorCode::InvalidAttribute,
+        op + " output tensor SCALE must be Float [rows, 1]");
+    if (a.getWEIGHT())
+      FUSILLI_RETURN_ERROR_IF(a.getWEIGHT()->getDim() !=
+                                  (std::vector<int64_t>{1, x[1]}),
+                              ErrorCode::InvalidAttribute,
+                              op + " tensor WEIGHT must be [1, " +
+                                  std::to_string(x[1]) + "]");
+    return ok();
+  }
+
+private:
+  static constexpr const char *kOp = "Quantize rows";
+};
+
+class MatmulQuantizedNode : public NodeCRTP<MatmulQuantizedNode> {
+public:
+  MatmulQuantizedAttr matmulQuantizedAttr;
+  MatmulQuantizedNode(MatmulQuantizedAttr &&attr, const Context &ctx)
+      : NodeCRTP(ctx), matmulQuantizedAttr(std::move(attr)) {}
+  const std::string &getName() const override final {
+    return matmulQuantizedAttr.getName();
+  }
+  Type getType() const override final { return Type::MatmulQuantized; }
+
+  ErrorObject preValidateNode() const override final {
+    const auto &a = matmulQuantizedAttr;
+    FUSILLI_CHECK_ERROR(quantized_utils::checkMatrix(a.getA(), kOp, "A"));
+    FUSILLI_CHECK_ERROR(quantized_utils::checkMatrix(a.getB(), kOp, "B"));
+    const int64_t aK = a.getA()->getDim()[1], bK = a.getB()->getDim()[0];
+    FUSILLI_RETURN_ERROR_IF(aK != bK, ErrorCode::InvalidAttribute,
+                            std::string(kOp) +
+                                " input tensors A and B have incompatible "
+                                "inner dimensions (K): A has K=" +
+                                std::to_string(aK) +
+                                ", B has K=" + std::to_string(bK));
+    FUSILLI_RETURN_ERROR_IF(!a.getA_SCALE() || !a.getB_SCALE(),
+                            ErrorCode::AttributeNotSet,
+                            std::string(kOp) +
+                                " tensors A_SCALE and B_SCALE must be set");
+    return ok();
+  }
+  ErrorObject inferPropertiesNode() override final {
+    const auto &a = matmulQuantizedAttr;
+    quantized_utils::infer(a.getC(),
+                           {a.getA()->getDim()[0], a.getB()->getDim()[1]},
+                           DataType::NotSet);
+    matmulQuantizedAttr.fillFromContext(context);
+    return ok();
+  }
+  ErrorObject postValidateNode() const override final {
+    return checkShapes(matmulQuantizedAttr, kOp);
+  }
+  static ErrorObject checkShapes(const MatmulQuantizedAttr &a,
+                                 const std::string &op) {
+    const int64_t m = a.getA()->getDim()[0], n = a.getB()->getDim()[1];
+    FUSILLI_CHECK_ERROR(quantized_utils::checkAlong(a.getA_SCALE(), op,
+                                                    "A_SCALE", {m, 1}, true));
+    FUSILLI_CHECK_ERROR(quantized_utils::checkAlong(a.getB_SCALE(), op,
+                                                    "B_SCALE", {1, n}, true));
+    if (a.getBIAS())
+      FUSILLI_CHECK_ERROR(quantized_utils::checkAlong(a.getBIAS(), op, "BIAS",
+                                                      {1, n}, false));
+    FUSILLI_RETURN_ERROR_IF(a.getC()->getDim() !=
+                                (std::vector<int64_t>{m, n}),
+                            ErrorCode::InvalidAttribute,
+                            op + " output tensor C must be [M, N]");
+    return ok();
+  }
+
+private:
+  static constexpr const char *kOp = "Quantized matmul";
+};
+
+class SampleNode : public NodeCRTP<SampleNode> {
+public:
+  SampleAttr sampleAttr;
+  SampleNode(SampleAttr &&attr, const Context &ctx)
+      : NodeCRTP(ctx), sampleAttr(std::move(attr)) {}
+  const std::string &getName() const override final {
+    return sampleAttr.getName();
+  }
+  Type getType() const override final { return Type::Sample; }
+
+  ErrorObject preValidateNode() const override final {
+    const auto &a = sampleAttr;
+    FUSILLI_CHECK_ERROR(
+        quantized_utils::checkMatrix(a.getLOGITS(), kOp, "LOGITS"));
+    FUSILLI_RETURN_ERROR_IF(!a.getUNIFORM(), ErrorCode::AttributeNotSet,
+                            std::string(kOp) + " tensor UNIFORM not set");
+    return ok();
+  }
+  ErrorObject inferPropertiesNode() override final {
+    const auto &a = sampleAttr;
+    const int64_t rows = a.getLOGITS()->getDim()[0];
+    quantized_utils::infer(a.getTOKEN(), {rows}, DataType::Int32);
+    quantized_utils::infer(a.getPROBABILITY(), {rows}, DataType::Float);
+    sampleAttr.fillFromContext(context);
+    return ok();
+  }
+  ErrorObject postValidateNode() const override final {
+    return checkShapes(sampleAttr, kOp);
+  }
+  static ErrorObject checkShapes(const SampleAttr &a, const std::string &op) {
+    const int64_t rows = a.getLOGITS()->getDim()[0];
+    auto check = [&](const TensorPtr &t, const std::string &which,
+                     DataType type) {
+      return t && !t->isScalar()
+                 ? quantized_utils::checkVector(t, op, which, rows, type)
+                 : ok();
+    };
+    FUSILLI_RETURN_ERROR_IF(a.getUNIFORM()->isScalar(),
+                            ErrorCode::InvalidAttribute,
+                            op + " tensor UNIFORM must not be a constant");
+    FUSILLI_CHECK_ERROR(check(a.getUNIFORM(), "UNIFORM", DataType::Float));
+    FUSILLI_CHECK_ERROR(
+        check(a.getTEMPERATURE(), "TEMPERATURE", DataType::Float));
+    FUSILLI_CHECK_ERROR(check(a.getTOP_K(), "TOP_K", DataType::Int32));
+    FUSILLI_CHECK_ERROR(check(a.getTOP_P(), "TOP_P", DataType::Float));
+    FUSILLI_CHECK_ERROR(check(a.getMIN_P(), "MIN_P", DataType::Float));
+    FUSILLI_CHECK_ERROR(check(a.getTOKEN(), "TOKEN", DataType::Int32));
+    return check(a.getPROBABILITY(), "PROBABILITY", DataType::Float);
+  }
+
+private:
+  static constexpr const char *kOp = "Sample";
 };
 
 // ---- norms ------------------------------------------------------------------

@@ -554,6 +554,74 @@ public:
   FUSILLI_OUT_SLOT(CacheReadAttr, V)
 };
 
+// ---- models served in 8 bits (no counterpart in the reference) -----------------
+// Rows [rows, K] to Int8 codes with a Float scale each, behind what FRONT names:
+// nothing, an RMS norm (WEIGHT [1, K] optional, EPSILON a scalar) or swish(X) * UP.
+class QuantizeRowsAttr : public AttributesCRTP<QuantizeRowsAttr> {
+public:
+  enum class InputNames : uint8_t { X, UP, WEIGHT, EPSILON };
+  enum class OutputNames : uint8_t { Q, SCALE };
+  enum class Front : uint8_t { NONE, RMSNORM, SWISH_GATE };
+  FUSILLI_SLOT_MAPS
+  FUSILLI_IN_SLOT(QuantizeRowsAttr, X)
+  FUSILLI_IN_SLOT(QuantizeRowsAttr, UP)
+  FUSILLI_IN_SLOT(QuantizeRowsAttr, WEIGHT)
+  FUSILLI_OUT_SLOT(QuantizeRowsAttr, Q)
+  FUSILLI_OUT_SLOT(QuantizeRowsAttr, SCALE)
+
+  QuantizeRowsAttr &setEpsilon(const TensorPtr &eps) {
+    return setInput(InputNames::EPSILON, eps);
+  }
+  TensorPtr getEpsilon() const { return getInput(InputNames::EPSILON); }
+  QuantizeRowsAttr &setFront(Front f) {
+    front_ = f;
+    return *this;
+  }
+  Front getFront() const { return front_; }
+
+private:
+  Front front_ = Front::NONE;
+};
+
+// C = A B of Int8 codes, times A_SCALE [M, 1] (or [1, 1]) and B_SCALE [1, N] (or
+// [1, 1]), plus BIAS [1, N].
+class MatmulQuantizedAttr : public AttributesCRTP<MatmulQuantizedAttr> {
+public:
+  enum class InputNames : uint8_t { A, B, A_SCALE, B_SCALE, BIAS };
+  enum class OutputNames : uint8_t { C };
+  FUSILLI_SLOT_MAPS
+  FUSILLI_IN_SLOT(MatmulQuantizedAttr, A)
+  FUSILLI_IN_SLOT(MatmulQuantizedAttr, B)
+  FUSILLI_IN_SLOT(MatmulQuantizedAttr, A_SCALE)
+  FUSILLI_IN_SLOT(MatmulQuantizedAttr, B_SCALE)
+  FUSILLI_IN_SLOT(MatmulQuantizedAttr, BIAS)
+  FUSILLI_OUT_SLOT(MatmulQuantizedAttr, C)
+};
+
+// A token for each row of LOGITS [rows, words].  UNIFORM and those settings that
+// are no scalar constants are vectors [rows]; a setting that is null is off.
+class SampleAttr : public AttributesCRTP<SampleAttr> {
+public:
+  enum class InputNames : uint8_t {
+    LOGITS,
+    UNIFORM,
+    TEMPERATURE,
+    TOP_K,
+    TOP_P,
+    MIN_P
+  };
+  enum class OutputNames : uint8_t { TOKEN, PROBABILITY };
+  FUSILLI_SLOT_MAPS
+  FUSILLI_IN_SLOT(SampleAttr, LOGITS)
+  FUSILLI_IN_SLOT(SampleAttr, UNIFORM)
+  FUSILLI_IN_SLOT(SampleAttr, TEMPERATURE)
+  FUSILLI_IN_SLOT(SampleAttr, TOP_K)
+  FUSILLI_IN_SLOT(SampleAttr, TOP_P)
+  FUSILLI_IN_SLOT(SampleAttr, MIN_P)
+  FUSILLI_OUT_SLOT(SampleAttr, TOKEN)
+  FUSILLI_OUT_SLOT(SampleAttr, PROBABILITY)
+};
+
 // ---- RMSNorm (attributes/rmsnorm_attributes.h) ------------------------------
 class RmsnormAttr : public AttributesCRTP<RmsnormAttr> {
 public:

@@ -46,6 +46,9 @@ enum class StepKind : uint32_t {
   SdpaPaged = 11,
   CacheAppend = 12,
   CacheRead = 13,
+  QuantizeRows = 14,
+  MatmulQuantized = 15,
+  Sample = 16,
 };
 
 constexpr int kMaxSlots = 12;
@@ -75,6 +78,9 @@ union StepDesc {
   fhip_sdpa_paged_desc sdpaPaged;
   CacheAppendStep cacheAppend;
   fhip_cache_read_desc cacheRead;
+  fhip_quantize_rows_desc quantizeRows;
+  fhip_matmul_quantized_desc matmulQuantized;
+  fhip_sample_desc sample;
 };
 // A step's size is part of a saved plan's format.
 static_assert(sizeof(StepDesc) == sizeof(fhip_norm_desc));
@@ -148,6 +154,24 @@ enum : int { // the cache of the three operations on one: from kCa
   kAppPositions = 11,
   kReadK = 7,
   kReadV = 8
+};
+enum : int { kQrX = 0, kQrUp = 1, kQrWeight = 2, kQrQ = 3, kQrScale = 4 };
+enum : int {
+  kMqA = 0,
+  kMqB = 1,
+  kMqAScale = 2,
+  kMqBScale = 3,
+  kMqBias = 4,
+  kMqOut = 5,
+  kMqEpi = 6
+};
+enum : int { // the settings from kSmSettings: temperature, top-k, top-p, min-p
+  kSmLogits = 0,
+  kSmUniform = 1,
+  kSmSettings = 2,
+  kSmToken = 6,
+  kSmProbability = 7,
+  kSmScratch = 8
 };
 enum : int { kRdX = 0, kRdY = 1 };
 enum : int { kPwIn0 = 0, kPwIn1 = 1, kPwIn2 = 2, kPwOut = 3 };
@@ -370,6 +394,19 @@ public:
         FUSILLI_CHECK_ERROR(planCacheRead(i));
         ++i;
         break;
+      case INode::Type::QuantizeRows:
+        FUSILLI_CHECK_ERROR(planQuantizeRows(i));
+        ++i;
+        break;
+      case INode::Type::MatmulQuantized: {
+        FUSILLI_ASSIGN_OR_RETURN(size_t next, planMatmulQuantized(i));
+        i = next;
+        break;
+      }
+      case INode::Type::Sample:
+        FUSILLI_CHECK_ERROR(planSample(i));
+        ++i;
+        break;
       case INode::Type::Reduction:
         FUSILLI_CHECK_ERROR(planReduction(i));
         ++i;
@@ -442,6 +479,15 @@ private:
       break;
     case INode::Type::CacheRead:
       each(static_cast<const CacheReadNode &>(n).cacheReadAttr);
+      break;
+    case INode::Type::QuantizeRows:
+      each(static_cast<const QuantizeRowsNode &>(n).quantizeRowsAttr);
+      break;
+    case INode::Type::MatmulQuantized:
+      each(static_cast<const MatmulQuantizedNode &>(n).matmulQuantizedAttr);
+      break;
+    case INode::Type::Sample:
+      each(static_cast<const SampleNode &>(n).sampleAttr);
       break;
     case INode::Type::RmsNorm:
       each(static_cast<const RmsNormNode &>(n).rmsnormAttr);
@@ -954,6 +1000,148 @@ private:
     return ok();
   }
 
+  // -- models served in 8 bits -----------------------------------------------------
+  ErrorObject planQuantizeRows(size_t i) {
+    using Front = QuantizeRowsAttr::Front;
+    const auto &attr =
+        static_cast<const QuantizeRowsNode &>(*nodes_[i]).quantizeRowsAttr;
+    FUSILLI_CHECK_ERROR(QuantizeRowsNode::checkShapes(
+        attr, "Node '" + attr.getName() + "':"));
+    Step s;
+    s.kind = static_cast<uint32_t>(StepKind::QuantizeRows);
+    fhip_quantize_rows_desc &d = s.desc.quantizeRows;
+    FUSILLI_ASSIGN_OR_RETURN(d.x, toDesc(attr.getX()));
+    FUSILLI_ASSIGN_OR_RETURN(d.q, toDesc(attr.getQ()));
+    d.scale_stride = attr.getSCALE()->getStride()[0];
+    d.front = attr.getFront() == Front::RMSNORM      ? FHIP_QUANTIZE_RMSNORM
+              : attr.getFront() == Front::SWISH_GATE ? FHIP_QUANTIZE_SWISH_GATE
+                                                     : FHIP_QUANTIZE_NONE;
+    if (attr.getFront() == Front::RMSNORM)
+      d.epsilon = static_cast<float>(scalarAsDouble(*attr.getEpsilon()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kQrX], readSlot(attr.getX()));
+    if (const TensorPtr t = attr.getUP()) {
+      FUSILLI_ASSIGN_OR_RETURN(d.up, toDesc(t));
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kQrUp], readSlot(t));
+    }
+    if (const TensorPtr t = attr.getWEIGHT()) {
+      d.has_weight = 1;
+      d.weight_dtype = static_cast<int32_t>(t->getDataType());
+      d.weight_stride = t->getStride()[1];
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kQrWeight], readSlot(t));
+    }
+    FUSILLI_CHECK_ERROR(mustRun(fhip_quantize_rows_supported(&d) != 0,
+                                "Quantize rows", attr.getName()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kQrQ], writeSlot(attr.getQ()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kQrScale], writeSlot(attr.getSCALE()));
+    plan_.steps.push_back(s);
+    return ok();
+  }
+
+  ErrorOr<size_t> planMatmulQuantized(size_t i) {
+    const auto &attr = static_cast<const MatmulQuantizedNode &>(*nodes_[i])
+                           .matmulQuantizedAttr;
+    FUSILLI_CHECK_ERROR(MatmulQuantizedNode::checkShapes(
+        attr, "Node '" + attr.getName() + "':"));
+    Step s;
+    s.kind = static_cast<uint32_t>(StepKind::MatmulQuantized);
+    fhip_matmul_quantized_desc &d = s.desc.matmulQuantized;
+    FUSILLI_ASSIGN_OR_RETURN(d.a, toDesc(attr.getA()));
+    FUSILLI_ASSIGN_OR_RETURN(d.b, toDesc(attr.getB()));
+    FUSILLI_ASSIGN_OR_RETURN(d.c, toDesc(attr.getC()));
+    // (one value for all: a stride of 0)
+    auto along = [](const TensorPtr &t, size_t dim) {
+      return t->getDim()[dim] == 1 ? int64_t{0} : t->getStride()[dim];
+    };
+    d.a_scale_stride = along(attr.getA_SCALE(), 0);
+    d.b_scale_stride = along(attr.getB_SCALE(), 1);
+    if (const TensorPtr t = attr.getBIAS()) {
+      d.has_bias = 1;
+      d.bias_dtype = static_cast<int32_t>(t->getDataType());
+      d.bias_stride = along(t, 1);
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kMqBias], readSlot(t));
+    }
+    d.out = d.c;
+    d.out_dtype = d.c.dtype;
+    TensorPtr cur = attr.getC();
+    std::vector<TensorPtr> operands;
+    FUSILLI_ASSIGN_OR_RETURN(
+        size_t next,
+        fuseFollowers(i, cur, d.epilogue, operands,
+                      [&](const fhip_epilogue &e, const TensorPtr &out) {
+                        fhip_matmul_quantized_desc t;
+                        std::memcpy(&t, &d, sizeof(d));
+                        std::memcpy(&t.epilogue, &e, sizeof(e));
+                        auto od = toDesc(out);
+                        if (isError(od))
+                          return false;
+                        std::memcpy(&t.out, &*od, sizeof(t.out));
+                        t.out_dtype = od->dtype;
+                        if (fhip_matmul_quantized_supported(&t) == 0)
+                          return false;
+                        std::memcpy(&d, &t, sizeof(d));
+                        return true;
+                      }));
+    FUSILLI_CHECK_ERROR(mustRun(fhip_matmul_quantized_supported(&d) != 0,
+                                "Quantized matmul", attr.getName()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kMqA], readSlot(attr.getA()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kMqB], readSlot(attr.getB()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kMqAScale], readSlot(attr.getA_SCALE()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kMqBScale], readSlot(attr.getB_SCALE()));
+    for (size_t k = 0; k < operands.size(); ++k) {
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kMqEpi + k], readSlot(operands[k]));
+    }
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kMqOut], writeSlot(cur));
+    plan_.steps.push_back(s);
+    return ok(next);
+  }
+
+  ErrorObject planSample(size_t i) {
+    const auto &attr = static_cast<const SampleNode &>(*nodes_[i]).sampleAttr;
+    FUSILLI_CHECK_ERROR(
+        SampleNode::checkShapes(attr, "Node '" + attr.getName() + "':"));
+    Step s;
+    s.kind = static_cast<uint32_t>(StepKind::Sample);
+    fhip_sample_desc &d = s.desc.sample;
+    FUSILLI_ASSIGN_OR_RETURN(d.logits, toDesc(attr.getLOGITS()));
+    d.temperature = d.top_p = 1.0f;
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSmLogits], readSlot(attr.getLOGITS()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSmUniform], readSlot(attr.getUNIFORM()));
+    const TensorPtr settings[4] = {attr.getTEMPERATURE(), attr.getTOP_K(),
+                                   attr.getTOP_P(), attr.getMIN_P()};
+    int32_t *has[4] = {&d.has_temperature, &d.has_top_k, &d.has_top_p,
+                       &d.has_min_p};
+    for (int k = 0; k < 4; ++k) {
+      if (!settings[k])
+        continue;
+      if (settings[k]->isScalar()) {
+        const double v = scalarAsDouble(*settings[k]);
+        if (k == 1) // (0 or less: off; more than there are words: all)
+          d.top_k = v < 1 ? 0 : v > 2147483647.0 ? 2147483647 : static_cast<int32_t>(v);
+        else
+          (k == 0 ? d.temperature : k == 2 ? d.top_p : d.min_p) =
+              static_cast<float>(v);
+        continue;
+      }
+      *has[k] = 1;
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kSmSettings + k], readSlot(settings[k]));
+    }
+    FUSILLI_CHECK_ERROR(
+        mustRun(fhip_sample_supported(&d) != 0, "Sample", attr.getName()));
+    FUSILLI_ASSIGN_OR_RETURN(s.slot[kSmToken], writeSlot(attr.getTOKEN()));
+    // (a virtual PROBABILITY that no node reads is not written)
+    const TensorPtr p = attr.getPROBABILITY();
+    if (!p->isVirtual() || consumers_.count(p.get()) > 0) {
+      FUSILLI_ASSIGN_OR_RETURN(s.slot[kSmProbability], writeSlot(p));
+    }
+    size_t scratch = 0;
+    FUSILLI_RETURN_ERROR_IF(fhip_sample_workspace_size(&d, &scratch) != 0,
+                            ErrorCode::InternalError,
+                            std::string(fhip_last_error(nullptr)));
+    s.slot[kSmScratch] = scratchSlot(scratch);
+    plan_.steps.push_back(s);
+    return ok();
+  }
+
   ErrorObject planReduction(size_t i) {
     const auto &attr =
         static_cast<const ReductionNode &>(*nodes_[i]).reductionAttr;
@@ -1252,6 +1440,29 @@ inline ErrorObject execute(fhip_ctx *ctx, const Plan &p,
                            ptr(s.slot[kReadV]), nullptr, 0);
       break;
     }
+    case StepKind::QuantizeRows:
+      rc = fhip_quantize_rows(ctx, &s.desc.quantizeRows, ptr(s.slot[kQrX]),
+                              ptr(s.slot[kQrUp]), ptr(s.slot[kQrWeight]),
+                              ptr(s.slot[kQrQ]), ptr(s.slot[kQrScale]), nullptr,
+                              0);
+      break;
+    case StepKind::MatmulQuantized:
+      for (int k = 0; k < FHIP_MAX_EPILOGUE; ++k)
+        epi[k] = ptr(s.slot[kMqEpi + k]);
+      rc = fhip_matmul_quantized(
+          ctx, &s.desc.matmulQuantized, ptr(s.slot[kMqA]), ptr(s.slot[kMqB]),
+          ptr(s.slot[kMqAScale]), ptr(s.slot[kMqBScale]), ptr(s.slot[kMqBias]),
+          epi, ptr(s.slot[kMqOut]), nullptr, 0);
+      break;
+    case StepKind::Sample:
+      rc = fhip_sample(ctx, &s.desc.sample, ptr(s.slot[kSmLogits]),
+                       ptr(s.slot[kSmUniform]), ptr(s.slot[kSmSettings]),
+                       ptr(s.slot[kSmSettings + 1]),
+                       ptr(s.slot[kSmSettings + 2]),
+                       ptr(s.slot[kSmSettings + 3]), ptr(s.slot[kSmToken]),
+                       ptr(s.slot[kSmProbability]), ptr(s.slot[kSmScratch]),
+                       bytesOf(s.slot[kSmScratch]));
+      break;
     case StepKind::Reduce:
       rc = fhip_reduce(ctx, &s.desc.reduce, ptr(s.slot[kRdX]),
                        ptr(s.slot[kRdY]), nullptr, 0);

@@ -6,6 +6,7 @@ import pytest
 
 from fusilli_amd import capi
 from quantized import codes_in_f32, matrix, token
+from serving import cpp_binary
 
 LIB = capi.load()
 BF16, F16, F32, I8 = capi.BFLOAT16, capi.HALF, capi.FLOAT, capi.INT8
@@ -132,3 +133,8 @@ def test_the_formulas_on_known_rows():
     assert token(l, 0.99, k=2) == (2, pytest.approx(2 / 6))
     assert token(l, 0.99, p=0.8)[0] == 0 and token(l, 0.99, least=0.3)[0] == 2 and token(l, 0.99, t=0) == (1, 1.0)
     assert token([-np.inf, np.nan], 0.5) == (-1, 0.0)
+
+
+# -- the C++ graph API (tests/cpp/test_quantized_api.cpp) -------------------------
+def test_cpp_nodes_and_plans():
+    cpp_binary("test_quantized_api", 120, "host")

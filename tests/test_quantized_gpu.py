@@ -4,7 +4,8 @@ import pytest
 
 from fusilli_amd import capi
 from helpers import HT
-from quantized import check_codes, check_product, codes_in_f32, front, guarded, product, token, tokens
+from quantized import check_codes, check_product, codes_in_f32, front, guarded, product, tokens
+from serving import cpp_binary
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = capi.BFLOAT16, capi.HALF, capi.FLOAT
@@ -425,3 +426,8 @@ def test_sample_covers_the_distribution(ctx):
     w /= w.sum()
     assert (np.abs(np.bincount(got, minlength=words) - n * w) <= 1.01).all()
     assert np.allclose(chance, w[got], rtol=3e-7)
+
+
+# ---- the C++ graph API -------------------------------------------------------------------
+def test_graphs():
+    cpp_binary("test_quantized_api", 120)
