@@ -323,11 +323,13 @@ def settings(rng, rows, words):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAME.get)
 @pytest.mark.parametrize("rows,words", [(1, 1), (3, 2), (40, 63), (9, 64), (33, 500), (5, 1025), (3, 4099), (4, 32000), (1, 70001),
-                                        (2, 131072), (300, 200), (260, 5000)])
+                                        (2, 131072), (300, 200), (260, 5000), (130, 9000), (127, 4100)])
 def test_sample(ctx, dtype, rows, words):
     rng = rng_of(13, rows, words, dtype)
     x = HT.from_logical(rng.normal(size=[rows, words]) * rng.choice([0.3, 1.5, 4.0], [rows, 1]), dtype)
-    check_tokens(ctx, x, rng.random(rows).astype(np.float32), *settings(rng, rows, words))
+    check_tokens(ctx, x, rng.random(rows).astype(np.float32), *settings(rng, rows, words), fast=True)
+    parts = max(1, min(512 // rows if rows < 128 else 1, (words + 4095) // 4096, 32))
+    assert ctx.last_kernel() == f"sample parts={parts}"
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAME.get)
