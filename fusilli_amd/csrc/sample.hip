@@ -31,8 +31,8 @@ struct SampleArgs {
   int32_t parts, part_words;
   uint64_t *part_most; // [row][part]: largest key, then the lowest index that has it
   float *part_least;   // [row][part]: smallest logit that may be drawn
-  uint64_t *sums;      // [row][part][bucket]
-  uint32_t *counts;    // the same
+  unsigned long long *sums; // [row][bucket], cleared by the first launch
+  uint32_t *counts;         // the same
 };
 
 // Ascending with the logit: 0 for what is never drawn (NaN, -inf); -0 is 0.
@@ -48,8 +48,10 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 
 // A row's settings.
 struct Settings {
-  double most, by; // the largest logit, 1 / T
-  double unit;     // 2^bits
+  double most, by;  // the largest logit, 1 / T
+  double cut, by2;  // (logits this far below weigh nothing), log2(e) / T
+  float top;        // the largest logit
+  int bits;
   float p, least, u;
   int k;
   bool greedy;
@@ -62,13 +64,35 @@ struct Settings {
     most = (double)largest;
     greedy = !(t > 0.f);
     by = greedy ? 1.0 : fmax(1.0 / (double)t, 1e-300); // (T infinite: -inf times it is -inf)
-    unit = (double)(1ull << g.bits);
+    cut = -32.0 / by;
+    by2 = by * 1.44269504088896340736;
+    top = largest;
+    bits = g.bits;
   }
-  __device__ __forceinline__ double down(float l) const { return l == (float)most ? 0.0 : ((double)l - most) * by; }
-  __device__ __forceinline__ double weight(float l) const { return exp(down(l)); }
+  __device__ __forceinline__ double weight(float l) const { return l == top ? 1.0 : exp(((double)l - most) * by); }
+  // The weight in units of 2^-bits, rounded; 0 from exp(-32) = 2^-46.2 on.  2^x with x = n + f, |f| at
+  // most 1/2: a polynomial of degree 10 through 1 at 0 that meets 2^f at the zeros of a Chebyshev
+  // polynomial (6e-16 of it off at most); the unit's power goes into n, and 2^52 on top leaves the
+  // rounded value in the low bits.  16 instructions; the library's exp and the conversion to 64 bits
+  // take more than twice as many.
   __device__ __forceinline__ uint64_t held(float l) const {
-    const double x = down(l);
-    return x > -32.0 ? (uint64_t)rint(exp(x) * unit) : 0; // (exp(-32) is 2^-46.2)
+    const double d = l == top ? 0.0 : (double)l - most;
+    const double x = (d > cut ? d : 0.0) * by2;
+    const double n = rint(x), f = x - n;
+    double y = 7.0709662925771758e-09;
+    y = __builtin_fma(y, f, 1.0205905366447884e-07);
+    y = __builtin_fma(y, f, 1.3215451705400571e-06);
+    y = __builtin_fma(y, f, 1.5252672925113478e-05);
+    y = __builtin_fma(y, f, 1.5403530424618647e-04);
+    y = __builtin_fma(y, f, 1.3333558200794100e-03);
+    y = __builtin_fma(y, f, 9.6181291076188023e-03);
+    y = __builtin_fma(y, f, 5.5504108664651677e-02);
+    y = __builtin_fma(y, f, 2.4022650695910075e-01);
+    y = __builtin_fma(y, f, 6.9314718055994617e-01);
+    y = __builtin_fma(y, f, 1.0);
+    y = __builtin_amdgcn_ldexp(y, (int)n + bits) + 0x1p52;
+    const uint64_t v = __builtin_bit_cast(uint64_t, y) & ((1ull << 52) - 1);
+    return d > cut ? v : 0;
   }
   // the weights' sum that top_p asks for of `all`; the sum that the token's exceeds of `kept`
   __device__ __forceinline__ uint64_t share(uint64_t all) const {
@@ -284,120 +308,281 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs g) 
 // over parts of rows.
 //
 // Buckets cover what words have above a weight of 0, less than 32 of (m - l) / T.
+//
+// Which buckets matter one wavefront finds, without a barrier: sixteen that execute the same few hundred
+// instructions between barriers take three times as long.
 constexpr int kBuckets = 1024, kThreads = 1024;
 constexpr int kList = 8192; // words of the buckets in question
 
 // N words from `at` of a row whose words lie side by side, at element alignment.
+template <typename E, int COUNT> struct WordsOf {
+  static constexpr int N = COUNT;
+  typedef E V __attribute__((ext_vector_type(COUNT), aligned(sizeof(E))));
+  static __device__ __forceinline__ float one(const void *p, int64_t at) { return (float)((const E *)p)[at]; }
+  static __device__ __forceinline__ V load(const void *p, int64_t at) { return *(const V *)((const E *)p + at); }
+};
 template <int DT> struct Words;
-template <> struct Words<FHIP_FLOAT> {
-  static constexpr int N = 4;
-  typedef float V __attribute__((ext_vector_type(4), aligned(4)));
-  static __device__ __forceinline__ float one(const void *p, int64_t at) { return ((const float *)p)[at]; }
-  static __device__ __forceinline__ void load(const void *p, int64_t at, float (&v)[N]) {
-    const V x = *(const V *)((const float *)p + at);
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-  }
-};
-template <typename H> struct HalfWords {
-  static constexpr int N = 8;
-  typedef H V __attribute__((ext_vector_type(8), aligned(2)));
-  static __device__ __forceinline__ float one(const void *p, int64_t at) { return (float)((const H *)p)[at]; }
-  static __device__ __forceinline__ void load(const void *p, int64_t at, float (&v)[N]) {
-    const V x = *(const V *)((const H *)p + at);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      v[i] = (float)x[i];
-  }
-};
-template <> struct Words<FHIP_BFLOAT16> : HalfWords<__bf16> {};
-template <> struct Words<FHIP_HALF> : HalfWords<_Float16> {};
+template <> struct Words<FHIP_FLOAT> : WordsOf<float, 4> {};
+template <> struct Words<FHIP_BFLOAT16> : WordsOf<__bf16, 8> {};
+template <> struct Words<FHIP_HALF> : WordsOf<_Float16, 8> {};
 
-// take(logit, index) of the words from .. to - 1 of a row
-template <int DT, int NT, typename Take>
+// take(logits, first index) of the words from .. to - 1 of a row, N of them at a time (-inf where
+// fewer are left), with U loads on their way.
+template <int DT, int U, typename Take>
 __device__ __forceinline__ void for_words(const SampleArgs &g, int64_t row, int from, int to, Take take) {
   using W = Words<DT>;
+  constexpr int STEP = kThreads * W::N;
   const int64_t base = row * g.row_s;
-  const int whole = from + (to - from) / W::N * W::N;
-#pragma unroll 4
-  for (int i = from + (int)threadIdx.x * W::N; i < whole; i += NT * W::N) {
-    float v[W::N];
-    W::load(g.logits, base + i, v);
+  const int whole = from + (to - from) / W::N * W::N, last = whole - W::N;
+  const int first = from + (int)threadIdx.x * W::N;
+  typename W::V raw[U];
+  auto fetch = [&](int u, int i) { raw[u] = W::load(g.logits, base + (i < last ? i : last)); };
+  if (last >= from) {
 #pragma unroll
-    for (int e = 0; e < W::N; ++e)
-      take(v[e], i + e);
+    for (int u = 0; u < U; ++u)
+      fetch(u, first + u * STEP);
+#pragma clang loop unroll(disable)
+    for (int i = first; i < whole; i += U * STEP) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[W::N];
+#pragma unroll
+        for (int e = 0; e < W::N; ++e)
+          v[e] = (float)raw[u][e];
+        fetch(u, i + (u + U) * STEP);
+        if (u == 0 || i + u * STEP < whole)
+          take(v, i + u * STEP);
+      }
+    }
   }
-  for (int i = whole + (int)threadIdx.x; i < to; i += NT)
-    take(W::one(g.logits, base + i), i);
+  if (whole + (int)threadIdx.x < to) { // (fewer than a vector)
+    float v[W::N];
+    v[0] = W::one(g.logits, base + whole + threadIdx.x);
+#pragma unroll
+    for (int e = 1; e < W::N; ++e)
+      v[e] = -INFINITY;
+    take(v, whole + (int)threadIdx.x);
+  }
 }
 
-// What is known of a row, or a part of it: its largest key and the lowest index that has it (0: no
-// word may be drawn), its smallest logit that may be drawn.
+// Sums over the lanes up to each, and the largest value of a wavefront.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t from_lane(uint32_t v) { // (0 where there is none)
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 15, false);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t from_lane(uint64_t v) {
+  return (uint64_t)from_lane<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | from_lane<CTRL, ROWS>((uint32_t)v);
+}
+template <typename T, typename F> __device__ __forceinline__ T up_to_lane(T v, F join) {
+  v = join(v, from_lane<0x111, 15>(v)); // from 1, 2, 4 and 8 lanes below in a row of 16
+  v = join(v, from_lane<0x112, 15>(v));
+  v = join(v, from_lane<0x114, 15>(v));
+  v = join(v, from_lane<0x118, 15>(v));
+  v = join(v, from_lane<0x142, 10>(v)); // a row's last lane to the next row, the first half's to the second
+  v = join(v, from_lane<0x143, 12>(v));
+  return v;
+}
+template <typename T> __device__ __forceinline__ T sum_up_to_lane(T v) {
+  return up_to_lane(v, [](T a, T b) { return a + b; });
+}
+__device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+__device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+template <typename T> __device__ __forceinline__ T largest_of_wave(T v) {
+  return of_lane(up_to_lane(v, [](T a, T b) { return a > b ? a : b; }), 63);
+}
+// (a wavefront's LDS accesses keep their order; this keeps the compiler from changing it)
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// What is known of a row, or a part of it: its largest key and the complement of the lowest index that has
+// it (0: no word may be drawn), its smallest logit that may be drawn.
 struct Range {
   uint64_t most;
   float least;
   __device__ __forceinline__ float largest() const { return logit_of((uint32_t)(most >> 32)); }
 };
-template <int DT> __device__ __forceinline__ Range range_of(const SampleArgs &g, int64_t row, int from, int to, Shared<kThreads> &s) {
-  uint64_t most = 0;
-  float least = INFINITY;
-  for_words<DT, kThreads>(g, row, from, to, [&](float l, int i) {
-    const uint64_t x = (uint64_t)key_of(l) << 32 | ~(uint32_t)i;
-    most = l > -INFINITY && x > most ? x : most;
-    least = l > -INFINITY ? fminf(least, l) : least;
+struct RangeRoom {
+  uint64_t most[kThreads / 64];
+  uint32_t least[kThreads / 64];
+};
+template <int DT>
+__device__ __forceinline__ Range range_of(const SampleArgs &g, int64_t row, int from, int to, RangeRoom &room) {
+  using W = Words<DT>;
+  // (a thread's indices ascend: a later word has to be larger)
+  float top = -INFINITY, least = INFINITY;
+  int place = 0;
+  for_words<DT, 4>(g, row, from, to, [&](const float(&v)[W::N], int i) {
+#pragma unroll
+    for (int e = 0; e < W::N; ++e) {
+      place = v[e] > top ? i + e : place;
+      top = v[e] > top ? v[e] : top;
+      least = v[e] > -INFINITY && v[e] < least ? v[e] : least;
+    }
   });
-  auto larger = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
+  const uint64_t most = largest_of_wave<uint64_t>(top > -INFINITY ? (uint64_t)key_of(top) << 32 | ~(uint32_t)place : 0);
+  const uint32_t low = largest_of_wave<uint32_t>(~key_of(least));
+  if ((threadIdx.x & 63) == 0)
+    room.most[threadIdx.x >> 6] = most, room.least[threadIdx.x >> 6] = low;
+  __syncthreads();
+  const int w = threadIdx.x & (kThreads / 64 - 1);
   Range r;
-  r.most = over_workgroup<kThreads>(most, s, larger);
-  r.least = logit_of(0xffffffffu - (uint32_t)over_workgroup<kThreads>((uint64_t)(0xffffffffu - key_of(least)), s, larger));
+  r.most = largest_of_wave<uint64_t>(room.most[w]);
+  r.least = logit_of(~largest_of_wave<uint32_t>(room.least[w]));
   return r;
 }
 
-// A row's buckets: the first holds the largest logits.
+// A row's buckets: the first holds the largest logits.  In f32, whose differences and products keep the
+// order; halves, as a difference may be twice the largest number.
 struct Buckets {
-  double most, by;
-  float top;
-  __device__ __forceinline__ Buckets(const Settings &set, float least) : most(set.most), top((float)set.most) {
-    const double wide = -set.down(least);
-    // (a little less than the range takes, so that the last word is inside)
-    by = wide > 0.0 ? set.by * (kBuckets * (1.0 - 0x1p-20)) / (wide < 32.0 ? wide : 32.0) : 0.0;
+  float half, top, by;
+  double wide; // of (m - l) / T, all of them
+  __device__ __forceinline__ Buckets(const Settings &set, float least) : half(0.5f * set.top), top(set.top) {
+    const double range = least == top ? 0.0 : (set.most - (double)least) * set.by;
+    wide = range < 32.0 ? range : 32.0;
+    // (a little less than the range takes, so that the last word is inside for all roundings)
+    const double x = range > 0.0 ? 2.0 * set.by * (kBuckets * (1.0 - 0x1p-20)) / wide : 0.0;
+    by = x < 3.0e38 ? (float)x : 3.0e38f;
   }
-  __device__ __forceinline__ int of(float l) const { // kBuckets and more: none
-    const double b = l == top ? 0.0 : (most - (double)l) * by;
-    return b < (double)kBuckets ? (int)b : kBuckets;
+  __device__ __forceinline__ int of(float l) const { // kBuckets: none
+    const float b = l == top ? 0.f : (half - 0.5f * l) * by; // (NaN, -inf: none)
+    return b < (float)kBuckets ? (int)b : kBuckets;
   }
 };
+// Where a bucket lies in LDS: a lane's sixteen in a row, lanes on banks of their own.
+__device__ __forceinline__ int bucket_place(int b) { return b + (b >> 4); }
+constexpr int kPlaces = kBuckets + kBuckets / 16 + 1;
 
 struct Sums {
-  uint64_t sum[kBuckets];
-  uint32_t count[kBuckets];
+  unsigned long long sum[kPlaces];
+  uint32_t count[kPlaces];
 };
 template <int DT>
 __device__ __forceinline__ void sums_of(const SampleArgs &g, int64_t row, int from, int to, const Settings &set,
                                         const Buckets &buckets, bool count, Sums &s) {
-  s.sum[threadIdx.x] = 0, s.count[threadIdx.x] = 0;
+  using W = Words<DT>;
+  for (int i = threadIdx.x; i < kPlaces; i += kThreads)
+    s.sum[i] = 0, s.count[i] = 0;
   __syncthreads();
-  for_words<DT, kThreads>(g, row, from, to, [&](float l, int) {
-    if (!(l > -INFINITY))
-      return;
-    const int b = buckets.of(l);
-    if (b >= kBuckets)
-      return;
-    atomicAdd((unsigned long long *)&s.sum[b], (unsigned long long)set.held(l));
-    if (count)
-      atomicAdd(&s.count[b], 1u);
+  for_words<DT, 1>(g, row, from, to, [&](const float(&v)[W::N], int) {
+#pragma unroll
+    for (int e = 0; e < W::N; ++e) {
+      const int b = buckets.of(v[e]);
+      if (b < kBuckets) {
+        atomicAdd(&s.sum[bucket_place(b)], (unsigned long long)set.held(v[e]));
+        if (count)
+          atomicAdd(&s.count[bucket_place(b)], 1u);
+      }
+    }
   });
   __syncthreads();
 }
 
-struct Draw {
-  Shared<kThreads> s;
-  uint64_t before[kBuckets + 1]; // weights in front of a bucket
-  uint8_t asked[kBuckets];
-  int located[6], filled;
-  uint32_t count_before;
-  uint32_t keys[kList], places[kList];
-  uint16_t homes[kList];
+struct Bins {
+  uint64_t sum[256];
+  uint32_t count[256];
 };
+struct Draw {
+  union {
+    Bins bins;
+    Shared<kThreads> whole; // of a row that does not fit the list
+  };
+  uint64_t before[kPlaces];        // weights in front of a bucket
+  uint32_t first[kPlaces];         // words in front of it
+  uint32_t asked[kBuckets / 32 + 1]; // a bit a bucket (the last: none)
+  uint64_t all;
+  float floor; // no word in question is smaller
+  int by_k, least_from, least_to;
+  int filled;
+  uint32_t high, low; // largest key, complement of the smallest
+  End end;
+  float logits[kList];
+  uint32_t places[kList];
+};
+
+// find_end above over the list.  (d.high and d.low are 0 before and after.)
+template <typename Key, typename Held>
+__device__ __forceinline__ End list_end(bool by_count, uint64_t need, int n, Draw &d, Key key_at, Held held) {
+  const int t = threadIdx.x, l = t & 63;
+  auto clear = [&] {
+    if (t < 256)
+      d.bins.sum[t] = 0, d.bins.count[t] = 0;
+  };
+  uint32_t high = 0, low = 0;
+  for (int i = t; i < n; i += kThreads) {
+    const uint32_t key = key_at(i);
+    high = key > high ? key : high;
+    low = key && ~key > low ? ~key : low;
+  }
+  if (t / 64 * 64 < n) {
+    high = largest_of_wave<uint32_t>(high), low = largest_of_wave<uint32_t>(low);
+    if (l == 0 && high)
+      atomicMax(&d.high, high), atomicMax(&d.low, low);
+  }
+  clear();
+  __syncthreads();
+  high = d.high, low = ~d.low;
+  int left = high == low ? 0 : 32 - __builtin_clz(high ^ low); // bits in which keys differ
+  uint32_t prefix = left == 32 ? 0 : high >> left << left;
+  End e{prefix, 0, 0, 0};
+  for (;;) {
+    const int shift = left > 8 ? left - 8 : 0;
+    const uint32_t above = left == 32 ? 0 : ~0u << left; // bits that the prefix has
+    for (int i = t; i < n; i += kThreads) {
+      const uint32_t key = key_at(i);
+      if (key == 0 || (key & above) != e.key)
+        continue;
+      const int digit = (int)((key & ~above) >> shift);
+      atomicAdd(&d.bins.count[digit], 1u);
+      atomicAdd((unsigned long long *)&d.bins.sum[digit], (unsigned long long)held(key));
+    }
+    __syncthreads();
+    if (t < 64) {
+      // (four digits a lane, the largest first)
+      uint32_t c[4], cs = 0;
+      uint64_t w[4], ws = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] = d.bins.count[255 - 4 * l - i], w[i] = d.bins.sum[255 - 4 * l - i];
+        cs += c[i], ws += w[i];
+      }
+      uint32_t c0 = e.count + sum_up_to_lane(cs) - cs; // in front of this lane's
+      uint64_t w0 = e.sum + sum_up_to_lane(ws) - ws;
+      int found = -1;
+      uint32_t own = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool here = c[i] != 0 && (by_count ? c0 + c[i] >= need : w0 + w[i] >= need);
+        if (here && found < 0)
+          found = i, own = c[i];
+        if (found < 0)
+          c0 += c[i], w0 += w[i];
+      }
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(found >= 0);
+      if (l == (hit ? __builtin_ctzll(hit) : 0))
+        d.end = End{e.key | (uint32_t)(255 - 4 * l - (found < 0 ? 0 : found)) << shift, c0, w0, own};
+      if (l == 0)
+        d.high = d.low = 0;
+    }
+    __syncthreads();
+    e = d.end;
+    left = shift;
+    if (left == 0)
+      break;
+    clear();
+    __syncthreads();
+  }
+  const uint32_t same = e.ties;
+  const uint64_t each = held(e.key);
+  const uint64_t ties = by_count ? need - e.count : need <= e.sum || each == 0 ? 1 : (need - e.sum + each - 1) / each;
+  e.ties = (uint32_t)(ties < 1 ? 1 : ties > same ? same : ties);
+  return e;
+}
 
 // A row without a question; false: there are some.
 __device__ __forceinline__ bool settled(const SampleArgs &g, int64_t row, const Range &range) {
@@ -412,144 +597,197 @@ __device__ __forceinline__ bool settled(const SampleArgs &g, int64_t row, const 
   return true;
 }
 
-// The token of a row; `mine` and `here`: weights and words of this thread's bucket.
-template <int DT>
+// The token of a row; `sums` and `counts`: where lane l of the first wavefront finds its sixteen buckets.
+template <int DT, typename Sum, typename Count>
 __device__ __forceinline__ void draw_row(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets,
-                                         bool count, uint64_t mine, uint32_t here, Draw &d) {
-  constexpr int NT = kThreads;
-  static_assert(NT == kBuckets, "a thread a bucket");
-  const int b = threadIdx.x;
-  auto in_front = [&](uint64_t v) { // exclusive sums over the threads
-    uint64_t x = v;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-      const uint64_t y = __shfl_up((unsigned long long)x, k);
-      x += (threadIdx.x & 63) >= k ? y : 0;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63)
-      d.s.wave[threadIdx.x >> 6] = x;
-    __syncthreads();
-    for (int w = 0; w < (int)(threadIdx.x >> 6); ++w)
-      x += d.s.wave[w];
-    return x - v;
-  };
-  const uint64_t start = in_front(mine);
-  const uint32_t first = count ? (uint32_t)in_front(here) : 0;
-  d.before[b] = start;
-  if (b == NT - 1)
-    d.before[kBuckets] = start + mine;
-  if (b < 6)
-    d.located[b] = -1;
-  if (b == 0)
-    d.filled = 0;
-  __syncthreads();
-  const uint64_t all = d.before[kBuckets];
-  // which bucket holds the `need`-th unit of weight
-  auto locate = [&](int slot, uint64_t need) {
-    if (start < need && need <= start + mine)
-      d.located[slot] = b;
-  };
-  // What is kept weighs between `low` and `high`, until the words are known in which a prefix ends.
-  if (count && first < (uint32_t)set.k && (uint32_t)set.k <= first + here) {
-    d.located[0] = b;
-    d.count_before = first;
-  }
-  __syncthreads();
-  const int by_k = d.located[0]; // (-1: fewer words than k weigh anything)
-  uint64_t low = all, high = all;
-  if (by_k >= 0)
-    low = d.before[by_k], high = d.before[by_k + 1];
-  low = low < 1 ? 1 : low;
-  const bool by_p = set.p < 1.f;
-  if (by_p) {
-    locate(1, set.share(low));
-    locate(2, set.share(high));
-    __syncthreads();
-    low = d.before[d.located[1]], high = d.before[d.located[2] + 1];
-  }
-  const bool by_least = set.least > 0.f;
+                                         bool count, const Sum *sums, const Count *counts, Draw &d) {
+  const int l = threadIdx.x & 63;
+  const bool leads = threadIdx.x < 64;
+  const bool by_p = set.p < 1.f, by_least = set.least > 0.f;
   const double bound = set.least < 1.f ? (double)set.least : 1.0;
-  int least_from = kBuckets, least_to = kBuckets;
-  if (by_least) {
-    const double at = -log(bound) / set.by * buckets.by;
-    const double a = at - 1e-6, z = at + 1e-6;
-    least_from = a < 0.0 ? 0 : a < (double)kBuckets ? (int)a : kBuckets;
-    least_to = z < (double)kBuckets ? (int)z : kBuckets;
-    if (least_from < kBuckets) {
-      const uint64_t a_sum = d.before[least_from], z_sum = d.before[least_to < kBuckets ? least_to + 1 : kBuckets];
-      low = a_sum < low ? a_sum : low;
-      high = z_sum < high ? z_sum : high;
+  const uint64_t one = (uint64_t)1 << g.bits; // (the largest is always kept)
+  uint64_t all = 0, lane_start = 0, lane_end = 0; // of a lane's buckets
+  int by_k = -1, least_from = kBuckets, least_to = kBuckets;
+  // which bucket holds the `need`-th unit of weight (1 .. all)
+  auto locate = [&](uint64_t need) {
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane_start < need && need <= lane_end);
+    const int lane = hit ? __builtin_ctzll(hit) : 0;
+    const uint64_t front = __builtin_amdgcn_ballot_w64(l < 16 && d.before[lane * 17 + (l & 15)] < need);
+    return lane * 16 + (front ? __builtin_popcountll(front) - 1 : 0);
+  };
+  auto start_of = [&](int b) { return d.before[bucket_place(b)]; };
+  auto end_of = [&](int b) { return b + 1 < kBuckets ? d.before[bucket_place(b + 1)] : all; };
+  if (leads) {
+    uint64_t w[16];
+    uint32_t c[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      w[i] = sums[i], c[i] = 0;
+    if (count) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        c[i] = counts[i];
+    }
+    uint64_t ws = 0;
+    uint32_t cs = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      ws += w[i], cs += c[i];
+    lane_end = sum_up_to_lane(ws), lane_start = lane_end - ws;
+    all = of_lane(lane_end, 63);
+    const uint32_t words_end = sum_up_to_lane(cs);
+    uint64_t at = lane_start;
+    uint32_t words = words_end - cs;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      d.before[l * 17 + i] = at, d.first[l * 17 + i] = words;
+      at += w[i], words += c[i];
+    }
+    if (l <= kBuckets / 32)
+      d.asked[l] = 0;
+    if (l == 0)
+      d.filled = 0, d.high = 0, d.low = 0;
+    wave_fence();
+    // What is kept weighs between `low` and `high`, until the words are known in which a prefix ends.
+    uint64_t low = all, high = all;
+    const uint32_t k = (uint32_t)set.k;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(count && words_end - cs < k && k <= words_end);
+    if (hit) { // (otherwise fewer words than k weigh anything)
+      const int lane = __builtin_ctzll(hit);
+      const uint64_t front = __builtin_amdgcn_ballot_w64(l < 16 && d.first[lane * 17 + (l & 15)] < k);
+      by_k = lane * 16 + __builtin_popcountll(front) - 1;
+      low = start_of(by_k), high = end_of(by_k);
+    }
+    int lowest = 0; // bucket in question
+    auto ask = [&](int from, int to) { // (few, or one range of many)
+      lowest = to > lowest ? to : lowest;
+      for (int i = from + l; i <= to; i += 64)
+        atomicOr(&d.asked[i >> 5], 1u << (i & 31));
+    };
+    if (by_k >= 0)
+      ask(by_k, by_k);
+    low = low < 1 ? 1 : low;
+    if (by_p) {
+      const int a = locate(set.share(low)), z = locate(set.share(high));
+      ask(a, z);
+      low = start_of(a), high = end_of(z);
+    }
+    if (by_least) {
+      // (buckets are of f32, three roundings: less than a thousandth of one)
+      const double at = -log(bound) / buckets.wide * kBuckets * (1.0 - 0x1p-20);
+      const double a = at - 1e-3, z = at + 1e-3;
+      least_from = !(a > 0.0) ? 0 : a < (double)kBuckets ? (int)a : kBuckets; // (one bucket for all: 0)
+      least_to = !(z > 0.0) ? 0 : z < (double)kBuckets ? (int)z : kBuckets - 1;
+      if (least_from < kBuckets) {
+        ask(least_from, least_to);
+        const uint64_t a_sum = start_of(least_from), z_sum = end_of(least_to);
+        low = a_sum < low ? a_sum : low;
+        high = z_sum < high ? z_sum : high;
+      }
+    }
+    low = low < one ? one : low;
+    high = high < low ? low : high;
+    if (set.least > 1.f)
+      low = high = one;
+    ask(locate(set.below(low) + 1), locate(set.below(high) + 1));
+    if (l == 0) {
+      d.all = all, d.by_k = by_k, d.least_from = least_from, d.least_to = least_to;
+      // (below the last bucket's end, for all roundings)
+      const double end = set.most - (lowest + 2) * 2.0 / (double)buckets.by;
+      d.floor = buckets.by > 0.f && set.top < INFINITY ? (float)(end - 1e-6 * (fabs(end) + fabs(set.most))) : -INFINITY;
     }
   }
-  const uint64_t one = (uint64_t)1 << g.bits; // (the largest is always kept)
-  low = low < one ? one : low;
-  high = high < low ? low : high;
-  if (set.least > 1.f)
-    low = high = one;
-  locate(3, set.below(low) + 1);
-  locate(4, set.below(high) + 1);
   __syncthreads();
-  d.asked[b] = b == by_k || (by_p && b >= d.located[1] && b <= d.located[2]) || (b >= least_from && b <= least_to) ||
-               (b >= d.located[3] && b <= d.located[4]);
-  __syncthreads();
+  const float floor = d.floor;
   // the words of those buckets
-  for_words<DT, NT>(g, row, 0, g.words, [&](float l, int i) {
-    if (!(l > -INFINITY))
+  using W = Words<DT>;
+  for_words<DT, 4>(g, row, 0, g.words, [&](const float(&v)[W::N], int i) {
+    uint32_t hits = 0;
+    float top = v[0];
+#pragma unroll
+    for (int e = 1; e < W::N; ++e)
+      top = fmaxf(top, v[e]);
+    if (!(top >= floor)) // (most, where few words weigh much)
       return;
-    const int home = buckets.of(l);
-    if (home >= kBuckets || !d.asked[home])
-      return;
-    const int to = atomicAdd(&d.filled, 1);
-    if (to < kList)
-      d.keys[to] = key_of(l), d.places[to] = (uint32_t)i, d.homes[to] = (uint16_t)home;
+#pragma unroll
+    for (int e = 0; e < W::N; ++e) {
+      const int b = buckets.of(v[e]);
+      hits |= (d.asked[b >> 5] >> (b & 31) & 1) << e;
+    }
+    if (hits) { // (few)
+#pragma unroll
+      for (int e = 0; e < W::N; ++e)
+        if (hits >> e & 1) {
+          const int to = atomicAdd(&d.filled, 1);
+          if (to < kList)
+            d.logits[to] = v[e], d.places[to] = (uint32_t)(i + e);
+        }
+    }
   });
   __syncthreads();
   const int n = d.filled;
   if (n > kList) { // (many equal logits)
-    sample_row<NT>(g, row, d.s);
+    sample_row<kThreads>(g, row, d.whole);
     return;
   }
-  auto held = [&](uint32_t key) { return set.held(logit_of(key)); };
-  auto of_bucket = [&](int home) { return [&, home](int i) { return d.homes[i] == home ? d.keys[i] : 0u; }; };
-  auto bucket_of = [&](uint64_t need) {
-    __syncthreads();
-    locate(5, need);
-    __syncthreads();
-    return d.located[5];
-  };
+  all = d.all, by_k = d.by_k, least_from = d.least_from, least_to = d.least_to;
+  lane_start = d.before[l * 17], lane_end = l < 63 ? d.before[l * 17 + 17] : all;
+  // The questions in turn: what the first k weigh, how far top_p reaches, which word is drawn, and its
+  // index among those that are equal.  (One loop, so that the search is in the code once.)
   uint64_t kept = all;
-  if (by_k >= 0) {
-    const End e = find_end<NT>(true, (uint64_t)set.k - d.count_before, n, d.s, of_bucket(by_k), held);
-    kept = d.before[by_k] + e.sum + e.ties * held(e.key);
-  }
-  uint64_t strict = kept;
-  if (by_p) {
-    const uint64_t need = set.share(kept);
-    const int home = bucket_of(need);
-    const End e = find_end<NT>(false, need - d.before[home], n, d.s, of_bucket(home), held);
-    strict = d.before[home] + e.sum + e.ties * held(e.key);
-  }
-  if (by_least && least_from < kBuckets) {
-    uint64_t large = 0;
-    for (int i = threadIdx.x; i < n; i += NT)
-      if (d.homes[i] >= least_from && d.homes[i] <= least_to && set.weight(logit_of(d.keys[i])) >= bound)
-        large += held(d.keys[i]);
-    large = d.before[least_from] + over_workgroup<NT>(large, d.s, [](uint64_t a, uint64_t c) { return a + c; });
-    strict = large < strict ? large : strict;
-  }
-  kept = strict < kept ? strict : kept;
-  if (set.least > 1.f)
-    kept = one;
-  const uint64_t need = set.below(kept) + 1;
-  const int home = bucket_of(need);
-  const End e = find_end<NT>(false, need - d.before[home], n, d.s, of_bucket(home), held);
-  const End at = find_end<NT>(true, e.ties, n, d.s, [&](int i) { return d.keys[i] == e.key ? ~d.places[i] : 0u; },
-                              [](uint32_t) { return 0ull; });
-  if (b == 0) {
-    g.token[row] = (int32_t)~at.key;
-    if (g.probability)
-      g.probability[row] = (float)((double)held(e.key) / (double)kept);
+  float word = 0.f;
+  uint32_t drawn = 0;
+  for (int q = by_k >= 0 ? 0 : by_p ? 1 : 2;; q = q == 0 && !by_p ? 2 : q + 1) {
+    uint64_t need = drawn;
+    int home = by_k;
+    if (q == 0) {
+      need = (uint64_t)set.k - d.first[bucket_place(home)];
+    } else if (q < 3) {
+      if (q == 2 && by_least && least_from < kBuckets) {
+        uint64_t large = 0;
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+          const int at = buckets.of(d.logits[i]);
+          if (at >= least_from && at <= least_to && set.weight(d.logits[i]) >= bound)
+            large += set.held(d.logits[i]);
+        }
+        if (threadIdx.x == 0)
+          d.bins.sum[0] = 0;
+        __syncthreads();
+        large = of_lane(sum_up_to_lane(large), 63);
+        if (l == 0 && large)
+          atomicAdd((unsigned long long *)&d.bins.sum[0], (unsigned long long)large);
+        __syncthreads();
+        large = start_of(least_from) + d.bins.sum[0];
+        kept = large < kept ? large : kept;
+        __syncthreads();
+      }
+      if (q == 2 && set.least > 1.f)
+        kept = one;
+      need = q == 1 ? set.share(kept) : set.below(kept) + 1;
+      home = locate(need);
+      need -= start_of(home);
+    }
+    const bool by_place = q == 3;
+    const End e = list_end(
+        q == 0 || by_place, need, n, d,
+        [&](int i) {
+          const float x = d.logits[i];
+          return by_place ? (x == word ? ~d.places[i] : 0u) : buckets.of(x) == home ? key_of(x) : 0u;
+        },
+        [&](uint32_t key) { return by_place ? 0ull : set.held(logit_of(key)); });
+    if (q < 2) {
+      kept = start_of(home) + e.sum + e.ties * set.held(logit_of(e.key));
+    } else if (q == 2) {
+      drawn = e.ties;
+      word = logit_of(e.key);
+      if (threadIdx.x == 0 && g.probability)
+        g.probability[row] = (float)((double)set.held(word) / (double)kept);
+    } else {
+      if (threadIdx.x == 0)
+        g.token[row] = (int32_t)~e.key;
+      return;
+    }
+    __syncthreads();
   }
 }
 
@@ -559,36 +797,38 @@ __device__ __forceinline__ bool counts_words(const SampleArgs &g, const Settings
 template <int DT> __global__ __launch_bounds__(kThreads) void sample_whole_kernel(SampleArgs g) {
   __shared__ Draw d;
   __shared__ Sums sums;
+  __shared__ RangeRoom room;
   const int64_t row = blockIdx.x;
-  const Range range = range_of<DT>(g, row, 0, g.words, d.s);
+  const Range range = range_of<DT>(g, row, 0, g.words, room);
   if (settled(g, row, range))
     return;
   const Settings set(g, row, range.largest());
   const Buckets buckets(set, range.least);
   const bool count = counts_words(g, set);
   sums_of<DT>(g, row, 0, g.words, set, buckets, count, sums);
-  draw_row<DT>(g, row, set, buckets, count, sums.sum[threadIdx.x], sums.count[threadIdx.x], d);
+  draw_row<DT>(g, row, set, buckets, count, &sums.sum[(threadIdx.x & 63) * 17], &sums.count[(threadIdx.x & 63) * 17], d);
 }
 
 template <int DT> __global__ __launch_bounds__(kThreads) void sample_most_kernel(SampleArgs g) {
-  __shared__ Shared<kThreads> s;
+  __shared__ RangeRoom room;
   const int part = blockIdx.x;
   const int64_t row = blockIdx.y;
+  if (part == 0)
+    g.sums[row * kBuckets + threadIdx.x] = 0, g.counts[row * kBuckets + threadIdx.x] = 0;
   const int from = part * g.part_words, to = from + g.part_words < g.words ? from + g.part_words : g.words;
-  const Range r = range_of<DT>(g, row, from, to, s);
+  const Range r = range_of<DT>(g, row, from, to, room);
   if (threadIdx.x == 0) {
     g.part_most[row * g.parts + part] = r.most;
     g.part_least[row * g.parts + part] = r.least;
   }
 }
 
+// (a lane a part, at most 32)
 __device__ __forceinline__ Range range_of_parts(const SampleArgs &g, int64_t row) {
-  Range r{0, INFINITY};
-  for (int p = 0; p < g.parts; ++p) {
-    const uint64_t m = g.part_most[row * g.parts + p];
-    r.most = m > r.most ? m : r.most;
-    r.least = fminf(r.least, g.part_least[row * g.parts + p]);
-  }
+  const int p = threadIdx.x & 31, at = p < g.parts ? p : 0;
+  Range r;
+  r.most = largest_of_wave<uint64_t>(g.part_most[row * g.parts + at]);
+  r.least = logit_of(~largest_of_wave<uint32_t>(~key_of(g.part_least[row * g.parts + at])));
   return r;
 }
 
@@ -606,10 +846,11 @@ template <int DT> __global__ __launch_bounds__(kThreads) void sample_sums_kernel
   const bool count = counts_words(g, set);
   const int from = part * g.part_words, to = from + g.part_words < g.words ? from + g.part_words : g.words;
   sums_of<DT>(g, row, from, to, set, buckets, count, sums);
-  const int64_t at = (row * g.parts + part) * kBuckets + threadIdx.x;
-  g.sums[at] = sums.sum[threadIdx.x];
-  if (count)
-    g.counts[at] = sums.count[threadIdx.x];
+  const int at = bucket_place((int)threadIdx.x);
+  if (sums.sum[at])
+    atomicAdd(&g.sums[row * kBuckets + threadIdx.x], sums.sum[at]);
+  if (count && sums.count[at])
+    atomicAdd(&g.counts[row * kBuckets + threadIdx.x], sums.count[at]);
 }
 
 template <int DT> __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs g) {
@@ -620,16 +861,8 @@ template <int DT> __global__ __launch_bounds__(kThreads) void sample_draw_kernel
     return;
   const Settings set(g, row, range.largest());
   const Buckets buckets(set, range.least);
-  const bool count = counts_words(g, set);
-  uint64_t mine = 0;
-  uint32_t here = 0;
-  for (int p = 0; p < g.parts; ++p) {
-    const int64_t at = (row * g.parts + p) * kBuckets + threadIdx.x;
-    mine += g.sums[at];
-    if (count)
-      here += g.counts[at];
-  }
-  draw_row<DT>(g, row, set, buckets, count, mine, here, d);
+  const int64_t at = row * kBuckets + (threadIdx.x & 63) * 16;
+  draw_row<DT>(g, row, set, buckets, counts_words(g, set), g.sums + at, g.counts + at, d);
 }
 
 // How rows are cut: parts that fill the chip, of 4096 words at least (one part: a workgroup a row).
@@ -675,8 +908,8 @@ static Places places_of(const fhip_sample_desc &d) {
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   p.least = up(n * 8);
   p.sums = p.least + up(n * 4);
-  p.counts = p.sums + n * kBuckets * 8;
-  p.bytes = p.counts + n * kBuckets * 4;
+  p.counts = p.sums + (size_t)d.logits.dim[0] * kBuckets * 8;
+  p.bytes = p.counts + (size_t)d.logits.dim[0] * kBuckets * 4;
   return p;
 }
 
@@ -740,7 +973,7 @@ int fhip_sample(fhip_ctx *ctx, const fhip_sample_desc *d, const void *logits, co
     g.parts = c.parts, g.part_words = c.words;
     char *w = (char *)workspace;
     g.part_most = (uint64_t *)w, g.part_least = (float *)(w + at.least);
-    g.sums = (uint64_t *)(w + at.sums), g.counts = (uint32_t *)(w + at.counts);
+    g.sums = (unsigned long long *)(w + at.sums), g.counts = (uint32_t *)(w + at.counts);
     fhip_note_kernel(ctx, "sample parts=%d", c.parts);
     switch (g.dtype) {
     case FHIP_FLOAT: return launch<FHIP_FLOAT>(ctx, g);
