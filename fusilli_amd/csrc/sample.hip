@@ -46,53 +46,68 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// A row's settings.
-struct Settings {
+// A row's settings as they are given.  All loads at once, those of absent vectors from the uniform
+// numbers: behind a branch each would wait for memory by itself, a microsecond every time.
+struct Asked {
+  float t, p, least, u;
+  int k;
+  __device__ __forceinline__ Asked(const SampleArgs &g, int64_t row) {
+    const float *const vt = g.temperature ? g.temperature : g.uniform, *const vp = g.top_p ? g.top_p : g.uniform;
+    const float *const vl = g.min_p ? g.min_p : g.uniform;
+    const int32_t *const vk = g.top_k ? g.top_k : (const int32_t *)g.uniform;
+    t = vt[row], p = vp[row], least = vl[row], k = vk[row], u = g.uniform[row];
+    t = g.temperature ? t : g.one_temperature;
+    k = g.top_k ? k : g.one_top_k;
+    p = g.top_p ? p : g.one_top_p;
+    least = g.min_p ? least : g.one_min_p;
+  }
+};
+
+struct Settings : Asked {
   double most, by;  // the largest logit, 1 / T
-  double cut, by2;  // (logits this far below weigh nothing), log2(e) / T
+  double by2;       // log2(e) / T
   float top;        // the largest logit
   int bits;
-  float p, least, u;
-  int k;
   bool greedy;
-  __device__ __forceinline__ Settings(const SampleArgs &g, int64_t row, float largest) {
-    const float t = g.temperature ? g.temperature[row] : g.one_temperature;
-    k = g.top_k ? g.top_k[row] : g.one_top_k;
-    p = g.top_p ? g.top_p[row] : g.one_top_p;
-    least = g.min_p ? g.min_p[row] : g.one_min_p;
-    u = g.uniform[row];
+  __device__ __forceinline__ Settings(const SampleArgs &g, const Asked &asked, float largest) : Asked(asked) {
     most = (double)largest;
     greedy = !(t > 0.f);
     by = greedy ? 1.0 : fmax(1.0 / (double)t, 1e-300); // (T infinite: -inf times it is -inf)
-    cut = -32.0 / by;
     by2 = by * 1.44269504088896340736;
     top = largest;
     bits = g.bits;
   }
   __device__ __forceinline__ double weight(float l) const { return l == top ? 1.0 : exp(((double)l - most) * by); }
-  // The weight in units of 2^-bits, rounded; 0 from exp(-32) = 2^-46.2 on.  2^x with x = n + f, |f| at
-  // most 1/2: a polynomial of degree 10 through 1 at 0 that meets 2^f at the zeros of a Chebyshev
-  // polynomial (6e-16 of it off at most); the unit's power goes into n, and 2^52 on top leaves the
-  // rounded value in the low bits.  16 instructions; the library's exp and the conversion to 64 bits
-  // take more than twice as many.
-  __device__ __forceinline__ uint64_t held(float l) const {
-    const double d = l == top ? 0.0 : (double)l - most;
-    const double x = (d > cut ? d : 0.0) * by2;
+  // The weight in units of 2^-bits, rounded, of a logit that is finite like the largest and less than
+  // 40 T below it.  2^x with x = n + f, |f| at most 1/2: a polynomial of degree 10 through 1 at 0 that
+  // meets 2^f at the zeros of a Chebyshev polynomial (6e-16 of it off at most); the unit's power goes
+  // into n, and 2^52 on top leaves the rounded value in the low bits.  20 instructions; the library's
+  // exp and the conversion to 64 bits take more than twice as many.
+  __device__ __forceinline__ uint64_t held_near(float l) const {
+    const double x = ((double)l - most) * by2;
     const double n = rint(x), f = x - n;
-    double y = 7.0709662925771758e-09;
-    y = __builtin_fma(y, f, 1.0205905366447884e-07);
-    y = __builtin_fma(y, f, 1.3215451705400571e-06);
-    y = __builtin_fma(y, f, 1.5252672925113478e-05);
-    y = __builtin_fma(y, f, 1.5403530424618647e-04);
-    y = __builtin_fma(y, f, 1.3333558200794100e-03);
-    y = __builtin_fma(y, f, 9.6181291076188023e-03);
-    y = __builtin_fma(y, f, 5.5504108664651677e-02);
-    y = __builtin_fma(y, f, 2.4022650695910075e-01);
-    y = __builtin_fma(y, f, 6.9314718055994617e-01);
+    // (the constants keep their registers: in C++ each becomes a copy and an instruction that overwrites it)
+    auto step = [&](double y, double c) {
+      double r;
+      asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(y), "v"(f), "s"(c));
+      return r;
+    };
+    double y = step(7.0709662925771758e-09, 1.0205905366447884e-07);
+    y = step(y, 1.3215451705400571e-06);
+    y = step(y, 1.5252672925113478e-05);
+    y = step(y, 1.5403530424618647e-04);
+    y = step(y, 1.3333558200794100e-03);
+    y = step(y, 9.6181291076188023e-03);
+    y = step(y, 5.5504108664651677e-02);
+    y = step(y, 2.4022650695910075e-01);
+    y = step(y, 6.9314718055994617e-01);
     y = __builtin_fma(y, f, 1.0);
     y = __builtin_amdgcn_ldexp(y, (int)n + bits) + 0x1p52;
-    const uint64_t v = __builtin_bit_cast(uint64_t, y) & ((1ull << 52) - 1);
-    return d > cut ? v : 0;
+    return __builtin_bit_cast(uint64_t, y) & ((1ull << 52) - 1);
+  }
+  // The same of any; 0 from exp(-32) = 2^-46.2 on.
+  __device__ __forceinline__ uint64_t held(float l) const {
+    return l == top ? 1ull << bits : ((double)l - most) * by > -32.0 ? held_near(l) : 0;
   }
   // the weights' sum that top_p asks for of `all`; the sum that the token's exceeds of `kept`
   __device__ __forceinline__ uint64_t share(uint64_t all) const {
@@ -112,7 +127,7 @@ struct End {
   uint32_t key;
   uint32_t count;
   uint64_t sum;
-  uint32_t ties;
+  uint32_t ties, same; // (all words of that value: those of the items that were asked for)
 };
 
 template <int NT> struct Shared {
@@ -217,6 +232,7 @@ __device__ __forceinline__ End find_end(bool by_count, uint64_t need, int n, Sha
   } while (left > 0);
   End e;
   e.key = prefix, e.count = count, e.sum = sum;
+  e.same = same;
   const uint64_t each = held(prefix);
   const uint64_t ties = by_count ? need - count : need <= sum || each == 0 ? 1 : (need - sum + each - 1) / each;
   e.ties = (uint32_t)(ties < 1 ? 1 : ties > same ? same : ties);
@@ -244,7 +260,7 @@ template <int NT> __device__ __noinline__ void sample_row(const SampleArgs &g, i
     }
     return;
   }
-  const Settings set(g, row, logit_of((uint32_t)most));
+  const Settings set(g, Asked(g, row), logit_of((uint32_t)most));
   auto held = [&](uint32_t key) { return set.held(logit_of(key)); };
   uint64_t kept = (uint64_t)1 << g.bits; // (greedy: the first word's weight)
   if (!set.greedy) {
@@ -438,29 +454,29 @@ __device__ __forceinline__ Range range_of(const SampleArgs &g, int64_t row, int 
 }
 
 // A row's buckets: the first holds the largest logits.  In f32, whose differences and products keep the
-// order; halves, as a difference may be twice the largest number.
+// order; halves, as a difference may be twice the largest number.  (Of rows whose largest logit is finite.)
 struct Buckets {
-  float half, top, by;
+  float half, by;
   double wide; // of (m - l) / T, all of them
-  __device__ __forceinline__ Buckets(const Settings &set, float least) : half(0.5f * set.top), top(set.top) {
-    const double range = least == top ? 0.0 : (set.most - (double)least) * set.by;
+  __device__ __forceinline__ Buckets(const Settings &set, float least) : half(0.5f * set.top) {
+    const double range = (set.most - (double)least) * set.by;
     wide = range < 32.0 ? range : 32.0;
     // (a little less than the range takes, so that the last word is inside for all roundings)
     const double x = range > 0.0 ? 2.0 * set.by * (kBuckets * (1.0 - 0x1p-20)) / wide : 0.0;
     by = x < 3.0e38 ? (float)x : 3.0e38f;
   }
   __device__ __forceinline__ int of(float l) const { // kBuckets: none
-    const float b = l == top ? 0.f : (half - 0.5f * l) * by; // (NaN, -inf: none)
-    return b < (float)kBuckets ? (int)b : kBuckets;
+    return (int)fminf((half - 0.5f * l) * by, (float)kBuckets); // (NaN, -inf: none)
   }
 };
 // Where a bucket lies in LDS: a lane's sixteen in a row, lanes on banks of their own.
 __device__ __forceinline__ int bucket_place(int b) { return b + (b >> 4); }
 constexpr int kPlaces = kBuckets + kBuckets / 16 + 1;
+constexpr int kNowhere = kPlaces, kAllPlaces = kPlaces + 64; // what is in none, by lane
 
 struct Sums {
-  unsigned long long sum[kPlaces];
-  uint32_t count[kPlaces];
+  unsigned long long sum[kAllPlaces];
+  uint32_t count[kAllPlaces];
 };
 template <int DT>
 __device__ __forceinline__ void sums_of(const SampleArgs &g, int64_t row, int from, int to, const Settings &set,
@@ -473,11 +489,10 @@ __device__ __forceinline__ void sums_of(const SampleArgs &g, int64_t row, int fr
 #pragma unroll
     for (int e = 0; e < W::N; ++e) {
       const int b = buckets.of(v[e]);
-      if (b < kBuckets) {
-        atomicAdd(&s.sum[bucket_place(b)], (unsigned long long)set.held(v[e]));
-        if (count)
-          atomicAdd(&s.count[bucket_place(b)], 1u);
-      }
+      const int at = b < kBuckets ? bucket_place(b) : kNowhere + (int)(threadIdx.x & 63);
+      atomicAdd(&s.sum[at], (unsigned long long)set.held_near(v[e]));
+      if (count)
+        atomicAdd(&s.count[at], 1u);
     }
   });
   __syncthreads();
@@ -487,25 +502,32 @@ struct Bins {
   uint64_t sum[256];
   uint32_t count[256];
 };
+// What is known of a row when its buckets' sums are.
+struct Front {
+  uint64_t before[kPlaces]; // weights in front of a bucket
+  uint32_t first[kPlaces];  // words in front of it
+  uint64_t all;
+  float floor; // no word in question is smaller
+  int by_k, least_from, least_to;
+};
 struct Draw {
   union {
     Bins bins;
     Shared<kThreads> whole; // of a row that does not fit the list
   };
-  uint64_t before[kPlaces];        // weights in front of a bucket
-  uint32_t first[kPlaces];         // words in front of it
+  Front f;
   uint32_t asked[kBuckets / 32 + 1]; // a bit a bucket (the last: none)
-  uint64_t all;
-  float floor; // no word in question is smaller
-  int by_k, least_from, least_to;
+  uint64_t swap[2][kThreads];
+  uint64_t kept;
+  uint64_t least_front; // weights in front of the first bucket that min_p's end may lie in
   int filled;
-  uint32_t high, low; // largest key, complement of the smallest
+  uint32_t high, low, items; // largest key, complement of the smallest; how many
   End end;
   float logits[kList];
   uint32_t places[kList];
 };
 
-// find_end above over the list.  (d.high and d.low are 0 before and after.)
+// find_end above over the list.  (d.high, d.low and d.items are 0 before and after.)
 template <typename Key, typename Held>
 __device__ __forceinline__ End list_end(bool by_count, uint64_t need, int n, Draw &d, Key key_at, Held held) {
   const int t = threadIdx.x, l = t & 63;
@@ -513,24 +535,30 @@ __device__ __forceinline__ End list_end(bool by_count, uint64_t need, int n, Dra
     if (t < 256)
       d.bins.sum[t] = 0, d.bins.count[t] = 0;
   };
-  uint32_t high = 0, low = 0;
-  for (int i = t; i < n; i += kThreads) {
-    const uint32_t key = key_at(i);
+  uint32_t high = 0, low = 0, items = 0;
+  for (int i = t; i - l < n; i += kThreads) {
+    const uint32_t key = i < n ? key_at(i) : 0;
     high = key > high ? key : high;
     low = key && ~key > low ? ~key : low;
+    items += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key != 0));
   }
-  if (t / 64 * 64 < n) {
+  if (items) {
     high = largest_of_wave<uint32_t>(high), low = largest_of_wave<uint32_t>(low);
-    if (l == 0 && high)
-      atomicMax(&d.high, high), atomicMax(&d.low, low);
+    if (l == 0)
+      atomicMax(&d.high, high), atomicMax(&d.low, low), atomicAdd(&d.items, items);
   }
   clear();
   __syncthreads();
-  high = d.high, low = ~d.low;
+  high = d.high, low = ~d.low, items = d.items;
   int left = high == low ? 0 : 32 - __builtin_clz(high ^ low); // bits in which keys differ
   uint32_t prefix = left == 32 ? 0 : high >> left << left;
-  End e{prefix, 0, 0, 0};
-  for (;;) {
+  End e{prefix, 0, 0, items, 0};
+  if (left == 0) { // (equal ones: nothing to search)
+    __syncthreads();
+    if (t == 0)
+      d.high = d.low = d.items = 0;
+  }
+  while (left > 0) {
     const int shift = left > 8 ? left - 8 : 0;
     const uint32_t above = left == 32 ? 0 : ~0u << left; // bits that the prefix has
     for (int i = t; i < n; i += kThreads) {
@@ -565,30 +593,37 @@ __device__ __forceinline__ End list_end(bool by_count, uint64_t need, int n, Dra
       }
       const uint64_t hit = __builtin_amdgcn_ballot_w64(found >= 0);
       if (l == (hit ? __builtin_ctzll(hit) : 0))
-        d.end = End{e.key | (uint32_t)(255 - 4 * l - (found < 0 ? 0 : found)) << shift, c0, w0, own};
+        d.end = End{e.key | (uint32_t)(255 - 4 * l - (found < 0 ? 0 : found)) << shift, c0, w0, own, 0};
       if (l == 0)
-        d.high = d.low = 0;
+        d.high = d.low = d.items = 0;
     }
     __syncthreads();
     e = d.end;
     left = shift;
-    if (left == 0)
-      break;
-    clear();
-    __syncthreads();
+    if (left > 0) {
+      clear();
+      __syncthreads();
+    }
   }
-  const uint32_t same = e.ties;
+  const uint32_t same = e.same = e.ties;
   const uint64_t each = held(e.key);
   const uint64_t ties = by_count ? need - e.count : need <= e.sum || each == 0 ? 1 : (need - e.sum + each - 1) / each;
   e.ties = (uint32_t)(ties < 1 ? 1 : ties > same ? same : ties);
   return e;
 }
 
-// A row without a question; false: there are some.
-__device__ __forceinline__ bool settled(const SampleArgs &g, int64_t row, const Range &range) {
-  const float t = g.temperature ? g.temperature[row] : g.one_temperature;
-  if (range.most != 0 && t > 0.f)
+// Rows of no word and greedy ones have none, and those whose largest logit is infinite go to sample_row.
+__device__ __forceinline__ bool has_questions(const Range &range, float t) {
+  return range.most != 0 && t > 0.f && range.largest() < INFINITY;
+}
+// Does a row without questions; false: it has some.
+__device__ __forceinline__ bool settled(const SampleArgs &g, int64_t row, const Range &range, float t, Shared<kThreads> &s) {
+  if (has_questions(range, t))
     return false;
+  if (range.most != 0 && t > 0.f) {
+    sample_row<kThreads>(g, row, s);
+    return true;
+  }
   if (threadIdx.x == 0) {
     g.token[row] = range.most == 0 ? -1 : (int32_t)~(uint32_t)range.most;
     if (g.probability)
@@ -597,110 +632,119 @@ __device__ __forceinline__ bool settled(const SampleArgs &g, int64_t row, const 
   return true;
 }
 
-// The token of a row; `sums` and `counts`: where lane l of the first wavefront finds its sixteen buckets.
-template <int DT, typename Sum, typename Count>
-__device__ __forceinline__ void draw_row(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets,
-                                         bool count, const Sum *sums, const Count *counts, Draw &d) {
-  const int l = threadIdx.x & 63;
-  const bool leads = threadIdx.x < 64;
-  const bool by_p = set.p < 1.f, by_least = set.least > 0.f;
-  const double bound = set.least < 1.f ? (double)set.least : 1.0;
-  const uint64_t one = (uint64_t)1 << g.bits; // (the largest is always kept)
-  uint64_t all = 0, lane_start = 0, lane_end = 0; // of a lane's buckets
-  int by_k = -1, least_from = kBuckets, least_to = kBuckets;
+// Where a sum ends, by a wavefront: of a lane's sixteen buckets and of all.
+struct Locator {
+  const Front &f;
+  uint64_t start, end;
   // which bucket holds the `need`-th unit of weight (1 .. all)
-  auto locate = [&](uint64_t need) {
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane_start < need && need <= lane_end);
+  __device__ __forceinline__ int operator()(uint64_t need) const {
+    const int l = threadIdx.x & 63;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(start < need && need <= end);
     const int lane = hit ? __builtin_ctzll(hit) : 0;
-    const uint64_t front = __builtin_amdgcn_ballot_w64(l < 16 && d.before[lane * 17 + (l & 15)] < need);
+    const uint64_t front = __builtin_amdgcn_ballot_w64(l < 16 && f.before[lane * 17 + (l & 15)] < need);
     return lane * 16 + (front ? __builtin_popcountll(front) - 1 : 0);
+  }
+  __device__ __forceinline__ uint64_t start_of(int b) const { return f.before[bucket_place(b)]; }
+  __device__ __forceinline__ uint64_t end_of(int b, uint64_t all) const {
+    return b + 1 < kBuckets ? f.before[bucket_place(b + 1)] : all;
+  }
+};
+
+__device__ __forceinline__ double least_bound(const Settings &set) { return set.least < 1.f ? (double)set.least : 1.0; }
+
+// A lane's sixteen buckets.
+struct Sixteen {
+  uint64_t w[16];
+  uint32_t c[16];
+  template <typename Sum, typename Count> __device__ __forceinline__ void load(const Sum *sums, const Count *counts) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      w[i] = sums[i], c[i] = counts[i]; // (0 where they are not asked for)
+  }
+};
+
+// The buckets in question, by the first wavefront.
+__device__ __forceinline__ void ask_buckets(const Settings &set, const Buckets &buckets, bool count, const Sixteen &own,
+                                            Draw &d) {
+  const int l = threadIdx.x;
+  const uint64_t one = (uint64_t)1 << set.bits; // (the largest is always kept)
+  const uint64_t(&w)[16] = own.w;
+  const uint32_t(&c)[16] = own.c;
+  uint64_t ws = 0;
+  uint32_t cs = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    ws += w[i], cs += c[i];
+  Locator locate{d.f, 0, sum_up_to_lane(ws)};
+  locate.start = locate.end - ws;
+  const uint64_t all = of_lane(locate.end, 63);
+  const uint32_t words_end = sum_up_to_lane(cs);
+  uint64_t at = locate.start;
+  uint32_t words = words_end - cs;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    d.f.before[l * 17 + i] = at, d.f.first[l * 17 + i] = words;
+    at += w[i], words += c[i];
+  }
+  if (l <= kBuckets / 32)
+    d.asked[l] = 0;
+  if (l == 0)
+    d.filled = 0, d.high = 0, d.low = 0, d.items = 0;
+  wave_fence();
+  int lowest = 0; // bucket in question
+  auto ask = [&](int from, int to) { // (few, or one range of many)
+    lowest = to > lowest ? to : lowest;
+    for (int i = from + l; i <= to; i += 64)
+      atomicOr(&d.asked[i >> 5], 1u << (i & 31));
   };
-  auto start_of = [&](int b) { return d.before[bucket_place(b)]; };
-  auto end_of = [&](int b) { return b + 1 < kBuckets ? d.before[bucket_place(b + 1)] : all; };
-  if (leads) {
-    uint64_t w[16];
-    uint32_t c[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      w[i] = sums[i], c[i] = 0;
-    if (count) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        c[i] = counts[i];
-    }
-    uint64_t ws = 0;
-    uint32_t cs = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      ws += w[i], cs += c[i];
-    lane_end = sum_up_to_lane(ws), lane_start = lane_end - ws;
-    all = of_lane(lane_end, 63);
-    const uint32_t words_end = sum_up_to_lane(cs);
-    uint64_t at = lane_start;
-    uint32_t words = words_end - cs;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      d.before[l * 17 + i] = at, d.first[l * 17 + i] = words;
-      at += w[i], words += c[i];
-    }
-    if (l <= kBuckets / 32)
-      d.asked[l] = 0;
-    if (l == 0)
-      d.filled = 0, d.high = 0, d.low = 0;
-    wave_fence();
-    // What is kept weighs between `low` and `high`, until the words are known in which a prefix ends.
-    uint64_t low = all, high = all;
-    const uint32_t k = (uint32_t)set.k;
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(count && words_end - cs < k && k <= words_end);
-    if (hit) { // (otherwise fewer words than k weigh anything)
-      const int lane = __builtin_ctzll(hit);
-      const uint64_t front = __builtin_amdgcn_ballot_w64(l < 16 && d.first[lane * 17 + (l & 15)] < k);
-      by_k = lane * 16 + __builtin_popcountll(front) - 1;
-      low = start_of(by_k), high = end_of(by_k);
-    }
-    int lowest = 0; // bucket in question
-    auto ask = [&](int from, int to) { // (few, or one range of many)
-      lowest = to > lowest ? to : lowest;
-      for (int i = from + l; i <= to; i += 64)
-        atomicOr(&d.asked[i >> 5], 1u << (i & 31));
-    };
-    if (by_k >= 0)
-      ask(by_k, by_k);
-    low = low < 1 ? 1 : low;
-    if (by_p) {
-      const int a = locate(set.share(low)), z = locate(set.share(high));
-      ask(a, z);
-      low = start_of(a), high = end_of(z);
-    }
-    if (by_least) {
-      // (buckets are of f32, three roundings: less than a thousandth of one)
-      const double at = -log(bound) / buckets.wide * kBuckets * (1.0 - 0x1p-20);
-      const double a = at - 1e-3, z = at + 1e-3;
-      least_from = !(a > 0.0) ? 0 : a < (double)kBuckets ? (int)a : kBuckets; // (one bucket for all: 0)
-      least_to = !(z > 0.0) ? 0 : z < (double)kBuckets ? (int)z : kBuckets - 1;
-      if (least_from < kBuckets) {
-        ask(least_from, least_to);
-        const uint64_t a_sum = start_of(least_from), z_sum = end_of(least_to);
-        low = a_sum < low ? a_sum : low;
-        high = z_sum < high ? z_sum : high;
-      }
-    }
-    low = low < one ? one : low;
-    high = high < low ? low : high;
-    if (set.least > 1.f)
-      low = high = one;
-    ask(locate(set.below(low) + 1), locate(set.below(high) + 1));
-    if (l == 0) {
-      d.all = all, d.by_k = by_k, d.least_from = least_from, d.least_to = least_to;
-      // (below the last bucket's end, for all roundings)
-      const double end = set.most - (lowest + 2) * 2.0 / (double)buckets.by;
-      d.floor = buckets.by > 0.f && set.top < INFINITY ? (float)(end - 1e-6 * (fabs(end) + fabs(set.most))) : -INFINITY;
+  // What is kept weighs between `low` and `high`, until the words are known in which a prefix ends.
+  uint64_t low = all, high = all;
+  int by_k = -1, least_from = kBuckets, least_to = kBuckets;
+  const uint32_t k = (uint32_t)set.k;
+  const uint64_t hit = __builtin_amdgcn_ballot_w64(count && words_end - cs < k && k <= words_end);
+  if (hit) { // (otherwise fewer words than k weigh anything)
+    const int lane = __builtin_ctzll(hit);
+    const uint64_t front = __builtin_amdgcn_ballot_w64(l < 16 && d.f.first[lane * 17 + (l & 15)] < k);
+    by_k = lane * 16 + __builtin_popcountll(front) - 1;
+    low = locate.start_of(by_k), high = locate.end_of(by_k, all);
+    ask(by_k, by_k);
+  }
+  low = low < 1 ? 1 : low;
+  if (set.p < 1.f) {
+    const int a = locate(set.share(low)), z = locate(set.share(high));
+    ask(a, z);
+    low = locate.start_of(a), high = locate.end_of(z, all);
+  }
+  if (set.least > 0.f) {
+    // (buckets are of f32, three roundings: less than a thousandth of one)
+    const double edge = -log(least_bound(set)) / buckets.wide * kBuckets * (1.0 - 0x1p-20);
+    const double a = edge - 1e-3, z = edge + 1e-3;
+    least_from = !(a > 0.0) ? 0 : a < (double)kBuckets ? (int)a : kBuckets; // (one bucket for all: 0)
+    least_to = !(z > 0.0) ? 0 : z < (double)kBuckets ? (int)z : kBuckets - 1;
+    if (least_from < kBuckets) {
+      ask(least_from, least_to);
+      const uint64_t a_sum = locate.start_of(least_from), z_sum = locate.end_of(least_to, all);
+      low = a_sum < low ? a_sum : low;
+      high = z_sum < high ? z_sum : high;
     }
   }
-  __syncthreads();
-  const float floor = d.floor;
-  // the words of those buckets
+  low = low < one ? one : low;
+  high = high < low ? low : high;
+  if (set.least > 1.f)
+    low = high = one;
+  ask(locate(set.below(low) + 1), locate(set.below(high) + 1));
+  if (l == 0) {
+    d.f.all = all, d.f.by_k = by_k, d.f.least_from = least_from, d.f.least_to = least_to;
+    // (below the last bucket's end, for all roundings)
+    const double end = set.most - (lowest + 2) * 2.0 / (double)buckets.by;
+    d.f.floor = buckets.by > 0.f ? (float)(end - 1e-6 * (fabs(end) + fabs(set.most))) : -INFINITY;
+  }
+}
+
+// The words of those buckets, to the list.
+template <int DT> __device__ __forceinline__ void gather(const SampleArgs &g, int64_t row, const Buckets &buckets, Draw &d) {
   using W = Words<DT>;
+  const float floor = d.f.floor;
   for_words<DT, 4>(g, row, 0, g.words, [&](const float(&v)[W::N], int i) {
     uint32_t hits = 0;
     float top = v[0];
@@ -718,20 +762,122 @@ __device__ __forceinline__ void draw_row(const SampleArgs &g, int64_t row, const
 #pragma unroll
       for (int e = 0; e < W::N; ++e)
         if (hits >> e & 1) {
-          const int to = atomicAdd(&d.filled, 1);
-          if (to < kList)
-            d.logits[to] = v[e], d.places[to] = (uint32_t)(i + e);
+          const int at = atomicAdd(&d.filled, 1);
+          if (at < kList)
+            d.logits[at] = v[e], d.places[at] = (uint32_t)(i + e);
         }
     }
   });
   __syncthreads();
-  const int n = d.filled;
+}
+
+// The token of a row, from at most a word a thread: in order, with their sums next to them, they answer
+// every question by a comparison.  (A search for each of them in the list takes three times as long.)
+__device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets,
+                                              int n, Draw &d) {
+  const int t = threadIdx.x, l = t & 63;
+  uint64_t v = t < n ? (uint64_t)key_of(d.logits[t]) << 32 | ~d.places[t] : 0;
+  // exchanges at distances below 64 inside a wavefront, the others through LDS (two places in turn: one
+  // barrier each); wavefronts without a word keep the barriers only
+  int turn = 0;
+  for (int size = 2; size < 2 * n; size *= 2)
+    for (int far = size / 2; far > 0; far /= 2) {
+      uint64_t w;
+      if (far >= 64) {
+        d.swap[turn][t] = v;
+        __syncthreads();
+        w = d.swap[turn][t ^ far];
+        turn ^= 1;
+      } else {
+        if (t - l >= n && size <= 64)
+          continue;
+        w = (uint64_t)__shfl_xor((unsigned long long)v, far);
+      }
+      const bool larger = ((t & far) == 0) == ((t & size) == 0);
+      v = (w > v) == larger ? w : v;
+    }
+  const float x = logit_of((uint32_t)(v >> 32));
+  const bool mine = v != 0;
+  const uint64_t weight = mine ? set.held(x) : 0;
+  const int home = mine ? buckets.of(x) : kBuckets;
+  // sums up to each word of the list, then of the row: a bucket's begin at its first word
+  uint64_t sum = sum_up_to_lane(weight);
+  if (l == 63)
+    d.bins.sum[t >> 6] = sum;
+  d.swap[turn][t] = (uint64_t)home;
+  __syncthreads();
+  for (int w = 0; w < t >> 6; ++w)
+    sum += d.bins.sum[w];
+  if (mine && (t == 0 || (int)d.swap[turn][t - 1] != home)) {
+    d.f.before[bucket_place(home)] -= sum - weight; // (unsigned: wraps and wraps back)
+    d.f.first[bucket_place(home)] -= (uint32_t)t;
+  }
+  __syncthreads();
+  const int least_from = d.f.least_from, least_to = d.f.least_to;
+  const uint64_t one = (uint64_t)1 << set.bits;
+  const uint64_t up_to = mine ? d.f.before[bucket_place(home)] + sum : 0;
+  const uint32_t rank = mine ? d.f.first[bucket_place(home)] + (uint32_t)t : 0;
+  // whoever ends a prefix says so
+  auto told = [&](bool says, uint64_t otherwise) {
+    if (t == 0)
+      d.kept = otherwise;
+    __syncthreads();
+    if (says)
+      d.kept = up_to;
+    __syncthreads();
+    const uint64_t kept = d.kept;
+    __syncthreads();
+    return kept;
+  };
+  uint64_t kept = d.f.all;
+  if (d.f.by_k >= 0)
+    kept = told(mine && rank + 1 == (uint32_t)set.k, kept);
+  if (set.p < 1.f) {
+    const uint64_t need = set.share(kept);
+    kept = told(mine && up_to - weight < need && need <= up_to, kept);
+  }
+  if (set.least > 0.f && least_from < kBuckets) {
+    const bool large = mine && home >= least_from && home <= least_to && set.weight(x) >= least_bound(set);
+    // (the largest sum among them, or what lies in front of their buckets)
+    const uint64_t most = largest_of_wave<uint64_t>(large ? up_to : 0);
+    if (t == 0)
+      d.kept = d.least_front;
+    __syncthreads();
+    if (l == 0 && most)
+      atomicMax((unsigned long long *)&d.kept, (unsigned long long)most);
+    __syncthreads();
+    kept = d.kept < kept ? d.kept : kept;
+    __syncthreads();
+  }
+  if (set.least > 1.f)
+    kept = one;
+  const uint64_t need = set.below(kept) + 1;
+  if (mine && up_to - weight < need && need <= up_to) {
+    g.token[row] = (int32_t)~(uint32_t)v;
+    if (g.probability)
+      g.probability[row] = (float)((double)weight / (double)kept);
+  }
+}
+
+// The token of a row, from the n words of the list.
+__device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets, int n,
+                                       Draw &d) {
+  const int l = threadIdx.x & 63;
   if (n > kList) { // (many equal logits)
     sample_row<kThreads>(g, row, d.whole);
     return;
   }
-  all = d.all, by_k = d.by_k, least_from = d.least_from, least_to = d.least_to;
-  lane_start = d.before[l * 17], lane_end = l < 63 ? d.before[l * 17 + 17] : all;
+  if (n <= kThreads) {
+    if (threadIdx.x == 0)
+      d.least_front = d.f.least_from < kBuckets ? d.f.before[bucket_place(d.f.least_from)] : 0;
+    answer_sorted(g, row, set, buckets, n, d);
+    return;
+  }
+  const uint64_t one = (uint64_t)1 << set.bits;
+  const uint64_t all = d.f.all;
+  const Locator locate{d.f, d.f.before[l * 17], l < 63 ? d.f.before[l * 17 + 17] : all};
+  const int by_k = d.f.by_k, least_from = d.f.least_from, least_to = d.f.least_to;
+  const bool by_p = set.p < 1.f;
   // The questions in turn: what the first k weigh, how far top_p reaches, which word is drawn, and its
   // index among those that are equal.  (One loop, so that the search is in the code once.)
   uint64_t kept = all;
@@ -741,9 +887,10 @@ __device__ __forceinline__ void draw_row(const SampleArgs &g, int64_t row, const
     uint64_t need = drawn;
     int home = by_k;
     if (q == 0) {
-      need = (uint64_t)set.k - d.first[bucket_place(home)];
+      need = (uint64_t)set.k - d.f.first[bucket_place(home)];
     } else if (q < 3) {
-      if (q == 2 && by_least && least_from < kBuckets) {
+      if (q == 2 && set.least > 0.f && least_from < kBuckets) {
+        const double bound = least_bound(set);
         uint64_t large = 0;
         for (int i = threadIdx.x; i < n; i += kThreads) {
           const int at = buckets.of(d.logits[i]);
@@ -757,7 +904,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs &g, int64_t row, const
         if (l == 0 && large)
           atomicAdd((unsigned long long *)&d.bins.sum[0], (unsigned long long)large);
         __syncthreads();
-        large = start_of(least_from) + d.bins.sum[0];
+        large = locate.start_of(least_from) + d.bins.sum[0];
         kept = large < kept ? large : kept;
         __syncthreads();
       }
@@ -765,7 +912,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs &g, int64_t row, const
         kept = one;
       need = q == 1 ? set.share(kept) : set.below(kept) + 1;
       home = locate(need);
-      need -= start_of(home);
+      need -= locate.start_of(home);
     }
     const bool by_place = q == 3;
     const End e = list_end(
@@ -776,12 +923,18 @@ __device__ __forceinline__ void draw_row(const SampleArgs &g, int64_t row, const
         },
         [&](uint32_t key) { return by_place ? 0ull : set.held(logit_of(key)); });
     if (q < 2) {
-      kept = start_of(home) + e.sum + e.ties * set.held(logit_of(e.key));
+      kept = locate.start_of(home) + e.sum + e.ties * set.held(logit_of(e.key));
     } else if (q == 2) {
       drawn = e.ties;
       word = logit_of(e.key);
       if (threadIdx.x == 0 && g.probability)
         g.probability[row] = (float)((double)set.held(word) / (double)kept);
+      if (e.same == 1) { // (its only place)
+        for (int i = threadIdx.x; i < n; i += kThreads)
+          if (d.logits[i] == word)
+            g.token[row] = (int32_t)d.places[i];
+        return;
+      }
     } else {
       if (threadIdx.x == 0)
         g.token[row] = (int32_t)~e.key;
@@ -791,7 +944,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs &g, int64_t row, const
   }
 }
 
-__device__ __forceinline__ bool counts_words(const SampleArgs &g, const Settings &set) { return set.k > 0 && set.k < g.words; }
+__device__ __forceinline__ bool counts_words(const SampleArgs &g, int k) { return k > 0 && k < g.words; }
 
 // A workgroup a row.
 template <int DT> __global__ __launch_bounds__(kThreads) void sample_whole_kernel(SampleArgs g) {
@@ -799,14 +952,22 @@ template <int DT> __global__ __launch_bounds__(kThreads) void sample_whole_kerne
   __shared__ Sums sums;
   __shared__ RangeRoom room;
   const int64_t row = blockIdx.x;
+  const Asked asked(g, row);
   const Range range = range_of<DT>(g, row, 0, g.words, room);
-  if (settled(g, row, range))
+  if (settled(g, row, range, asked.t, d.whole))
     return;
-  const Settings set(g, row, range.largest());
+  const Settings set(g, asked, range.largest());
   const Buckets buckets(set, range.least);
-  const bool count = counts_words(g, set);
+  const bool count = counts_words(g, set.k);
   sums_of<DT>(g, row, 0, g.words, set, buckets, count, sums);
-  draw_row<DT>(g, row, set, buckets, count, &sums.sum[(threadIdx.x & 63) * 17], &sums.count[(threadIdx.x & 63) * 17], d);
+  if (threadIdx.x < 64) {
+    Sixteen own;
+    own.load(&sums.sum[threadIdx.x * 17], &sums.count[threadIdx.x * 17]);
+    ask_buckets(set, buckets, count, own, d);
+  }
+  __syncthreads();
+  gather<DT>(g, row, buckets, d);
+  answer(g, row, set, buckets, d.filled, d);
 }
 
 template <int DT> __global__ __launch_bounds__(kThreads) void sample_most_kernel(SampleArgs g) {
@@ -836,14 +997,13 @@ template <int DT> __global__ __launch_bounds__(kThreads) void sample_sums_kernel
   __shared__ Sums sums;
   const int part = blockIdx.x;
   const int64_t row = blockIdx.y;
+  const Asked asked(g, row);
   const Range range = range_of_parts(g, row);
-  if (range.most == 0)
+  if (!has_questions(range, asked.t))
     return;
-  const Settings set(g, row, range.largest());
-  if (set.greedy)
-    return;
+  const Settings set(g, asked, range.largest());
   const Buckets buckets(set, range.least);
-  const bool count = counts_words(g, set);
+  const bool count = counts_words(g, set.k);
   const int from = part * g.part_words, to = from + g.part_words < g.words ? from + g.part_words : g.words;
   sums_of<DT>(g, row, from, to, set, buckets, count, sums);
   const int at = bucket_place((int)threadIdx.x);
@@ -856,13 +1016,20 @@ template <int DT> __global__ __launch_bounds__(kThreads) void sample_sums_kernel
 template <int DT> __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs g) {
   __shared__ Draw d;
   const int64_t row = blockIdx.x;
+  const Asked asked(g, row);
+  Sixteen own;
+  if (threadIdx.x < 64)
+    own.load(g.sums + row * kBuckets + threadIdx.x * 16, g.counts + row * kBuckets + threadIdx.x * 16);
   const Range range = range_of_parts(g, row);
-  if (settled(g, row, range))
+  if (settled(g, row, range, asked.t, d.whole))
     return;
-  const Settings set(g, row, range.largest());
+  const Settings set(g, asked, range.largest());
   const Buckets buckets(set, range.least);
-  const int64_t at = row * kBuckets + (threadIdx.x & 63) * 16;
-  draw_row<DT>(g, row, set, buckets, counts_words(g, set), g.sums + at, g.counts + at, d);
+  if (threadIdx.x < 64)
+    ask_buckets(set, buckets, counts_words(g, asked.k), own, d);
+  __syncthreads();
+  gather<DT>(g, row, buckets, d);
+  answer(g, row, set, buckets, d.filled, d);
 }
 
 // How rows are cut: parts that fill the chip, of 4096 words at least (one part: a workgroup a row).
