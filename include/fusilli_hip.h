@@ -516,9 +516,10 @@ int fhip_cache_read(fhip_ctx *ctx, const fhip_cache_read_desc *d,
  *      codes 0, a row whose y holds a NaN or an infinity scale NaN and codes 0.
  *      (Where a is below 2^-100 both factors of the product are taken 2^64
  *      times as large; scales below 2^-126 are subnormal and lose bits.)
- *      X's type: f32, bf16 or f16; strides are free.  supported: 2 for rows and
- *      codes with a last stride of 1 whose starts and K lie on 16 bytes of X (and UP) and 8
- *      codes, K at most 16384, X and weight of one type; otherwise 1. ------- */
+ *      A row whose squares' sum leaves f32 counts as not finite for the norm.
+ *      X's type: f32, bf16 or f16; strides are free.  supported: 2 (rows held in
+ *      registers) for X, UP, Q and the weight with a last stride of 1, K at most
+ *      32768 and fewer than 2^21 rows; otherwise 1. ------------------------- */
 typedef enum {
   FHIP_QUANTIZE_NONE = 0,
   FHIP_QUANTIZE_RMSNORM = 1,
@@ -580,7 +581,7 @@ int fhip_matmul_quantized(fhip_ctx *ctx, const fhip_matmul_quantized_desc *d,
 /* A token for each row of logits, drawn with the caller's random numbers.  With m
  * a row's largest logit and T its temperature, word i has the weight
  *   w_i = exp((logit_i - m) / T), 1 for the largest,
- * in f64, held as a whole multiple of 2^-40.  Words are ordered by their logits, the
+ * in f64, held as a whole multiple of 2^-46 (of 2^-38 for the longest rows).  Words are ordered by their logits, the
  * largest first, equal ones by their index, and the first so many are kept as the
  * strictest of these says:
  *   top_k   the first top_k (0 or less: all);

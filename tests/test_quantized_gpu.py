@@ -18,8 +18,7 @@ def rng_of(*seed):
 
 
 # ---- rows to codes ----------------------------------------------------------------
-def quantize(ctx, x, kind="NONE", weight=None, up=None, eps=1e-6, q_strides=None, scale_stride=1, x_shift=0, q_shift=0,
-             fast=None):
+def quantize(ctx, x, kind="NONE", weight=None, up=None, eps=1e-6, q_strides=None, scale_stride=1, x_shift=0, q_shift=0):
     """x, up, weight: HT.  -> (codes, scales)"""
     rows, k = x.dims
     d = capi.QuantizeRowsDesc()
@@ -30,8 +29,8 @@ def quantize(ctx, x, kind="NONE", weight=None, up=None, eps=1e-6, q_strides=None
         d.has_weight, d.weight_dtype, d.weight_stride = 1, weight.dtype, weight.strides[0]
     if up is not None:
         d.up = up.desc()
-    supported = ctx.lib.fhip_quantize_rows_supported(d)
-    assert supported == (2 if fast else supported if fast is None else 1)
+    held = k <= 32768 and all(k == 1 or t.strides[-1] == 1 for t in (x, up, weight, q) if t is not None)
+    assert ctx.lib.fhip_quantize_rows_supported(d) == (2 if held else 1)
     bx, px, _ = guarded(ctx, x.storage, x_shift)
     bu, pu, _ = guarded(ctx, up.storage, x_shift) if up is not None else (None, None, None)
     bw, pw, _ = guarded(ctx, weight.storage) if weight is not None else (None, None, None)
@@ -39,6 +38,7 @@ def quantize(ctx, x, kind="NONE", weight=None, up=None, eps=1e-6, q_strides=None
     scales = np.full((rows - 1) * scale_stride + 1, -5.0, np.float32)
     bs, ps, scales_back = guarded(ctx, scales)
     ctx.quantize_rows(d, px, pq, ps, up=pu, weight=pw)
+    assert ctx.last_kernel() == ("quantize_rows_held" if held else "quantize_rows_generic")
     q.storage = codes()
     touched = np.zeros(q.storage.size, bool)
     touched[(np.arange(rows)[:, None] * q.strides[0] + np.arange(k) * q.strides[1]).reshape(-1)] = True
@@ -48,7 +48,8 @@ def quantize(ctx, x, kind="NONE", weight=None, up=None, eps=1e-6, q_strides=None
     return q.logical().astype(np.int64), s[::scale_stride]
 
 
-SIZES = [(1, 1), (1, 2048), (3, 7), (5, 1001), (17, 4096), (2, 16384), (2, 20008), (300, 96), (33, 8), (4, 5120)]
+SIZES = [(1, 1), (1, 2048), (3, 7), (5, 1001), (17, 4096), (2, 16384), (2, 20008), (300, 96), (33, 8), (4, 5120),
+         (2, 32768), (3, 32767), (2, 32769), (6, 511), (3, 513), (5, 8193)]
 
 
 @pytest.mark.parametrize("kind", ["NONE", "RMSNORM", "SWISH_GATE"])
@@ -129,7 +130,7 @@ def test_quantize_odd_rows_behind_a_front(ctx, front_kind):
     with np.errstate(all="ignore"):
         y, rel = front(x.logical(), front_kind, up=up and up.logical())
     keep = [0, 3, 5, 6, 7] + ([2] if front_kind == "SWISH_GATE" else [])
-    if front_kind == "SWISH_GATE":  # (exp(200) is beyond f32, whose quotient is 0; in 64 bits it is 1e-85)
+    if front_kind == "SWISH_GATE":  # (exp(-200) is 0 in f32; in 64 bits the row is 1e-85)
         assert s[4] == 0 and not q[4].any()
     else:
         keep.append(4)
@@ -141,9 +142,39 @@ def test_quantize_odd_rows_behind_a_front(ctx, front_kind):
 def test_quantize_weight_of_another_type_and_stride(ctx):
     rng = rng_of(5)
     x = HT.from_logical(rng.normal(size=[6, 768]), BF16)
-    for weight in (HT.from_logical(rng.normal(size=[768]), F32), HT.from_logical(rng.normal(size=[768]), BF16, [3]), None):
+    for weight in (HT.from_logical(rng.normal(size=[768]), F32), HT.from_logical(rng.normal(size=[768]), F16),
+                   HT.from_logical(rng.normal(size=[768]), BF16, [3]), None):
         q, s = quantize(ctx, x, "RMSNORM", weight, eps=1e-3)
         check_codes(q, s, *front(x.logical(), "RMSNORM", weight and weight.logical(), eps=1e-3))
+
+
+@pytest.mark.parametrize("k", [96, 1024, 40000])
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=NAME.get)
+def test_quantize_squares_beyond_f32(ctx, dtype, k):
+    """A row of finite numbers whose squares' sum is infinite has no scale, rather than codes of zeros."""
+    x = np.ones([3, k])
+    x[1, k // 3] = 1e25
+    q, s = quantize(ctx, HT.from_logical(x, dtype), "RMSNORM")
+    assert np.isnan(s[1]) and not q[1].any()
+    assert (q[[0, 2]] == 127).all() and np.isfinite(s[[0, 2]]).all()
+
+
+@pytest.mark.parametrize("k", [96, 1024, 40000])
+def test_quantize_gate_of_large_numbers(ctx, k):
+    """x / (1 + exp(-x)) where exp leaves f32's range: nearly x, or nearly nothing."""
+    x = rng_of(6, k).normal(size=[6, k])
+    x[0] = 1e30
+    x[1] = np.linspace(-95, -85, k)  # (a row of the smallest results: scales stay normal numbers)
+    x[2] = np.where(np.arange(k) % 2, -3e38, 3e38)
+    x[3, 1] = -np.inf
+    x[4] = np.linspace(-150, 150, k)
+    x = HT.from_logical(x, F32)
+    up = HT.from_logical(np.where(np.arange(k) % 3, 1.0, -0.5)[None].repeat(6, 0), F32)
+    q, s = quantize(ctx, x, "SWISH_GATE", up=up)
+    y, rel = front(x.logical(), "SWISH_GATE", up=up.logical())
+    keep = [0, 1, 2, 4, 5]
+    check_codes(q[keep], s[keep], y[keep], rel)
+    assert np.isnan(s[3]) and not q[3].any()
 
 
 # ---- products ------------------------------------------------------------------------
