@@ -13,6 +13,8 @@
 // one border in 10^7, and a row has 10^5 of them.)
 #include "common.h"
 
+#include <type_traits>
+
 namespace {
 
 struct SampleArgs {
@@ -63,6 +65,14 @@ struct Asked {
   }
 };
 
+// 1 / x, good to two steps or so of f64 (x = 0: infinity or NaN; infinite: 0 or NaN): a seed that is good to
+// 2^-24 and two of Newton's steps.
+__device__ __forceinline__ double reciprocal(double x) {
+  double y = __builtin_amdgcn_rcp(x);
+  y = __builtin_fma(y, __builtin_fma(-x, y, 1.0), y);
+  return __builtin_fma(y, __builtin_fma(-x, y, 1.0), y);
+}
+
 struct Settings : Asked {
   double most, by;  // the largest logit, 1 / T
   double by2;       // log2(e) / T
@@ -72,20 +82,19 @@ struct Settings : Asked {
   __device__ __forceinline__ Settings(const SampleArgs &g, const Asked &asked, float largest) : Asked(asked) {
     most = (double)largest;
     greedy = !(t > 0.f);
-    by = greedy ? 1.0 : fmax(1.0 / (double)t, 1e-300); // (T infinite: -inf times it is -inf)
+    by = greedy ? 1.0 : fmax(reciprocal((double)t), 1e-300); // (T infinite: NaN; -inf times it is -inf)
     by2 = by * 1.44269504088896340736;
     top = largest;
     bits = g.bits;
   }
-  __device__ __forceinline__ double weight(float l) const { return l == top ? 1.0 : exp(((double)l - most) * by); }
-  // The weight in units of 2^-bits, rounded, of a logit that is finite like the largest and less than
-  // 40 T below it.  2^x with x = n + f, |f| at most 1/2: a polynomial of degree 10 through 1 at 0 that
-  // meets 2^f at the zeros of a Chebyshev polynomial (6e-16 of it off at most); the unit's power goes
-  // into n, and 2^52 on top leaves the rounded value in the low bits.  20 instructions; the library's
-  // exp and the conversion to 64 bits take more than twice as many.
-  __device__ __forceinline__ uint64_t held_near(float l) const {
-    const double x = ((double)l - most) * by2;
-    const double n = rint(x), f = x - n;
+  // The weight of a logit that is finite like the largest and less than 64 T below it, times 2^up.  2^x
+  // with x = n + f, |f| at most 1/2: a polynomial of degree 10 through 1 at 0 that meets 2^f at the zeros of a
+  // Chebyshev polynomial (6e-16 of it off at most).  Adding 3 * 2^51 rounds x to its n, which stands in the
+  // sum's low bits and is added to the exponent from there: f64's own rint, conversion and ldexp are
+  // issued at a quarter of the rate.
+  __device__ __forceinline__ double near_weight(float l, int up) const {
+    const double off = (double)l - most, whole = __builtin_fma(off, by2, 0x1.8p52);
+    const double f = __builtin_fma(off, by2, 0x1.8p52 - whole);
     // (the constants keep their registers: in C++ each becomes a copy and an instruction that overwrites it)
     auto step = [&](double y, double c) {
       double r;
@@ -102,8 +111,16 @@ struct Settings : Asked {
     y = step(y, 2.4022650695910075e-01);
     y = step(y, 6.9314718055994617e-01);
     y = __builtin_fma(y, f, 1.0);
-    y = __builtin_amdgcn_ldexp(y, (int)n + bits) + 0x1p52;
-    return __builtin_bit_cast(uint64_t, y) & ((1ull << 52) - 1);
+    const uint64_t bits_of = __builtin_bit_cast(uint64_t, y);
+    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, whole) + (uint32_t)up;
+    return __builtin_bit_cast(double, (uint64_t)((uint32_t)(bits_of >> 32) + (n << 20)) << 32 | (uint32_t)bits_of);
+  }
+  __device__ __forceinline__ double weight(float l) const {
+    return l == top ? 1.0 : ((double)l - most) * by > -40.0 ? near_weight(l, 0) : 0.0;
+  }
+  // The weight in units of 2^-bits, rounded: 2^52 on top leaves it in the low bits.
+  __device__ __forceinline__ uint64_t held_near(float l) const {
+    return __builtin_bit_cast(uint64_t, near_weight(l, bits) + 0x1p52) & ((1ull << 52) - 1);
   }
   // The same of any; 0 from exp(-32) = 2^-46.2 on.
   __device__ __forceinline__ uint64_t held(float l) const {
@@ -327,8 +344,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs g) 
 //
 // Which buckets matter one wavefront finds, without a barrier: sixteen that execute the same few hundred
 // instructions between barriers take three times as long.
-constexpr int kBuckets = 1024, kThreads = 1024;
-constexpr int kList = 8192; // words of the buckets in question
+constexpr int kBuckets = 1024;
+constexpr int kThreads = 1024; // of the launches over parts
+// How many words of the buckets in question NT threads hold, and how many of them they sort.
+constexpr int list_of(int nt) { return nt == 64 ? 1024 : 8192; }
+constexpr int sorted_of(int nt) { return nt == 1024 ? 2048 : 4 * nt; }
 
 // N words from `at` of a row whose words lie side by side, at element alignment.
 template <typename E, int COUNT> struct WordsOf {
@@ -344,10 +364,10 @@ template <> struct Words<FHIP_HALF> : WordsOf<_Float16, 8> {};
 
 // take(logits, first index) of the words from .. to - 1 of a row, N of them at a time (-inf where
 // fewer are left), with U loads on their way.
-template <int DT, int U, typename Take>
+template <int NT, int DT, int U, typename Take>
 __device__ __forceinline__ void for_words(const SampleArgs &g, int64_t row, int from, int to, Take take) {
   using W = Words<DT>;
-  constexpr int STEP = kThreads * W::N;
+  constexpr int STEP = NT * W::N;
   const int64_t base = row * g.row_s;
   const int whole = from + (to - from) / W::N * W::N, last = whole - W::N;
   const int first = from + (int)threadIdx.x * W::N;
@@ -407,6 +427,20 @@ __device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) {
 __device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
+// All lanes' values joined (a value joined with itself is the same).
+template <int CTRL, int ROWS, typename T> __device__ __forceinline__ T lane_or_own(T v) {
+  const int own = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(own, own, CTRL, ROWS, 15, false));
+}
+template <typename T, typename F> __device__ __forceinline__ T joined_lanes(T v, F join) {
+  v = join(v, lane_or_own<0x111, 15>(v));
+  v = join(v, lane_or_own<0x112, 15>(v));
+  v = join(v, lane_or_own<0x114, 15>(v));
+  v = join(v, lane_or_own<0x118, 15>(v));
+  v = join(v, lane_or_own<0x142, 10>(v));
+  v = join(v, lane_or_own<0x143, 12>(v));
+  return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
 template <typename T> __device__ __forceinline__ T largest_of_wave(T v) {
   return of_lane(up_to_lane(v, [](T a, T b) { return a > b ? a : b; }), 63);
 }
@@ -423,17 +457,27 @@ struct Range {
   float least;
   __device__ __forceinline__ float largest() const { return logit_of((uint32_t)(most >> 32)); }
 };
-struct RangeRoom {
-  uint64_t most[kThreads / 64];
-  uint32_t least[kThreads / 64];
+template <int NT> struct RangeRoom {
+  float top[NT / 64], least[NT / 64];
+  uint32_t place[NT / 64];
 };
-template <int DT>
-__device__ __forceinline__ Range range_of(const SampleArgs &g, int64_t row, int from, int to, RangeRoom &room) {
+// The same of 64 values that lanes hold: a largest value and the lowest place that has it.
+__device__ __forceinline__ Range range_of_lanes(float top, uint32_t place, float least) {
+  auto larger = [](float a, float b) { return fmaxf(a, b); };
+  const float most = joined_lanes(top, larger);
+  const uint32_t first = joined_lanes(top == most ? place : ~0u, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+  Range r;
+  r.most = most > -INFINITY ? (uint64_t)key_of(most) << 32 | ~first : 0;
+  r.least = joined_lanes(least, [](float a, float b) { return fminf(a, b); });
+  return r;
+}
+template <int NT, int DT>
+__device__ __forceinline__ Range range_of(const SampleArgs &g, int64_t row, int from, int to, RangeRoom<NT> &room) {
   using W = Words<DT>;
   // (a thread's indices ascend: a later word has to be larger)
   float top = -INFINITY, least = INFINITY;
   int place = 0;
-  for_words<DT, 4>(g, row, from, to, [&](const float(&v)[W::N], int i) {
+  for_words<NT, DT, NT == 64 ? 2 : 4>(g, row, from, to, [&](const float(&v)[W::N], int i) {
 #pragma unroll
     for (int e = 0; e < W::N; ++e) {
       place = v[e] > top ? i + e : place;
@@ -441,15 +485,17 @@ __device__ __forceinline__ Range range_of(const SampleArgs &g, int64_t row, int 
       least = v[e] > -INFINITY && v[e] < least ? v[e] : least;
     }
   });
-  const uint64_t most = largest_of_wave<uint64_t>(top > -INFINITY ? (uint64_t)key_of(top) << 32 | ~(uint32_t)place : 0);
-  const uint32_t low = largest_of_wave<uint32_t>(~key_of(least));
-  if ((threadIdx.x & 63) == 0)
-    room.most[threadIdx.x >> 6] = most, room.least[threadIdx.x >> 6] = low;
-  __syncthreads();
-  const int w = threadIdx.x & (kThreads / 64 - 1);
-  Range r;
-  r.most = largest_of_wave<uint64_t>(room.most[w]);
-  r.least = logit_of(~largest_of_wave<uint32_t>(room.least[w]));
+  Range r = range_of_lanes(top, (uint32_t)place, least);
+  if constexpr (NT > 64) {
+    if ((threadIdx.x & 63) == 0) {
+      room.top[threadIdx.x >> 6] = r.most ? r.largest() : -INFINITY;
+      room.place[threadIdx.x >> 6] = ~(uint32_t)r.most;
+      room.least[threadIdx.x >> 6] = r.least;
+    }
+    __syncthreads();
+    const int w = threadIdx.x & (NT / 64 - 1);
+    r = range_of_lanes(room.top[w], room.place[w], room.least[w]);
+  }
   return r;
 }
 
@@ -457,13 +503,14 @@ __device__ __forceinline__ Range range_of(const SampleArgs &g, int64_t row, int 
 // order; halves, as a difference may be twice the largest number.  (Of rows whose largest logit is finite.)
 struct Buckets {
   float half, by;
-  double wide; // of (m - l) / T, all of them
+  float a_unit; // buckets to a unit of (m - l) / T
   __device__ __forceinline__ Buckets(const Settings &set, float least) : half(0.5f * set.top) {
     const double range = (set.most - (double)least) * set.by;
-    wide = range < 32.0 ? range : 32.0;
     // (a little less than the range takes, so that the last word is inside for all roundings)
-    const double x = range > 0.0 ? 2.0 * set.by * (kBuckets * (1.0 - 0x1p-20)) / wide : 0.0;
+    const double unit = range > 0.0 ? kBuckets * (1.0 - 0x1p-20) * reciprocal(range < 32.0 ? range : 32.0) : 0.0;
+    const double x = 2.0 * set.by * unit;
     by = x < 3.0e38 ? (float)x : 3.0e38f;
+    a_unit = unit < 3.0e38 ? (float)unit : 3.0e38f;
   }
   __device__ __forceinline__ int of(float l) const { // kBuckets: none
     return (int)fminf((half - 0.5f * l) * by, (float)kBuckets); // (NaN, -inf: none)
@@ -478,14 +525,14 @@ struct Sums {
   unsigned long long sum[kAllPlaces];
   uint32_t count[kAllPlaces];
 };
-template <int DT>
+template <int NT, int DT>
 __device__ __forceinline__ void sums_of(const SampleArgs &g, int64_t row, int from, int to, const Settings &set,
                                         const Buckets &buckets, bool count, Sums &s) {
   using W = Words<DT>;
-  for (int i = threadIdx.x; i < kPlaces; i += kThreads)
+  for (int i = threadIdx.x; i < kPlaces; i += NT)
     s.sum[i] = 0, s.count[i] = 0;
   __syncthreads();
-  for_words<DT, 1>(g, row, from, to, [&](const float(&v)[W::N], int) {
+  for_words<NT, DT, 1>(g, row, from, to, [&](const float(&v)[W::N], int) {
 #pragma unroll
     for (int e = 0; e < W::N; ++e) {
       const int b = buckets.of(v[e]);
@@ -510,33 +557,36 @@ struct Front {
   float floor; // no word in question is smaller
   int by_k, least_from, least_to;
 };
-struct Draw {
+template <int NT> struct Draw {
   union {
     Bins bins;
-    Shared<kThreads> whole; // of a row that does not fit the list
+    Shared<NT> whole; // of a row that does not fit the list
   };
   Front f;
   uint32_t asked[kBuckets / 32 + 1]; // a bit a bucket (the last: none)
-  uint64_t swap[2][kThreads];
-  uint64_t kept;
-  uint64_t least_front; // weights in front of the first bucket that min_p's end may lie in
+  uint64_t kept[3]; // what weighs no more than top_k, top_p and min_p keep
   int filled;
   uint32_t high, low, items; // largest key, complement of the smallest; how many
   End end;
-  float logits[kList];
-  uint32_t places[kList];
+  union {
+    struct {
+      float logits[list_of(NT)];
+      uint32_t places[list_of(NT)];
+    };
+    uint64_t swap[2][sorted_of(NT)]; // (of words that registers hold)
+  };
 };
 
 // find_end above over the list.  (d.high, d.low and d.items are 0 before and after.)
-template <typename Key, typename Held>
-__device__ __forceinline__ End list_end(bool by_count, uint64_t need, int n, Draw &d, Key key_at, Held held) {
+template <int NT, typename Key, typename Held>
+__device__ __forceinline__ End list_end(bool by_count, uint64_t need, int n, Draw<NT> &d, Key key_at, Held held) {
   const int t = threadIdx.x, l = t & 63;
   auto clear = [&] {
-    if (t < 256)
-      d.bins.sum[t] = 0, d.bins.count[t] = 0;
+    for (int i = t; i < 256; i += NT)
+      d.bins.sum[i] = 0, d.bins.count[i] = 0;
   };
   uint32_t high = 0, low = 0, items = 0;
-  for (int i = t; i - l < n; i += kThreads) {
+  for (int i = t; i - l < n; i += NT) {
     const uint32_t key = i < n ? key_at(i) : 0;
     high = key > high ? key : high;
     low = key && ~key > low ? ~key : low;
@@ -561,7 +611,7 @@ __device__ __forceinline__ End list_end(bool by_count, uint64_t need, int n, Dra
   while (left > 0) {
     const int shift = left > 8 ? left - 8 : 0;
     const uint32_t above = left == 32 ? 0 : ~0u << left; // bits that the prefix has
-    for (int i = t; i < n; i += kThreads) {
+    for (int i = t; i < n; i += NT) {
       const uint32_t key = key_at(i);
       if (key == 0 || (key & above) != e.key)
         continue;
@@ -617,11 +667,12 @@ __device__ __forceinline__ bool has_questions(const Range &range, float t) {
   return range.most != 0 && t > 0.f && range.largest() < INFINITY;
 }
 // Does a row without questions; false: it has some.
-__device__ __forceinline__ bool settled(const SampleArgs &g, int64_t row, const Range &range, float t, Shared<kThreads> &s) {
+template <int NT>
+__device__ __forceinline__ bool settled(const SampleArgs &g, int64_t row, const Range &range, float t, Shared<NT> &s) {
   if (has_questions(range, t))
     return false;
   if (range.most != 0 && t > 0.f) {
-    sample_row<kThreads>(g, row, s);
+    sample_row<NT>(g, row, s);
     return true;
   }
   if (threadIdx.x == 0) {
@@ -664,8 +715,9 @@ struct Sixteen {
 };
 
 // The buckets in question, by the first wavefront.
+template <int NT>
 __device__ __forceinline__ void ask_buckets(const Settings &set, const Buckets &buckets, bool count, const Sixteen &own,
-                                            Draw &d) {
+                                            Draw<NT> &d) {
   const int l = threadIdx.x;
   const uint64_t one = (uint64_t)1 << set.bits; // (the largest is always kept)
   const uint64_t(&w)[16] = own.w;
@@ -716,11 +768,13 @@ __device__ __forceinline__ void ask_buckets(const Settings &set, const Buckets &
     low = locate.start_of(a), high = locate.end_of(z, all);
   }
   if (set.least > 0.f) {
-    // (buckets are of f32, three roundings: less than a thousandth of one)
-    const double edge = -log(least_bound(set)) / buckets.wide * kBuckets * (1.0 - 0x1p-20);
-    const double a = edge - 1e-3, z = edge + 1e-3;
-    least_from = !(a > 0.0) ? 0 : a < (double)kBuckets ? (int)a : kBuckets; // (one bucket for all: 0)
-    least_to = !(z > 0.0) ? 0 : z < (double)kBuckets ? (int)z : kBuckets - 1;
+    // (the logarithm is good to 2^-21 and 2^-21 of itself; buckets are of f32, a few roundings: less than a
+    // thousandth of one)
+    const float edge = -0.69314718f * __builtin_amdgcn_logf((float)least_bound(set));
+    const float a = edge * (1.f - 0x1p-20f) * buckets.a_unit - buckets.a_unit * 0x1p-20f - 2e-3f;
+    const float z = edge * (1.f + 0x1p-20f) * buckets.a_unit + buckets.a_unit * 0x1p-20f + 2e-3f;
+    least_from = !(a > 0.f) ? 0 : a < (float)kBuckets ? (int)a : kBuckets; // (one bucket for all: 0)
+    least_to = !(z > 0.f) ? 0 : z < (float)kBuckets ? (int)z : kBuckets - 1;
     if (least_from < kBuckets) {
       ask(least_from, least_to);
       const uint64_t a_sum = locate.start_of(least_from), z_sum = locate.end_of(least_to, all);
@@ -735,6 +789,8 @@ __device__ __forceinline__ void ask_buckets(const Settings &set, const Buckets &
   ask(locate(set.below(low) + 1), locate(set.below(high) + 1));
   if (l == 0) {
     d.f.all = all, d.f.by_k = by_k, d.f.least_from = least_from, d.f.least_to = least_to;
+    d.kept[0] = d.kept[1] = all; // (until a word says less; and what lies in front of min_p's buckets)
+    d.kept[2] = least_from < kBuckets ? locate.start_of(least_from) : all;
     // (below the last bucket's end, for all roundings)
     const double end = set.most - (lowest + 2) * 2.0 / (double)buckets.by;
     d.f.floor = buckets.by > 0.f ? (float)(end - 1e-6 * (fabs(end) + fabs(set.most))) : -INFINITY;
@@ -742,10 +798,11 @@ __device__ __forceinline__ void ask_buckets(const Settings &set, const Buckets &
 }
 
 // The words of those buckets, to the list.
-template <int DT> __device__ __forceinline__ void gather(const SampleArgs &g, int64_t row, const Buckets &buckets, Draw &d) {
+template <int NT, int DT>
+__device__ __forceinline__ void gather(const SampleArgs &g, int64_t row, const Buckets &buckets, Draw<NT> &d) {
   using W = Words<DT>;
   const float floor = d.f.floor;
-  for_words<DT, 4>(g, row, 0, g.words, [&](const float(&v)[W::N], int i) {
+  for_words<NT, DT, NT == 64 ? 2 : 4>(g, row, 0, g.words, [&](const float(&v)[W::N], int i) {
     uint32_t hits = 0;
     float top = v[0];
 #pragma unroll
@@ -763,7 +820,7 @@ template <int DT> __device__ __forceinline__ void gather(const SampleArgs &g, in
       for (int e = 0; e < W::N; ++e)
         if (hits >> e & 1) {
           const int at = atomicAdd(&d.filled, 1);
-          if (at < kList)
+          if (at < list_of(NT))
             d.logits[at] = v[e], d.places[at] = (uint32_t)(i + e);
         }
     }
@@ -771,106 +828,192 @@ template <int DT> __device__ __forceinline__ void gather(const SampleArgs &g, in
   __syncthreads();
 }
 
-// The token of a row, from at most a word a thread: in order, with their sums next to them, they answer
-// every question by a comparison.  (A search for each of them in the list takes three times as long.)
-__device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets,
-                                              int n, Draw &d) {
-  const int t = threadIdx.x, l = t & 63;
-  uint64_t v = t < n ? (uint64_t)key_of(d.logits[t]) << 32 | ~d.places[t] : 0;
-  // exchanges at distances below 64 inside a wavefront, the others through LDS (two places in turn: one
-  // barrier each); wavefronts without a word keep the barriers only
-  int turn = 0;
-  for (int size = 2; size < 2 * n; size *= 2)
-    for (int far = size / 2; far > 0; far /= 2) {
-      uint64_t w;
-      if (far >= 64) {
-        d.swap[turn][t] = v;
-        __syncthreads();
-        w = d.swap[turn][t ^ far];
-        turn ^= 1;
-      } else {
-        if (t - l >= n && size <= 64)
-          continue;
-        w = (uint64_t)__shfl_xor((unsigned long long)v, far);
-      }
-      const bool larger = ((t & far) == 0) == ((t & size) == 0);
-      v = (w > v) == larger ? w : v;
-    }
-  const float x = logit_of((uint32_t)(v >> 32));
-  const bool mine = v != 0;
-  const uint64_t weight = mine ? set.held(x) : 0;
-  const int home = mine ? buckets.of(x) : kBuckets;
-  // sums up to each word of the list, then of the row: a bucket's begin at its first word
-  uint64_t sum = sum_up_to_lane(weight);
-  if (l == 63)
-    d.bins.sum[t >> 6] = sum;
-  d.swap[turn][t] = (uint64_t)home;
-  __syncthreads();
-  for (int w = 0; w < t >> 6; ++w)
-    sum += d.bins.sum[w];
-  if (mine && (t == 0 || (int)d.swap[turn][t - 1] != home)) {
-    d.f.before[bucket_place(home)] -= sum - weight; // (unsigned: wraps and wraps back)
-    d.f.first[bucket_place(home)] -= (uint32_t)t;
-  }
-  __syncthreads();
-  const int least_from = d.f.least_from, least_to = d.f.least_to;
-  const uint64_t one = (uint64_t)1 << set.bits;
-  const uint64_t up_to = mine ? d.f.before[bucket_place(home)] + sum : 0;
-  const uint32_t rank = mine ? d.f.first[bucket_place(home)] + (uint32_t)t : 0;
-  // whoever ends a prefix says so
-  auto told = [&](bool says, uint64_t otherwise) {
-    if (t == 0)
-      d.kept = otherwise;
-    __syncthreads();
-    if (says)
-      d.kept = up_to;
-    __syncthreads();
-    const uint64_t kept = d.kept;
-    __syncthreads();
-    return kept;
+// The value of the lane whose number differs in one bit.
+template <int FAR> __device__ __forceinline__ uint32_t other_lane(uint32_t v) {
+  auto move = [](uint32_t x, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 15, 15, false);
   };
-  uint64_t kept = d.f.all;
-  if (d.f.by_k >= 0)
-    kept = told(mine && rank + 1 == (uint32_t)set.k, kept);
-  if (set.p < 1.f) {
-    const uint64_t need = set.share(kept);
-    kept = told(mine && up_to - weight < need && need <= up_to, kept);
+  if constexpr (FAR == 1)
+    return move(v, std::integral_constant<int, 0xB1>{}); // quad_perm [1,0,3,2]
+  else if constexpr (FAR == 2)
+    return move(v, std::integral_constant<int, 0x4E>{}); // quad_perm [2,3,0,1]
+  else if constexpr (FAR == 4) // mirrored in halves of a row, then in quads
+    return move(move(v, std::integral_constant<int, 0x141>{}), std::integral_constant<int, 0x1B>{});
+  else if constexpr (FAR == 8)
+    return move(v, std::integral_constant<int, 0x128>{}); // row_ror 8
+  else {
+    // odd rows (or the upper half) of one copy against even ones (the lower half) of another
+    const auto both = FAR == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false)
+                                : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & FAR ? both[0] : both[1];
   }
-  if (set.least > 0.f && least_from < kBuckets) {
-    const bool large = mine && home >= least_from && home <= least_to && set.weight(x) >= least_bound(set);
-    // (the largest sum among them, or what lies in front of their buckets)
-    const uint64_t most = largest_of_wave<uint64_t>(large ? up_to : 0);
-    if (t == 0)
-      d.kept = d.least_front;
-    __syncthreads();
-    if (l == 0 && most)
-      atomicMax((unsigned long long *)&d.kept, (unsigned long long)most);
-    __syncthreads();
-    kept = d.kept < kept ? d.kept : kept;
-    __syncthreads();
-  }
-  if (set.least > 1.f)
-    kept = one;
-  const uint64_t need = set.below(kept) + 1;
-  if (mine && up_to - weight < need && need <= up_to) {
-    g.token[row] = (int32_t)~(uint32_t)v;
-    if (g.probability)
-      g.probability[row] = (float)((double)weight / (double)kept);
+}
+template <int FAR> __device__ __forceinline__ void exchange(uint64_t &v, bool descending) {
+  const uint64_t w = (uint64_t)other_lane<FAR>((uint32_t)(v >> 32)) << 32 | other_lane<FAR>((uint32_t)v);
+  v = (w > v) == (((threadIdx.x & FAR) == 0) == descending) ? w : v;
+}
+
+// n words in descending order, words h * NT + thread in a thread (0 behind the last): a bitonic
+// network.  Exchanges at distances below 64 by DPP inside a wavefront, others through LDS (two places in
+// turn: one barrier each) or inside a thread; wavefronts in whose block nothing lies only keep the barriers.
+template <int NT, int E> __device__ __forceinline__ void sort_words(uint64_t (&v)[E], int n, uint64_t (*swap)[NT * E]) {
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t & ~63);
+  int turn = 0;
+#pragma clang loop unroll(disable)
+  for (int size = 2; size < 2 * n; size *= 2) {
+    auto used = [&](int h) { return ((h * NT + wave) & -size) < n; };
+#pragma clang loop unroll(disable)
+    for (int far = size / 2; far >= 64; far /= 2) {
+      if (far >= NT) {
+#pragma unroll
+        for (int gap = E / 2; gap > 0; gap /= 2)
+          if (far == gap * NT) {
+#pragma unroll
+            for (int h = 0; h < E; ++h)
+              if ((h & gap) == 0) {
+                const bool descending = ((h * NT + t) & size) == 0;
+                const uint64_t a = v[h], b = v[h + gap];
+                const bool swaps = (b > a) == descending;
+                v[h] = swaps ? b : a, v[h + gap] = swaps ? a : b;
+              }
+          }
+        continue;
+      }
+#pragma unroll
+      for (int h = 0; h < E; ++h)
+        if (used(h))
+          swap[turn][h * NT + t] = v[h];
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < E; ++h)
+        if (used(h)) {
+          const uint64_t w = swap[turn][h * NT + (t ^ far)];
+          v[h] = (w > v[h]) == (((t & far) == 0) == (((h * NT + t) & size) == 0)) ? w : v[h];
+        }
+      turn ^= 1;
+    }
+#pragma unroll
+    for (int h = 0; h < E; ++h)
+      if (used(h)) {
+        const bool descending = ((h * NT + t) & size) == 0;
+        if (size > 32)
+          exchange<32>(v[h], descending);
+        if (size > 16)
+          exchange<16>(v[h], descending);
+        if (size > 8)
+          exchange<8>(v[h], descending);
+        if (size > 4)
+          exchange<4>(v[h], descending);
+        if (size > 2)
+          exchange<2>(v[h], descending);
+        exchange<1>(v[h], descending);
+      }
   }
 }
 
+// The token of a row, from words that registers hold: in order, with their sums next to them, they answer
+// every question by a comparison.  (A search for each of them in the list takes three times as long.)
+template <int NT>
+__device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets,
+                                              int n, Draw<NT> &d) {
+  constexpr int E = sorted_of(NT) / NT, WAVES = NT / 64;
+  const int t = threadIdx.x, l = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  uint64_t v[E];
+#pragma unroll
+  for (int h = 0; h < E; ++h) {
+    const int i = h * NT + t;
+    v[h] = i < n ? (uint64_t)key_of(d.logits[i]) << 32 | ~d.places[i] : 0;
+  }
+  __syncthreads(); // (the exchanges lie where the list does)
+  sort_words<NT, E>(v, n, d.swap);
+  // sums up to each word of the list, then of the row: a bucket's begin at its first word
+  auto each = [&](auto take) {
+#pragma unroll
+    for (int h = 0; h < E; ++h)
+      if (h * NT + wave * 64 < n)
+        take(h, h * NT + t);
+  };
+  uint64_t weight[E], up_to[E];
+  float x[E];
+  int home[E];
+  uint32_t rank[E];
+  __syncthreads();
+  each([&](int h, int i) {
+    x[h] = logit_of((uint32_t)(v[h] >> 32));
+    weight[h] = v[h] ? set.held(x[h]) : 0;
+    home[h] = v[h] ? buckets.of(x[h]) : kBuckets;
+    up_to[h] = sum_up_to_lane(weight[h]);
+    if (l == 63)
+      d.bins.sum[h * WAVES + wave] = up_to[h];
+    d.swap[0][i] = (uint64_t)home[h];
+  });
+  __syncthreads();
+  each([&](int h, int i) {
+    for (int w = 0; w < h * WAVES + wave; ++w)
+      up_to[h] += d.bins.sum[w];
+    if (v[h] && (i == 0 || (int)d.swap[0][i - 1] != home[h])) {
+      d.f.before[bucket_place(home[h])] -= up_to[h] - weight[h]; // (unsigned: wraps and wraps back)
+      d.f.first[bucket_place(home[h])] -= (uint32_t)i;
+    }
+  });
+  __syncthreads();
+  const int least_from = d.f.least_from, least_to = d.f.least_to, by_k = d.f.by_k;
+  each([&](int h, int i) {
+    up_to[h] += d.f.before[bucket_place(home[h])];
+    rank[h] = d.f.first[bucket_place(home[h])] + (uint32_t)i;
+    if (v[h] && by_k >= 0 && rank[h] + 1 == (uint32_t)set.k)
+      d.kept[0] = up_to[h];
+  });
+  // whoever ends a prefix says so
+  auto ends = [&](int h, uint64_t need) { return v[h] && up_to[h] - weight[h] < need && need <= up_to[h]; };
+  uint64_t kept = d.f.all;
+  if (by_k >= 0) {
+    __syncthreads();
+    kept = d.kept[0];
+  }
+  if (set.p < 1.f) {
+    const uint64_t need = set.share(kept);
+    each([&](int h, int) {
+      if (ends(h, need))
+        d.kept[1] = up_to[h];
+    });
+    __syncthreads();
+    kept = d.kept[1] < kept ? d.kept[1] : kept;
+  }
+  if (set.least > 0.f && least_from < kBuckets) {
+    // (the largest sum among them, or what lies in front of their buckets)
+    each([&](int h, int) {
+      const bool large = v[h] && home[h] >= least_from && home[h] <= least_to && set.weight(x[h]) >= least_bound(set);
+      const uint64_t most = largest_of_wave<uint64_t>(large ? up_to[h] : 0);
+      if (l == 0 && most)
+        atomicMax((unsigned long long *)&d.kept[2], (unsigned long long)most);
+    });
+    __syncthreads();
+    kept = d.kept[2] < kept ? d.kept[2] : kept;
+  }
+  if (set.least > 1.f)
+    kept = (uint64_t)1 << set.bits;
+  const uint64_t need = set.below(kept) + 1;
+  each([&](int h, int) {
+    if (ends(h, need)) {
+      g.token[row] = (int32_t)~(uint32_t)v[h];
+      if (g.probability)
+        g.probability[row] = (float)((double)weight[h] / (double)kept);
+    }
+  });
+}
+
 // The token of a row, from the n words of the list.
+template <int NT>
 __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets, int n,
-                                       Draw &d) {
+                                       Draw<NT> &d) {
   const int l = threadIdx.x & 63;
-  if (n > kList) { // (many equal logits)
-    sample_row<kThreads>(g, row, d.whole);
+  if (n > list_of(NT)) { // (many equal logits)
+    sample_row<NT>(g, row, d.whole);
     return;
   }
-  if (n <= kThreads) {
-    if (threadIdx.x == 0)
-      d.least_front = d.f.least_from < kBuckets ? d.f.before[bucket_place(d.f.least_from)] : 0;
-    answer_sorted(g, row, set, buckets, n, d);
+  if (n <= sorted_of(NT)) {
+    answer_sorted<NT>(g, row, set, buckets, n, d);
     return;
   }
   const uint64_t one = (uint64_t)1 << set.bits;
@@ -892,7 +1035,7 @@ __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const S
       if (q == 2 && set.least > 0.f && least_from < kBuckets) {
         const double bound = least_bound(set);
         uint64_t large = 0;
-        for (int i = threadIdx.x; i < n; i += kThreads) {
+        for (int i = threadIdx.x; i < n; i += NT) {
           const int at = buckets.of(d.logits[i]);
           if (at >= least_from && at <= least_to && set.weight(d.logits[i]) >= bound)
             large += set.held(d.logits[i]);
@@ -915,7 +1058,7 @@ __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const S
       need -= locate.start_of(home);
     }
     const bool by_place = q == 3;
-    const End e = list_end(
+    const End e = list_end<NT>(
         q == 0 || by_place, need, n, d,
         [&](int i) {
           const float x = d.logits[i];
@@ -930,7 +1073,7 @@ __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const S
       if (threadIdx.x == 0 && g.probability)
         g.probability[row] = (float)((double)set.held(word) / (double)kept);
       if (e.same == 1) { // (its only place)
-        for (int i = threadIdx.x; i < n; i += kThreads)
+        for (int i = threadIdx.x; i < n; i += NT)
           if (d.logits[i] == word)
             g.token[row] = (int32_t)d.places[i];
         return;
@@ -947,37 +1090,37 @@ __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const S
 __device__ __forceinline__ bool counts_words(const SampleArgs &g, int k) { return k > 0 && k < g.words; }
 
 // A workgroup a row.
-template <int DT> __global__ __launch_bounds__(kThreads) void sample_whole_kernel(SampleArgs g) {
-  __shared__ Draw d;
+template <int NT, int DT> __global__ __launch_bounds__(NT) void sample_whole_kernel(SampleArgs g) {
+  __shared__ Draw<NT> d;
   __shared__ Sums sums;
-  __shared__ RangeRoom room;
+  __shared__ RangeRoom<NT> room;
   const int64_t row = blockIdx.x;
   const Asked asked(g, row);
-  const Range range = range_of<DT>(g, row, 0, g.words, room);
-  if (settled(g, row, range, asked.t, d.whole))
+  const Range range = range_of<NT, DT>(g, row, 0, g.words, room);
+  if (settled<NT>(g, row, range, asked.t, d.whole))
     return;
   const Settings set(g, asked, range.largest());
   const Buckets buckets(set, range.least);
   const bool count = counts_words(g, set.k);
-  sums_of<DT>(g, row, 0, g.words, set, buckets, count, sums);
+  sums_of<NT, DT>(g, row, 0, g.words, set, buckets, count, sums);
   if (threadIdx.x < 64) {
     Sixteen own;
     own.load(&sums.sum[threadIdx.x * 17], &sums.count[threadIdx.x * 17]);
-    ask_buckets(set, buckets, count, own, d);
+    ask_buckets<NT>(set, buckets, count, own, d);
   }
   __syncthreads();
-  gather<DT>(g, row, buckets, d);
-  answer(g, row, set, buckets, d.filled, d);
+  gather<NT, DT>(g, row, buckets, d);
+  answer<NT>(g, row, set, buckets, d.filled, d);
 }
 
 template <int DT> __global__ __launch_bounds__(kThreads) void sample_most_kernel(SampleArgs g) {
-  __shared__ RangeRoom room;
+  __shared__ RangeRoom<kThreads> room;
   const int part = blockIdx.x;
   const int64_t row = blockIdx.y;
   if (part == 0)
     g.sums[row * kBuckets + threadIdx.x] = 0, g.counts[row * kBuckets + threadIdx.x] = 0;
   const int from = part * g.part_words, to = from + g.part_words < g.words ? from + g.part_words : g.words;
-  const Range r = range_of<DT>(g, row, from, to, room);
+  const Range r = range_of<kThreads, DT>(g, row, from, to, room);
   if (threadIdx.x == 0) {
     g.part_most[row * g.parts + part] = r.most;
     g.part_least[row * g.parts + part] = r.least;
@@ -1005,7 +1148,7 @@ template <int DT> __global__ __launch_bounds__(kThreads) void sample_sums_kernel
   const Buckets buckets(set, range.least);
   const bool count = counts_words(g, set.k);
   const int from = part * g.part_words, to = from + g.part_words < g.words ? from + g.part_words : g.words;
-  sums_of<DT>(g, row, from, to, set, buckets, count, sums);
+  sums_of<kThreads, DT>(g, row, from, to, set, buckets, count, sums);
   const int at = bucket_place((int)threadIdx.x);
   if (sums.sum[at])
     atomicAdd(&g.sums[row * kBuckets + threadIdx.x], sums.sum[at]);
@@ -1014,22 +1157,22 @@ template <int DT> __global__ __launch_bounds__(kThreads) void sample_sums_kernel
 }
 
 template <int DT> __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs g) {
-  __shared__ Draw d;
+  __shared__ Draw<kThreads> d;
   const int64_t row = blockIdx.x;
   const Asked asked(g, row);
   Sixteen own;
   if (threadIdx.x < 64)
     own.load(g.sums + row * kBuckets + threadIdx.x * 16, g.counts + row * kBuckets + threadIdx.x * 16);
   const Range range = range_of_parts(g, row);
-  if (settled(g, row, range, asked.t, d.whole))
+  if (settled<kThreads>(g, row, range, asked.t, d.whole))
     return;
   const Settings set(g, asked, range.largest());
   const Buckets buckets(set, range.least);
   if (threadIdx.x < 64)
-    ask_buckets(set, buckets, counts_words(g, asked.k), own, d);
+    ask_buckets<kThreads>(set, buckets, counts_words(g, asked.k), own, d);
   __syncthreads();
-  gather<DT>(g, row, buckets, d);
-  answer(g, row, set, buckets, d.filled, d);
+  gather<kThreads, DT>(g, row, buckets, d);
+  answer<kThreads>(g, row, set, buckets, d.filled, d);
 }
 
 // How rows are cut: parts that fill the chip, of 4096 words at least (one part: a workgroup a row).
@@ -1082,7 +1225,13 @@ static Places places_of(const fhip_sample_desc &d) {
 
 template <int DT> static int launch(fhip_ctx *ctx, const SampleArgs &g) {
   if (g.parts == 1) {
-    hipLaunchKernelGGL(sample_whole_kernel<DT>, dim3((unsigned)g.rows), dim3(kThreads), 0, ctx->stream, g);
+    const dim3 grid((unsigned)g.rows);
+    if (g.words <= 1024)
+      hipLaunchKernelGGL((sample_whole_kernel<64, DT>), grid, dim3(64), 0, ctx->stream, g);
+    else if (g.words <= 8192)
+      hipLaunchKernelGGL((sample_whole_kernel<256, DT>), grid, dim3(256), 0, ctx->stream, g);
+    else
+      hipLaunchKernelGGL((sample_whole_kernel<1024, DT>), grid, dim3(1024), 0, ctx->stream, g);
   } else { // (fewer than 128 rows)
     const dim3 grid((unsigned)g.parts, (unsigned)g.rows);
     hipLaunchKernelGGL(sample_most_kernel<DT>, grid, dim3(kThreads), 0, ctx->stream, g);
