@@ -35,6 +35,8 @@ struct SampleArgs {
   float *part_least;   // [row][part]: smallest logit that may be drawn
   unsigned long long *sums; // [row][bucket], cleared by the first launch
   uint32_t *counts;         // the same
+  uint32_t *filled, *arrived; // [row]: words of the buckets in question, parts that have written theirs; cleared too
+  unsigned long long *list;   // [row][kList]: such a word's index, logit
 };
 
 // Ascending with the logit: 0 for what is never drawn (NaN, -inf); -0 is 0.
@@ -257,8 +259,9 @@ __device__ __forceinline__ End find_end(bool by_count, uint64_t need, int n, Sha
   return e;
 }
 
-// One row, which is read again for each digit.
-template <int NT> __device__ __noinline__ void sample_row(const SampleArgs &g, int64_t row, Shared<NT> &s) {
+// One row, which is read again for each digit.  (Inlined: a call would give its callers a stack, which
+// costs 3 us or so a launch, and its registers, with which half as many wavefronts fit.)
+template <int NT> __device__ __forceinline__ void sample_row(const SampleArgs &g, int64_t row, Shared<NT> &s) {
   auto key_at = [&](int i) { return key_of(fhip_load_float(g.logits, g.dtype, row * g.row_s + i * g.word_s)); };
   auto add = [](uint64_t a, uint64_t b) { return a + b; };
   uint64_t most = 0, some = 0;
@@ -347,8 +350,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs g) 
 constexpr int kBuckets = 1024;
 constexpr int kThreads = 1024; // of the launches over parts
 // How many words of the buckets in question NT threads hold, and how many of them they sort.
-constexpr int list_of(int nt) { return nt == 64 ? 1024 : 8192; }
-constexpr int sorted_of(int nt) { return nt == 1024 ? 2048 : 4 * nt; }
+constexpr int list_of(int nt) { return nt == 64 ? 1024 : nt == 1024 ? 8192 : 4096; }
+constexpr int sorted_of(int nt) { return nt == 1024 ? 2048 : nt == 64 ? 256 : 2048; }
+constexpr int kDraw = 512; // threads of the launch that draws, if it is one of its own
+constexpr int kRanked = 512; // up to so many words a place is counted
+constexpr int kList = 8192; // words that its workgroups hand over, of a row
 
 // N words from `at` of a row whose words lie side by side, at element alignment.
 template <typename E, int COUNT> struct WordsOf {
@@ -573,7 +579,7 @@ template <int NT> struct Draw {
       float logits[list_of(NT)];
       uint32_t places[list_of(NT)];
     };
-    uint64_t swap[2][sorted_of(NT)]; // (of words that registers hold)
+    alignas(16) double swap[2][sorted_of(NT)]; // (of words that registers hold)
   };
 };
 
@@ -799,10 +805,10 @@ __device__ __forceinline__ void ask_buckets(const Settings &set, const Buckets &
 
 // The words of those buckets, to the list.
 template <int NT, int DT>
-__device__ __forceinline__ void gather(const SampleArgs &g, int64_t row, const Buckets &buckets, Draw<NT> &d) {
+__device__ __forceinline__ void gather(const SampleArgs &g, int64_t row, int from, int to, const Buckets &buckets, Draw<NT> &d) {
   using W = Words<DT>;
   const float floor = d.f.floor;
-  for_words<NT, DT, NT == 64 ? 2 : 4>(g, row, 0, g.words, [&](const float(&v)[W::N], int i) {
+  for_words<NT, DT, NT == 64 ? 2 : 4>(g, row, from, to, [&](const float(&v)[W::N], int i) {
     uint32_t hits = 0;
     float top = v[0];
 #pragma unroll
@@ -848,15 +854,27 @@ template <int FAR> __device__ __forceinline__ uint32_t other_lane(uint32_t v) {
     return threadIdx.x & FAR ? both[0] : both[1];
   }
 }
-template <int FAR> __device__ __forceinline__ void exchange(uint64_t &v, bool descending) {
-  const uint64_t w = (uint64_t)other_lane<FAR>((uint32_t)(v >> 32)) << 32 | other_lane<FAR>((uint32_t)v);
+// A word as one number, the larger the earlier in the order: key and index are 56 bits, and as many bits
+// of a positive f64 below 2 compare as they do, at four times the rate of whole numbers of 64 bits.  0: none.
+__device__ __forceinline__ double word_of(float logit, uint32_t place) {
+  return __builtin_bit_cast(double, (uint64_t)key_of(logit) << 30 | (uint64_t)(~place & 0xFFFFFFu) << 6);
+}
+__device__ __forceinline__ float logit_of_word(double v) {
+  return logit_of((uint32_t)(__builtin_bit_cast(uint64_t, v) >> 30));
+}
+__device__ __forceinline__ int32_t place_of_word(double v) {
+  return (int32_t)(~(uint32_t)(__builtin_bit_cast(uint64_t, v) >> 6) & 0xFFFFFFu);
+}
+template <int FAR> __device__ __forceinline__ void exchange(double &v, bool descending) {
+  const uint64_t own = __builtin_bit_cast(uint64_t, v);
+  const double w = __builtin_bit_cast(double, (uint64_t)other_lane<FAR>((uint32_t)(own >> 32)) << 32 | other_lane<FAR>((uint32_t)own));
   v = (w > v) == (((threadIdx.x & FAR) == 0) == descending) ? w : v;
 }
 
 // n words in descending order, words h * NT + thread in a thread (0 behind the last): a bitonic
 // network.  Exchanges at distances below 64 by DPP inside a wavefront, others through LDS (two places in
 // turn: one barrier each) or inside a thread; wavefronts in whose block nothing lies only keep the barriers.
-template <int NT, int E> __device__ __forceinline__ void sort_words(uint64_t (&v)[E], int n, uint64_t (*swap)[NT * E]) {
+template <int NT, int E> __device__ __forceinline__ void sort_words(double (&v)[E], int n, double (*swap)[NT * E]) {
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t & ~63);
   int turn = 0;
 #pragma clang loop unroll(disable)
@@ -872,7 +890,7 @@ template <int NT, int E> __device__ __forceinline__ void sort_words(uint64_t (&v
             for (int h = 0; h < E; ++h)
               if ((h & gap) == 0) {
                 const bool descending = ((h * NT + t) & size) == 0;
-                const uint64_t a = v[h], b = v[h + gap];
+                const double a = v[h], b = v[h + gap];
                 const bool swaps = (b > a) == descending;
                 v[h] = swaps ? b : a, v[h + gap] = swaps ? a : b;
               }
@@ -887,7 +905,7 @@ template <int NT, int E> __device__ __forceinline__ void sort_words(uint64_t (&v
 #pragma unroll
       for (int h = 0; h < E; ++h)
         if (used(h)) {
-          const uint64_t w = swap[turn][h * NT + (t ^ far)];
+          const double w = swap[turn][h * NT + (t ^ far)];
           v[h] = (w > v[h]) == (((t & far) == 0) == (((h * NT + t) & size) == 0)) ? w : v[h];
         }
       turn ^= 1;
@@ -911,6 +929,32 @@ template <int NT, int E> __device__ __forceinline__ void sort_words(uint64_t (&v
   }
 }
 
+// The same of at most NT words, one in a thread: a word's place is how many are larger.  Shorter code
+// than the network's, which is what counts where few words make code run once; NT^2 comparisons in all.
+template <int NT, int ROOM> __device__ __forceinline__ void rank_words(double &v, int n, double (*swap)[ROOM]) {
+  typedef double Two __attribute__((ext_vector_type(2)));
+  constexpr int STEP = 8;
+  const int t = threadIdx.x;
+  const bool used = __builtin_amdgcn_readfirstlane(t & ~63) < n;
+  swap[0][t] = v; // (zeros behind the last)
+  __syncthreads();
+  if (used) {
+    int larger = 0;
+    for (int i = 0; i < n; i += STEP)
+#pragma unroll
+      for (int e = 0; e < STEP; e += 2) {
+        const Two w = *(const Two *)&swap[0][i + e];
+        larger += w[0] > v;
+        larger += w[1] > v;
+      }
+    if (t < n)
+      swap[1][larger] = v;
+  }
+  __syncthreads();
+  if (used)
+    v = t < n ? swap[1][t] : 0.0;
+}
+
 // The token of a row, from words that registers hold: in order, with their sums next to them, they answer
 // every question by a comparison.  (A search for each of them in the list takes three times as long.)
 template <int NT>
@@ -918,14 +962,17 @@ __device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, 
                                               int n, Draw<NT> &d) {
   constexpr int E = sorted_of(NT) / NT, WAVES = NT / 64;
   const int t = threadIdx.x, l = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  uint64_t v[E];
+  double v[E];
 #pragma unroll
   for (int h = 0; h < E; ++h) {
     const int i = h * NT + t;
-    v[h] = i < n ? (uint64_t)key_of(d.logits[i]) << 32 | ~d.places[i] : 0;
+    v[h] = i < n ? word_of(d.logits[i], d.places[i]) : 0.0;
   }
   __syncthreads(); // (the exchanges lie where the list does)
-  sort_words<NT, E>(v, n, d.swap);
+  if (n <= kRanked && n <= NT)
+    rank_words<NT>(v[0], n, d.swap);
+  else
+    sort_words<NT, E>(v, n, d.swap);
   // sums up to each word of the list, then of the row: a bucket's begin at its first word
   auto each = [&](auto take) {
 #pragma unroll
@@ -939,19 +986,19 @@ __device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, 
   uint32_t rank[E];
   __syncthreads();
   each([&](int h, int i) {
-    x[h] = logit_of((uint32_t)(v[h] >> 32));
-    weight[h] = v[h] ? set.held(x[h]) : 0;
-    home[h] = v[h] ? buckets.of(x[h]) : kBuckets;
+    x[h] = logit_of_word(v[h]);
+    weight[h] = v[h] > 0.0 ? set.held(x[h]) : 0;
+    home[h] = v[h] > 0.0 ? buckets.of(x[h]) : kBuckets;
     up_to[h] = sum_up_to_lane(weight[h]);
     if (l == 63)
       d.bins.sum[h * WAVES + wave] = up_to[h];
-    d.swap[0][i] = (uint64_t)home[h];
+    d.swap[0][i] = home[h];
   });
   __syncthreads();
   each([&](int h, int i) {
     for (int w = 0; w < h * WAVES + wave; ++w)
       up_to[h] += d.bins.sum[w];
-    if (v[h] && (i == 0 || (int)d.swap[0][i - 1] != home[h])) {
+    if (v[h] > 0.0 && (i == 0 || (int)d.swap[0][i - 1] != home[h])) {
       d.f.before[bucket_place(home[h])] -= up_to[h] - weight[h]; // (unsigned: wraps and wraps back)
       d.f.first[bucket_place(home[h])] -= (uint32_t)i;
     }
@@ -961,11 +1008,11 @@ __device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, 
   each([&](int h, int i) {
     up_to[h] += d.f.before[bucket_place(home[h])];
     rank[h] = d.f.first[bucket_place(home[h])] + (uint32_t)i;
-    if (v[h] && by_k >= 0 && rank[h] + 1 == (uint32_t)set.k)
+    if (v[h] > 0.0 && by_k >= 0 && rank[h] + 1 == (uint32_t)set.k)
       d.kept[0] = up_to[h];
   });
   // whoever ends a prefix says so
-  auto ends = [&](int h, uint64_t need) { return v[h] && up_to[h] - weight[h] < need && need <= up_to[h]; };
+  auto ends = [&](int h, uint64_t need) { return v[h] > 0.0 && up_to[h] - weight[h] < need && need <= up_to[h]; };
   uint64_t kept = d.f.all;
   if (by_k >= 0) {
     __syncthreads();
@@ -983,7 +1030,7 @@ __device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, 
   if (set.least > 0.f && least_from < kBuckets) {
     // (the largest sum among them, or what lies in front of their buckets)
     each([&](int h, int) {
-      const bool large = v[h] && home[h] >= least_from && home[h] <= least_to && set.weight(x[h]) >= least_bound(set);
+      const bool large = v[h] > 0.0 && home[h] >= least_from && home[h] <= least_to && set.weight(x[h]) >= least_bound(set);
       const uint64_t most = largest_of_wave<uint64_t>(large ? up_to[h] : 0);
       if (l == 0 && most)
         atomicMax((unsigned long long *)&d.kept[2], (unsigned long long)most);
@@ -996,19 +1043,19 @@ __device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, 
   const uint64_t need = set.below(kept) + 1;
   each([&](int h, int) {
     if (ends(h, need)) {
-      g.token[row] = (int32_t)~(uint32_t)v[h];
+      g.token[row] = place_of_word(v[h]);
       if (g.probability)
         g.probability[row] = (float)((double)weight[h] / (double)kept);
     }
   });
 }
 
-// The token of a row, from the n words of the list.
+// The token of a row, from the n words of the list; `handed` holds those that LDS does not.
 template <int NT>
 __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets, int n,
-                                       Draw<NT> &d) {
+                                       Draw<NT> &d, const unsigned long long *handed = nullptr) {
   const int l = threadIdx.x & 63;
-  if (n > list_of(NT)) { // (many equal logits)
+  if (n > (handed ? kList : list_of(NT))) { // (many equal logits)
     sample_row<NT>(g, row, d.whole);
     return;
   }
@@ -1016,6 +1063,11 @@ __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const S
     answer_sorted<NT>(g, row, set, buckets, n, d);
     return;
   }
+  auto of_memory = [&](int i) { return __hip_atomic_load(&handed[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  auto logit_at = [&](int i) {
+    return !handed || i < list_of(NT) ? d.logits[i] : __builtin_bit_cast(float, (uint32_t)of_memory(i));
+  };
+  auto place_at = [&](int i) { return !handed || i < list_of(NT) ? d.places[i] : (uint32_t)(of_memory(i) >> 32); };
   const uint64_t one = (uint64_t)1 << set.bits;
   const uint64_t all = d.f.all;
   const Locator locate{d.f, d.f.before[l * 17], l < 63 ? d.f.before[l * 17 + 17] : all};
@@ -1036,9 +1088,10 @@ __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const S
         const double bound = least_bound(set);
         uint64_t large = 0;
         for (int i = threadIdx.x; i < n; i += NT) {
-          const int at = buckets.of(d.logits[i]);
-          if (at >= least_from && at <= least_to && set.weight(d.logits[i]) >= bound)
-            large += set.held(d.logits[i]);
+          const float x = logit_at(i);
+          const int at = buckets.of(x);
+          if (at >= least_from && at <= least_to && set.weight(x) >= bound)
+            large += set.held(x);
         }
         if (threadIdx.x == 0)
           d.bins.sum[0] = 0;
@@ -1061,8 +1114,8 @@ __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const S
     const End e = list_end<NT>(
         q == 0 || by_place, need, n, d,
         [&](int i) {
-          const float x = d.logits[i];
-          return by_place ? (x == word ? ~d.places[i] : 0u) : buckets.of(x) == home ? key_of(x) : 0u;
+          const float x = logit_at(i);
+          return by_place ? (x == word ? ~place_at(i) : 0u) : buckets.of(x) == home ? key_of(x) : 0u;
         },
         [&](uint32_t key) { return by_place ? 0ull : set.held(logit_of(key)); });
     if (q < 2) {
@@ -1074,8 +1127,8 @@ __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const S
         g.probability[row] = (float)((double)set.held(word) / (double)kept);
       if (e.same == 1) { // (its only place)
         for (int i = threadIdx.x; i < n; i += NT)
-          if (d.logits[i] == word)
-            g.token[row] = (int32_t)d.places[i];
+          if (logit_at(i) == word)
+            g.token[row] = (int32_t)place_at(i);
         return;
       }
     } else {
@@ -1109,7 +1162,7 @@ template <int NT, int DT> __global__ __launch_bounds__(NT) void sample_whole_ker
     ask_buckets<NT>(set, buckets, count, own, d);
   }
   __syncthreads();
-  gather<NT, DT>(g, row, buckets, d);
+  gather<NT, DT>(g, row, 0, g.words, buckets, d);
   answer<NT>(g, row, set, buckets, d.filled, d);
 }
 
@@ -1117,8 +1170,11 @@ template <int DT> __global__ __launch_bounds__(kThreads) void sample_most_kernel
   __shared__ RangeRoom<kThreads> room;
   const int part = blockIdx.x;
   const int64_t row = blockIdx.y;
-  if (part == 0)
+  if (part == 0) {
     g.sums[row * kBuckets + threadIdx.x] = 0, g.counts[row * kBuckets + threadIdx.x] = 0;
+    if (threadIdx.x == 0)
+      g.filled[row] = 0, g.arrived[row] = 0;
+  }
   const int from = part * g.part_words, to = from + g.part_words < g.words ? from + g.part_words : g.words;
   const Range r = range_of<kThreads, DT>(g, row, from, to, room);
   if (threadIdx.x == 0) {
@@ -1156,23 +1212,60 @@ template <int DT> __global__ __launch_bounds__(kThreads) void sample_sums_kernel
     atomicAdd(&g.counts[row * kBuckets + threadIdx.x], sums.count[at]);
 }
 
-template <int DT> __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs g) {
-  __shared__ Draw<kThreads> d;
-  const int64_t row = blockIdx.x;
+// A workgroup a part: all find the buckets in question for themselves and bring the words of their part
+// together; the last one to have written them answers.
+//
+// What they hand over goes through atomics of device scope, which are coherent over the chip by
+// themselves: every thread waits for its stores, then the workgroup adds itself to those that have
+// arrived.  (Fences would write back and discard the L2 caches: 165 us for 48 rows, all in all.)
+template <int DT> __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs g) {
+  __shared__ Draw<kDraw> d;
+  __shared__ uint32_t told;
+  const int part = blockIdx.x;
+  const int64_t row = blockIdx.y;
   const Asked asked(g, row);
   Sixteen own;
   if (threadIdx.x < 64)
     own.load(g.sums + row * kBuckets + threadIdx.x * 16, g.counts + row * kBuckets + threadIdx.x * 16);
   const Range range = range_of_parts(g, row);
-  if (settled<kThreads>(g, row, range, asked.t, d.whole))
+  if (!has_questions(range, asked.t)) {
+    if (part == 0)
+      settled<kDraw>(g, row, range, asked.t, d.whole);
     return;
+  }
   const Settings set(g, asked, range.largest());
   const Buckets buckets(set, range.least);
   if (threadIdx.x < 64)
-    ask_buckets<kThreads>(set, buckets, counts_words(g, asked.k), own, d);
+    ask_buckets<kDraw>(set, buckets, counts_words(g, asked.k), own, d);
   __syncthreads();
-  gather<kThreads, DT>(g, row, buckets, d);
-  answer<kThreads>(g, row, set, buckets, d.filled, d);
+  const int from = part * g.part_words, to = from + g.part_words < g.words ? from + g.part_words : g.words;
+  gather<kDraw, DT>(g, row, from, to, buckets, d);
+  constexpr uint32_t HERE = list_of(kDraw);
+  unsigned long long *const list = g.list + row * kList;
+  const uint32_t mine = (uint32_t)d.filled;
+  if (threadIdx.x == 0)
+    told = mine ? __hip_atomic_fetch_add(&g.filled[row], mine > HERE ? kList + 1 : mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+  __syncthreads();
+  const uint32_t first = told;
+  for (uint32_t i = threadIdx.x; i < mine && i < HERE && first + i < kList; i += kDraw)
+    __hip_atomic_store(&list[first + i],
+                       (unsigned long long)d.places[i] << 32 | __builtin_bit_cast(uint32_t, d.logits[i]), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup"); // (for the compiler)
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0)
+    told = __hip_atomic_fetch_add(&g.arrived[row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (told != (uint32_t)g.parts - 1)
+    return;
+  const uint32_t n = __hip_atomic_load(&g.filled[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (uint32_t i = threadIdx.x; i < n && i < HERE; i += kDraw) {
+    const unsigned long long v = __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    d.logits[i] = __builtin_bit_cast(float, (uint32_t)v), d.places[i] = (uint32_t)(v >> 32);
+  }
+  __syncthreads();
+  answer<kDraw>(g, row, set, buckets, (int)n, d, list);
 }
 
 // How rows are cut: parts that fill the chip, of 4096 words at least (one part: a workgroup a row).
@@ -1207,7 +1300,7 @@ static int validate(fhip_ctx *ctx, const fhip_sample_desc *d) {
 static bool side_by_side(const fhip_sample_desc &d) { return d.logits.stride[1] == 1 || d.logits.dim[1] == 1; }
 // Where things lie in the workspace, which begins with the parts' largest logits.
 struct Places {
-  size_t least, sums, counts, bytes;
+  size_t least, sums, counts, filled, list, bytes;
 };
 static Places places_of(const fhip_sample_desc &d) {
   Places p{};
@@ -1219,7 +1312,9 @@ static Places places_of(const fhip_sample_desc &d) {
   p.least = up(n * 8);
   p.sums = p.least + up(n * 4);
   p.counts = p.sums + (size_t)d.logits.dim[0] * kBuckets * 8;
-  p.bytes = p.counts + (size_t)d.logits.dim[0] * kBuckets * 4;
+  p.filled = p.counts + (size_t)d.logits.dim[0] * kBuckets * 4;
+  p.list = p.filled + up((size_t)d.logits.dim[0] * 8);
+  p.bytes = p.list + (size_t)d.logits.dim[0] * kList * 8;
   return p;
 }
 
@@ -1236,7 +1331,7 @@ template <int DT> static int launch(fhip_ctx *ctx, const SampleArgs &g) {
     const dim3 grid((unsigned)g.parts, (unsigned)g.rows);
     hipLaunchKernelGGL(sample_most_kernel<DT>, grid, dim3(kThreads), 0, ctx->stream, g);
     hipLaunchKernelGGL(sample_sums_kernel<DT>, grid, dim3(kThreads), 0, ctx->stream, g);
-    hipLaunchKernelGGL(sample_draw_kernel<DT>, dim3((unsigned)g.rows), dim3(kThreads), 0, ctx->stream, g);
+    hipLaunchKernelGGL(sample_draw_kernel<DT>, grid, dim3(kDraw), 0, ctx->stream, g);
   }
   FHIP_HIP_CHECK(ctx, hipGetLastError());
   return 0;
@@ -1290,6 +1385,7 @@ int fhip_sample(fhip_ctx *ctx, const fhip_sample_desc *d, const void *logits, co
     char *w = (char *)workspace;
     g.part_most = (uint64_t *)w, g.part_least = (float *)(w + at.least);
     g.sums = (unsigned long long *)(w + at.sums), g.counts = (uint32_t *)(w + at.counts);
+    g.filled = (uint32_t *)(w + at.filled), g.arrived = g.filled + g.rows, g.list = (unsigned long long *)(w + at.list);
     fhip_note_kernel(ctx, "sample parts=%d", c.parts);
     switch (g.dtype) {
     case FHIP_FLOAT: return launch<FHIP_FLOAT>(ctx, g);
