@@ -351,9 +351,10 @@ constexpr int kBuckets = 1024;
 constexpr int kThreads = 1024; // of the launches over parts
 // How many words of the buckets in question NT threads hold, and how many of them they sort.
 constexpr int list_of(int nt) { return nt == 64 ? 1024 : nt == 1024 ? 8192 : 4096; }
-constexpr int sorted_of(int nt) { return nt == 1024 ? 2048 : nt == 64 ? 256 : 2048; }
+constexpr int kOwn = 4; // of them in a thread
+constexpr int sorted_of(int nt) { return kOwn * nt; }
 constexpr int kDraw = 512; // threads of the launch that draws, if it is one of its own
-constexpr int kRanked = 512; // up to so many words a place is counted
+constexpr int kRanked = 256; // up to so many words a place is counted
 constexpr int kList = 8192; // words that its workgroups hand over, of a row
 
 // N words from `at` of a row whose words lie side by side, at element alignment.
@@ -865,80 +866,87 @@ __device__ __forceinline__ float logit_of_word(double v) {
 __device__ __forceinline__ int32_t place_of_word(double v) {
   return (int32_t)(~(uint32_t)(__builtin_bit_cast(uint64_t, v) >> 6) & 0xFFFFFFu);
 }
-template <int FAR> __device__ __forceinline__ void exchange(double &v, bool descending) {
-  const uint64_t own = __builtin_bit_cast(uint64_t, v);
-  const double w = __builtin_bit_cast(double, (uint64_t)other_lane<FAR>((uint32_t)(own >> 32)) << 32 | other_lane<FAR>((uint32_t)own));
-  v = (w > v) == (((threadIdx.x & FAR) == 0) == descending) ? w : v;
+__device__ __forceinline__ void exchange(double &larger, double &smaller) {
+  const double a = larger, b = smaller;
+  const bool turned = b > a;
+  larger = turned ? b : a, smaller = turned ? a : b;
 }
-
-// n words in descending order, words h * NT + thread in a thread (0 behind the last): a bitonic
-// network.  Exchanges at distances below 64 by DPP inside a wavefront, others through LDS (two places in
-// turn: one barrier each) or inside a thread; wavefronts in whose block nothing lies only keep the barriers.
-template <int NT, int E> __device__ __forceinline__ void sort_words(double (&v)[E], int n, double (*swap)[NT * E]) {
-  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t & ~63);
-  int turn = 0;
-#pragma clang loop unroll(disable)
-  for (int size = 2; size < 2 * n; size *= 2) {
-    auto used = [&](int h) { return ((h * NT + wave) & -size) < n; };
-#pragma clang loop unroll(disable)
-    for (int far = size / 2; far >= 64; far /= 2) {
-      if (far >= NT) {
+template <int FAR> __device__ __forceinline__ void exchange_lanes(double (&v)[kOwn]) {
 #pragma unroll
-        for (int gap = E / 2; gap > 0; gap /= 2)
-          if (far == gap * NT) {
-#pragma unroll
-            for (int h = 0; h < E; ++h)
-              if ((h & gap) == 0) {
-                const bool descending = ((h * NT + t) & size) == 0;
-                const double a = v[h], b = v[h + gap];
-                const bool swaps = (b > a) == descending;
-                v[h] = swaps ? b : a, v[h + gap] = swaps ? a : b;
-              }
-          }
-        continue;
-      }
-#pragma unroll
-      for (int h = 0; h < E; ++h)
-        if (used(h))
-          swap[turn][h * NT + t] = v[h];
-      __syncthreads();
-#pragma unroll
-      for (int h = 0; h < E; ++h)
-        if (used(h)) {
-          const double w = swap[turn][h * NT + (t ^ far)];
-          v[h] = (w > v[h]) == (((t & far) == 0) == (((h * NT + t) & size) == 0)) ? w : v[h];
-        }
-      turn ^= 1;
-    }
-#pragma unroll
-    for (int h = 0; h < E; ++h)
-      if (used(h)) {
-        const bool descending = ((h * NT + t) & size) == 0;
-        if (size > 32)
-          exchange<32>(v[h], descending);
-        if (size > 16)
-          exchange<16>(v[h], descending);
-        if (size > 8)
-          exchange<8>(v[h], descending);
-        if (size > 4)
-          exchange<4>(v[h], descending);
-        if (size > 2)
-          exchange<2>(v[h], descending);
-        exchange<1>(v[h], descending);
-      }
+  for (int h = 0; h < kOwn; ++h) {
+    const uint64_t own = __builtin_bit_cast(uint64_t, v[h]);
+    const double w = __builtin_bit_cast(double, (uint64_t)other_lane<FAR>((uint32_t)(own >> 32)) << 32 | other_lane<FAR>((uint32_t)own));
+    v[h] = (w > v[h]) == ((threadIdx.x & FAR) == 0) ? w : v[h];
   }
 }
 
-// The same of at most NT words, one in a thread: a word's place is how many are larger.  Shorter code
-// than the network's, which is what counts where few words make code run once; NT^2 comparisons in all.
-template <int NT, int ROOM> __device__ __forceinline__ void rank_words(double &v, int n, double (*swap)[ROOM]) {
+// n words in descending order, words kOwn * thread + h in a thread (0 behind the last): a bitonic network.
+// Where a block is to ascend its words change their sign meanwhile.  Exchanges at distances below
+// kOwn inside a thread, below 64 kOwn by DPP inside a wavefront, others through LDS (two places in turn: one
+// barrier each); wavefronts in whose block nothing lies only keep the barriers.
+template <int NT> __device__ __forceinline__ void sort_words(double (&v)[kOwn], int n, double (*swap)[NT * kOwn]) {
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t & ~63);
+  exchange(v[0], v[1]);
+  exchange(v[3], v[2]);
+  uint32_t signs = 0;
+  auto ascend = [&](uint32_t now) {
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h)
+      v[h] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, v[h]) ^ (uint64_t)(signs ^ now) << 32);
+    signs = now;
+  };
+  int turn = 0;
+#pragma clang loop unroll(disable)
+  for (int size = 4; size < 2 * n; size *= 2) {
+    const bool used = (wave * kOwn & -size) < n;
+    if (used)
+      ascend((t * kOwn & size) != 0 ? 0x80000000u : 0u);
+#pragma clang loop unroll(disable)
+    for (int far = size / 2; far >= 64 * kOwn; far /= 2) {
+      if (used)
+#pragma unroll
+        for (int h = 0; h < kOwn; ++h)
+          swap[turn][h * NT + t] = v[h];
+      __syncthreads();
+      if (used)
+#pragma unroll
+        for (int h = 0; h < kOwn; ++h) {
+          const double w = swap[turn][h * NT + (t ^ far / kOwn)];
+          v[h] = (w > v[h]) == ((t * kOwn & far) == 0) ? w : v[h];
+        }
+      turn ^= 1;
+    }
+    if (used) {
+      if (size > 32 * kOwn)
+        exchange_lanes<32>(v);
+      if (size > 16 * kOwn)
+        exchange_lanes<16>(v);
+      if (size > 8 * kOwn)
+        exchange_lanes<8>(v);
+      if (size > 4 * kOwn)
+        exchange_lanes<4>(v);
+      if (size > 2 * kOwn)
+        exchange_lanes<2>(v);
+      if (size > kOwn)
+        exchange_lanes<1>(v);
+      exchange(v[0], v[2]);
+      exchange(v[1], v[3]);
+      exchange(v[0], v[1]);
+      exchange(v[2], v[3]);
+    }
+  }
+  ascend(0);
+}
+
+// The same of at most NT words, one in a thread (to swap[1]): a word's place is how many are larger.  Shorter code
+// than the network's, which is what counts where few words make code run once.
+template <int NT, int ROOM> __device__ __forceinline__ void rank_words(double v, int n, double (*swap)[ROOM]) {
   typedef double Two __attribute__((ext_vector_type(2)));
   constexpr int STEP = 8;
   const int t = threadIdx.x;
-  const bool used = __builtin_amdgcn_readfirstlane(t & ~63) < n;
   swap[0][t] = v; // (zeros behind the last)
   __syncthreads();
-  if (used) {
+  if (__builtin_amdgcn_readfirstlane(t & ~63) < n) {
     int larger = 0;
     for (int i = 0; i < n; i += STEP)
 #pragma unroll
@@ -951,8 +959,6 @@ template <int NT, int ROOM> __device__ __forceinline__ void rank_words(double &v
       swap[1][larger] = v;
   }
   __syncthreads();
-  if (used)
-    v = t < n ? swap[1][t] : 0.0;
 }
 
 // The token of a row, from words that registers hold: in order, with their sums next to them, they answer
@@ -960,59 +966,78 @@ template <int NT, int ROOM> __device__ __forceinline__ void rank_words(double &v
 template <int NT>
 __device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets,
                                               int n, Draw<NT> &d) {
-  constexpr int E = sorted_of(NT) / NT, WAVES = NT / 64;
   const int t = threadIdx.x, l = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  double v[E];
+  double v[kOwn];
+  if (n <= kRanked && n <= NT) {
+    const double own = t < n ? word_of(d.logits[t], d.places[t]) : 0.0;
+    __syncthreads(); // (the words to sort lie where the list does)
+    rank_words<NT>(own, n, d.swap);
 #pragma unroll
-  for (int h = 0; h < E; ++h) {
-    const int i = h * NT + t;
-    v[h] = i < n ? word_of(d.logits[i], d.places[i]) : 0.0;
-  }
-  __syncthreads(); // (the exchanges lie where the list does)
-  if (n <= kRanked && n <= NT)
-    rank_words<NT>(v[0], n, d.swap);
-  else
-    sort_words<NT, E>(v, n, d.swap);
-  // sums up to each word of the list, then of the row: a bucket's begin at its first word
-  auto each = [&](auto take) {
+    for (int h = 0; h < kOwn; ++h)
+      v[h] = t * kOwn + h < n ? d.swap[1][t * kOwn + h] : 0.0;
+  } else {
 #pragma unroll
-    for (int h = 0; h < E; ++h)
-      if (h * NT + wave * 64 < n)
-        take(h, h * NT + t);
-  };
-  uint64_t weight[E], up_to[E];
-  float x[E];
-  int home[E];
-  uint32_t rank[E];
-  __syncthreads();
-  each([&](int h, int i) {
-    x[h] = logit_of_word(v[h]);
-    weight[h] = v[h] > 0.0 ? set.held(x[h]) : 0;
-    home[h] = v[h] > 0.0 ? buckets.of(x[h]) : kBuckets;
-    up_to[h] = sum_up_to_lane(weight[h]);
-    if (l == 63)
-      d.bins.sum[h * WAVES + wave] = up_to[h];
-    d.swap[0][i] = home[h];
-  });
-  __syncthreads();
-  each([&](int h, int i) {
-    for (int w = 0; w < h * WAVES + wave; ++w)
-      up_to[h] += d.bins.sum[w];
-    if (v[h] > 0.0 && (i == 0 || (int)d.swap[0][i - 1] != home[h])) {
-      d.f.before[bucket_place(home[h])] -= up_to[h] - weight[h]; // (unsigned: wraps and wraps back)
-      d.f.first[bucket_place(home[h])] -= (uint32_t)i;
+    for (int h = 0; h < kOwn; ++h) {
+      const int i = t * kOwn + h;
+      v[h] = i < n ? word_of(d.logits[i], d.places[i]) : 0.0;
     }
-  });
+    __syncthreads();
+    sort_words<NT>(v, n, d.swap);
+  }
+  // sums up to each word of the list, then of the row: a bucket's begin at its first word
+  const bool used = wave * 64 * kOwn < n;
+  uint64_t weight[kOwn], up_to[kOwn], sum = 0;
+  float x[kOwn];
+  int home[kOwn];
+  __syncthreads();
+  if (used) {
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+      const bool mine = v[h] > 0.0;
+      x[h] = logit_of_word(v[h]);
+      weight[h] = mine ? set.held(x[h]) : 0;
+      home[h] = mine ? buckets.of(x[h]) : kBuckets;
+      up_to[h] = sum += weight[h];
+    }
+    sum = sum_up_to_lane(sum);
+    if (l == 63)
+      d.bins.sum[wave] = sum;
+    d.swap[0][t] = home[kOwn - 1];
+  }
+  __syncthreads();
+  if (used) {
+    sum -= up_to[kOwn - 1];
+    for (int w = 0; w < wave; ++w)
+      sum += d.bins.sum[w];
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+      up_to[h] += sum;
+      const int before = h > 0 ? home[h > 0 ? h - 1 : 0] : t > 0 ? (int)d.swap[0][t - 1] : -1;
+      if (home[h] < kBuckets && before != home[h]) {
+        d.f.before[bucket_place(home[h])] -= up_to[h] - weight[h]; // (unsigned: wraps and wraps back)
+        d.f.first[bucket_place(home[h])] -= (uint32_t)(t * kOwn + h);
+      }
+    }
+  }
   __syncthreads();
   const int least_from = d.f.least_from, least_to = d.f.least_to, by_k = d.f.by_k;
-  each([&](int h, int i) {
+  // (those behind the last word end nothing: their weight is 0)
+  auto each = [&](auto take) {
+    if (used)
+#pragma unroll
+      for (int h = 0; h < kOwn; ++h)
+        take(h);
+  };
+  each([&](int h) {
+    if (home[h] == kBuckets)
+      return;
     up_to[h] += d.f.before[bucket_place(home[h])];
-    rank[h] = d.f.first[bucket_place(home[h])] + (uint32_t)i;
-    if (v[h] > 0.0 && by_k >= 0 && rank[h] + 1 == (uint32_t)set.k)
+    const uint32_t rank = d.f.first[bucket_place(home[h])] + (uint32_t)(t * kOwn + h);
+    if (by_k >= 0 && rank + 1 == (uint32_t)set.k)
       d.kept[0] = up_to[h];
   });
   // whoever ends a prefix says so
-  auto ends = [&](int h, uint64_t need) { return v[h] > 0.0 && up_to[h] - weight[h] < need && need <= up_to[h]; };
+  auto ends = [&](int h, uint64_t need) { return up_to[h] - weight[h] < need && need <= up_to[h]; };
   uint64_t kept = d.f.all;
   if (by_k >= 0) {
     __syncthreads();
@@ -1020,7 +1045,7 @@ __device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, 
   }
   if (set.p < 1.f) {
     const uint64_t need = set.share(kept);
-    each([&](int h, int) {
+    each([&](int h) {
       if (ends(h, need))
         d.kept[1] = up_to[h];
     });
@@ -1029,19 +1054,23 @@ __device__ __forceinline__ void answer_sorted(const SampleArgs &g, int64_t row, 
   }
   if (set.least > 0.f && least_from < kBuckets) {
     // (the largest sum among them, or what lies in front of their buckets)
-    each([&](int h, int) {
-      const bool large = v[h] > 0.0 && home[h] >= least_from && home[h] <= least_to && set.weight(x[h]) >= least_bound(set);
-      const uint64_t most = largest_of_wave<uint64_t>(large ? up_to[h] : 0);
+    uint64_t most = 0;
+    each([&](int h) {
+      if (home[h] >= least_from && home[h] <= least_to && set.weight(x[h]) >= least_bound(set))
+        most = up_to[h];
+    });
+    if (used) {
+      most = largest_of_wave<uint64_t>(most);
       if (l == 0 && most)
         atomicMax((unsigned long long *)&d.kept[2], (unsigned long long)most);
-    });
+    }
     __syncthreads();
     kept = d.kept[2] < kept ? d.kept[2] : kept;
   }
   if (set.least > 1.f)
     kept = (uint64_t)1 << set.bits;
   const uint64_t need = set.below(kept) + 1;
-  each([&](int h, int) {
+  each([&](int h) {
     if (ends(h, need)) {
       g.token[row] = place_of_word(v[h]);
       if (g.probability)
