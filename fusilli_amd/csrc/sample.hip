@@ -338,15 +338,21 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs g) 
 
 // ---- rows whose words lie side by side ------------------------------------------------------
 // Three steps: the largest logit; sums of weights in 1024 buckets of equal width in (m - l) / T; then
-// the buckets in which the prefixes can end, their words brought together in LDS and the
-// questions answered there as above.  The buckets' sums are exact, so are the prefixes.  One workgroup
-// takes all steps of a row where rows fill the chip or are short; otherwise the first two are launches
-// over parts of rows.
+// the buckets in which the prefixes can end, their words brought together in LDS, put in order there, and
+// every question answered by the word whose sum says so.  The buckets' sums are exact, so are the prefixes.
+// One workgroup takes all steps of a row where rows fill the chip or are short; otherwise they are three
+// launches over parts of rows, the last part of a row answering.
 //
-// Buckets cover what words have above a weight of 0, less than 32 of (m - l) / T.
+// Buckets cover what words have above a weight of 0, less than 32 of (m - l) / T.  Which of them matter one
+// wavefront finds, without a barrier: sixteen that execute the same few hundred instructions
+// between barriers take three times as long.
 //
-// Which buckets matter one wavefront finds, without a barrier: sixteen that execute the same few hundred
-// instructions between barriers take three times as long.
+// Bound by memory (three walks, of which caches feed the last two) and by f64 arithmetic, 30 instructions a
+// word, where rows are many: f32 256 x 131072, 134 MB, 97 us, of it 28 for the largest logits (4.8 TB/s), 39 for
+// the sums (20 without the exponentials), 16 for bringing together; by what runs once where they are few: code
+// that no cache holds yet, loads that wait for each other, three launches.  1 x 65536 16.4 us, bf16 48 x 131072
+// 40 us (launches 6.6, 12 and 21, of which putting 1300 words of its flattest row in order takes 10), f16
+// 7 x 100003 22, f32 25 x 536 10.
 constexpr int kBuckets = 1024;
 constexpr int kThreads = 1024; // of the launches over parts
 // How many words of the buckets in question NT threads hold, and how many of them they sort.
@@ -1297,11 +1303,14 @@ template <int DT> __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel
   answer<kDraw>(g, row, set, buckets, (int)n, d, list);
 }
 
-// How rows are cut: parts that fill the chip, of 4096 words at least (one part: a workgroup a row).
+// How rows are cut: a workgroup a row where rows are short or fill the chip, otherwise parts that do, of
+// 4096 words at least.  us, one part / parts: bf16 33 x 16384 17.2 / 20.9 (four), f32 4 x 8192 13.7 / 17.9;
+// f32 130 x 131072 80 / 67 (four), 256 x 131072 94 / 108 (two), bf16 257 x 32000 31 / 40.
+constexpr int64_t kFull = 192, kShort = 20480;
 struct Cut {
   int parts, words;
   Cut(int64_t rows, int64_t row_words) {
-    int64_t n = rows >= 128 ? 1 : 512 / rows;
+    int64_t n = rows >= kFull || row_words <= kShort ? 1 : (512 + rows - 1) / rows;
     const int64_t most = (row_words + 4095) / 4096;
     n = n < most ? n : most;
     n = n < 32 ? n : 32;
@@ -1356,7 +1365,7 @@ template <int DT> static int launch(fhip_ctx *ctx, const SampleArgs &g) {
       hipLaunchKernelGGL((sample_whole_kernel<256, DT>), grid, dim3(256), 0, ctx->stream, g);
     else
       hipLaunchKernelGGL((sample_whole_kernel<1024, DT>), grid, dim3(1024), 0, ctx->stream, g);
-  } else { // (fewer than 128 rows)
+  } else { // (fewer than kFull rows)
     const dim3 grid((unsigned)g.parts, (unsigned)g.rows);
     hipLaunchKernelGGL(sample_most_kernel<DT>, grid, dim3(kThreads), 0, ctx->stream, g);
     hipLaunchKernelGGL(sample_sums_kernel<DT>, grid, dim3(kThreads), 0, ctx->stream, g);

@@ -3,6 +3,7 @@ f32 steps where the formula says so), and the bounds that their roundings allow.
 from __future__ import annotations
 
 import numpy as np
+import torch  # noqa: F401 (before the library, which then shares its runtime)
 
 from fusilli_amd import capi
 
@@ -40,7 +41,7 @@ def front(x, kind, weight=None, up=None, eps=1e-6):
         return y, ((k / 64 + 12) / 2 + 6) * UNIT
     if kind == "SWISH_GATE":
         # exp is good to 2 steps of 2^-23, the sum, the quotient (2 steps of 2^-23) and the product round once each
-        with np.errstate(over="ignore"):
+        with np.errstate(over="ignore", invalid="ignore"):
             return x / (1.0 + np.exp(-x)) * np.asarray(up, np.float64), 12 * UNIT
     return x, 0.0
 

@@ -1,6 +1,7 @@
 """Rows in 8-bit codes, products of codes and tokens from logits against their formulas in 64 bits, through the C ABI."""
 import numpy as np
 import pytest
+import torch  # (before the library, which then shares its runtime)
 
 from fusilli_amd import capi
 from helpers import HT
@@ -29,7 +30,7 @@ def quantize(ctx, x, kind="NONE", weight=None, up=None, eps=1e-6, q_strides=None
         d.has_weight, d.weight_dtype, d.weight_stride = 1, weight.dtype, weight.strides[0]
     if up is not None:
         d.up = up.desc()
-    held = k <= 32768 and all(k == 1 or t.strides[-1] == 1 for t in (x, up, weight, q) if t is not None)
+    held = k <= 32768 and rows < 2 ** 21 and all(k == 1 or t.strides[-1] == 1 for t in (x, up, weight, q) if t is not None)
     assert ctx.lib.fhip_quantize_rows_supported(d) == (2 if held else 1)
     bx, px, _ = guarded(ctx, x.storage, x_shift)
     bu, pu, _ = guarded(ctx, up.storage, x_shift) if up is not None else (None, None, None)
@@ -354,12 +355,13 @@ def settings(rng, rows, words):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAME.get)
 @pytest.mark.parametrize("rows,words", [(1, 1), (3, 2), (40, 63), (9, 64), (33, 500), (5, 1025), (3, 4099), (4, 32000), (1, 70001),
-                                        (2, 131072), (300, 200), (260, 5000), (130, 9000), (127, 4100)])
+                                        (2, 131072), (300, 200), (260, 5000), (130, 9000), (127, 4100), (150, 21000),
+                                        (2, 1024), (2, 8192), (2, 8193), (3, 20480), (3, 20481), (1, 1000003)])
 def test_sample(ctx, dtype, rows, words):
     rng = rng_of(13, rows, words, dtype)
     x = HT.from_logical(rng.normal(size=[rows, words]) * rng.choice([0.3, 1.5, 4.0], [rows, 1]), dtype)
     check_tokens(ctx, x, rng.random(rows).astype(np.float32), *settings(rng, rows, words), fast=True)
-    parts = max(1, min(512 // rows if rows < 128 else 1, (words + 4095) // 4096, 32))
+    parts = 1 if rows >= 192 or words <= 20480 else min(-(-512 // rows), -(-words // 4096), 32)
     assert ctx.last_kernel() == f"sample parts={parts}"
 
 
@@ -396,7 +398,7 @@ def test_sample_equal_logits(ctx, words):
         check_tokens(ctx, x, np.full(n, u, np.float32), t, k, p, np.tile([0.0, 0.0, 0.0, 0.0, 0.9, 0.0], 8))
 
 
-@pytest.mark.parametrize("words", [4, 300, 20000])
+@pytest.mark.parametrize("words", [4, 300, 5000, 20000, 24000])
 def test_sample_masked_rows(ctx, words):
     """NaN and -inf are never drawn; rows of nothing else have no token; infinities outweigh all."""
     rng = rng_of(16, words)
@@ -416,6 +418,159 @@ def test_sample_masked_rows(ctx, words):
         u = rng.random(10).astype(np.float32)
         check_tokens(ctx, x, u, np.full(10, [1.0, 0.0, 0.7, 2.0][i]), np.full(10, [0, 5, 2, 0][i]), np.full(10, [1.0, 0.9, 0.5, 0.99][i]),
                      np.full(10, [0.0, 0.1, 0.0, 1.0][i]))
+
+
+@pytest.mark.parametrize("rows,words", [(3, 900), (2, 6000), (2, 18000), (2, 40000), (1, 150000)])
+def test_sample_many_words_in_question(ctx, rows, words):
+    """Logits so close together, or one so far above, that the words in question are hundreds, thousands or all: each way
+    of ordering them, lists that LDS does not hold and rows that no list holds."""
+    rng = rng_of(20, rows, words)
+    values = rng.normal(size=[rows, words])
+    for i in range(rows):
+        if i % 3 == 0:
+            values[i] *= 1e-3
+            values[i, words // 3] = [31.0, 8.0, 2.0][i // 3 % 3]
+        elif i % 3 == 1:
+            values[i] = np.round(values[i] * 4) / 4
+        else:
+            values[i, :words // 2] *= 0.01
+    x = HT.from_logical(values, F32)
+    for j in range(3):
+        u = rng.random(rows).astype(np.float32)
+        k, p = np.full(rows, [words // 2, 0, words // 3][j]), np.full(rows, [1.0, 0.7, 0.8][j])
+        check_tokens(ctx, x, u, np.full(rows, [1.0, 1.0, 4.0][j]), k, p, np.full(rows, [0.0, 0.0, 0.01][j]))
+
+
+@pytest.mark.parametrize("n", [3, 60, 130, 255, 257, 500, 1000, 1500, 2047, 2049, 3900, 4100, 8000, 8200, 9000])
+@pytest.mark.parametrize("words", [24000, 18000])
+def test_sample_words_in_question(ctx, words, n):
+    """Exactly n words near each other below one that is far above, and nothing else to draw."""
+    rng = rng_of(21, words, n)
+    values = np.full([2, words], -np.inf)
+    for row in values:
+        at = rng.choice(words, n + 1, replace=False)
+        row[at] = rng.permutation(n + 1) * (1e-3 / n)
+        row[at[0]] = 12.0
+    x = HT.from_logical(values, F32)
+    for u in (0.1, 0.37, 0.99):
+        check_tokens(ctx, x, np.full(2, u, np.float32), np.full(2, 1.5), np.array([0, n // 2]), np.array([0.9, 1.0]), np.zeros(2))
+
+
+def test_sample_many_rows(ctx):
+    """More rows than a grid has workgroups of a row each."""
+    rows = 2 ** 21 + 5
+    x = HT.from_logical(np.tile(np.float32([[0.0, 1.0]]), [rows, 1]), F32)
+    got, chance = sample(ctx, x, np.tile(np.float32([0.7, 0.8]), rows // 2 + 1)[:rows])
+    # (1 weighs 1 and comes first, 0 weighs 1 / e: the first up to 0.731)
+    assert (got[::2] == 1).all() and (got[1::2] == 0).all()
+    assert np.allclose(chance[::2], 1 / (1 + np.exp(-1.0)), rtol=2e-7)
+
+
+def test_quantize_many_rows(ctx):
+    rows = 2 ** 21 + 3
+    q, s = quantize(ctx, HT.from_logical(np.tile(np.float32([[3.0], [-5.0], [0.0]]), [rows // 3 + 1, 1])[:rows], F32))
+    assert (q[0::3] == 127).all() and (q[1::3] == -127).all() and (q[2::3] == 0).all()
+    assert (s[0::3] == np.float32(3) / np.float32(127)).all() and (s[2::3] == 0).all()
+
+
+# ---- streams, graphs, calls side by side -------------------------------------------------
+def serving_step(c, dev, seed, rows=24, k=1024, hidden=2048, words=32768):
+    """Norm, codes, product; gate, codes, product onto words; tokens.  -> (run on a context, check)"""
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    randn = lambda *s: torch.randn(*s, generator=gen, device=dev)
+    x = randn(rows, k).to(torch.bfloat16)
+    w1 = torch.randint(-127, 128, (2 * hidden, k), generator=gen, device=dev, dtype=torch.int8)
+    w2 = torch.randint(-127, 128, (words, hidden), generator=gen, device=dev, dtype=torch.int8)
+    s1, s2 = torch.full((2 * hidden,), 4e-4, device=dev), torch.full((words,), 2e-3, device=dev)
+    u = torch.rand(rows, generator=gen, device=dev)
+    q1, q2 = (torch.empty(rows, n, dtype=torch.int8, device=dev) for n in (k, hidden))
+    a1, a2 = (torch.empty(rows, device=dev) for _ in range(2))
+    mid, logits = torch.empty(rows, 2 * hidden, dtype=torch.bfloat16, device=dev), torch.empty(rows, words, device=dev)
+    token, chance = torch.empty(rows, dtype=torch.int32, device=dev), torch.empty(rows, device=dev)
+    T = capi.TensorDesc.make
+    n1, n2 = capi.QuantizeRowsDesc(), capi.QuantizeRowsDesc()
+    n1.x, n1.q, n1.scale_stride, n1.front, n1.epsilon = T([rows, k], [k, 1], BF16), T([rows, k], [k, 1], capi.INT8), 1, \
+        capi.QUANTIZE_FRONT["RMSNORM"], 1e-5
+    n2.x, n2.q, n2.scale_stride, n2.front = T([rows, hidden], [2 * hidden, 1], BF16), T([rows, hidden], [hidden, 1], capi.INT8), 1, \
+        capi.QUANTIZE_FRONT["SWISH_GATE"]
+    n2.up = T([rows, hidden], [2 * hidden, 1], BF16)
+    m1, m2 = capi.MatmulQuantizedDesc(), capi.MatmulQuantizedDesc()
+    for m, kk, nn, t in ((m1, k, 2 * hidden, BF16), (m2, hidden, words, F32)):
+        m.a, m.b, m.c = T([rows, kk], [kk, 1], capi.INT8), T([kk, nn], [1, kk], capi.INT8), T([rows, nn], [nn, 1], t)
+        m.out, m.out_dtype, m.a_scale_stride, m.b_scale_stride = m.c, t, 1, 1
+    d = capi.SampleDesc()
+    d.logits, d.temperature, d.top_k, d.top_p = T([rows, words], [words, 1], F32), 0.9, 50, 0.95
+    work = torch.empty(c.sample_workspace(d), dtype=torch.uint8, device=dev)
+
+    def run():
+        c.quantize_rows(n1, x.data_ptr(), q1.data_ptr(), a1.data_ptr())
+        c.matmul_quantized(m1, q1.data_ptr(), w1.data_ptr(), a1.data_ptr(), s1.data_ptr(), mid.data_ptr())
+        c.quantize_rows(n2, mid.data_ptr(), q2.data_ptr(), a2.data_ptr(), up=mid.data_ptr() + 2 * hidden)
+        c.matmul_quantized(m2, q2.data_ptr(), w2.data_ptr(), a2.data_ptr(), s2.data_ptr(), logits.data_ptr())
+        c.sample(d, logits.data_ptr(), u.data_ptr(), token.data_ptr(), probability=chance.data_ptr(), workspace=work.data_ptr())
+
+    def check():
+        codes, scale = q1.cpu().numpy(), a1.cpu().numpy()
+        check_codes(codes, scale, *front(x.float().cpu().numpy(), "RMSNORM", eps=1e-5))
+        middle = mid.float().cpu().numpy()
+        check_product(middle, *product(codes, w1.cpu().numpy().T, scale, s1.cpu().numpy()), BF16)
+        y, rel = front(middle[:, :hidden], "SWISH_GATE", up=middle[:, hidden:])
+        check_codes(q2.cpu().numpy(), a2.cpu().numpy(), y, rel)
+        l = logits.cpu().numpy()
+        check_product(l, *product(q2.cpu().numpy(), w2.cpu().numpy().T, a2.cpu().numpy(), s2.cpu().numpy()), F32)
+        want, expected = tokens(l, u.cpu().numpy(), [0.9] * rows, [50] * rows, [0.95] * rows, [0.0] * rows)
+        assert np.array_equal(token.cpu().numpy(), want)
+        assert np.allclose(chance.cpu().numpy(), expected, rtol=2e-7, atol=1e-10)
+
+    def change(seed):
+        gen.manual_seed(seed)
+        x.copy_(randn(rows, k))
+        u.copy_(torch.rand(rows, generator=gen, device=dev))
+    return run, check, change
+
+
+def test_step_on_a_stream_and_captured(ctx):
+    """The operators one after another as a decoder uses them: on a stream of the caller's, then captured and replayed with
+    other inputs, with other work between the replays."""
+    dev = torch.device("cuda")
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        c = capi.Context(torch.cuda.current_device(), stream.cuda_stream)
+        run, check, change = serving_step(c, dev, 31)
+        stream.synchronize()
+        run()
+        stream.synchronize()
+        check()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            run()
+        for i in range(4):
+            change(40 + i)
+            graph.replay()
+            stream.synchronize()
+            check()
+            run()  # eager work between, of the same operators
+            torch.randn(512, 512, device=dev).sum()
+            stream.synchronize()
+            check()
+
+
+def test_two_steps_at_once(ctx):
+    """Two contexts on streams of their own, with workspaces of their own, side by side."""
+    dev = torch.device("cuda")
+    steps = []
+    for i in range(2):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            c = capi.Context(torch.cuda.current_device(), stream.cuda_stream)
+            steps.append((c, stream, *serving_step(c, dev, 50 + i, rows=5 + 40 * i)))
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for _, _, run, _, _ in steps:
+            run()
+    torch.cuda.synchronize()
+    for _, _, _, check, _ in steps:
+        check()
 
 
 def test_sample_settings_at_their_ends(ctx):
