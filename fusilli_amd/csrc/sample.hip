@@ -1335,7 +1335,10 @@ static int validate(fhip_ctx *ctx, const fhip_sample_desc *d) {
   return 0;
 }
 
-static bool side_by_side(const fhip_sample_desc &d) { return d.logits.stride[1] == 1 || d.logits.dim[1] == 1; }
+// (a grid's threads are a number below 2^32)
+static bool side_by_side(const fhip_sample_desc &d) {
+  return (d.logits.stride[1] == 1 || d.logits.dim[1] == 1) && d.logits.dim[0] < (1 << 21);
+}
 // Where things lie in the workspace, which begins with the parts' largest logits.
 struct Places {
   size_t least, sums, counts, filled, list, bytes;
@@ -1417,7 +1420,7 @@ int fhip_sample(fhip_ctx *ctx, const fhip_sample_desc *d, const void *logits, co
   g.bits = 0;
   while (g.bits < 46 && ((int64_t)g.words << (g.bits + 1)) <= (1ll << 62))
     ++g.bits;
-  if (side_by_side(*d) && g.rows < (1 << 21)) { // (a grid's threads are a number below 2^32)
+  if (side_by_side(*d)) {
     const Cut c(g.rows, g.words);
     g.parts = c.parts, g.part_words = c.words;
     char *w = (char *)workspace;

@@ -596,7 +596,8 @@ int fhip_matmul_quantized(fhip_ctx *ctx, const fhip_matmul_quantized_desc *d,
  * are vectors of `rows` elements on the device or, where there is none, the
  * descriptor's.  At most 2^24 words.  Needs 256-byte aligned workspace of
  * fhip_sample_workspace_size bytes; it holds nothing between calls, and calls that
- * overlap need one each.  supported: 2 for a last stride of 1; otherwise 1. */
+ * overlap need one each.  supported: 2 for a last stride of 1 and fewer than 2^21
+ * rows; otherwise 1. */
 typedef struct {
   fhip_tensor_desc logits; /* [rows, words] f32, bf16 or f16 */
   int32_t has_temperature, has_top_k, has_top_p, has_min_p;

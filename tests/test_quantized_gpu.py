@@ -1,4 +1,6 @@
 """Rows in 8-bit codes, products of codes and tokens from logits against their formulas in 64 bits, through the C ABI."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch  # (before the library, which then shares its runtime)
@@ -456,11 +458,48 @@ def test_sample_words_in_question(ctx, words, n):
         check_tokens(ctx, x, np.full(2, u, np.float32), np.full(2, 1.5), np.array([0, n // 2]), np.array([0.9, 1.0]), np.zeros(2))
 
 
+def test_calls_are_refused(ctx):
+    """What a descriptor does not show: missing pointers, settings without their vector, small or unaligned workspace."""
+    d = capi.SampleDesc()
+    d.logits, d.temperature, d.top_p = capi.TensorDesc.make([2, 30000], [30000, 1], F32), 1.0, 1.0
+    x, u = ctx.to_device(np.zeros([2, 30000], np.float32)), ctx.to_device(np.zeros(2, np.float32))
+    _, tok, tokens_back = guarded(ctx, np.full(2, -9, np.int32))
+    need = ctx.sample_workspace(d)
+    room = ctx.alloc(need + 512)
+    at = room.ptr + -room.ptr % 256
+
+    def call(logits=x.ptr, uniform=u.ptr, t=None, token=tok, work=at, size=need):
+        return ctx.lib.fhip_sample(ctx.handle, ctypes.byref(d), logits, uniform, t, None, None, None, token, None, work, size)
+    for bad in (dict(logits=None), dict(uniform=None), dict(token=None), dict(t=u.ptr), dict(work=None), dict(work=at + 64), dict(size=need - 1)):
+        assert call(**bad) != 0, bad
+        said = ctx.lib.fhip_last_error(ctx.handle).decode()
+        assert "fhip_sample" in said and ("workspace" in said) == bool({"work", "size"} & set(bad)), said
+    d.has_top_k = 1
+    assert call() != 0
+    d.has_top_k = 0
+    ctx.sync()
+    assert (tokens_back() == -9).all()
+    assert call() == 0
+    assert (tokens_back() == 0).all()
+
+    q = capi.QuantizeRowsDesc()
+    q.x, q.q, q.scale_stride = capi.TensorDesc.make([2, 64], [64, 1], F32), capi.TensorDesc.make([2, 64], [64, 1], capi.INT8), 1
+    _, codes, codes_back = guarded(ctx, np.full([2, 64], 5, np.int8))
+    run = lambda x, q_, s, up=None, w=None: ctx.lib.fhip_quantize_rows(  # noqa: E731
+        ctx.handle, ctypes.byref(q), x, up, w, q_, s, None, 0)
+    for bad in ((None, codes, u.ptr), (x.ptr, None, u.ptr), (x.ptr, codes, None), (x.ptr, codes, u.ptr, x.ptr), (x.ptr, codes, u.ptr, None, x.ptr)):
+        assert run(*bad) != 0 and "fhip_quantize_rows" in ctx.lib.fhip_last_error(ctx.handle).decode()
+    ctx.sync()
+    assert (codes_back() == 5).all()
+    assert run(x.ptr, codes, u.ptr) == 0 and (codes_back() == 0).all()
+
+
 def test_sample_many_rows(ctx):
     """More rows than a grid has workgroups of a row each."""
     rows = 2 ** 21 + 5
     x = HT.from_logical(np.tile(np.float32([[0.0, 1.0]]), [rows, 1]), F32)
     got, chance = sample(ctx, x, np.tile(np.float32([0.7, 0.8]), rows // 2 + 1)[:rows])
+    assert ctx.last_kernel() == "sample_rows"
     # (1 weighs 1 and comes first, 0 weighs 1 / e: the first up to 0.731)
     assert (got[::2] == 1).all() and (got[1::2] == 0).all()
     assert np.allclose(chance[::2], 1 / (1 + np.exp(-1.0)), rtol=2e-7)
