@@ -309,9 +309,10 @@ __device__ __forceinline__ void direct_coord(int q, int *m, int *dm, int *n) {
 // Finishes and stores N values of column n, value i at row rows[i] (all values of
 // a thread together: a fused operand's loads are then one round trip, not one per
 // four values -- a bias on 64 x 64 tiles cost 6 us).
+// `early`: the rows' and the column's scale, if they are there already.
 template <typename Acc, int N, bool SCALED = false>
 __device__ __forceinline__ void direct_store(const DirectArgs &g, int64_t batch, const int (&row)[N], int n,
-                                             const Acc (&acc)[N]) {
+                                             const Acc (&acc)[N], const float (*early)[N + 1] = nullptr) {
   if (n >= g.N)
     return;
   int64_t at[N], rows[N];
@@ -330,10 +331,10 @@ __device__ __forceinline__ void direct_store(const DirectArgs &g, int64_t batch,
   } else {
     float v[N];
     if constexpr (SCALED) {
-      const float column = g.scales.column(n), bias = g.scales.bias_of(n);
+      const float column = early ? (*early)[N] : g.scales.column(n), bias = g.scales.bias_of(n);
 #pragma unroll
       for (int r = 0; r < N; ++r)
-        v[r] = g.scales.row(rows[r]);
+        v[r] = early ? (*early)[r] : g.scales.row(rows[r]);
 #pragma unroll
       for (int r = 0; r < N; ++r)
         v[r] = fhip_scaled(acc[r], v[r], column, bias);
@@ -397,6 +398,21 @@ __attribute__((amdgpu_waves_per_eu(
   OB ob;
   oa.setup(g.a + batch * g.a_batch * D::ELEM, g.a_ldb, m0, g.M, (int64_t)s0 * D::SK, lds0);
   ob.setup(g.b + batch * g.b_batch * D::ELEM, g.b_ldb, n0, g.N, (int64_t)s0 * D::SK, lds0 + OA::LDS);
+  // A thread's scales, requested ahead of everything else: behind the sums they are a round trip of their own
+  // (us, so / there: M1 N2560 K2048 into f16 4.6 / 5.0, M16 N4096 K4096 7.0 / 7.4).  For 16 x 16 tiles, of which there
+  // are few: thousands of workgroups hide it (M5 N131072 K4096 in 16 x 32 91.7 / 90.2).
+  constexpr bool EARLY = KIND == GK_I8S && MT * NT == 1;
+  float early[EARLY ? 5 : 1];
+  if (EARLY && threadIdx.x < F / 4 && !g.partial) {
+    int m, dm, n;
+    direct_coord<A_KC, B_KC, MT, NT>(threadIdx.x, &m, &dm, &n);
+    early[EARLY ? 4 : 0] = g.scales.column(n0 + n < g.N ? n0 + n : g.N - 1);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = m0 + m + r * dm;
+      early[EARLY ? r : 0] = g.scales.row(row < g.M ? row : g.M - 1);
+    }
+  }
   typename D::Acc4 acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -496,8 +512,12 @@ __attribute__((amdgpu_waves_per_eu(
     for (int r = 0; r < 4; ++r)
       row[e * 4 + r] = m0 + m + r * dm, vals[e * 4 + r] = v[r];
   }
-  if (!g.partial)
-    direct_store<Acc, PER * 4, KIND == GK_I8S>(g, batch, row, n0 + n, vals);
+  if (!g.partial) {
+    if constexpr (EARLY)
+      direct_store<Acc, 4, true>(g, batch, row, n0 + n, vals, &early);
+    else
+      direct_store<Acc, PER * 4, KIND == GK_I8S>(g, batch, row, n0 + n, vals);
+  }
 }
 
 // Adds the split parts of every tile in order and finishes as above.
