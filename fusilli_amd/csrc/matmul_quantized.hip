@@ -6,7 +6,7 @@
 // that a split of K adds whole numbers and changes no result.  Bound by the matrix pipes from a few hundred rows on
 // (4096 x 8192 x 4096 into bf16 106-113 us, 2.4 to 2.6 POP/s), by the weights below (5 x 4096 x 131072 into
 // f32 90 us, 5.9 TB/s; 48 x 4096 x 12288 12.9, 3.9 TB/s), by a launch, the first loads and the epilogue for small ones
-// (1 x 2048 x 2560 5.0).
+// (1 x 2048 x 2560 4.6).
 #include "fast_paths.h"
 
 namespace {
