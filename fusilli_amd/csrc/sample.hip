@@ -75,6 +75,9 @@ __device__ __forceinline__ double reciprocal(double x) {
   return __builtin_fma(y, __builtin_fma(-x, y, 1.0), y);
 }
 
+// (m - l) / T from which on no weight is held.
+constexpr double kFar = 33.0;
+
 struct Settings : Asked {
   double most, by;  // the largest logit, 1 / T
   double by2;       // log2(e) / T
@@ -124,9 +127,10 @@ struct Settings : Asked {
   __device__ __forceinline__ uint64_t held_near(float l) const {
     return __builtin_bit_cast(uint64_t, near_weight(l, bits) + 0x1p52) & ((1ull << 52) - 1);
   }
-  // The same of any; 0 from exp(-32) = 2^-46.2 on.
+  // The same of any.  0 beyond kFar, where held_near is 0 as well (from exp(-32.58) = 2^-47 on): whichever of the
+  // two a kernel asks, sums and the words that they are made of agree, also where buckets end a rounding off kFar.
   __device__ __forceinline__ uint64_t held(float l) const {
-    return l == top ? 1ull << bits : ((double)l - most) * by > -32.0 ? held_near(l) : 0;
+    return l == top ? 1ull << bits : ((double)l - most) * by > -kFar ? held_near(l) : 0;
   }
   // the weights' sum that top_p asks for of `all`; the sum that the token's exceeds of `kept`
   __device__ __forceinline__ uint64_t share(uint64_t all) const {
@@ -343,7 +347,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs g) 
 // One workgroup takes all steps of a row where rows fill the chip or are short; otherwise they are three
 // launches over parts of rows, the last part of a row answering.
 //
-// Buckets cover what words have above a weight of 0, less than 32 of (m - l) / T.  Which of them matter one
+// Buckets cover what words have above a weight of 0, less than 33 of (m - l) / T (kFar).  Which of them matter one
 // wavefront finds, without a barrier: sixteen that execute the same few hundred instructions
 // between barriers take three times as long.
 //
@@ -520,7 +524,7 @@ struct Buckets {
   __device__ __forceinline__ Buckets(const Settings &set, float least) : half(0.5f * set.top) {
     const double range = (set.most - (double)least) * set.by;
     // (a little less than the range takes, so that the last word is inside for all roundings)
-    const double unit = range > 0.0 ? kBuckets * (1.0 - 0x1p-20) * reciprocal(range < 32.0 ? range : 32.0) : 0.0;
+    const double unit = range > 0.0 ? kBuckets * (1.0 - 0x1p-20) * reciprocal(range < kFar ? range : kFar) : 0.0;
     const double x = 2.0 * set.by * unit;
     by = x < 3.0e38 ? (float)x : 3.0e38f;
     a_unit = unit < 3.0e38 ? (float)unit : 3.0e38f;

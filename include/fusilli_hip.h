@@ -581,16 +581,18 @@ int fhip_matmul_quantized(fhip_ctx *ctx, const fhip_matmul_quantized_desc *d,
 /* A token for each row of logits, drawn with the caller's random numbers.  With m
  * a row's largest logit and T its temperature, word i has the weight
  *   w_i = exp((logit_i - m) / T), 1 for the largest,
- * in f64, held as a whole multiple of 2^-46 (of 2^-38 for the longest rows).  Words are ordered by their logits, the
- * largest first, equal ones by their index, and the first so many are kept as the
- * strictest of these says:
+ * in f64, held as the nearest whole multiple of 2^-46 (of 2^-38 for the longest
+ * rows; 0 from (m - logit_i) / T = 32.6 on).  Words are ordered by their logits,
+ * the largest first, equal ones by their index, and the first so many are kept as
+ * the strictest of these says:
  *   top_k   the first top_k (0 or less: all);
  *   top_p   of what top_k keeps, the fewest whose weights' sum reaches top_p of
  *           all of it (1 or more, or NaN: all; 0 or less: the first);
  *   min_p   those whose weight is at least min_p (NaN: all);
  * one at least.  TOKEN is the first word in that order up to which the kept weights'
  * sum exceeds uniform times all of it (uniform in [0, 1); values outside count as
- * the nearest inside, NaN as 0), PROBABILITY its weight over that sum.  T that is
+ * the nearest inside, so that those from 1 on draw the last word that weighs
+ * anything, NaN as 0), PROBABILITY its weight over that sum.  T that is
  * not above 0: the first word, with probability 1.  Logits that are NaN or -inf are
  * never drawn; a row of nothing else has token -1 and probability 0.  The settings
  * are vectors of `rows` elements on the device or, where there is none, the
