@@ -679,9 +679,12 @@ __device__ __forceinline__ End list_end(bool by_count, uint64_t need, int n, Dra
   return e;
 }
 
-// Rows of no word and greedy ones have none, and those whose largest logit is infinite go to sample_row.
+// Rows of no word and greedy ones have none; those whose largest logit is infinite and those at a temperature below
+// 2^-90 go to sample_row.  (Further down f32 may have no number for Buckets::by, which is capped; from 2^-90 on it is
+// where all words are within 6.8e-36 of the largest, hence 2^-26 of a temperature: min_p below 1 keeps them all.)
+constexpr float kColdest = 0x1p-90f;
 __device__ __forceinline__ bool has_questions(const Range &range, float t) {
-  return range.most != 0 && t > 0.f && range.largest() < INFINITY;
+  return range.most != 0 && t >= kColdest && range.largest() < INFINITY;
 }
 // Does a row without questions; false: it has some.
 template <int NT>

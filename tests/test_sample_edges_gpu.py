@@ -79,3 +79,26 @@ def test_numbers_beyond_their_range(ctx, words, stride, dtype_seed):
     p, least = rng.choice([1.0, 0.9, 0.5], n), rng.choice([0.0, 0.05, 1.0], n)
     for u in (1.0, 1.5, np.inf, -1.0, -np.inf, np.nan):
         check(ctx, rows, u, t, k, p, least, stride=stride)
+
+
+COLD = PATHS[1:]
+
+
+@pytest.mark.parametrize("words,stride", COLD)
+@pytest.mark.parametrize("t", [1e-45, 1e-42, 1e-39, 2e-38, 1e-33, 1e-29, 8.07e-28, 8.08e-28, 1e-26])
+def test_rows_that_are_nearly_greedy(ctx, words, stride, t):
+    """Temperatures down to the smallest number above 0, with words a few of them apart and others beyond 64 of them."""
+    rng = np.random.default_rng([3, words])
+    t = float(np.float32(t))
+    rows = np.full([8, words], -1.0, np.float32)
+    for i, row in enumerate(rows):
+        at = rng.permutation(words)[:200]
+        row[at] = -np.float32(np.maximum(np.rint(rng.uniform(0, [5, 40, 200, 1000][i % 4], 200)), 0) * t)
+        row[at[0]] = 0
+        row[at[1]] = [-1e-30, -7e-36, -3e-36, -1e-37][i % 4]
+        if i >= 4:  # (every word near the largest)
+            row[:] = np.where(row == -1, np.float32(-0.25 * t), row)
+    for u in (0.05, 0.4, 0.8, 0.99, 1.0):
+        check(ctx, rows, u, t, stride=stride)
+        check(ctx, rows, u, t, k=[0, 3, 50, 0, 0, 7, 0, 100], p=[0.9, 1.0, 0.5, 0.99, 0.9, 1.0, 0.5, 0.99],
+              least=[0.0, 0.02, 0.0, 0.3, 0.02, 0.0, 0.99999994, 1.0], stride=stride)
