@@ -87,7 +87,9 @@ struct Settings : Asked {
   __device__ __forceinline__ Settings(const SampleArgs &g, const Asked &asked, float largest) : Asked(asked) {
     most = (double)largest;
     greedy = !(t > 0.f);
-    by = greedy ? 1.0 : fmax(reciprocal((double)t), 1e-300); // (T infinite: NaN; -inf times it is -inf)
+    // (T infinite: NaN here, and 1e-100, with which -inf is -inf, any other difference times it less than 2^-200 and
+    // the smallest one's reciprocal a number)
+    by = greedy ? 1.0 : fmax(reciprocal((double)t), 1e-100);
     by2 = by * 1.44269504088896340736;
     top = largest;
     bits = g.bits;

@@ -102,3 +102,16 @@ def test_rows_that_are_nearly_greedy(ctx, words, stride, t):
         check(ctx, rows, u, t, stride=stride)
         check(ctx, rows, u, t, k=[0, 3, 50, 0, 0, 7, 0, 100], p=[0.9, 1.0, 0.5, 0.99, 0.9, 1.0, 0.5, 0.99],
               least=[0.0, 0.02, 0.0, 0.3, 0.02, 0.0, 0.99999994, 1.0], stride=stride)
+
+
+@pytest.mark.parametrize("words,stride", COLD)
+@pytest.mark.parametrize("apart", [1e-45, 1e-30, 1e-12, 1e-10, 1e-9, 1e-8, 1e-7, 1.0, 1e30])
+def test_rows_of_infinite_temperature(ctx, words, stride, apart):
+    """Every word weighs the same, however close together or far apart they are."""
+    rng = np.random.default_rng([4, words])
+    rows = (-rng.integers(0, 50, [4, words]) * np.float64(apart)).astype(np.float32)
+    rows[1, ::3] = -np.inf
+    rows[2, 1::2] = 0
+    for u in (0.0, 0.3, 0.7, JUST_BELOW_ONE, 1.0):
+        check(ctx, rows, u, np.inf, stride=stride)
+        check(ctx, rows, u, np.inf, k=[0, 9, words // 2, 0], p=[0.5, 1.0, 0.9, 0.25], least=[0.0, 0.5, 1.0, 0.0], stride=stride)
