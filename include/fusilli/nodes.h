@@ -1299,7 +1299,10 @@ public:
   ErrorObject postValidateNode() const override final {
     return checkShapes(sampleAttr, kOp);
   }
-  static ErrorObject checkShapes(const SampleAttr &a, const std::string &op) {
+  // `probability` false: nothing reads or writes it, and it keeps the extents
+  // that it was declared with.
+  static ErrorObject checkShapes(const SampleAttr &a, const std::string &op,
+                                 bool probability = true) {
     const int64_t rows = a.getLOGITS()->getDim()[0];
     auto check = [&](const TensorPtr &t, const std::string &which,
                      DataType type) {
@@ -1317,7 +1320,9 @@ public:
     FUSILLI_CHECK_ERROR(check(a.getTOP_P(), "TOP_P", DataType::Float));
     FUSILLI_CHECK_ERROR(check(a.getMIN_P(), "MIN_P", DataType::Float));
     FUSILLI_CHECK_ERROR(check(a.getTOKEN(), "TOKEN", DataType::Int32));
-    return check(a.getPROBABILITY(), "PROBABILITY", DataType::Float);
+    return probability
+               ? check(a.getPROBABILITY(), "PROBABILITY", DataType::Float)
+               : ok();
   }
 
 private:

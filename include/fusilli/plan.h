@@ -1097,8 +1097,11 @@ private:
 
   ErrorObject planSample(size_t i) {
     const auto &attr = static_cast<const SampleNode &>(*nodes_[i]).sampleAttr;
-    FUSILLI_CHECK_ERROR(
-        SampleNode::checkShapes(attr, "Node '" + attr.getName() + "':"));
+    // (a virtual PROBABILITY that no node reads is not written)
+    const TensorPtr p = attr.getPROBABILITY();
+    const bool asked = !p->isVirtual() || consumers_.count(p.get()) > 0;
+    FUSILLI_CHECK_ERROR(SampleNode::checkShapes(
+        attr, "Node '" + attr.getName() + "':", asked));
     Step s;
     s.kind = static_cast<uint32_t>(StepKind::Sample);
     fhip_sample_desc &d = s.desc.sample;
@@ -1128,9 +1131,7 @@ private:
     FUSILLI_CHECK_ERROR(
         mustRun(fhip_sample_supported(&d) != 0, "Sample", attr.getName()));
     FUSILLI_ASSIGN_OR_RETURN(s.slot[kSmToken], writeSlot(attr.getTOKEN()));
-    // (a virtual PROBABILITY that no node reads is not written)
-    const TensorPtr p = attr.getPROBABILITY();
-    if (!p->isVirtual() || consumers_.count(p.get()) > 0) {
+    if (asked) {
       FUSILLI_ASSIGN_OR_RETURN(s.slot[kSmProbability], writeSlot(p));
     }
     size_t scratch = 0;

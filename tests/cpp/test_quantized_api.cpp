@@ -204,6 +204,47 @@ TEST("host: what no kernel takes is refused by compile") {
               "Quantized matmul node 'm' is not executable by this backend: fhip_matmul_quantized: A and B must be Int8");
 }
 
+TEST("host: buffers give a draw another number of rows, also where nothing asks for the probability") {
+  for (bool asked : {false, true}) {
+    Graph g = newGraph("dynamic_draw");
+    auto logits = g.tensor(mk("logits", {kRows, kWords}, DataType::Float).setDynamicDims({0}));
+    auto u = g.tensor(mk("u", {kRows}, DataType::Float).setDynamicDims({0}));
+    SampleAttr a;
+    a.setName("s");
+    auto [token, probability] = g.sample(logits, u, g.tensor(TensorAttr(0.8f)), nullptr, nullptr, nullptr, a);
+    token->setOutput(true).setDim({kRows}).setStride({1}).setDynamicDims({0});
+    if (asked)
+      probability->setOutput(true).setDim({kRows}).setStride({1}).setDynamicDims({0});
+    REQUIRE_OK(g.validate());
+    REQUIRE_ASSIGN(Handle cpu, Handle::create(Backend::CPU));
+    REQUIRE_OK(g.compile(cpu, true));
+    auto need = g.getWorkspaceSize();
+    REQUIRE(!isError(need) && **need == 0);
+    for (int64_t rows : {kRows, int64_t{1}, int64_t{50}}) {
+      auto buf = [&](int64_t cols, const Dims &dims) {
+        return std::make_shared<Buffer>(std::move(*Buffer::allocate(
+            cpu, std::vector<size_t>(dims.begin(), dims.end()), std::vector<float>(rows * cols))));
+      };
+      Pack pack;
+      pack[logits] = buf(kWords, {rows, kWords});
+      pack[u] = buf(1, {rows});
+      pack[token] = std::make_shared<Buffer>(
+          std::move(*Buffer::allocate(cpu, {(size_t)rows}, std::vector<int32_t>(rows))));
+      if (asked)
+        pack[probability] = buf(1, {rows});
+      // (planned for these rows: only then the backend is looked at)
+      CHECK_ERROR(g.execute(cpu, pack, nullptr), ErrorCode::NotImplemented,
+                  "Backend::CPU has no execution engine in this build: graphs run on Backend::AMDGPU (gfx950) only");
+      if (asked && rows != kRows) {
+        pack[probability] = std::make_shared<Buffer>(
+            std::move(*Buffer::allocate(cpu, {(size_t)kRows}, std::vector<float>(kRows))));
+        CHECK_ERROR(g.execute(cpu, pack, nullptr), ErrorCode::InvalidAttribute,
+                    "Node 's': tensor PROBABILITY must be contiguous [" + std::to_string(rows) + "]");
+      }
+    }
+  }
+}
+
 // ---- on the GPU ----------------------------------------------------------------
 static Handle &gpu() {
   static Handle h = [] {
