@@ -18,6 +18,7 @@
 #ifndef FUSILLI_PLAN_H
 #define FUSILLI_PLAN_H
 
+#include <algorithm>
 #include <cstring>
 #include <map>
 #include <set>
@@ -1138,6 +1139,17 @@ private:
     FUSILLI_RETURN_ERROR_IF(fhip_sample_workspace_size(&d, &scratch) != 0,
                             ErrorCode::InternalError,
                             std::string(fhip_last_error(nullptr)));
+    // Few long rows need workspace, many do not: where buffers may give fewer
+    // than are declared, as much as any count of them.  (None of 1024 and more
+    // does; fewer words never need more.)
+    fhip_sample_desc fewer = d;
+    for (int64_t r = std::min<int64_t>(d.logits.dim[0], 1024);
+         r > 0 && attr.getLOGITS()->isDynamicDim(0); --r) {
+      size_t need = 0;
+      fewer.logits.dim[0] = r;
+      if (fhip_sample_workspace_size(&fewer, &need) == 0)
+        scratch = std::max(scratch, need);
+    }
     s.slot[kSmScratch] = scratchSlot(scratch);
     plan_.steps.push_back(s);
     return ok();

@@ -245,6 +245,38 @@ TEST("host: buffers give a draw another number of rows, also where nothing asks 
   }
 }
 
+TEST("host: the workspace of a draw with dynamic rows serves every number of rows up to the declared one") {
+  constexpr int64_t kLong = 30000;
+  auto needOf = [&](int64_t rows, bool dynamic) {
+    Graph g = newGraph("dynamic_room");
+    auto logits = g.tensor(mk("logits", {rows, kLong}, DataType::Half));
+    auto u = g.tensor(mk("u", {rows}, DataType::Float));
+    SampleAttr a;
+    a.setName("s");
+    auto token = g.sample(logits, u, nullptr, nullptr, nullptr, nullptr, a)[0];
+    token->setOutput(true);
+    if (dynamic) {
+      logits->setDynamicDims({0});
+      u->setDynamicDims({0});
+      token->setDim({rows}).setStride({1}).setDynamicDims({0});
+    }
+    REQUIRE_OK(g.validate());
+    REQUIRE_ASSIGN(Handle cpu, Handle::create(Backend::CPU));
+    REQUIRE_OK(g.compile(cpu, true));
+    auto need = g.getWorkspaceSize();
+    REQUIRE(!isError(need) && need->has_value());
+    return **need;
+  };
+  // (few long rows are cut into parts, many are not)
+  CHECK(needOf(256, false) == 0);
+  for (int64_t rows : {2, 100, 256, 1000}) {
+    const size_t room = needOf(rows, true);
+    for (int64_t now : {1, 2, 5, 60, 127, 128, 190, 191, 192, 256})
+      if (now <= rows)
+        CHECK(room >= needOf(now, false));
+  }
+}
+
 // ---- on the GPU ----------------------------------------------------------------
 static Handle &gpu() {
   static Handle h = [] {
