@@ -1119,8 +1119,10 @@ private:
         continue;
       if (settings[k]->isScalar()) {
         const double v = scalarAsDouble(*settings[k]);
-        if (k == 1) // (0 or less: off; more than there are words: all)
-          d.top_k = v < 1 ? 0 : v > 2147483647.0 ? 2147483647 : static_cast<int32_t>(v);
+        if (k == 1) // (0 or less, or NaN: off; more than there are words: all)
+          d.top_k = !(v >= 1) ? 0
+                    : v > 2147483647.0 ? 2147483647
+                                       : static_cast<int32_t>(v);
         else
           (k == 0 ? d.temperature : k == 2 ? d.top_p : d.min_p) =
               static_cast<float>(v);

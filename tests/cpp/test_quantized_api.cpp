@@ -277,6 +277,26 @@ TEST("host: the workspace of a draw with dynamic rows serves every number of row
   }
 }
 
+TEST("host: constants of TOP_K that are no count are off, larger ones all words") {
+  auto planOf = [](float k) {
+    Graph g = newGraph("constant_top_k");
+    auto logits = g.tensor(mk("logits", {kRows, kWords}, DataType::Float));
+    SampleAttr a;
+    a.setName("s");
+    g.sample(logits, g.tensor(mk("u", {kRows}, DataType::Float)), nullptr, g.tensor(TensorAttr(k)), nullptr, nullptr, a)[0]
+        ->setOutput(true);
+    REQUIRE_OK(g.validate());
+    REQUIRE_ASSIGN(auto bytes, g.compileToArtifact(Backend::CPU, /*remove=*/true));
+    return bytes;
+  };
+  const auto off = planOf(0.f), all = planOf(2147483648.f);
+  CHECK(off != all && off != planOf(1.f));
+  for (float k : {std::nanf(""), -1.f, 0.5f, -INFINITY})
+    CHECK(planOf(k) == off);
+  for (float k : {1e30f, INFINITY})
+    CHECK(planOf(k) == all);
+}
+
 // ---- on the GPU ----------------------------------------------------------------
 static Handle &gpu() {
   static Handle h = [] {
