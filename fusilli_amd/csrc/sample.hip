@@ -1099,7 +1099,9 @@ template <int NT>
 __device__ __forceinline__ void answer(const SampleArgs &g, int64_t row, const Settings &set, const Buckets &buckets, int n,
                                        Draw<NT> &d, const unsigned long long *handed = nullptr) {
   const int l = threadIdx.x & 63;
-  if (n > (handed ? kList : list_of(NT))) { // (many equal logits)
+  // (Many equal logits, many that are close below one far above them, or distinct ones of a million words and more, of
+  // which a bucket holds thousands: f32 2^20 normal ones 33 to 60 us, 2^22 94 us on the list and 29 to 46 ms here.)
+  if (n > (handed ? kList : list_of(NT))) {
     sample_row<NT>(g, row, d.whole);
     return;
   }

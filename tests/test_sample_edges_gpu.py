@@ -115,3 +115,11 @@ def test_rows_of_infinite_temperature(ctx, words, stride, apart):
     for u in (0.0, 0.3, 0.7, JUST_BELOW_ONE, 1.0):
         check(ctx, rows, u, np.inf, stride=stride)
         check(ctx, rows, u, np.inf, k=[0, 9, words // 2, 0], p=[0.5, 1.0, 0.9, 0.25], least=[0.0, 0.5, 1.0, 0.0], stride=stride)
+
+
+@pytest.mark.parametrize("rows,words", [(2, 1 << 20), (2, (1 << 22) + 3), (1, 1 << 24)])
+def test_large_vocabularies_of_distinct_logits(ctx, rows, words):
+    """So many words in each bucket that those in question outnumber what a list holds: all of the row's words answer."""
+    rows = np.random.default_rng([5, words]).normal(size=[rows, words]).astype(np.float32) * np.float32([[1.5], [3.0]][:rows])
+    check(ctx, rows, [0.83, 0.4][:len(rows)], p=0.95)
+    check(ctx, rows, [0.02, 0.99][:len(rows)], t=1.25, k=words // 3, p=0.9, least=[1e-6, 0.0][:len(rows)])
