@@ -300,7 +300,7 @@ int fhip_direct_matmul(fhip_ctx *ctx, const fhip_matmul_desc *d, const void *a, 
   const bool f32_out = p.kind != GK_I8 && !scales && d->c.dtype == FHIP_FLOAT && d->out.dtype == FHIP_FLOAT;
   // Split products over a long K stay on the tiled GEMM, and so do those over one whole slice (bf16
   // 5696 x 5184 x 64 in four batches 59 us, here 416; 1536 x 448 x 64 5.7 / 9.5); those over less
-  // than a slice stay here.
+  // than a slice stay here, whatever they cost (scaled int8, M4096 N10624: K127 157 us, K128 on the tiled GEMM 33).
   if (whole && (f32_out || g.slices >= 128 || g.slices == 1))
     return 0;
   if (p.kind != GK_F32 && !f32_out && g.slices > 1) {

@@ -354,11 +354,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs g) 
 // between barriers take three times as long.
 //
 // Bound by memory (three walks, of which caches feed the last two) and by f64 arithmetic, 30 instructions a
-// word, where rows are many: f32 256 x 131072, 134 MB, 97 us, of it 28 for the largest logits (4.8 TB/s), 39 for
+// word, where rows are many: f32 256 x 131072, 134 MB, 93 to 97 us, of it 28 for the largest logits (4.8 TB/s), 39 for
 // the sums (20 without the exponentials), 16 for bringing together; by what runs once where they are few: code
-// that no cache holds yet, loads that wait for each other, three launches.  1 x 65536 16.4 us, bf16 48 x 131072
-// 40 us (launches 6.6, 12 and 21, of which putting 1300 words of its flattest row in order takes 10), f16
-// 7 x 100003 22, f32 25 x 536 10.
+// that no cache holds yet, loads that wait for each other, three launches.  1 x 65536 17 to 19 us, bf16 48 x 131072
+// 39 to 40 us (launches 6.6, 12 and 21, of which putting 1300 words of its flattest row in order takes 10), f16
+// 7 x 100003 24 to 27, f32 25 x 536 10.
 constexpr int kBuckets = 1024;
 constexpr int kThreads = 1024; // of the launches over parts
 // How many words of the buckets in question NT threads hold, and how many of them they sort.
@@ -1316,7 +1316,10 @@ template <int DT> __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel
 
 // How rows are cut: a workgroup a row where rows are short or fill the chip, otherwise parts that do, of
 // 4096 words at least.  us, one part / parts: bf16 33 x 16384 17.2 / 20.9 (four), f32 4 x 8192 13.7 / 17.9;
-// f32 130 x 131072 80 / 67 (four), 256 x 131072 94 / 108 (two), bf16 257 x 32000 31 / 40.
+// f32 130 x 131072 80 / 67 (four), 256 x 131072 94 / 108 (two), bf16 257 x 32000 31 / 40.  As it is, over
+// 131072 words f32 (128256 words bf16): 128 rows 65 us (59), 191 92 (79), 192 82 (74), 256 88 (76), 257 126 (77),
+// 300 138 (116), 512 163 (144): a workgroup of 1024 threads has a compute unit to itself, and more of them than units
+// take a second round.
 constexpr int64_t kFull = 192, kShort = 20480;
 struct Cut {
   int parts, words;

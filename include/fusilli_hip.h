@@ -516,7 +516,8 @@ int fhip_cache_read(fhip_ctx *ctx, const fhip_cache_read_desc *d,
  *      codes 0, a row whose y holds a NaN or an infinity scale NaN and codes 0.
  *      (Where a is below 2^-100 both factors of the product are taken 2^64
  *      times as large; scales below 2^-126 are subnormal and lose bits.)
- *      A row whose squares' sum leaves f32 counts as not finite for the norm.
+ *      A row whose squares' sum leaves f32 counts as not finite for the norm, and
+ *      so does one whose squares are all 0 in f32 with an epsilon of 0.
  *      X's type: f32, bf16 or f16; strides are free.  supported: 2 (rows held in
  *      registers) for X, UP, Q and the weight with a last stride of 1, K at most
  *      32768 and fewer than 2^21 rows; otherwise 1. ------------------------- */
@@ -599,7 +600,9 @@ int fhip_matmul_quantized(fhip_ctx *ctx, const fhip_matmul_quantized_desc *d,
  * descriptor's.  At most 2^24 words.  Needs 256-byte aligned workspace of
  * fhip_sample_workspace_size bytes; it holds nothing between calls, and calls that
  * overlap need one each.  supported: 2 for a last stride of 1 and fewer than 2^21
- * rows; otherwise 1. */
+ * rows; otherwise 1.  (Single rows may still take the slower way of the latter:
+ * those with an infinite logit, with T below 2^-90, with thousands of equal or
+ * nearly equal logits about a border, or of 2^20 words and more.) */
 typedef struct {
   fhip_tensor_desc logits; /* [rows, words] f32, bf16 or f16 */
   int32_t has_temperature, has_top_k, has_top_p, has_min_p;

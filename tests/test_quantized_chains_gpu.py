@@ -41,3 +41,22 @@ def test_columns_multiplied_cut_and_added(ctx, m, n, k, c_dtype, dtype):
     y = np.maximum(c * by, 0) + t.logical()
     # (the product and the sum round once each, or once together)
     check_product(out.logical(), y, bound * by + UNIT * (np.abs(c * by) * 1.01 + np.abs(y)), dtype)
+
+
+@pytest.mark.parametrize("m,n,k", [(1000, 1100, 15), (1000, 1100, 16), (1024, 2048, 64), (1500, 1032, 100), (2050, 1300, 127), (1152, 1024, 128)])
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=NAME.get)
+@pytest.mark.parametrize("along_k", [True, False])
+def test_many_results_of_a_short_reduction(ctx, m, n, k, dtype, along_k):
+    rng = np.random.default_rng([m, n, k])
+    a, b = (rng.integers(-128, 128, s, np.int8) for s in ([m, k], [k, n]))
+    sa, sb = ((0.5 + rng.random(s)).astype(np.float32) * np.float32(0.01) for s in (m, n))
+    hb, out = HT.from_logical(b, capi.INT8, [1, k] if along_k else None), HT.empty([m, n], dtype, [n + 3, 1], fill=3)
+    d = capi.MatmulQuantizedDesc()
+    d.a, d.b, d.c = capi.TensorDesc.make([m, k], [k, 1], capi.INT8), hb.desc(), capi.TensorDesc.make([m, n], [n, 1], dtype)
+    d.out, d.out_dtype, d.a_scale_stride, d.b_scale_stride = out.desc(), dtype, 1, 1
+    o = guarded(ctx, out.storage)
+    ctx.matmul_quantized(d, *[ctx.to_device(x) for x in (a, hb.storage, sa, sb)], o[1])
+    out.storage = o[2]()
+    assert (out.storage[: (m - 1) * (n + 3)].reshape(m - 1, n + 3)[:, n:] == 3).all()
+    c = a.astype(np.float64) @ b.astype(np.float64) * sa.astype(np.float64)[:, None] * sb.astype(np.float64)
+    check_product(out.logical(), c, 3 * UNIT * np.abs(c) * 1.001, dtype)
